@@ -6,8 +6,8 @@
 - ``linear``: the product of a few tokens with a 4-bit weight, stored in the activations' type, in float32, or with a SiLU gate.
 
 What 4 bits hold: ``group`` neighbouring values share a minimum z and a step s, both float16, and a value is c s + z with c in 0 .. 15:
-z = float16(min x), s = float16((max x - z) / 15) with the difference and the quotient in float32, c = (x - z) / s rounded to the
-nearest, ties to even, and cut to 0 .. 15; s = 0 gives c = 0.  A group that holds a value beyond 60000, or one that is not finite, is
+z = float16(min x), s = float16((max x - z) f) with f the float32 next to 1/15, the difference and the product in float32,
+c = (x - z) / s rounded to the nearest, ties to even, and cut to 0 .. 15; s = 0 gives c = 0.  A group that holds a value beyond 60000, or one that is not finite, is
 not a number as a whole.
 
 Sizes are those of the engine's 1b, 8b and 14b layers and of its tiny models.  Inputs are normal (keys with the louder channels that
@@ -219,7 +219,7 @@ def quantise(x, group):
     x = x.unflatten(-1, (-1, group))
     lo, hi = x.amin(-1).float(), x.amax(-1).float()
     z = lo.half()
-    s = ((hi - z.float()) / 15.0).half()
+    s = ((hi - z.float()) * torch.tensor(1.0 / 15.0, dtype=torch.float32, device=x.device)).half()
     bad = ~((x.float().abs() <= LIMIT).all(-1))
     s, z = s.masked_fill(bad, math.nan), z.masked_fill(bad, math.nan)
     code = ((x.double() - z.double()[..., None]) / s.double()[..., None]).round().clamp(0, 15)
@@ -326,7 +326,9 @@ def held_values(x, group):
     rows = x.reshape(-1, group)
     least, most = rows.min(dim=1).values.to(torch.float32), rows.max(dim=1).values.to(torch.float32)
     z = least.to(torch.float16).double()
-    s = torch.div(torch.sub(most, z.to(torch.float32)), 15.0).to(torch.float16).double()
+    # (the product of two float32 numbers is exact in float64)
+    f = float(torch.tensor(1.0 / 15.0, dtype=torch.float32))
+    s = (torch.sub(most, z.to(torch.float32)).double() * f).to(torch.float32).to(torch.float16).double()
     y = rows.double()
     t = (y - z[:, None]) / torch.where(s > 0, s, torch.ones_like(s))[:, None]
     whole = torch.floor(t)
