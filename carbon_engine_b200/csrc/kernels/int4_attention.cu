@@ -1,0 +1,572 @@
+// Attention over a paged cache held in 4 bits (int4.cuh): rows of queries against the tiles of 16 keys of one KV head.
+//
+// For a query row q and the keys j it sees, with group g of the channels:
+//   S_j = scale sum_g (s_jg (q_g . c_jg) + z_jg sum q_g),   p_j = exp(S_j - max S),
+//   out_g = sum_j (p_j s_jg c_jg + p_j z_jg) / sum_j p_j
+// so the codes themselves are the operands of both products, and steps and minima never touch a value: a step scales a group's partial score
+// (keys) or the probability (values), a minimum takes part in float32.  Keys (values' channels) are the 16 rows of mma.sync m16n8k16, query
+// rows its 8 columns, which is how the heads of a group that share a KV head fill a tile.
+//
+// Roundings: a query row is brought into [2^14, 2^15) by a power of two and rounded to float16, which is exact for bfloat16 (to 2^-30 of the
+// row's largest); float32 rows are two float16 pieces, 22 bits.  p_j s_jg is rounded to float16 (2^-12 of itself; two pieces for float32),
+// scaled so that the largest lies near 2^10: sums of thousands of small weights keep their bits.  Everything else is float32.
+//
+// A block takes up to 8 or 16 rows (tokens by heads of the KV head) and a run of the keys; its 8 warps take tiles in turn, each with a ring
+// of its own that one lane fills with bulk copies (a tile is one run of bytes in the page); warps, then blocks, are joined in a fixed order.
+#include "int4.cuh"
+
+namespace {
+
+constexpr int WARPS = 8, STAGES = 4;
+constexpr uint32_t SPIN = 1u << 20;
+constexpr float HEADROOM = 5.0f;               // scores may pass the running maximum by this many powers of two before it is moved
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Args {
+    const void* q;                 // [T, heads, d]: token stride q_stride, heads d apart
+    void* out;                     // [T, heads, d] contiguous
+    const unsigned char* pages;
+    const int *seq_slot, *q_start, *ctx_len, *block_table, *tiles;
+    int* status;
+    float *part_o, *part_ml;       // splits > 1: [row block, split, rows, d], [row block, split, rows, 2]
+    long long q_stride;
+    int nh, nkv, page_size, max_pages, num_pages, window, splits, subs;    // subs: row blocks of a sequence (or of a tile of 64 tokens)
+    int vec;
+    float scale;
+};
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < SPIN; ++i) {
+        uint32_t ok;
+        asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(smem_of(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+        if (i > 256) __nanosleep(64);
+    }
+    return false;
+}
+__device__ __forceinline__ void copy_tile(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_of(bar)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_of(dst)), "l"(src), "r"(bytes), "r"(smem_of(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// What a block works on: rows [row0, row0 + 8 NT) of the (token, head) pairs of tokens q0 .. of a sequence
+struct Job {
+    int b, slot, t0, token0, tokens, base, row0, kvh;        // base: position of token 0 of the tile
+};
+__device__ __forceinline__ Job job_of(const Args& a, int job, int rows) {
+    Job j;
+    const int sub = job % a.subs, rest = job / a.subs, i = rest / a.nkv;
+    j.kvh = rest - i * a.nkv;
+    int q0 = 0;
+    if (a.tiles) { j.b = a.tiles[2 * i]; q0 = a.tiles[2 * i + 1]; }
+    else j.b = i;
+    const int start = a.q_start[j.b], n = a.q_start[j.b + 1] - start;
+    j.slot = a.seq_slot[j.b];
+    j.t0 = start + q0;
+    j.tokens = a.tiles ? min(64, n - q0) : 1;
+    j.base = a.ctx_len[j.b] - n + q0;
+    j.row0 = sub * rows;
+    return j;
+}
+
+template <typename T> struct Pieces;
+template <> struct Pieces<__nv_bfloat16> { static constexpr int N = 1; };
+template <> struct Pieces<float> { static constexpr int N = 2; };
+
+// (s, z) of one token's groups out of shared memory, as they lie: NG words
+template <int NG>
+__device__ __forceinline__ void load_steps(const unsigned char* p, uint32_t (&v)[NG]) {
+    if constexpr (NG == 1) v[0] = *reinterpret_cast<const uint32_t*>(p);
+    else if constexpr (NG == 2) { const uint2 x = *reinterpret_cast<const uint2*>(p); v[0] = x.x; v[1] = x.y; }
+    else if constexpr (NG == 3 || NG == 6) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) v[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NG / 4; ++i) {
+            const uint4 x = reinterpret_cast<const uint4*>(p)[i];
+            v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+        }
+    }
+}
+
+template <typename T, int D, int G, int NT>
+__global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
+    constexpr int NB = D / 64, NG = D / G, P = Pieces<T>::N, ROWS = 8 * NT, TILE = i4_cache_tile_bytes(D, G), CH = D / 32;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) uint64_t full[WARPS][STAGES];
+    __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
+    ce_pdl_begin();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3;
+    const int split = blockIdx.x % a.splits, job_id = blockIdx.x / a.splits;
+    const Job j = job_of(a, job_id, ROWS);
+    const int each = a.nh / a.nkv, rows = min(ROWS, j.tokens * each - j.row0);
+    if (rows <= 0) return;                            // a tile with fewer tokens than its row blocks take
+    const int first_pos = j.base + j.row0 / each, last_pos = j.base + (j.row0 + rows - 1) / each;
+    const int block_lo = a.window > 0 ? max(0, first_pos - a.window + 1) : 0;
+    const int tile_lo = block_lo >> 4, tiles = last_pos < block_lo ? 0 : (last_pos >> 4) + 1 - tile_lo;
+    const int share = (tiles + a.splits - 1) / a.splits, begin = min(split * share, tiles), end = min(begin + share, tiles);
+    const int mine = end - begin > warp ? (end - begin - warp + WARPS - 1) / WARPS : 0;      // tiles begin + warp, + WARPS, ...
+    const int* table = a.block_table + (size_t)j.slot * a.max_pages;
+    unsigned char* ring = smem + warp * (STAGES * TILE);
+    const int per_page = a.page_size >> 4;
+
+    if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(&full[warp][s])));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    // page ids of 32 of the warp's tiles at a time, one a lane
+    int looked = 0, page_ids = 0;
+    auto look_up = [&](int from) {
+        looked = from;
+        const int i = from + lane, pi = (tile_lo + begin + warp + i * WARPS) / per_page;
+        page_ids = i >= mine ? 0 : pi < a.max_pages ? table[pi] : -1;
+        if (page_ids < 0 || page_ids >= a.num_pages) { atomicExch(a.status, 4); page_ids = 0; }      // (the step's results are not used)
+    };
+    auto issue = [&](int i) {
+        if (i >= looked + 32) look_up(i);
+        const int page = __shfl_sync(0xffffffffu, page_ids, i - looked);
+        const int t = tile_lo + begin + warp + i * WARPS, in = t % per_page;
+        if (lane == 0)
+            copy_tile(ring + (i % STAGES) * TILE, a.pages + (((size_t)page * a.nkv + j.kvh) * per_page + in) * TILE, TILE, &full[warp][i % STAGES]);
+    };
+    look_up(0);
+    for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
+
+    // ---- queries: the second operand of K Q^T.  Lane (r, l) holds row 8 nt + r, channels 32 c + 8 l .. + 8; codes pair channels i and i + 4,
+    // and odd codes come 16 times too large
+    uint32_t qf[NT][P][CH][4];
+    float qsum[NT][NG][2], row_scale[NT][2];          // of rows 8 nt + 2 l and + 1, as the scores lie
+    int hi[NT][2], lo[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = nt * 8 + r;
+        float x[CH][8], largest = 0.f;
+        if (row < rows) {
+            const int rho = j.row0 + row, tok = rho / each;
+            const T* src = (const T*)a.q + (size_t)(j.t0 + tok) * a.q_stride + (size_t)(j.kvh * each + rho - tok * each) * D + 8 * l;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (a.vec) {
+                    const float4 u = ce_load4(src + 32 * c), v = ce_load4(src + 32 * c + 4);
+                    x[c][0] = u.x; x[c][1] = u.y; x[c][2] = u.z; x[c][3] = u.w; x[c][4] = v.x; x[c][5] = v.y; x[c][6] = v.z; x[c][7] = v.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[c][i] = CeType<T>::load(src + 32 * c + i);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[c][i] = 0.f;
+        }
+        bool finite = true;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { largest = fmaxf(largest, fabsf(x[c][i])); finite = finite && fabsf(x[c][i]) <= 3.402823466e38f; }
+        if (!finite) largest = INFINITY;
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        const float up = i4_row_scale(largest);
+        float sums[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) sums[g] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[c][i] * up;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f = i & 1 ? 0.0625f : 1.0f;
+                    qf[nt][p][c][i] = i4_pack(y[i] * f, y[i + 4] * f);
+                    const float2 got = i4_unpack(qf[nt][p][c][i]);
+                    const float g0 = got.x * (i & 1 ? 16.0f : 1.0f), g1 = got.y * (i & 1 ? 16.0f : 1.0f);
+                    sums[c * 32 / G] += g0 + g1;
+                    y[i] -= g0; y[i + 4] -= g1;
+                }
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qsum[nt][g][e] = __shfl_sync(0xffffffffu, sums[g], 4 * (2 * l + e)) * 0x1p-24f;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float u = __shfl_sync(0xffffffffu, up, 4 * (2 * l + e));
+            row_scale[nt][e] = a.scale * LOG2E * 0x1p24f / u;
+            const int rr = nt * 8 + 2 * l + e, pos = j.base + (j.row0 + rr) / each;
+            hi[nt][e] = rr < rows ? pos : -1;
+            lo[nt][e] = a.window > 0 ? pos - a.window + 1 : 0;
+        }
+    }
+
+    float o[NT][NB * 4][4], oz[NT][NG][2], m[NT][2], sum[NT][2];
+    float top = 0x1p-24f, norm = 1024.0f / top;       // a power of two that no step of V seen so far passes
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < NB * 4; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) oz[nt][g][0] = oz[nt][g][1] = 0.f;
+        m[nt][0] = m[nt][1] = -INFINITY;
+        sum[nt][0] = sum[nt][1] = 0.f;
+    }
+    // tiles in [whole_lo, whole_hi] hold only keys that every row sees
+    const int inner_lo = a.window > 0 ? max(0, last_pos - a.window + 1) : 0;
+
+    bool ok = true;
+    int gone = 0;                                     // tiles whose copies this warp has waited for
+    for (int i = 0; i < mine; ++i, ++gone) {
+        ok = wait_full(&full[warp][i % STAGES], (i / STAGES) & 1);
+        if (!ok) { if (lane == 0) atomicExch(a.status, 7); break; }
+        const unsigned char* tile = ring + (i % STAGES) * TILE;
+        const int key0 = (tile_lo + begin + warp + i * WARPS) * 16;
+        const bool cut = key0 < inner_lo || key0 + 15 > first_pos;
+        // ---- scores of keys r and r + 8 (rows of the tile) for query rows 2 l and 2 l + 1
+        uint32_t ka[NG], kb[NG];
+        load_steps<NG>(tile + 16 * D + r * NG * 4, ka);
+        load_steps<NG>(tile + 16 * D + (r + 8) * NG * 4, kb);
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+        float acc[NT][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint4 w = *reinterpret_cast<const uint4*>(tile + b * 512 + lane * 16);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int c = 2 * b + half;
+                const uint32_t wa = half ? w.z : w.x, wb = half ? w.w : w.y;
+                if ((c * 32) % G == 0)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const uint32_t ua = st ? wa >> 8 : wa, ub = st ? wb >> 8 : wb;
+                    const uint32_t a0 = ua & 0x000f000fu, a1 = ub & 0x000f000fu, a2 = ua & 0x00f000f0u, a3 = ub & 0x00f000f0u;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) i4_mma(acc[nt], a0, a1, a2, a3, qf[nt][p][c][2 * st], qf[nt][p][c][2 * st + 1]);
+                }
+                if ((c * 32 + 32) % G == 0) {
+                    const int g = c * 32 / G;
+                    const float2 fa = i4_unpack(ka[g]), fb = i4_unpack(kb[g]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            s[nt][e] = fmaf(fa.x, acc[nt][e], fmaf(fa.y, qsum[nt][g][e], s[nt][e]));
+                            s[nt][2 + e] = fmaf(fb.x, acc[nt][2 + e], fmaf(fb.y, qsum[nt][g][e], s[nt][2 + e]));
+                        }
+                }
+            }
+        }
+        const int key_a = key0 + r, key_b = key_a + 8;
+        // steps and minima of V; keys outside the block's reach may hold anything
+        uint32_t va[NG], vb[NG];
+        load_steps<NG>(tile + 16 * D + 64 * NG + r * NG * 4, va);
+        load_steps<NG>(tile + 16 * D + 64 * NG + (r + 8) * NG * 4, vb);
+        if (cut) {
+            const bool in_a = key_a >= block_lo && key_a <= last_pos, in_b = key_b >= block_lo && key_b <= last_pos;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                // a group that is not a number reaches the rows that see its key, and no others (0 times NaN would)
+                const bool nan_a = isnan(i4_unpack(va[g]).x), nan_b = isnan(i4_unpack(vb[g]).x);
+                if (__any_sync(0xffffffffu, nan_a || nan_b)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            if (nan_a && in_a && key_a <= hi[nt][e] && key_a >= lo[nt][e]) oz[nt][g][e] = __int_as_float(0x7fc00000);
+                            if (nan_b && in_b && key_b <= hi[nt][e] && key_b >= lo[nt][e]) oz[nt][g][e] = __int_as_float(0x7fc00000);
+                        }
+                }
+                if (!in_a || nan_a) va[g] = 0;
+                if (!in_b || nan_b) vb[g] = 0;
+            }
+        }
+        bool move = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s[nt][e] *= row_scale[nt][e];
+                s[nt][2 + e] *= row_scale[nt][e];
+                if (cut) {
+                    if (key_a > hi[nt][e] || key_a < lo[nt][e]) s[nt][e] = -INFINITY;
+                    if (key_b > hi[nt][e] || key_b < lo[nt][e]) s[nt][2 + e] = -INFINITY;
+                }
+                move = move || fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + HEADROOM;
+            }
+        float step_max = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) step_max = fmaxf(step_max, fmaxf(i4_unpack(va[g]).x, i4_unpack(vb[g]).x));
+        move = move || step_max > top;
+        if (__any_sync(0xffffffffu, move)) {
+            // maxima over the 8 lanes that share l, the largest step over all
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) step_max = fmaxf(step_max, __shfl_xor_sync(0xffffffffu, step_max, w));
+            const float before = top;
+            // the next power of two: a number's exponent, one up where it has bits below
+            if (step_max > top) top = __uint_as_float((__float_as_uint(step_max) + 0x007fffffu) & 0x7f800000u);
+            const float shrink = before / top;
+            norm = 1024.0f / top;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float mx = fmaxf(s[nt][e], s[nt][2 + e]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float mn = fmaxf(m[nt][e], mx), alpha = mn == -INFINITY ? 1.0f : exp2f(m[nt][e] - mn);
+                    m[nt][e] = mn;
+                    sum[nt][e] *= alpha;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) oz[nt][g][e] *= alpha;
+#pragma unroll
+                    for (int i2 = 0; i2 < NB * 4; ++i2) { o[nt][i2][e] *= alpha * shrink; o[nt][i2][2 + e] *= alpha * shrink; }
+                }
+        }
+        float pr[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+                pr[nt][e] = ce_exp2_fast(s[nt][e] - base);
+                pr[nt][2 + e] = ce_exp2_fast(s[nt][2 + e] - base);
+                sum[nt][e] += pr[nt][e] + pr[nt][2 + e];
+            }
+        // ---- V^T P^T, group by group: the probability carries the step
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint4 w = *reinterpret_cast<const uint4*>(tile + 8 * D + b * 512 + lane * 16);
+            uint32_t bf[NT][P][2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int g = (64 * b + 32 * half) / G;
+                if ((32 * half) % G == 0) {
+                    const float2 fa = i4_unpack(va[g]), fb = i4_unpack(vb[g]);
+                    const float sa = fa.x * norm, sb = fb.x * norm;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        oz[nt][g][0] = fmaf(pr[nt][0], fa.y, fmaf(pr[nt][2], fb.y, oz[nt][g][0]));
+                        oz[nt][g][1] = fmaf(pr[nt][1], fa.y, fmaf(pr[nt][3], fb.y, oz[nt][g][1]));
+                        float x0 = pr[nt][0] * sa, x1 = pr[nt][1] * sa, x2 = pr[nt][2] * sb, x3 = pr[nt][3] * sb;
+#pragma unroll
+                        for (int p = 0; p < P; ++p) {
+                            const uint32_t ab = i4_pack(x0, x1), cd = i4_pack(x2, x3);
+                            bf[nt][p][0] = transpose8(ab);
+                            bf[nt][p][1] = transpose8(cd);
+                            if (p + 1 < P) {
+                                const float2 g0 = i4_unpack(ab), g1 = i4_unpack(cd);
+                                x0 -= g0.x; x1 -= g0.y; x2 -= g1.x; x3 -= g1.y;
+                            }
+                        }
+                    }
+                }
+                // the halves of a word are the two halves of the block's channels; two tokens' words side by side
+                const uint32_t pick = half ? 0x7632u : 0x5410u;
+                const uint32_t u = __byte_perm(w.x, w.y, pick), v = __byte_perm(w.z, w.w, pick);
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const uint32_t us = st ? u >> 8 : u, vs = st ? v >> 8 : v;
+                    const uint32_t a0 = us & 0x000f000fu, a1 = us & 0x00f000f0u, a2 = vs & 0x000f000fu, a3 = vs & 0x00f000f0u;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) i4_mma(o[nt][b * 4 + half * 2 + st], a0, a1, a2, a3, bf[nt][p][0], bf[nt][p][1]);
+                }
+            }
+        }
+        __syncwarp();
+        if (i + STAGES < mine) issue(i + STAGES);
+    }
+    if (!ok) {
+        // the copies still in flight land in this block's memory: wait for them, with a limit, before it is used for anything else
+        for (int i = gone; i < min(gone + STAGES, mine); ++i) wait_full(&full[warp][i % STAGES], (i / STAGES) & 1);
+    }
+    __syncthreads();                                  // the rings are free: the warps' outputs take their place
+
+    float* so = reinterpret_cast<float*>(smem);       // [WARPS][ROWS][D + 4]
+    constexpr int LD = D + 4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = nt * 8 + 2 * l + e;
+            float t = sum[nt][e];
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) t += __shfl_xor_sync(0xffffffffu, t, w);
+            if (r == 0) { s_m[warp][row] = m[nt][e]; s_l[warp][row] = t; }
+            const float even = top * 0x1p14f, odd = top * 0x1p10f;
+            float zs[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                zs[g] = oz[nt][g][e];
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) zs[g] += __shfl_xor_sync(0xffffffffu, zs[g], w);
+            }
+#pragma unroll
+            for (int i = 0; i < NB * 4; ++i) {
+                const int ch = 64 * (i >> 2) + 32 * ((i >> 1) & 1) + 4 * r + 2 * (i & 1), g = (64 * (i >> 2) + 32 * ((i >> 1) & 1)) / G;
+                float2 v = make_float2(fmaf(o[nt][i][e], even, zs[g]), fmaf(o[nt][i][2 + e], odd, zs[g]));
+                *reinterpret_cast<float2*>(so + (warp * ROWS + row) * LD + ch) = v;
+            }
+        }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < rows * (D / 4); x += WARPS * 32) {
+        const int row = x / (D / 4), ch = (x - row * (D / 4)) * 4;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][row]);
+        float L = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = s_m[w][row] == -INFINITY ? (s_l[w][row] == 0.f ? 0.f : 1.f) : exp2f(s_m[w][row] - M);
+            const float4 u = *reinterpret_cast<const float4*>(so + (w * ROWS + row) * LD + ch);
+            L += s_l[w][row] * f;
+            v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+        }
+        if (a.splits > 1) {
+            const size_t at = ((size_t)job_id * a.splits + split) * ROWS + row;
+            *reinterpret_cast<float4*>(a.part_o + at * D + ch) = v;
+            if (ch == 0) { a.part_ml[2 * at] = M; a.part_ml[2 * at + 1] = L; }
+        } else {
+            const float inv = L == 0.f ? 0.f : 1.0f / L;
+            const int rho = j.row0 + row, tok = rho / each;
+            T* dst = (T*)a.out + ((size_t)(j.t0 + tok) * a.nh + j.kvh * each + rho - tok * each) * D + ch;
+            CeType<T>::store(dst, v.x * inv); CeType<T>::store(dst + 1, v.y * inv);
+            CeType<T>::store(dst + 2, v.z * inv); CeType<T>::store(dst + 3, v.w * inv);
+        }
+    }
+}
+
+// Joins the runs of keys of a row block, in their order: one block a row, four channels a thread
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(64) int4_attention_merge_kernel(Args a) {
+    ce_pdl_begin();
+    const int job_id = blockIdx.x / ROWS, row = blockIdx.x - job_id * ROWS;
+    const Job j = job_of(a, job_id, ROWS);
+    const int each = a.nh / a.nkv;
+    if (row >= j.tokens * each - j.row0) return;
+    const int ch = threadIdx.x * 4;
+    if (ch >= D) return;
+    float M = -INFINITY, L = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const size_t at = (size_t)job_id * a.splits * ROWS + row;
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (at + (size_t)s * ROWS)]);
+    for (int s = 0; s < a.splits; ++s) {
+        const size_t p = at + (size_t)s * ROWS;
+        const float ms = a.part_ml[2 * p], ls = a.part_ml[2 * p + 1];
+        const float f = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : exp2f(ms - M);
+        const float4 u = *reinterpret_cast<const float4*>(a.part_o + p * D + ch);
+        L += ls * f;
+        v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    const int rho = j.row0 + row, tok = rho / each;
+    T* dst = (T*)a.out + ((size_t)(j.t0 + tok) * a.nh + j.kvh * each + rho - tok * each) * D + ch;
+    CeType<T>::store(dst, v.x * inv); CeType<T>::store(dst + 1, v.y * inv);
+    CeType<T>::store(dst + 2, v.z * inv); CeType<T>::store(dst + 3, v.w * inv);
+}
+
+template <typename T, int D, int G, int NT>
+int run(const Args& a, int jobs, cudaStream_t stream) {
+    constexpr int TILE = i4_cache_tile_bytes(D, G), RING = WARPS * STAGES * TILE, OUT = WARPS * 8 * NT * (D + 4) * 4;
+    constexpr int SMEM = RING > OUT ? RING : OUT;
+    static_assert(SMEM <= 220 * 1024, "a block's shared memory");
+    static std::atomic<unsigned long long> done{0};
+    cudaError_t e = ce_allow_smem(done, int4_attention_kernel<T, D, G, NT>, SMEM);
+    if (e == cudaSuccess) {
+        ce_note("int4_attention_kernel");
+        e = ce_launch(int4_attention_kernel<T, D, G, NT>, dim3((unsigned)(jobs * a.splits)), dim3(WARPS * 32), SMEM, stream, a);
+    }
+    if (e == cudaSuccess && a.splits > 1) {
+        ce_note("int4_attention_merge_kernel");
+        e = ce_launch(int4_attention_merge_kernel<T, D, 8 * NT>, dim3((unsigned)(jobs * 8 * NT)), dim3(64), 0, stream, a);
+    }
+    if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_attention: %s", cudaGetErrorString(e)); }
+    return ce_check_launch("int4_attention");
+}
+
+template <typename T, int D, int G>
+int run_rows(const Args& a, int jobs, int rows, cudaStream_t stream) {
+    if constexpr (D <= 128) {
+        if (rows == 16) return run<T, D, G, 2>(a, jobs, stream);
+    }
+    return run<T, D, G, 1>(a, jobs, stream);
+}
+template <typename T, int D>
+int run_group(const Args& a, int group, int jobs, int rows, cudaStream_t stream) {
+    return group == 32 ? run_rows<T, D, 32>(a, jobs, rows, stream) : run_rows<T, D, 64>(a, jobs, rows, stream);
+}
+template <typename T>
+int run_type(const Args& a, int d, int group, int jobs, int rows, cudaStream_t stream) {
+    switch (d) {
+        case 64: return run_group<T, 64>(a, group, jobs, rows, stream);
+        case 128: return run_group<T, 128>(a, group, jobs, rows, stream);
+        case 192: return run_group<T, 192>(a, group, jobs, rows, stream);
+        default: return run_group<T, 256>(a, group, jobs, rows, stream);
+    }
+}
+
+// rows of a block: 8, or 16 where a KV head has more than 8 query rows to serve and the registers hold them (heads of at most 128)
+int block_rows(int each, int d, int tokens) { return d <= 128 && each * tokens > 8 ? 16 : 8; }
+
+}  // namespace
+
+// Rows a block takes, and the row blocks of a one-token sequence (tile 0) or of a tile of 64 tokens (tile 1)
+extern "C" int ce_int4_attention_rows(int each, int d, int tile) { return block_rows(each, d, tile ? 64 : 1); }
+extern "C" int ce_int4_attention_blocks(int each, int d, int tile) {
+    const int rows = block_rows(each, d, tile ? 64 : 1);
+    return ((tile ? 64 : 1) * each + rows - 1) / rows;
+}
+
+// dtype, q, q_stride, pages, out, seq_slot, q_start, ctx_len, block_table, tiles (or null: ``count`` one-token sequences), status, part_o,
+// part_ml, count, nh, nkv, d, group, page_size, max_pages, num_pages, window, splits, scale, stream
+extern "C" int ce_int4_attention(int dtype, const void* q, long long q_stride, const void* pages, void* out, const int* seq_slot, const int* q_start,
+                                 const int* ctx_len, const int* block_table, const int* tiles, int* status, float* part_o, float* part_ml, int count,
+                                 int nh, int nkv, int d, int group, int page_size, int max_pages, int num_pages, int window, int splits, float scale,
+                                 void* stream) {
+    if (!q || !pages || !out || !seq_slot || !q_start || !ctx_len || !block_table || !status) return ce_fail(CE_ERR_ARG, "int4_attention: null pointer");
+    if (dtype != CE_F32 && dtype != CE_BF16) return ce_fail(CE_ERR_ARG, "int4_attention: unknown dtype %d", dtype);
+    if (nkv < 1 || nh < 1 || nh % nkv) return ce_fail(CE_ERR_SIZE, "int4_attention: %d heads over %d kv heads", nh, nkv);
+    if (d < 64 || d > 256 || d % 64) return ce_fail(CE_ERR_SIZE, "int4_attention: head size %d (64, 128, 192 or 256)", d);
+    if (group != 32 && group != 64) return ce_fail(CE_ERR_SIZE, "int4_attention: group %d (32 or 64)", group);
+    if (page_size < 16 || page_size % 16) return ce_fail(CE_ERR_SIZE, "int4_attention: page size %d is not a multiple of 16", page_size);
+    if (((uintptr_t)pages & 15) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: the pages do not start on a 16-byte boundary");
+    if (max_pages < 1 || num_pages < 1 || splits < 1 || window < 0) return ce_fail(CE_ERR_SIZE, "int4_attention: bad sizes");
+    if (splits > 1 && (!part_o || !part_ml)) return ce_fail(CE_ERR_ARG, "int4_attention: shares of the keys need scratch memory");
+    if (count == 0) return CE_OK;
+    const int each = nh / nkv, rows = block_rows(each, d, tiles ? 64 : 1), subs = ((tiles ? 64 : 1) * each + rows - 1) / rows;
+    const long long jobs = (long long)count * nkv * subs;
+    if (count < 0 || jobs * splits * 16 > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_attention: too many rows");
+    const int el = dtype == CE_F32 ? 4 : 2;
+    Args a{q, out, (const unsigned char*)pages, seq_slot, q_start, ctx_len, block_table, tiles, status, part_o, part_ml, q_stride,
+           nh, nkv, page_size, max_pages, num_pages, window, splits, subs, ((uintptr_t)q % (4 * el)) == 0 && q_stride % 4 == 0, scale};
+    return dtype == CE_F32 ? run_type<float>(a, d, group, (int)jobs, rows, (cudaStream_t)stream)
+                           : run_type<__nv_bfloat16>(a, d, group, (int)jobs, rows, (cudaStream_t)stream);
+}

@@ -1,0 +1,267 @@
+// Quantisation into 4 bits and back: keys and values as they enter the pages of a cache, weights once when they are loaded (format and layout:
+// int4.cuh).
+//
+// One half of a warp takes 64 neighbouring channels, 4 a lane: a group's extremes are found with shuffles, two lanes put the 8 codes of a word
+// together.  Bound by memory for whole prompts and by the launch for single tokens.
+#include "int4.cuh"
+
+namespace {
+
+struct CacheArgs {
+    const void *k, *v;             // rows as given: [T, nkv, d], strides below (kv_read writes them)
+    unsigned char* pages;          // [num_pages, nkv, page_size / 16, tile]
+    const int *positions, *seq_of_token, *seq_slot, *block_table;
+    int* status;
+    long long k_token, k_head, v_token, v_head;      // strides in elements
+    int T, nkv, d, group, page_size, max_pages, num_pages, vec;
+};
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool vec, float (&x)[4]) {
+    if (vec) {
+        const float4 v = ce_load4(p);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = CeType<T>::load(p + i);
+    }
+}
+__device__ __forceinline__ void store4(float* p, bool vec, const float (&x)[4]) {
+    if (vec) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = x[i];
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, bool vec, const float (&x)[4]) {
+    __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+    if (vec) *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+    else { p[0] = a.x; p[1] = a.y; p[2] = b.x; p[3] = b.y; }
+}
+
+// (s, z) of this lane's group and its four codes as 16 bits; ``lanes``: lanes of a group (8, 16 or 32)
+__device__ __forceinline__ unsigned quantise4(const float (&x)[4], int lanes, __half2& sz) {
+    float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ok = ok && fabsf(x[i]) <= I4_LIMIT;
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        ok = __shfl_xor_sync(0xffffffffu, (int)ok, o) && ok;
+    }
+    sz = i4_step(lo, hi, ok);
+    const float s = __low2float(sz), z = __high2float(sz), inv = ok ? i4_inverse(s) : 0.0f;
+    unsigned q = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q |= (inv > 0.0f ? i4_code(x[i], s, z, inv) : 0u) << (4 * i);
+    return q;
+}
+
+// The tile of a token's position; null (and a status) where its request holds no such page.
+__device__ __forceinline__ unsigned char* tile_of(const CacheArgs& a, int t, int h, int& slot_in_tile, int code) {
+    const int pos = a.positions[t], pi = pos >= 0 ? pos / a.page_size : -1;
+    const int page = pi >= 0 && pi < a.max_pages ? a.block_table[(size_t)a.seq_slot[a.seq_of_token[t]] * a.max_pages + pi] : -1;
+    if (page < 0 || page >= a.num_pages) { atomicExch(a.status, code); return nullptr; }
+    const int in = pos - pi * a.page_size;
+    slot_in_tile = in & 15;
+    return a.pages + (((size_t)page * a.nkv + h) * (a.page_size >> 4) + (in >> 4)) * (size_t)i4_cache_tile_bytes(a.d, a.group);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) int4_kv_write_kernel(CacheArgs a) {
+    ce_pdl_begin();
+    const int blocks = a.d >> 6, groups = a.d / a.group, lane = threadIdx.x & 15;
+    const long long units = (long long)a.T * a.nkv * 2 * blocks;
+    const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const bool live = u < units;
+    long long rest = live ? u : units - 1;
+    const int b = (int)(rest % blocks); rest /= blocks;
+    const bool is_v = rest & 1; rest >>= 1;
+    const int h = (int)(rest % a.nkv), t = (int)(rest / a.nkv);
+    const T* src = is_v ? (const T*)a.v + t * a.v_token + h * a.v_head : (const T*)a.k + t * a.k_token + h * a.k_head;
+    float x[4];
+    load4(src + 64 * b + 4 * lane, a.vec, x);
+    __half2 sz;
+    const unsigned q = quantise4(x, a.group >> 2, sz);
+    const unsigned near = __shfl_xor_sync(0xffffffffu, q, 1), far = __shfl_xor_sync(0xffffffffu, q, 8);
+    int at = 0;
+    unsigned char* tile = live ? tile_of(a, t, h, at, 2) : nullptr;
+    if (!tile) return;
+    const int g = (64 * b + 4 * lane) / a.group;
+    const bool first = (4 * lane) % a.group == 0;
+    if (!is_v) {
+        if (!(lane & 1)) *reinterpret_cast<uint32_t*>(tile + i4_k_word(at, 64 * b + 4 * lane)) = q | near << 16;
+        if (first) *reinterpret_cast<__half2*>(tile + i4_k_step(a.d, groups, at, g)) = sz;
+    } else {
+        if (lane < 8) *reinterpret_cast<uint32_t*>(tile + i4_v_word(a.d, at, b, lane)) = q | far << 16;
+        if (first) *reinterpret_cast<__half2*>(tile + i4_v_step(a.d, groups, at, g)) = sz;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) int4_kv_read_kernel(CacheArgs a) {
+    ce_pdl_begin();
+    const int blocks = a.d >> 6, groups = a.d / a.group, lane = threadIdx.x & 15;
+    const long long units = (long long)a.T * a.nkv * 2 * blocks;
+    const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (u >= units) return;
+    long long rest = u;
+    const int b = (int)(rest % blocks); rest /= blocks;
+    const bool is_v = rest & 1; rest >>= 1;
+    const int h = (int)(rest % a.nkv), t = (int)(rest / a.nkv);
+    int at = 0;
+    const unsigned char* tile = tile_of(a, t, h, at, 4);
+    if (!tile) return;
+    const int g = (64 * b + 4 * lane) / a.group;
+    uint32_t w;
+    __half2 sz;
+    if (!is_v) {
+        w = *reinterpret_cast<const uint32_t*>(tile + i4_k_word(at, 64 * b + 4 * lane)) >> (lane & 1 ? 16 : 0);
+        sz = *reinterpret_cast<const __half2*>(tile + i4_k_step(a.d, groups, at, g));
+    } else {
+        w = *reinterpret_cast<const uint32_t*>(tile + i4_v_word(a.d, at, b, lane & 7)) >> (lane & 8 ? 16 : 0);
+        sz = *reinterpret_cast<const __half2*>(tile + i4_v_step(a.d, groups, at, g));
+    }
+    const float s = __low2float(sz), z = __high2float(sz);
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), s, z);
+    T* dst = is_v ? (T*)a.v + t * a.v_token + h * a.v_head : (T*)a.k + t * a.k_token + h * a.k_head;
+    store4(dst + 64 * b + 4 * lane, a.vec, x);
+}
+
+struct WeightArgs {
+    const void* w;                 // [rows, width], row stride ld (quantise reads it, dequantise writes it)
+    unsigned char* tiles;          // [row tiles, ceil(width / 64), tile]
+    long long ld;
+    int rows, part, padded, width, kblocks, group, vec;      // part: rows of a half that is padded to a multiple of 16 by itself
+};
+
+// a warp takes 128 neighbouring columns of one (padded) row: rows of padding, and columns beyond the width, hold zeros
+template <typename T>
+__global__ void __launch_bounds__(256) int4_quantise_weight_kernel(WeightArgs a) {
+    ce_pdl_begin();
+    const int lane = threadIdx.x & 31, pairs = (a.kblocks + 1) >> 1, kept = min(a.group, 64);
+    const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int row = (int)(u / pairs), col = (int)(u - (long long)row * pairs) * 128 + 4 * lane;
+    const int padded_rows = a.padded * (a.rows / a.part);
+    if (row >= padded_rows) return;
+    const int half = row / a.padded, in_half = row - half * a.padded;
+    const bool real = in_half < a.part && col < a.width;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (real) load4((const T*)a.w + (half * (long long)a.part + in_half) * a.ld + col, a.vec, x);
+    __half2 sz;
+    const unsigned q = quantise4(x, a.group >> 2, sz);
+    const unsigned near = __shfl_xor_sync(0xffffffffu, q, 1);
+    const int kb = col >> 6;
+    if (kb >= a.kblocks) return;
+    unsigned char* tile = a.tiles + ((size_t)(row >> 4) * a.kblocks + kb) * i4_weight_tile_bytes(kept);
+    if (!(lane & 1)) *reinterpret_cast<uint32_t*>(tile + i4_k_word(row & 15, col & 63)) = q | near << 16;
+    if ((4 * lane) % kept == 0) *reinterpret_cast<__half2*>(tile + 512 + ((row & 15) * (64 / kept) + (col & 63) / kept) * 4) = sz;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) int4_dequantise_weight_kernel(WeightArgs a) {
+    ce_pdl_begin();
+    const int lane = threadIdx.x & 15, kept = min(a.group, 64);
+    const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int r = (int)(u / a.kblocks), kb = (int)(u - (long long)r * a.kblocks), col = kb * 64 + 4 * lane;
+    if (r >= a.rows || col >= a.width) return;
+    const int half = r / a.part, row = half * a.padded + (r - half * a.part);
+    const unsigned char* tile = a.tiles + ((size_t)(row >> 4) * a.kblocks + kb) * i4_weight_tile_bytes(kept);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + i4_k_word(row & 15, col & 63)) >> (lane & 1 ? 16 : 0);
+    const __half2 sz = *reinterpret_cast<const __half2*>(tile + 512 + ((row & 15) * (64 / kept) + (col & 63) / kept) * 4);
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), __low2float(sz), __high2float(sz));
+    store4((T*)a.w + r * a.ld + col, a.vec, x);
+}
+
+int check_cache(const CacheArgs& a, int dtype, const char* who) {
+    if (!a.k || !a.v || !a.pages || !a.positions || !a.seq_of_token || !a.seq_slot || !a.block_table || !a.status)
+        return ce_fail(CE_ERR_ARG, "%s: null pointer", who);
+    if (dtype != CE_F32 && dtype != CE_BF16) return ce_fail(CE_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if (a.T < 0 || a.nkv < 1 || a.num_pages < 1 || a.max_pages < 1) return ce_fail(CE_ERR_SIZE, "%s: bad sizes", who);
+    if (a.d < 64 || a.d > 256 || a.d % 64) return ce_fail(CE_ERR_SIZE, "%s: head size %d (64, 128, 192 or 256)", who, a.d);
+    if (a.group != 32 && a.group != 64) return ce_fail(CE_ERR_SIZE, "%s: group %d (32 or 64)", who, a.group);
+    if (a.page_size < 16 || a.page_size % 16) return ce_fail(CE_ERR_SIZE, "%s: page size %d is not a multiple of 16", who, a.page_size);
+    return CE_OK;
+}
+
+bool aligned4(const void* p, long long s0, long long s1, int dtype) {
+    return ((uintptr_t)p % (dtype == CE_F32 ? 16 : 8)) == 0 && s0 % 4 == 0 && s1 % 4 == 0;
+}
+
+template <typename F32, typename BF16>
+int run_cache(CacheArgs& a, int dtype, F32 f32, BF16 bf16, const char* name, cudaStream_t stream) {
+    if (a.T == 0) return CE_OK;
+    a.vec = aligned4(a.k, a.k_token, a.k_head, dtype) && aligned4(a.v, a.v_token, a.v_head, dtype);
+    const long long units = (long long)a.T * a.nkv * 2 * (a.d >> 6), grid = (units + 15) / 16;
+    if (grid > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "%s: too many rows", name);
+    ce_note(name);
+    const cudaError_t e = dtype == CE_F32 ? ce_launch(f32, dim3((unsigned)grid), dim3(256), 0, stream, a)
+                                          : ce_launch(bf16, dim3((unsigned)grid), dim3(256), 0, stream, a);
+    if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e)); }
+    return ce_check_launch(name);
+}
+
+int check_weight(const WeightArgs& a, int dtype, const char* who) {
+    if (!a.w || !a.tiles) return ce_fail(CE_ERR_ARG, "%s: null pointer", who);
+    if (dtype != CE_F32 && dtype != CE_BF16) return ce_fail(CE_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if (a.group != 32 && a.group != 64 && a.group != 128) return ce_fail(CE_ERR_SIZE, "%s: group %d (32, 64 or 128)", who, a.group);
+    if (a.rows < 1 || a.width < 1 || a.part < 1 || a.rows % a.part || a.width % a.group || a.ld < a.width)
+        return ce_fail(CE_ERR_SIZE, "%s: %d rows of %d do not fit (the width is a multiple of the group)", who, a.rows, a.width);
+    return CE_OK;
+}
+
+}  // namespace
+
+extern "C" int ce_int4_cache_tile_bytes(int d, int group) { return i4_cache_tile_bytes(d, group); }
+extern "C" int ce_int4_weight_tile_bytes(int group) { return i4_weight_tile_bytes(group < 64 ? group : 64); }
+
+// dtype, k, v, their strides (token, head), pages, positions, seq_of_token, seq_slot, block_table, status, T, nkv, d, group, page_size,
+// max_pages, num_pages, stream
+extern "C" int ce_int4_kv_write(int dtype, const void* k, const void* v, long long k_token, long long k_head, long long v_token, long long v_head,
+                                void* pages, const int* positions, const int* seq_of_token, const int* seq_slot, const int* block_table,
+                                int* status, int T, int nkv, int d, int group, int page_size, int max_pages, int num_pages, void* stream) {
+    CacheArgs a{k, v, (unsigned char*)pages, positions, seq_of_token, seq_slot, block_table, status, k_token, k_head, v_token, v_head,
+                T, nkv, d, group, page_size, max_pages, num_pages, 0};
+    if (int e = check_cache(a, dtype, "int4_kv_write")) return e;
+    return run_cache(a, dtype, int4_kv_write_kernel<float>, int4_kv_write_kernel<__nv_bfloat16>, "int4_kv_write_kernel", (cudaStream_t)stream);
+}
+
+extern "C" int ce_int4_kv_read(int dtype, void* k, void* v, long long k_token, long long k_head, long long v_token, long long v_head,
+                               void* pages, const int* positions, const int* seq_of_token, const int* seq_slot, const int* block_table,
+                               int* status, int T, int nkv, int d, int group, int page_size, int max_pages, int num_pages, void* stream) {
+    CacheArgs a{k, v, (unsigned char*)pages, positions, seq_of_token, seq_slot, block_table, status, k_token, k_head, v_token, v_head,
+                T, nkv, d, group, page_size, max_pages, num_pages, 0};
+    if (int e = check_cache(a, dtype, "int4_kv_read")) return e;
+    return run_cache(a, dtype, int4_kv_read_kernel<float>, int4_kv_read_kernel<__nv_bfloat16>, "int4_kv_read_kernel", (cudaStream_t)stream);
+}
+
+// dtype, w, ld, tiles, rows, part, width, group, stream.  rows: a multiple of part; each part is padded to a multiple of 16 rows by itself.
+extern "C" int ce_int4_quantise_weight(int dtype, const void* w, long long ld, void* tiles, int rows, int part, int width, int group, void* stream) {
+    WeightArgs a{w, (unsigned char*)tiles, ld, rows, part, (part + 15) / 16 * 16, width, (width + 63) / 64, group, 0};
+    if (int e = check_weight(a, dtype, "int4_quantise_weight")) return e;
+    a.vec = aligned4(w, ld, 0, dtype);
+    const long long warps = (long long)a.padded * (rows / part) * ((a.kblocks + 1) / 2), grid = (warps + 7) / 8;
+    if (grid > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_quantise_weight: too large");
+    ce_note("int4_quantise_weight_kernel");
+    const cudaError_t e = dtype == CE_F32 ? ce_launch(int4_quantise_weight_kernel<float>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a)
+                                          : ce_launch(int4_quantise_weight_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a);
+    if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_quantise_weight: %s", cudaGetErrorString(e)); }
+    return ce_check_launch("int4_quantise_weight");
+}
+
+extern "C" int ce_int4_dequantise_weight(int dtype, void* w, long long ld, const void* tiles, int rows, int part, int width, int group, void* stream) {
+    WeightArgs a{w, (unsigned char*)tiles, ld, rows, part, (part + 15) / 16 * 16, width, (width + 63) / 64, group, 0};
+    if (int e = check_weight(a, dtype, "int4_dequantise_weight")) return e;
+    a.vec = aligned4(w, ld, 0, dtype);
+    const long long units = (long long)rows * a.kblocks, grid = (units + 15) / 16;
+    if (grid > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_dequantise_weight: too large");
+    ce_note("int4_dequantise_weight_kernel");
+    const cudaError_t e = dtype == CE_F32 ? ce_launch(int4_dequantise_weight_kernel<float>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a)
+                                          : ce_launch(int4_dequantise_weight_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a);
+    if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_dequantise_weight: %s", cudaGetErrorString(e)); }
+    return ce_check_launch("int4_dequantise_weight");
+}
