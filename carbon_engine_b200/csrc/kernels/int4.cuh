@@ -67,6 +67,33 @@ __device__ __forceinline__ void i4_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Four of a word's codes as operands (SHIFT 0 or 8): the even pair and the odd one, which is 16 times too large.  Plain: the bits of the codes,
+// float16 numbers of 2^-24.  CENTRED: codes less 8 as ordinary float16 numbers, which the float32 path takes for two instructions a word more:
+// tensor cores cut what they add to a sum, all the earlier where the operands are float16 numbers below 2^-14, and sums of codes that are all
+// positive lose, next to a result that their minimum's part nearly cancels, more of the bits that float32 is asked for.  (Attention of 4 x 700
+// keys, float32, off by 2.6e-5 of the result with the plain codes, 5.9e-6 with codes less 8 below 2^-14.)
+template <bool CENTRED> constexpr float i4_unit = CENTRED ? 1.0f : 0x1p24f;       // what a sum of products with the codes is multiplied by
+template <bool CENTRED, int SHIFT>
+__device__ __forceinline__ void i4_pairs(uint32_t w, uint32_t& even, uint32_t& odd) {
+    even = (w >> SHIFT) & 0x000f000fu;
+    odd = (w >> SHIFT) & 0x00f000f0u;
+    if (CENTRED) {
+        even |= 0x64006400u;                          // 1024 + c
+        odd |= 0x64006400u;                           // 1024 + 16 c
+        const uint32_t e8 = 0x64086408u, o8 = 0x64806480u;        // 1024 + 8, 1024 + 16 * 8
+        __half2 e = __hsub2(*reinterpret_cast<__half2*>(&even), *reinterpret_cast<const __half2*>(&e8));
+        __half2 o = __hsub2(*reinterpret_cast<__half2*>(&odd), *reinterpret_cast<const __half2*>(&o8));
+        even = *reinterpret_cast<uint32_t*>(&e);
+        odd = *reinterpret_cast<uint32_t*>(&o);
+    }
+}
+// (s, z) as float32; CENTRED: z is the value of code 8
+template <bool CENTRED>
+__device__ __forceinline__ float2 i4_step_of(uint32_t v) {
+    float2 f = __half22float2(*reinterpret_cast<__half2*>(&v));
+    if (CENTRED) f.y = fmaf(8.0f, f.x, f.y);
+    return f;
+}
 __device__ __forceinline__ uint32_t i4_pack(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);

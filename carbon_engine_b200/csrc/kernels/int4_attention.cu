@@ -100,6 +100,7 @@ __device__ __forceinline__ void load_steps(const unsigned char* p, uint32_t (&v)
 
 template <typename T, int D, int G, int NT>
 __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
+    constexpr bool C8 = Pieces<T>::N == 2;            // codes less 8: see i4_pairs
     constexpr int NB = D / 64, NG = D / G, P = Pieces<T>::N, ROWS = 8 * NT, TILE = i4_cache_tile_bytes(D, G), CH = D / 32;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[WARPS][STAGES];
@@ -206,12 +207,12 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
             sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
             sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) qsum[nt][g][e] = __shfl_sync(0xffffffffu, sums[g], 4 * (2 * l + e)) * 0x1p-24f;
+            for (int e = 0; e < 2; ++e) qsum[nt][g][e] = __shfl_sync(0xffffffffu, sums[g], 4 * (2 * l + e)) * (1.0f / i4_unit<C8>);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const float u = __shfl_sync(0xffffffffu, up, 4 * (2 * l + e));
-            row_scale[nt][e] = a.scale * LOG2E * 0x1p24f / u;
+            row_scale[nt][e] = a.scale * LOG2E * i4_unit<C8> / u;
             const int rr = nt * 8 + 2 * l + e, pos = j.base + (j.row0 + rr) / each;
             hi[nt][e] = rr < rows ? pos : -1;
             lo[nt][e] = a.window > 0 ? pos - a.window + 1 : 0;
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
         float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-        float acc[NT][4];
+        float acc[NT][P][4];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const uint4 w = *reinterpret_cast<const uint4*>(tile + b * 512 + lane * 16);
@@ -257,25 +258,30 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
                 const uint32_t wa = half ? w.z : w.x, wb = half ? w.w : w.y;
                 if ((c * 32) % G == 0)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) acc[nt][p][0] = acc[nt][p][1] = acc[nt][p][2] = acc[nt][p][3] = 0.f;
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
-                    const uint32_t ua = st ? wa >> 8 : wa, ub = st ? wb >> 8 : wb;
-                    const uint32_t a0 = ua & 0x000f000fu, a1 = ub & 0x000f000fu, a2 = ua & 0x00f000f0u, a3 = ub & 0x00f000f0u;
+                    uint32_t a0, a1, a2, a3;
+                    if (st) { i4_pairs<C8, 8>(wa, a0, a2); i4_pairs<C8, 8>(wb, a1, a3); }
+                    else { i4_pairs<C8, 0>(wa, a0, a2); i4_pairs<C8, 0>(wb, a1, a3); }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int p = 0; p < P; ++p) i4_mma(acc[nt], a0, a1, a2, a3, qf[nt][p][c][2 * st], qf[nt][p][c][2 * st + 1]);
+                        for (int p = 0; p < P; ++p) i4_mma(acc[nt][p], a0, a1, a2, a3, qf[nt][p][c][2 * st], qf[nt][p][c][2 * st + 1]);
                 }
                 if ((c * 32 + 32) % G == 0) {
                     const int g = c * 32 / G;
-                    const float2 fa = i4_unpack(ka[g]), fb = i4_unpack(kb[g]);
+                    const float2 fa = i4_step_of<C8>(ka[g]), fb = i4_step_of<C8>(kb[g]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            s[nt][e] = fmaf(fa.x, acc[nt][e], fmaf(fa.y, qsum[nt][g][e], s[nt][e]));
-                            s[nt][2 + e] = fmaf(fb.x, acc[nt][2 + e], fmaf(fb.y, qsum[nt][g][e], s[nt][2 + e]));
+                            float sa = acc[nt][0][e], sb = acc[nt][0][2 + e];
+                            if constexpr (P == 2) { sa += acc[nt][1][e]; sb += acc[nt][1][2 + e]; }
+                            s[nt][e] = fmaf(fa.x, sa, fmaf(fa.y, qsum[nt][g][e], s[nt][e]));
+                            s[nt][2 + e] = fmaf(fb.x, sb, fmaf(fb.y, qsum[nt][g][e], s[nt][2 + e]));
                         }
                 }
             }
@@ -366,7 +372,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
             for (int half = 0; half < 2; ++half) {
                 const int g = (64 * b + 32 * half) / G;
                 if ((32 * half) % G == 0) {
-                    const float2 fa = i4_unpack(va[g]), fb = i4_unpack(vb[g]);
+                    const float2 fa = i4_step_of<C8>(va[g]), fb = i4_step_of<C8>(vb[g]);
                     const float sa = fa.x * norm, sb = fb.x * norm;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -390,8 +396,9 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
                 const uint32_t u = __byte_perm(w.x, w.y, pick), v = __byte_perm(w.z, w.w, pick);
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
-                    const uint32_t us = st ? u >> 8 : u, vs = st ? v >> 8 : v;
-                    const uint32_t a0 = us & 0x000f000fu, a1 = us & 0x00f000f0u, a2 = vs & 0x000f000fu, a3 = vs & 0x00f000f0u;
+                    uint32_t a0, a1, a2, a3;
+                    if (st) { i4_pairs<C8, 8>(u, a0, a1); i4_pairs<C8, 8>(v, a2, a3); }
+                    else { i4_pairs<C8, 0>(u, a0, a1); i4_pairs<C8, 0>(v, a2, a3); }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -419,7 +426,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) t += __shfl_xor_sync(0xffffffffu, t, w);
             if (r == 0) { s_m[warp][row] = m[nt][e]; s_l[warp][row] = t; }
-            const float even = top * 0x1p14f, odd = top * 0x1p10f;
+            const float even = top * (i4_unit<C8> / 1024.0f), odd = even * 0.0625f;
             float zs[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(PrepareArgs a) {
             }
     largest = ce_block_max(finite ? largest : INFINITY, scratch);
     const float up = i4_row_scale(largest);
-    if (threadIdx.x == 0) a.to.back[t] = 0x1p24f / up;
+    if (threadIdx.x == 0) a.to.back[t] = i4_unit<P == 2> / up;
     // a thread takes 8 neighbouring columns: the four words of lane (r, l) for a half of a block; four threads hold a run of 32
     const int groups = 64 / a.group;
     for (int c = threadIdx.x * 8; c < a.kblocks * 64; c += 256 * 8) {
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(PrepareArgs a) {
         sum += __shfl_xor_sync(here, sum, 1);
         sum += __shfl_xor_sync(here, sum, 2);
         if (a.group == 64) sum += __shfl_xor_sync(here, sum, 4);
-        if (c % a.group == 0) a.to.sums[(size_t)(kb * groups + (c & 63) / a.group) * (tiles * 8) + t] = sum * 0x1p-24f;
+        if (c % a.group == 0) a.to.sums[(size_t)(kb * groups + (c & 63) / a.group) * (tiles * 8) + t] = sum * (1.0f / i4_unit<P == 2>);
     }
 }
 
@@ -113,35 +113,46 @@ __global__ void __launch_bounds__(WARPS * 32) int4_gemm_kernel(GemmArgs a) {
         for (int kb = warp; kb < a.kblocks; kb += WARPS) {
             const unsigned char* tile = rows + (size_t)kb * TILE;
             const uint4 w = *reinterpret_cast<const uint4*>(tile + lane * 16);
-            float acc[NT][4];
+            float acc[NT][P][4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const uint32_t wa = half ? w.z : w.x, wb = half ? w.w : w.y;
                 if ((half * 32) % G == 0)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) acc[nt][p][0] = acc[nt][p][1] = acc[nt][p][2] = acc[nt][p][3] = 0.f;
+                uint32_t e0, e1, e2, e3, o0, o1, o2, o3;
+                i4_pairs<P == 2, 0>(wa, e0, e2); i4_pairs<P == 2, 0>(wb, e1, e3);
+                i4_pairs<P == 2, 8>(wa, o0, o2); i4_pairs<P == 2, 8>(wb, o1, o3);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
                         if (nt < a.tiles) {
                             const uint4 x = *reinterpret_cast<const uint4*>(a.x.frag + ((((size_t)kb * a.tiles + nt) * P + p) * 2 + half) * 128 + lane * 4);
-                            i4_mma(acc[nt], wa & 0x000f000fu, wb & 0x000f000fu, wa & 0x00f000f0u, wb & 0x00f000f0u, x.x, x.y);
-                            i4_mma(acc[nt], wa >> 8 & 0x000f000fu, wb >> 8 & 0x000f000fu, wa >> 8 & 0x00f000f0u, wb >> 8 & 0x00f000f0u, x.z, x.w);
+                            i4_mma(acc[nt][p], e0, e1, e2, e3, x.x, x.y);
+                            i4_mma(acc[nt][p], o0, o1, o2, o3, x.z, x.w);
                         }
                     }
                 if ((half * 32 + 32) % G == 0) {
                     const int g = half * 32 / G;
-                    const float2 fa = i4_unpack(*reinterpret_cast<const uint32_t*>(tile + 512 + (r * GB + g) * 4));
-                    const float2 fb = i4_unpack(*reinterpret_cast<const uint32_t*>(tile + 512 + ((r + 8) * GB + g) * 4));
+                    const float2 fa = i4_step_of<P == 2>(*reinterpret_cast<const uint32_t*>(tile + 512 + (r * GB + g) * 4));
+                    const float2 fb = i4_step_of<P == 2>(*reinterpret_cast<const uint32_t*>(tile + 512 + ((r + 8) * GB + g) * 4));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         if (nt >= a.tiles) continue;
                         const float2 s = *reinterpret_cast<const float2*>(a.x.sums + (size_t)(kb * GB + g) * tokens + nt * 8 + 2 * l);
-                        y[nt][0] = fmaf(fa.x, acc[nt][0], fmaf(fa.y, s.x, y[nt][0]));
-                        y[nt][1] = fmaf(fa.x, acc[nt][1], fmaf(fa.y, s.y, y[nt][1]));
-                        y[nt][2] = fmaf(fb.x, acc[nt][2], fmaf(fb.y, s.x, y[nt][2]));
-                        y[nt][3] = fmaf(fb.x, acc[nt][3], fmaf(fb.y, s.y, y[nt][3]));
+                        float c[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            c[e] = acc[nt][0][e];
+                            if constexpr (P == 2) c[e] += acc[nt][1][e];
+                        }
+                        y[nt][0] = fmaf(fa.x, c[0], fmaf(fa.y, s.x, y[nt][0]));
+                        y[nt][1] = fmaf(fa.x, c[1], fmaf(fa.y, s.y, y[nt][1]));
+                        y[nt][2] = fmaf(fb.x, c[2], fmaf(fb.y, s.x, y[nt][2]));
+                        y[nt][3] = fmaf(fb.x, c[3], fmaf(fb.y, s.y, y[nt][3]));
                     }
                 }
             }
