@@ -552,12 +552,33 @@ extern "C" int ce_int4_attention_blocks(int each, int d, int tile) {
     return ((tile ? 64 : 1) * each + rows - 1) / rows;
 }
 
-// dtype, q, q_stride, pages, out, seq_slot, q_start, ctx_len, block_table, tiles (or null: ``count`` one-token sequences), status, part_o,
-// part_ml, count, nh, nkv, d, group, page_size, max_pages, num_pages, window, splits, scale, stream
-extern "C" int ce_int4_attention(int dtype, const void* q, long long q_stride, const void* pages, void* out, const int* seq_slot, const int* q_start,
-                                 const int* ctx_len, const int* block_table, const int* tiles, int* status, float* part_o, float* part_ml, int count,
-                                 int nh, int nkv, int d, int group, int page_size, int max_pages, int num_pages, int window, int splits, float scale,
-                                 void* stream) {
+// A call's arguments, 8 bytes each in this order
+struct Int4AttentionCall {
+    long long dtype;
+    const void* q;
+    long long q_stride;
+    const void* pages;
+    void* out;
+    const int *seq_slot, *q_start, *ctx_len, *block_table;
+    int* status;
+    const int* tiles;              // null: ``n`` one-token sequences
+    long long n, nh, nkv, d, group, page_size, max_pages, num_pages, window, splits;
+    float *part_o, *part_ml;
+    double scale;
+    void* stream;
+};
+
+extern "C" int ce_int4_attention(const Int4AttentionCall* c) {
+    const void *q = c->q, *pages = c->pages;
+    void* out = c->out;
+    const int *seq_slot = c->seq_slot, *q_start = c->q_start, *ctx_len = c->ctx_len, *block_table = c->block_table, *tiles = c->tiles;
+    int* status = c->status;
+    float *part_o = c->part_o, *part_ml = c->part_ml;
+    const long long q_stride = c->q_stride, count = c->n;
+    const int dtype = (int)c->dtype, nh = (int)c->nh, nkv = (int)c->nkv, d = (int)c->d, group = (int)c->group, page_size = (int)c->page_size,
+              max_pages = (int)c->max_pages, num_pages = (int)c->num_pages, window = (int)c->window, splits = (int)c->splits;
+    const float scale = (float)c->scale;
+    void* stream = c->stream;
     if (!q || !pages || !out || !seq_slot || !q_start || !ctx_len || !block_table || !status) return ce_fail(CE_ERR_ARG, "int4_attention: null pointer");
     if (dtype != CE_F32 && dtype != CE_BF16) return ce_fail(CE_ERR_ARG, "int4_attention: unknown dtype %d", dtype);
     if (nkv < 1 || nh < 1 || nh % nkv) return ce_fail(CE_ERR_SIZE, "int4_attention: %d heads over %d kv heads", nh, nkv);
@@ -569,7 +590,7 @@ extern "C" int ce_int4_attention(int dtype, const void* q, long long q_stride, c
     if (splits > 1 && (!part_o || !part_ml)) return ce_fail(CE_ERR_ARG, "int4_attention: shares of the keys need scratch memory");
     if (count == 0) return CE_OK;
     const int each = nh / nkv, rows = block_rows(each, d, tiles ? 64 : 1), subs = ((tiles ? 64 : 1) * each + rows - 1) / rows;
-    const long long jobs = (long long)count * nkv * subs;
+    const long long jobs = count * nkv * subs;
     if (count < 0 || jobs * splits * 16 > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_attention: too many rows");
     const int el = dtype == CE_F32 ? 4 : 2;
     Args a{q, out, (const unsigned char*)pages, seq_slot, q_start, ctx_len, block_table, tiles, status, part_o, part_ml, q_stride,

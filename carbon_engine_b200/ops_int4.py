@@ -11,35 +11,39 @@ tensors' device, which has to be the current one; scratch memory comes from torc
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
 
-from . import ops
+from . import ops, ops_tensor
 from .csrc import kernel_lib
 from .csrc.kernel_lib import KernelError, kernels
 
-_i, _f, _ll, _p = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_void_p
+_i, _ll, _p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
 kernel_lib.declare("ce_int4_cache_tile_bytes", _i, [_i, _i])
 kernel_lib.declare("ce_int4_weight_tile_bytes", _i, [_i])
+# These take one pointer to their arguments, 8 bytes each (ctypes takes 0.2 us for every argument of its own):
 # dtype, k, v, strides of k and v (token, head), pages, positions, seq_of_token, seq_slot, block_table, status,
 # T, nkv, d, group, page_size, max_pages, num_pages, stream
-_kv = [_i, _p, _p] + [_ll] * 4 + [_p] * 6 + [_i] * 7 + [_p]
-kernel_lib.declare("ce_int4_kv_write", _i, _kv)
-kernel_lib.declare("ce_int4_kv_read", _i, _kv)
+kernel_lib.declare("ce_int4_kv_write", _i, [ctypes.c_char_p])
+kernel_lib.declare("ce_int4_kv_read", _i, [ctypes.c_char_p])
+_KV = struct.Struct("=21q").pack
+# dtype, q, q_stride, pages, out, seq_slot, q_start, ctx_len, block_table, status, tiles, count, nh, nkv, d, group, page_size, max_pages,
+# num_pages, window, splits, part_o, part_ml, scale, stream
+kernel_lib.declare("ce_int4_attention", _i, [ctypes.c_char_p])
+_ATTENTION = struct.Struct("=23qdq").pack
+# dtype, x, ldx, w, out, ldo, M, N, K, group, mode, scratch, status, stream
+kernel_lib.declare("ce_int4_gemm", _i, [ctypes.c_char_p])
+_GEMM = struct.Struct("=14q").pack
 # dtype, w, ld, tiles, rows, part, width, group, stream
 kernel_lib.declare("ce_int4_quantise_weight", _i, [_i, _p, _ll, _p, _i, _i, _i, _i, _p])
 kernel_lib.declare("ce_int4_dequantise_weight", _i, [_i, _p, _ll, _p, _i, _i, _i, _i, _p])
 # each, d, tile
 kernel_lib.declare("ce_int4_attention_rows", _i, [_i] * 3)
 kernel_lib.declare("ce_int4_attention_blocks", _i, [_i] * 3)
-# dtype, q, q_stride, pages, out, seq_slot, q_start, ctx_len, block_table, tiles, status, part_o, part_ml, count, nh, nkv, d, group,
-# page_size, max_pages, num_pages, window, splits, scale, stream
-kernel_lib.declare("ce_int4_attention", _i, [_i, _p, _ll] + [_p] * 10 + [_i] * 10 + [_f, _p])
 # dtype, M, K, group
 kernel_lib.declare("ce_int4_gemm_scratch", _ll, [_i] * 4)
-# dtype, x, ldx, w, out, ldo, M, N, K, group, mode, scratch, stream
-kernel_lib.declare("ce_int4_gemm", _i, [_i, _p, _ll, _p, _p] + [_i] * 6 + [_p, _p])
 
 HEAD_SIZES = (64, 128, 192, 256)
 CACHE_GROUPS = (32, 64)
@@ -50,12 +54,35 @@ MAX_TOKENS = 64
 TILE_TOKENS = 16
 
 
-def _same_device(first: torch.Tensor, *others) -> None:
-    if first.device.index != torch.cuda.current_device():
-        raise KernelError(f"the tensors are on {first.device}, but the current device is cuda:{torch.cuda.current_device()}")
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise KernelError(f"tensors on {first.device} and {t.device} in one call")
+_CODES = {torch.float32: ops.F32, torch.bfloat16: ops.BF16}
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _code(t: torch.Tensor, name: str) -> int:
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise KernelError(f"{name} is {t.dtype} (float32 or bfloat16)")
+    return code
+
+
+def _ints(device: int, **tensors) -> None:
+    """Contiguous int32 tensors on the given device.  (A call's checks are most of its time where the kernel is short: they ask for what is cheap
+    to answer, and for the words of an error only when there is one.)"""
+    for name, t in tensors.items():
+        if t.dtype is not torch.int32 or t.get_device() != device or not t.is_contiguous():
+            ops._need(t, name, torch.int32)
+            raise KernelError(f"{name} is on {t.device}, the call's other tensors on cuda:{device}")
+
+
+def _current(t: torch.Tensor, name: str) -> int:
+    """The device of the call's first tensor, which has to be the current one."""
+    device = t.get_device()
+    if device < 0:
+        raise KernelError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if device != _device():
+        raise KernelError(f"{name} is on cuda:{device}, but the current device is cuda:{_device()}")
+    return device
 
 
 def cache_problem(head_dim: int, group: int, page_size: int) -> Optional[str]:
@@ -97,37 +124,29 @@ class Int4Pages:
         return 0.5 + 4.0 / self.group
 
 
-def _rows(t: torch.Tensor, name: str, pages: Int4Pages, tokens: int, dtype=None) -> None:
-    if not t.is_cuda:
-        raise KernelError(f"{name} must be a CUDA tensor (there is no CPU path)")
-    if t.dim() != 3 or t.shape != (tokens, pages.kv_heads, pages.head_dim):
-        raise KernelError(f"{name} is {tuple(t.shape)}, not {(tokens, pages.kv_heads, pages.head_dim)}")
-    if t.numel() and t.stride(2) != 1:
-        raise KernelError(f"{name}: the channels of a head must lie together")
-    if dtype is not None and t.dtype != dtype:
-        raise KernelError(f"{name} must be {dtype}, got {t.dtype}")
-
-
 def _kv_call(fn, k, v, pages, positions, seq_of_token, seq_slot, block_table, status) -> None:
-    T = positions.numel()
-    _rows(k, "k", pages, T)
-    _rows(v, "v", pages, T, k.dtype)
-    for name, t in (("positions", positions), ("seq_of_token", seq_of_token), ("seq_slot", seq_slot), ("block_table", block_table),
-                    ("status", status)):
-        ops._need(t, name, torch.int32)
+    device = _current(k, "k")
+    code = _code(k, "k")
+    shape = (positions.numel(), pages.kv_heads, pages.head_dim)
+    T = shape[0]
+    if k.shape != shape or v.shape != shape or v.dtype is not k.dtype or v.get_device() != device or pages.data.get_device() != device:
+        raise KernelError(f"k is {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} on {v.device}: not both {shape} of one type where the pages "
+                          f"are ({pages.data.device})")
+    k_token, k_head, k_channel = k.stride()
+    v_token, v_head, v_channel = v.stride()
+    if T and (k_channel != 1 or v_channel != 1):
+        raise KernelError("the channels of a head of k and v must lie together")
+    _ints(device, positions=positions, seq_of_token=seq_of_token, seq_slot=seq_slot, block_table=block_table, status=status)
     if seq_of_token.numel() != T or block_table.dim() != 2:
         raise KernelError("one position and one sequence a token, and a table of [slots, pages]")
-    code = ops.dtype_code(k.dtype)
-    _same_device(k, v, pages.data, positions, seq_of_token, seq_slot, block_table, status)
     if T == 0:
         return
-    prof = ops.profiling()
-    if prof is not None:
+    if ops._profile is not None:
         n = 2 * T * pages.kv_heads * pages.head_dim
-        prof.note_work(int(n * (k.element_size() + pages.element_size())), 0)
-    ops._ok(fn(code, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), pages.data.data_ptr(),
-               positions.data_ptr(), seq_of_token.data_ptr(), seq_slot.data_ptr(), block_table.data_ptr(), status.data_ptr(), T,
-               pages.kv_heads, pages.head_dim, pages.group, pages.page_size, block_table.shape[1], pages.num_pages, ops._stream()))
+        ops._profile.note_work(int(n * (k.element_size() + pages.element_size())), 0)
+    ops._ok(fn(_KV(code, k.data_ptr(), v.data_ptr(), k_token, k_head, v_token, v_head, pages.data.data_ptr(), positions.data_ptr(),
+                   seq_of_token.data_ptr(), seq_slot.data_ptr(), block_table.data_ptr(), status.data_ptr(), T, pages.kv_heads, pages.head_dim,
+                   pages.group, pages.page_size, block_table.shape[1], pages.num_pages, _stream(device))))
 
 
 def kv_write(pages: Int4Pages, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, seq_of_token: torch.Tensor,
@@ -152,9 +171,8 @@ def _splits(jobs: int, max_ctx: int, window: int, tokens: int) -> int:
     return max(1, min(most, 64, (2 * 148 + jobs - 1) // jobs))
 
 
-def _attend(q, pages, out, seq_slot, q_start, ctx_len, block_table, status, tiles, count, max_ctx, window, scale) -> None:
+def _attend(device, code, q, q_stride, heads, pages, out, seq_slot, q_start, ctx_len, block_table, status, tiles, count, max_ctx, window, scale) -> None:
     k = kernels()
-    heads = q.shape[1]
     each = heads // pages.kv_heads
     tile = 0 if tiles is None else 1
     jobs = count * pages.kv_heads * k.ce_int4_attention_blocks(each, pages.head_dim, tile)
@@ -162,13 +180,13 @@ def _attend(q, pages, out, seq_slot, q_start, ctx_len, block_table, status, tile
     part_o = part_ml = None
     if splits > 1:
         rows = jobs * splits * k.ce_int4_attention_rows(each, pages.head_dim, tile)
-        part_o = torch.empty(rows * pages.head_dim, dtype=torch.float32, device=q.device)
-        part_ml = torch.empty(rows * 2, dtype=torch.float32, device=q.device)
-    ops._ok(k.ce_int4_attention(
-        ops.dtype_code(q.dtype), q.data_ptr(), q.stride(0), pages.data.data_ptr(), out.data_ptr(), seq_slot.data_ptr(), q_start.data_ptr(),
-        ctx_len.data_ptr(), block_table.data_ptr(), ops._ptr(tiles), status.data_ptr(), ops._ptr(part_o), ops._ptr(part_ml), count, heads,
-        pages.kv_heads, pages.head_dim, pages.group, pages.page_size, block_table.shape[1], pages.num_pages, window, splits, scale,
-        ops._stream()), 2 if splits > 1 else 1)
+        part_o = torch.empty(rows * (pages.head_dim + 2), dtype=torch.float32, device=q.device)
+        part_ml = part_o.data_ptr() + 4 * rows * pages.head_dim
+    ops._ok(k.ce_int4_attention(_ATTENTION(
+        code, q.data_ptr(), q_stride, pages.data.data_ptr(), out.data_ptr(), seq_slot.data_ptr(), q_start.data_ptr(), ctx_len.data_ptr(),
+        block_table.data_ptr(), status.data_ptr(), 0 if tiles is None else tiles.data_ptr(), count, heads, pages.kv_heads, pages.head_dim,
+        pages.group, pages.page_size, block_table.shape[1], pages.num_pages, window, splits, 0 if part_o is None else part_o.data_ptr(),
+        part_ml or 0, scale, _stream(device))), 2 if splits > 1 else 1)
 
 
 def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor,
@@ -181,30 +199,32 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
     token each; the others are listed in ``tiles`` (int32 [n_tiles, 2]: sequence, first of up to 64 of its tokens).  ``max_ctx``: at least the longest
     ``ctx_len`` (it only shapes the launch: a smaller number is slower, not wrong).  ``window`` > 0: a query sees that many keys, itself the last of them.  A row that sees no key becomes zeros; rows of ``out`` that
     belong to no sequence stay as they were.  ``status`` becomes 4 where a page is not held, 7 where a wait gave up."""
-    if q.dim() != 3 or not q.is_cuda:
-        raise KernelError("q must be [tokens, heads, head_dim] on the GPU")
+    device = _current(q, "q")
+    code = _code(q, "q")
+    if q.dim() != 3:
+        raise KernelError("q must be [tokens, heads, head_dim]")
     T, heads, d = q.shape
     if d != pages.head_dim or heads % pages.kv_heads or heads == 0:
         raise KernelError(f"{heads} heads of {d} do not fit a cache of {pages.kv_heads} heads of {pages.head_dim}")
-    if T and (q.stride(2) != 1 or (heads > 1 and q.stride(1) != d)):
+    q_token, q_head, q_channel = q.stride()
+    if T and (q_channel != 1 or (heads > 1 and q_head != d)):
         raise KernelError("the heads of a token of q must lie together")
-    ops._need(out, "out", q.dtype)
-    if out.shape != q.shape:
-        raise KernelError(f"out is {tuple(out.shape)}, not {tuple(q.shape)}")
-    for name, t in (("seq_slot", seq_slot), ("q_start", q_start), ("ctx_len", ctx_len), ("block_table", block_table), ("status", status)):
-        ops._need(t, name, torch.int32)
+    if out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != device or not out.is_contiguous():
+        raise KernelError(f"out is {tuple(out.shape)} {out.dtype} on {out.device}, not {tuple(q.shape)} {q.dtype}, contiguous, where q is")
+    if pages.data.get_device() != device:
+        raise KernelError(f"the pages are on {pages.data.device}, q on {q.device}")
+    _ints(device, seq_slot=seq_slot, q_start=q_start, ctx_len=ctx_len, block_table=block_table, status=status)
     if block_table.dim() != 2 or window < 0 or n_decode < 0 or max_ctx < 0:
         raise KernelError("attention: a table of [slots, pages], no negative numbers")
-    if n_decode > seq_slot.numel() or q_start.numel() < seq_slot.numel() + 1 or ctx_len.numel() < seq_slot.numel():
+    seqs = seq_slot.numel()
+    if n_decode > seqs or q_start.numel() <= seqs or ctx_len.numel() < seqs:
         raise KernelError("attention: one slot and one length a sequence, one start more")
     if tiles is not None:
-        ops._need(tiles, "tiles", torch.int32)
+        _ints(device, tiles=tiles)
         n_tiles = tiles.numel() // 2 if n_tiles is None else int(n_tiles)
         if n_tiles < 0 or 2 * n_tiles > tiles.numel():
             raise KernelError(f"{n_tiles} tiles in a list of {tiles.numel() // 2}")
-    ops.dtype_code(q.dtype)
-    _same_device(q, out, pages.data, seq_slot, q_start, ctx_len, block_table, status, tiles)
-    args = (q, pages, out, seq_slot, q_start, ctx_len, block_table, status)
+    args = (device, code, q, q_token, heads, pages, out, seq_slot, q_start, ctx_len, block_table, status)
     if T and n_decode:
         _attend(*args, None, n_decode, int(max_ctx), int(window), float(scale))
     if T and tiles is not None and n_tiles:
@@ -212,7 +232,8 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
 
 
 class Int4Weight:
-    """A weight [rows, width] in 4 bits, laid out for :func:`matmul`.  ``gated``: the first half of the rows are gate rows, the
+    """A weight [rows, width] in 4 bits, laid out for :func:`matmul`, which reads it ahead of the kernels in front: :meth:`quantize` is what writes
+    it (whoever writes ``data`` otherwise synchronises before the next product).  ``gated``: the first half of the rows are gate rows, the
     second half the up rows that belong to them (for the gated epilogues, and only for them)."""
 
     def __init__(self, rows: int, width: int, group: int = 64, gated: bool = False, device="cuda"):
@@ -222,39 +243,41 @@ class Int4Weight:
             raise KernelError(f"a 4-bit weight of {rows} rows of {width}: the width must be a multiple of the group ({group})"
                               + (", the rows of two" if gated else ""))
         self.rows, self.width, self.group, self.gated = int(rows), int(width), int(group), bool(gated)
+        #: columns of the result
+        self.part = self.rows // 2 if self.gated else self.rows
         kept = min(group, 64)
         tiles = (self.part + 15) // 16 * (2 if gated else 1)
-        self.data = torch.empty((tiles, (width + 63) // 64, 512 + 64 * (64 // kept)), dtype=torch.uint8, device=device)
-
-    @property
-    def part(self) -> int:
-        """Columns of the result."""
-        return self.rows // 2 if self.gated else self.rows
+        self.kblocks = (self.width + 63) // 64
+        self.data = torch.empty((tiles, self.kblocks, 512 + 64 * (64 // kept)), dtype=torch.uint8, device=device)
+        #: the word that kernels of products report to (``ops_tensor.gemm_status``)
+        self.status = ops_tensor.gemm_workspace(self.data.device).status
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, group: int = 64, gated: bool = False) -> "Int4Weight":
         """``weight`` [rows, width] bfloat16 or float32 on the GPU."""
-        if weight.dim() != 2 or not weight.is_cuda or weight.stride(1) != 1:
-            raise KernelError("a weight is [rows, width] on the GPU, the columns of a row together")
+        device = _current(weight, "weight")
+        if weight.dim() != 2 or weight.stride(1) != 1:
+            raise KernelError("a weight is [rows, width], the columns of a row together")
         self = cls(weight.shape[0], weight.shape[1], group, gated, weight.device)
-        _same_device(weight)
         ld = weight.stride(0) if self.rows > 1 else self.width
-        ops._ok(kernels().ce_int4_quantise_weight(ops.dtype_code(weight.dtype), weight.data_ptr(), ld, self.data.data_ptr(),
-                                                  self.rows, self.part, self.width, self.group, ops._stream()))
+        ops._ok(kernels().ce_int4_quantise_weight(_code(weight, "weight"), weight.data_ptr(), ld, self.data.data_ptr(),
+                                                  self.rows, self.part, self.width, self.group, _stream(device)), 2)
         return self
 
     def dequantize(self, out: torch.Tensor) -> torch.Tensor:
         """The values held, rounded once to the type of ``out`` [rows, width]."""
-        if out.shape != (self.rows, self.width) or not out.is_cuda or out.stride(1) != 1:
-            raise KernelError(f"out is {tuple(out.shape)}, not {(self.rows, self.width)} on the GPU")
-        _same_device(out, self.data)
+        device = _current(out, "out")
+        if out.shape != (self.rows, self.width) or out.stride(1) != 1 or self.data.get_device() != device:
+            raise KernelError(f"out is {tuple(out.shape)} on {out.device}, not {(self.rows, self.width)} where the weight is ({self.data.device})")
         ld = out.stride(0) if self.rows > 1 else self.width
-        ops._ok(kernels().ce_int4_dequantise_weight(ops.dtype_code(out.dtype), out.data_ptr(), ld, self.data.data_ptr(),
-                                                    self.rows, self.part, self.width, self.group, ops._stream()))
+        ops._ok(kernels().ce_int4_dequantise_weight(_code(out, "out"), out.data_ptr(), ld, self.data.data_ptr(),
+                                                    self.rows, self.part, self.width, self.group, _stream(device)))
         return out
 
 
 _MODES = (ops.GEMM_STORE, ops.GEMM_STORE_F32, ops.GEMM_ACCUM_F32, ops.GEMM_SWIGLU, ops.GEMM_RELUGLU, ops.GEMM_RELU2)
+_GATED_MODES = (ops.GEMM_SWIGLU, ops.GEMM_RELUGLU)
+_F32_MODES = (ops.GEMM_STORE_F32, ops.GEMM_ACCUM_F32)
 
 
 def matmul(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, mode: int = ops.GEMM_STORE) -> None:
@@ -263,26 +286,31 @@ def matmul(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, mode: int = ops.GE
     ``GEMM_ACCUM_F32``; rows of both at any stride.  A token of x with a value that is not finite gives a row of NaN."""
     if mode not in _MODES:
         raise KernelError(f"a product with a 4-bit weight has no epilogue {mode}")
-    gated = mode in (ops.GEMM_SWIGLU, ops.GEMM_RELUGLU)
-    if gated != w.gated:
+    if (mode in _GATED_MODES) != w.gated:
         raise KernelError("a gated epilogue and a gated weight go together")
-    if x.dim() != 2 or not x.is_cuda or x.shape[1] != w.width or (x.shape[0] and x.stride(1) != 1):
-        raise KernelError(f"x is {tuple(x.shape)}, not [tokens, {w.width}] on the GPU with the columns of a row together")
-    M = x.shape[0]
+    device = _current(x, "x")
+    code = _code(x, "x")
+    if x.dim() != 2 or x.shape[1] != w.width:
+        raise KernelError(f"x is {tuple(x.shape)}, not [tokens, {w.width}]")
+    M, N = x.shape[0], w.part
     if M > MAX_TOKENS:
         raise KernelError(f"{M} tokens: a product with a 4-bit weight takes {MAX_TOKENS}")
-    want = torch.float32 if mode in (ops.GEMM_STORE_F32, ops.GEMM_ACCUM_F32) else x.dtype
-    if out.shape != (M, w.part) or out.dtype != want or not out.is_cuda or (M and out.stride(1) != 1):
-        raise KernelError(f"out is {tuple(out.shape)} {out.dtype}, not {(M, w.part)} {want} with the columns of a row together")
-    code = ops.dtype_code(x.dtype)
-    _same_device(x, w.data, out)
+    want = torch.float32 if mode in _F32_MODES else x.dtype
+    if out.shape != (M, N) or out.dtype is not want or out.get_device() != device or w.data.get_device() != device:
+        raise KernelError(f"out is {tuple(out.shape)} {out.dtype} on {out.device}, not {(M, N)} {want} where x and the weight are ({w.data.device})")
     if M == 0:
         return
+    (ldx, x_step), (ldo, out_step) = x.stride(), out.stride()
+    if x_step != 1 or (out_step != 1 and N > 1):
+        raise KernelError("the columns of a row of x and out must lie together")
+    if M == 1:
+        ldx, ldo = w.width, N               # (a single row's stride says nothing)
     k = kernels()
-    scratch = torch.empty(k.ce_int4_gemm_scratch(code, M, w.width, w.group), dtype=torch.float32, device=x.device)
-    prof = ops.profiling()
-    if prof is not None:
-        prof.note_work(w.data.numel() + M * w.width * x.element_size() + out.numel() * out.element_size(), 2 * M * w.rows * w.width)
-    ldx, ldo = (x.stride(0), out.stride(0)) if M > 1 else (w.width, w.part)           # (a single row's stride says nothing)
-    ops._ok(k.ce_int4_gemm(code, x.data_ptr(), ldx, w.data.data_ptr(), out.data_ptr(), ldo, M, w.part, w.width, w.group,
-                           mode, scratch.data_ptr(), ops._stream()), 2)
+    # up to 16 tokens that fit the registers of 8 blocks: no scratch memory, one launch (the launcher checks it too)
+    scratch = None
+    if (M + 7) // 8 * (1 if code else 2) * w.kblocks > 512 or M > 16:
+        scratch = torch.empty(k.ce_int4_gemm_scratch(code, M, w.width, w.group), dtype=torch.float32, device=x.device)
+    if ops._profile is not None:
+        ops._profile.note_work(w.data.numel() + M * w.width * x.element_size() + out.numel() * out.element_size(), 2 * M * w.rows * w.width)
+    ops._ok(k.ce_int4_gemm(_GEMM(code, x.data_ptr(), ldx, w.data.data_ptr(), out.data_ptr(), ldo, M, N, w.width, w.group, mode,
+                                 0 if scratch is None else scratch.data_ptr(), w.status.data_ptr(), _stream(device))), 1 if scratch is None else 2)
