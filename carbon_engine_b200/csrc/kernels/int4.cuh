@@ -21,7 +21,8 @@
 //   V codes   block b, lane (r, l): words of tokens 2 l, 2 l + 1, 2 l + 8, 2 l + 9; codes 0 .. 3 of a word are channels
 //             64 b + 4 r .. + 4, codes 4 .. 7 channels 64 b + 32 + 4 r .. + 4
 //   (s, z) of K, token by token and group by group, then those of V
-// A weight's tile has codes as K's and its (s, z) row by row.
+// A weight's tile has codes as K's and its (s, z) row by row; rows 0 .. 7 of a gated weight's tile are gate rows, 8 .. 15 the up rows that belong
+// to them, so that a lane's sums (rows r and r + 8) are the two halves of its results.
 #pragma once
 #include "common.cuh"
 #include <cuda_fp16.h>
@@ -63,10 +64,37 @@ __device__ __forceinline__ unsigned i4_code(float x, float s, float z, float inv
 }
 __device__ __forceinline__ float i4_inverse(float s) { return s > 0.0f ? 1.0f / s : 0.0f; }
 
+// (not volatile: the products are functions of their operands, and the compiler may order them)
 __device__ __forceinline__ void i4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the first product of a chain: nothing to add to
+__device__ __forceinline__ void i4_mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("{\n.reg .f32 z;\nmov.f32 z, 0f00000000;\n"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {z,z,z,z};\n}"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t i4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// A warp's wait for a copy, with a limit: the thread sleeps in the instruction itself, which leaves the issue slots to the warps that compute
+// (1 token, 75,776 x 4,096: 40.5 us with a loop of tests).
+__device__ __forceinline__ bool i4_wait(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < (1u << 16); ++i) {
+        uint32_t ok;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(i4_smem(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+// A run of bytes into shared memory, counted on the barrier (both addresses and the size in multiples of 16); one lane calls it.
+__device__ __forceinline__ void i4_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(i4_smem(bar)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(i4_smem(dst)), "l"(src), "r"(bytes), "r"(i4_smem(bar)) : "memory");
+}
+
 // Four of a word's codes as operands (SHIFT 0 or 8): the even pair and the odd one, which is 16 times too large.  Plain: the bits of the codes,
 // float16 numbers of 2^-24.  CENTRED: codes less 8 as ordinary float16 numbers, which the float32 path takes for two instructions a word more:
 // tensor cores cut what they add to a sum, all the earlier where the operands are float16 numbers below 2^-14, and sums of codes that are all

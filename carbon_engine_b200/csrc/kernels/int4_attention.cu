@@ -18,7 +18,6 @@
 namespace {
 
 constexpr int WARPS = 8, STAGES = 4;
-constexpr uint32_t SPIN = 1u << 20;
 constexpr float HEADROOM = 5.0f;               // scores may pass the running maximum by this many powers of two before it is moved
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -35,25 +34,9 @@ struct Args {
     float scale;
 };
 
-__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < SPIN; ++i) {
-        uint32_t ok;
-        asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(ok) : "r"(smem_of(bar)), "r"(parity) : "memory");
-        if (ok) return true;
-        if (i > 256) __nanosleep(64);
-    }
-    return false;
-}
-__device__ __forceinline__ void copy_tile(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_of(bar)), "r"(bytes) : "memory");
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_of(dst)), "l"(src), "r"(bytes), "r"(smem_of(bar)) : "memory");
-}
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 
@@ -122,7 +105,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
 
     if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < STAGES; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(&full[warp][s])));
+        for (int s = 0; s < STAGES; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(i4_smem(&full[warp][s])));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
@@ -139,7 +122,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
         const int page = __shfl_sync(0xffffffffu, page_ids, i - looked);
         const int t = tile_lo + begin + warp + i * WARPS, in = t % per_page;
         if (lane == 0)
-            copy_tile(ring + (i % STAGES) * TILE, a.pages + (((size_t)page * a.nkv + j.kvh) * per_page + in) * TILE, TILE, &full[warp][i % STAGES]);
+            i4_copy(ring + (i % STAGES) * TILE, a.pages + (((size_t)page * a.nkv + j.kvh) * per_page + in) * TILE, TILE, &full[warp][i % STAGES]);
     };
     look_up(0);
     for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
@@ -236,7 +219,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
     bool ok = true;
     int gone = 0;                                     // tiles whose copies this warp has waited for
     for (int i = 0; i < mine; ++i, ++gone) {
-        ok = wait_full(&full[warp][i % STAGES], (i / STAGES) & 1);
+        ok = i4_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
         if (!ok) { if (lane == 0) atomicExch(a.status, 7); break; }
         const unsigned char* tile = ring + (i % STAGES) * TILE;
         const int key0 = (tile_lo + begin + warp + i * WARPS) * 16;
@@ -256,11 +239,6 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
             for (int half = 0; half < 2; ++half) {
                 const int c = 2 * b + half;
                 const uint32_t wa = half ? w.z : w.x, wb = half ? w.w : w.y;
-                if ((c * 32) % G == 0)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int p = 0; p < P; ++p) acc[nt][p][0] = acc[nt][p][1] = acc[nt][p][2] = acc[nt][p][3] = 0.f;
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     uint32_t a0, a1, a2, a3;
@@ -269,7 +247,10 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int p = 0; p < P; ++p) i4_mma(acc[nt][p], a0, a1, a2, a3, qf[nt][p][c][2 * st], qf[nt][p][c][2 * st + 1]);
+                        for (int p = 0; p < P; ++p) {
+                            if (st == 0 && (c * 32) % G == 0) i4_mma_first(acc[nt][p], a0, a1, a2, a3, qf[nt][p][c][0], qf[nt][p][c][1]);
+                            else i4_mma(acc[nt][p], a0, a1, a2, a3, qf[nt][p][c][2 * st], qf[nt][p][c][2 * st + 1]);
+                        }
                 }
                 if ((c * 32 + 32) % G == 0) {
                     const int g = c * 32 / G;
@@ -411,7 +392,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
     }
     if (!ok) {
         // the copies still in flight land in this block's memory: wait for them, with a limit, before it is used for anything else
-        for (int i = gone; i < min(gone + STAGES, mine); ++i) wait_full(&full[warp][i % STAGES], (i / STAGES) & 1);
+        for (int i = gone; i < min(gone + STAGES, mine); ++i) i4_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
     }
     __syncthreads();                                  // the rings are free: the warps' outputs take their place
 

@@ -134,30 +134,36 @@ struct WeightArgs {
     const void* w;                 // [rows, width], row stride ld (quantise reads it, dequantise writes it)
     unsigned char* tiles;          // [row tiles, ceil(width / 64), tile]
     long long ld;
-    int rows, part, padded, width, kblocks, group, vec;      // part: rows of a half that is padded to a multiple of 16 by itself
+    int rows, gated, width, kblocks, group, vec;
 };
+// the row tile and the row in it of a weight's row: a gated weight's halves take eight rows of a tile each
+__device__ __forceinline__ int place_of(const WeightArgs& a, int row, int& in) {
+    const int half = a.rows >> 1;
+    if (!a.gated) { in = row & 15; return row >> 4; }
+    const int n = row < half ? row : row - half;
+    in = (n & 7) + (row < half ? 0 : 8);
+    return n >> 3;
+}
 
-// a warp takes 128 neighbouring columns of one (padded) row: rows of padding, and columns beyond the width, hold zeros
+// a warp takes 128 neighbouring columns of one row of a tile: rows of padding, and columns beyond the width, hold zeros
 template <typename T>
 __global__ void __launch_bounds__(256) int4_quantise_weight_kernel(WeightArgs a) {
     ce_pdl_begin();
     const int lane = threadIdx.x & 31, pairs = (a.kblocks + 1) >> 1, kept = min(a.group, 64);
     const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int row = (int)(u / pairs), col = (int)(u - (long long)row * pairs) * 128 + 4 * lane;
-    const int padded_rows = a.padded * (a.rows / a.part);
-    if (row >= padded_rows) return;
-    const int half = row / a.padded, in_half = row - half * a.padded;
-    const bool real = in_half < a.part && col < a.width;
+    const int padded = (int)(u / pairs), col = (int)(u - (long long)padded * pairs) * 128 + 4 * lane, tile_no = padded >> 4, in = padded & 15;
+    const int part = a.gated ? a.rows >> 1 : a.rows, n = a.gated ? tile_no * 8 + (in & 7) : padded;
+    if (tile_no * (a.gated ? 8 : 16) >= part) return;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (real) load4((const T*)a.w + (half * (long long)a.part + in_half) * a.ld + col, a.vec, x);
+    if (n < part && col < a.width) load4((const T*)a.w + (n + (a.gated && in >= 8 ? (long long)part : 0)) * a.ld + col, a.vec, x);
     __half2 sz;
     const unsigned q = quantise4(x, a.group >> 2, sz);
     const unsigned near = __shfl_xor_sync(0xffffffffu, q, 1);
     const int kb = col >> 6;
     if (kb >= a.kblocks) return;
-    unsigned char* tile = a.tiles + ((size_t)(row >> 4) * a.kblocks + kb) * i4_weight_tile_bytes(kept);
-    if (!(lane & 1)) *reinterpret_cast<uint32_t*>(tile + i4_k_word(row & 15, col & 63)) = q | near << 16;
-    if ((4 * lane) % kept == 0) *reinterpret_cast<__half2*>(tile + 512 + ((row & 15) * (64 / kept) + (col & 63) / kept) * 4) = sz;
+    unsigned char* tile = a.tiles + ((size_t)tile_no * a.kblocks + kb) * i4_weight_tile_bytes(kept);
+    if (!(lane & 1)) *reinterpret_cast<uint32_t*>(tile + i4_k_word(in, col & 63)) = q | near << 16;
+    if ((4 * lane) % kept == 0) *reinterpret_cast<__half2*>(tile + 512 + (in * (64 / kept) + (col & 63) / kept) * 4) = sz;
 }
 
 // Runs behind a weight's quantisation, launched the ordinary way, and so begins when that has ended: from here on, no kernel that starts early
@@ -171,10 +177,11 @@ __global__ void __launch_bounds__(256) int4_dequantise_weight_kernel(WeightArgs 
     const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
     const int r = (int)(u / a.kblocks), kb = (int)(u - (long long)r * a.kblocks), col = kb * 64 + 4 * lane;
     if (r >= a.rows || col >= a.width) return;
-    const int half = r / a.part, row = half * a.padded + (r - half * a.part);
-    const unsigned char* tile = a.tiles + ((size_t)(row >> 4) * a.kblocks + kb) * i4_weight_tile_bytes(kept);
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + i4_k_word(row & 15, col & 63)) >> (lane & 1 ? 16 : 0);
-    const __half2 sz = *reinterpret_cast<const __half2*>(tile + 512 + ((row & 15) * (64 / kept) + (col & 63) / kept) * 4);
+    int in;
+    const int tile_no = place_of(a, r, in);
+    const unsigned char* tile = a.tiles + ((size_t)tile_no * a.kblocks + kb) * i4_weight_tile_bytes(kept);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + i4_k_word(in, col & 63)) >> (lane & 1 ? 16 : 0);
+    const __half2 sz = *reinterpret_cast<const __half2*>(tile + 512 + (in * (64 / kept) + (col & 63) / kept) * 4);
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), __low2float(sz), __high2float(sz));
@@ -213,7 +220,7 @@ int check_weight(const WeightArgs& a, int dtype, const char* who) {
     if (!a.w || !a.tiles) return ce_fail(CE_ERR_ARG, "%s: null pointer", who);
     if (dtype != CE_F32 && dtype != CE_BF16) return ce_fail(CE_ERR_ARG, "%s: unknown dtype %d", who, dtype);
     if (a.group != 32 && a.group != 64 && a.group != 128) return ce_fail(CE_ERR_SIZE, "%s: group %d (32, 64 or 128)", who, a.group);
-    if (a.rows < 1 || a.width < 1 || a.part < 1 || a.rows % a.part || a.width % a.group || a.ld < a.width)
+    if (a.rows < 1 || a.width < 1 || (a.gated && a.rows % 2) || a.width % a.group || a.ld < a.width)
         return ce_fail(CE_ERR_SIZE, "%s: %d rows of %d do not fit (the width is a multiple of the group)", who, a.rows, a.width);
     return CE_OK;
 }
@@ -252,12 +259,12 @@ extern "C" int ce_int4_kv_read(const Int4KvCall* c) {
     return run_cache(a, (int)c->dtype, int4_kv_read_kernel<float>, int4_kv_read_kernel<__nv_bfloat16>, "int4_kv_read_kernel", (cudaStream_t)c->stream);
 }
 
-// dtype, w, ld, tiles, rows, part, width, group, stream.  rows: a multiple of part; each part is padded to a multiple of 16 rows by itself.
-extern "C" int ce_int4_quantise_weight(int dtype, const void* w, long long ld, void* tiles, int rows, int part, int width, int group, void* stream) {
-    WeightArgs a{w, (unsigned char*)tiles, ld, rows, part, (part + 15) / 16 * 16, width, (width + 63) / 64, group, 0};
+// dtype, w, ld, tiles, rows, gated, width, group, stream
+extern "C" int ce_int4_quantise_weight(int dtype, const void* w, long long ld, void* tiles, int rows, int gated, int width, int group, void* stream) {
+    WeightArgs a{w, (unsigned char*)tiles, ld, rows, gated, width, (width + 63) / 64, group, 0};
     if (int e = check_weight(a, dtype, "int4_quantise_weight")) return e;
     a.vec = aligned4(w, ld, 0, dtype);
-    const long long warps = (long long)a.padded * (rows / part) * ((a.kblocks + 1) / 2), grid = (warps + 7) / 8;
+    const long long tiles_n = gated ? (rows / 2 + 7) / 8 : (rows + 15) / 16, warps = tiles_n * 16 * ((a.kblocks + 1) / 2), grid = (warps + 7) / 8;
     if (grid > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_quantise_weight: too large");
     ce_note("int4_quantise_weight_kernel");
     const cudaError_t e = dtype == CE_F32 ? ce_launch(int4_quantise_weight_kernel<float>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a)
@@ -267,8 +274,8 @@ extern "C" int ce_int4_quantise_weight(int dtype, const void* w, long long ld, v
     return ce_check_launch("int4_quantise_weight");
 }
 
-extern "C" int ce_int4_dequantise_weight(int dtype, void* w, long long ld, const void* tiles, int rows, int part, int width, int group, void* stream) {
-    WeightArgs a{w, (unsigned char*)tiles, ld, rows, part, (part + 15) / 16 * 16, width, (width + 63) / 64, group, 0};
+extern "C" int ce_int4_dequantise_weight(int dtype, void* w, long long ld, const void* tiles, int rows, int gated, int width, int group, void* stream) {
+    WeightArgs a{w, (unsigned char*)tiles, ld, rows, gated, width, (width + 63) / 64, group, 0};
     if (int e = check_weight(a, dtype, "int4_dequantise_weight")) return e;
     a.vec = aligned4(w, ld, 0, dtype);
     const long long units = (long long)rows * a.kblocks, grid = (units + 15) / 16;

@@ -91,7 +91,7 @@ struct GemmArgs {
     const unsigned char* w;        // [row tiles][kblocks][tile]
     Operand x;
     void* out;
-    int M, N, kblocks, tiles, ldo, mode, up_tile;        // up_tile: row tiles between a gate row and its up row
+    int M, N, kblocks, tiles, ldo, mode, gated;
 };
 
 enum { STORE = 0, STORE_F32 = 1, ACCUM_F32 = 2, SWIGLU = 3, RELUGLU = 4, RELU2 = 5 };
@@ -108,20 +108,20 @@ __device__ __forceinline__ void finish(void* out, size_t at, int mode, float v, 
     }
 }
 
-// one block a tile of 16 rows (and the up rows that belong to it): its warps share K
-template <typename T, int G, int NT, int HALVES>
+// one block a tile of 16 rows: its warps share K
+template <typename T, int G, int NT>
 __global__ void __launch_bounds__(WARPS * 32) int4_gemm_kernel(GemmArgs a) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1, TILE = i4_weight_tile_bytes(G), GB = 64 / G;
     __shared__ float part[WARPS][16][NT * 8 + 1];
-    __shared__ float total[HALVES][16][NT * 8 + 1];
+    __shared__ float total[16][NT * 8 + 1];
     ce_pdl_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3;
     const int tokens = a.tiles * 8;
-    for (int h = 0; h < HALVES; ++h) {
+    {
         float y[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = 0.f;
-        const unsigned char* rows = a.w + (size_t)(blockIdx.x + h * a.up_tile) * a.kblocks * TILE;
+        const unsigned char* rows = a.w + (size_t)blockIdx.x * a.kblocks * TILE;
         for (int kb = warp; kb < a.kblocks; kb += WARPS) {
             const unsigned char* tile = rows + (size_t)kb * TILE;
             const uint4 w = *reinterpret_cast<const uint4*>(tile + lane * 16);
@@ -179,32 +179,29 @@ __global__ void __launch_bounds__(WARPS * 32) int4_gemm_kernel(GemmArgs a) {
             float v = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) v += part[w][row][t];
-            total[h][row][t] = v;
+            total[row][t] = v;
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < 16 * NT * 8; i += WARPS * 32) {
-        const int t = i >> 4, row = i & 15, n = blockIdx.x * 16 + row;
+    const int rows_out = a.gated ? 8 : 16;
+    for (int i = threadIdx.x; i < rows_out * NT * 8; i += WARPS * 32) {
+        const int t = i / rows_out, row = i - t * rows_out, n = blockIdx.x * rows_out + row;
         if (t >= a.M || n >= a.N) continue;
         const float back = a.x.back[t];
-        float v = total[0][row][t] * back;
-        const float u = HALVES == 2 ? total[HALVES - 1][row][t] * back : 0.f;
-        const size_t at = (size_t)t * a.ldo + n;
-        finish<T>(a.out, at, a.mode, v, u);
+        finish<T>(a.out, (size_t)t * a.ldo + n, a.mode, total[row][t] * back, a.gated ? total[row + 8][t] * back : 0.f);
     }
 }
 
 // ---------------------------------------------------------------------------------------------
 // Up to 16 tokens: a stream of weights past tokens that stay in registers.
 //
-// A block takes ``upb`` tiles of 16 rows (with a gate: pairs of tiles) and a slice of K; each of its 16 warps a run of up to KW blocks of 64
+// A block takes some tiles of 16 rows and a slice of K; each of its 16 warps a run of up to KW blocks of 64
 // columns of that slice.  A warp holds its run of all tokens as the second operand (laid out and scaled by itself: nothing to prepare, and one
 // launch) and meets the rows' tiles one after another, each a run of bytes that one lane copies into the warp's ring ahead of time.  What the
 // warps make of a tile is added up in their order, what the blocks of a cluster make of it (slices of K) in theirs, through shared memory.
 // The copies begin before the kernels in front have ended: no kernel writes a weight (ops_int4.Int4Weight sees to that).
 // ---------------------------------------------------------------------------------------------
 constexpr int SW = 16;             // warps
-constexpr uint32_t SPIN = 1u << 20;
 
 struct StreamArgs {
     const void* x;
@@ -212,25 +209,9 @@ struct StreamArgs {
     void* out;
     int* status;
     long long ldx;
-    int M, N, K, kblocks, ldo, mode, up_tile, units, upb, slices, overlap, vec;
+    int M, N, K, kblocks, ldo, mode, gated, units, each, slices, overlap, vec;
 };
 
-__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < SPIN; ++i) {
-        uint32_t ok;
-        asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(ok) : "r"(smem_of(bar)), "r"(parity) : "memory");
-        if (ok) return true;
-        if (i > 256) __nanosleep(64);
-    }
-    return false;
-}
-__device__ __forceinline__ void copy_in(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_of(bar)), "r"(bytes) : "memory");
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_of(dst)), "l"(src), "r"(bytes), "r"(smem_of(bar)) : "memory");
-}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -245,44 +226,143 @@ __device__ __forceinline__ float load_cluster(uint32_t local, int rank) {
 template <typename T, int G, int NT, int KW>
 struct StreamShape {
     static constexpr int TILE = i4_weight_tile_bytes(G), STAGE = KW * TILE, STAGES = 16 / KW, RING = SW * STAGES * STAGE;
-    static constexpr int PART = SW * NT * 128 * 4;                            // bytes of one tile's sums of all warps
-    static constexpr int ROOM = 227 * 1024 - 4096 - RING - 2 * PART;          // for the tiles' totals
-    static constexpr int MOST = ROOM / (NT * 128 * 4);                        // tiles a block can take
-    static constexpr size_t smem(int tiles) { return RING + 2 * PART + (size_t)tiles * NT * 128 * 4; }
+    static constexpr int LD = 20;                                             // floats of a token's 16 rows: no two lanes of a store meet in a bank
+    static constexpr int SUMS = NT * 8 * LD;                                  // floats of a tile's sums of one warp
+    static constexpr int BATCH = 4 / NT;                                      // tiles between two meetings of the warps
+    static constexpr int PART = BATCH * SW * SUMS * 4;
+    static constexpr int TOTAL = NT * 8 * 16 * 4;                             // bytes of a tile's sums of a slice, where others add theirs
+    static constexpr int MOST = (227 * 1024 - 4096 - RING - PART) / TOTAL;    // tiles a block can take
+    static constexpr size_t smem(int tiles, int slices) { return RING + PART + (slices > 1 ? (size_t)tiles * TOTAL : 0); }
 };
 
-template <typename T, int G, int NT, int KW, int HALVES>
+// The groups' sums of the tokens, which meet the minima.  bfloat16: as two float16 pieces (22 bits) of sum / 2^7, the second operand of ONE product
+// whose first holds the minima of the run's groups (2 l and 2 l + 1 at lane (r, l), twice: once for each piece) - instead of four fma, and
+// two conversions, a group.  float32: float32, since its minimum is that of code 8 and no float16.
+template <int P, int G, int NT, int KW> struct Sums { uint32_t b[NT][2]; };
+template <int G, int NT, int KW> struct Sums<2, G, NT, KW> { float f[KW][64 / G][NT][2]; };
+
+// A warp's run of one tile: its sums of 16 rows by the tokens, in float32.  ``at``: byte offsets of the run's blocks of 64 columns; a run with
+// fewer than KW repeats its last, against tokens that are zeros there (``z_at``: of the minima of this lane's groups): no question a block, and the loads and products of all of them overlap
+// (four chains of products side by side).
+template <typename T, int G, int NT, int KW>
+__device__ __forceinline__ void stream_run(const unsigned char* stage, const int (&at)[KW], const int (&z_at)[2], int lane, const uint32_t (&xf)[KW][NT][sizeof(T) == 4 ? 2 : 1][2][4],
+                                           const Sums<sizeof(T) == 4 ? 2 : 1, G, NT, KW>& sums, float (&y)[NT][4]) {
+    constexpr int P = sizeof(T) == 4 ? 2 : 1, GB = 64 / G;
+    constexpr bool C8 = P == 2;
+    const int r = lane >> 2;
+    if constexpr (P == 1) {
+        // minima of this lane's two groups for rows r and r + 8 (groups beyond the run: any of the row, their sums are 0)
+        uint32_t za, zb;
+        const unsigned char *p = stage + z_at[0], *q = stage + z_at[1];
+        if constexpr (GB == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p), v = *reinterpret_cast<const uint2*>(p + 64);
+            za = __byte_perm(u.x, u.y, 0x7632); zb = __byte_perm(v.x, v.y, 0x7632);
+        } else {
+            za = __byte_perm(*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(q), 0x7632);
+            zb = __byte_perm(*reinterpret_cast<const uint32_t*>(p + 32), *reinterpret_cast<const uint32_t*>(q + 32), 0x7632);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) i4_mma_first(y[nt], za, zb, za, zb, sums.b[nt][0], sums.b[nt][1]);
+    }
+    uint4 w[KW];
+    uint32_t sa[KW][GB], sb[KW][GB];
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+        const unsigned char* tile = stage + at[k];
+        w[k] = *reinterpret_cast<const uint4*>(tile + lane * 16);
+        if constexpr (GB == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(tile + 512 + r * 8), v = *reinterpret_cast<const uint2*>(tile + 512 + r * 8 + 64);
+            sa[k][0] = u.x; sa[k][1] = u.y; sb[k][0] = v.x; sb[k][1] = v.y;
+        } else {
+            sa[k][0] = *reinterpret_cast<const uint32_t*>(tile + 512 + r * 4);
+            sb[k][0] = *reinterpret_cast<const uint32_t*>(tile + 512 + r * 4 + 32);
+        }
+    }
+    float acc[KW][GB][NT][P][4];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int k = 0; k < KW; ++k) {
+                const uint32_t wa = half ? w[k].z : w[k].x, wb = half ? w[k].w : w[k].y;
+                uint32_t a0, a1, a2, a3;
+                if (st) { i4_pairs<C8, 8>(wa, a0, a2); i4_pairs<C8, 8>(wb, a1, a3); }
+                else { i4_pairs<C8, 0>(wa, a0, a2); i4_pairs<C8, 0>(wb, a1, a3); }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        float (&c)[4] = acc[k][half * 32 / G][nt][p];
+                        if (st == 0 && half * 32 % G == 0) i4_mma_first(c, a0, a1, a2, a3, xf[k][nt][p][half][0], xf[k][nt][p][half][1]);
+                        else i4_mma(c, a0, a1, a2, a3, xf[k][nt][p][half][2 * st], xf[k][nt][p][half][2 * st + 1]);
+                    }
+            }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[nt][e] = P == 1 ? y[nt][e] * (128.0f / i4_unit<false>) : 0.f;
+#pragma unroll
+    for (int k = 0; k < KW; ++k)
+#pragma unroll
+        for (int g = 0; g < GB; ++g) {
+            const float2 fa = i4_step_of<C8>(sa[k][g]), fb = i4_step_of<C8>(sb[k][g]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float c[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    c[e] = acc[k][g][nt][0][e];
+                    if constexpr (P == 2) c[e] += acc[k][g][nt][1][e];
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if constexpr (P == 2) {
+                        y[nt][e] = fmaf(fa.y, sums.f[k][g][nt][e], y[nt][e]);
+                        y[nt][2 + e] = fmaf(fb.y, sums.f[k][g][nt][e], y[nt][2 + e]);
+                    }
+                    y[nt][e] = fmaf(fa.x, c[e], y[nt][e]);
+                    y[nt][2 + e] = fmaf(fb.x, c[2 + e], y[nt][2 + e]);
+                }
+            }
+        }
+}
+
+template <typename T, int G, int NT, int KW>
 __global__ void __launch_bounds__(SW * 32) int4_stream_kernel(StreamArgs a) {
     using Shape = StreamShape<T, G, NT, KW>;
     constexpr int P = sizeof(T) == 4 ? 2 : 1, TILE = Shape::TILE, STAGES = Shape::STAGES, GB = 64 / G;
     constexpr bool C8 = P == 2;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[SW][STAGES];
-    float* part = reinterpret_cast<float*>(smem + Shape::RING);               // [2][SW][NT][32 lanes][4]
-    float* total = part + 2 * SW * NT * 128;                                  // [tiles of the block][NT][32 lanes][4]
+    constexpr int BATCH = Shape::BATCH, SUMS = Shape::SUMS, LD = Shape::LD;
+    float* part = reinterpret_cast<float*>(smem + Shape::RING);               // [BATCH][SW][tokens][LD]
+    float* total = reinterpret_cast<float*>(smem + Shape::RING + Shape::PART);    // [tiles of the block][tokens][16], where K has slices
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3;
-    const int slice = blockIdx.x % a.slices, first = blockIdx.x / a.slices * a.upb, units = min(a.upb, a.units - first), its = units * HALVES;
+    const int slice = blockIdx.x % a.slices, first = blockIdx.x / a.slices * a.each, its = min(a.each, a.units - first);
     const int kb_begin = (int)((long long)a.kblocks * slice / a.slices), kb_end = (int)((long long)a.kblocks * (slice + 1) / a.slices);
     const int run = (kb_end - kb_begin + SW - 1) / SW, kb0 = min(kb_begin + warp * run, kb_end), count = min(run, kb_end - kb0);
     unsigned char* ring = smem + warp * (STAGES * Shape::STAGE);
     if (a.overlap) ce_pdl_launch_dependents();
     if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < STAGES; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(&full[warp][s])));
+        for (int s = 0; s < STAGES; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(i4_smem(&full[warp][s])));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
+    const unsigned char* next = a.w + ((size_t)first * a.kblocks + kb0) * TILE;
+    const size_t step = (size_t)a.kblocks * TILE;
     auto issue = [&](int it) {
-        const int unit = first + it / HALVES, h = it % HALVES;
-        if (lane == 0 && count > 0)
-            copy_in(ring + it % STAGES * Shape::STAGE, a.w + ((size_t)(unit + h * a.up_tile) * a.kblocks + kb0) * TILE, count * TILE, &full[warp][it % STAGES]);
+        if (lane == 0 && count > 0) i4_copy(ring + it % STAGES * Shape::STAGE, next, count * TILE, &full[warp][it % STAGES]);
+        next += step;
     };
     for (int it = 0; it < min(STAGES, its); ++it) issue(it);
     ce_pdl_wait();
 
     // ---- the warp's run of the tokens: lane (r, l) lays out token 8 nt + r, columns 8 l .. + 8 of every 32
     uint32_t xf[KW][NT][P][2][4];
-    float sums[KW][GB][NT][2], back[NT][2];
+    Sums<P, G, NT, KW> sums;
+    float back[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int t = nt * 8 + r;
@@ -314,6 +394,7 @@ __global__ void __launch_bounds__(SW * 32) int4_stream_kernel(StreamArgs a) {
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         const float up = i4_row_scale(largest);
+        if constexpr (P == 1) sums.b[nt][0] = sums.b[nt][1] = 0;
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
             float sum[GB];
@@ -339,129 +420,106 @@ __global__ void __launch_bounds__(SW * 32) int4_stream_kernel(StreamArgs a) {
             for (int g = 0; g < GB; ++g) {
                 sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
                 sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+                if constexpr (P == 2) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) sums[k][g][nt][e] = __shfl_sync(0xffffffffu, sum[g], 4 * (2 * l + e)) * (1.0f / i4_unit<C8>);
+                    for (int e = 0; e < 2; ++e) sums.f[k][g][nt][e] = __shfl_sync(0xffffffffu, sum[g], 4 * (2 * l + e)) * (1.0f / i4_unit<C8>);
+                } else {
+                    const float part = sum[g] * (1.0f / 128.0f), high = __half2float(__float2half_rn(part));
+                    const int at = k * GB + g;                                // of the run's groups
+                    if (at >> 1 == l) {
+                        sums.b[nt][0] |= i4_pack(at & 1 ? 0.f : part, at & 1 ? part : 0.f);
+                        sums.b[nt][1] |= i4_pack(at & 1 ? 0.f : part - high, at & 1 ? part - high : 0.f);
+                    }
+                }
             }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) back[nt][e] = i4_unit<C8> / __shfl_sync(0xffffffffu, up, 4 * (2 * l + e));
     }
 
-    bool ok = true;
-    int gone = 0;                                     // tiles whose copies this warp has waited for
+    // a batch's sums, one a thread: of tile u of it, token t, row
+    static_assert(BATCH * NT * 8 * 16 == SW * 32, "one result a thread");
+    const int row = threadIdx.x & 15, u = (threadIdx.x >> 4) / a.M, t = (threadIdx.x >> 4) - u * a.M;
+    const bool sums_here = u < BATCH;
+    const float* from = part + u * SW * SUMS + t * LD + row;
+    float* mine = part + warp * SUMS + 2 * l * LD + r;
+    int at[KW];
+#pragma unroll
+    for (int k = 0; k < KW; ++k) at[k] = max(0, min(k, count - 1)) * TILE;
+    // where this lane's two minima lie: see stream_run
+    const int z_at[2] = {max(0, min(GB == 2 ? l : 2 * l, count - 1)) * TILE + 512 + r * (4 * GB), max(0, min(2 * l + 1, count - 1)) * TILE + 512 + r * 4};
+    int gave_up = -1;                                 // the tile whose copy was not waited for to the end
     for (int it = 0; it < its; ++it) {
-        float y[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = 0.f;
-        if (ok && count > 0) {
-            ok = wait_full(&full[warp][it % STAGES], (it / STAGES) & 1);
-            if (ok) ++gone;
-            else if (lane == 0) atomicExch(a.status, 59);
-        }
-#pragma unroll
-        for (int k = 0; k < KW; ++k) {
-            if (k >= count) break;
-            const unsigned char* tile = ring + it % STAGES * Shape::STAGE + k * TILE;
-            const uint4 w = *reinterpret_cast<const uint4*>(tile + lane * 16);
-            uint32_t sa[GB], sb[GB];
-#pragma unroll
-            for (int g = 0; g < GB; ++g) {
-                sa[g] = *reinterpret_cast<const uint32_t*>(tile + 512 + (r * GB + g) * 4);
-                sb[g] = *reinterpret_cast<const uint32_t*>(tile + 512 + ((r + 8) * GB + g) * 4);
+        float* to = mine + it % BATCH * (SW * SUMS);
+        if (count > 0) {
+            if (gave_up < 0 && !i4_wait(&full[warp][it % STAGES], (it / STAGES) & 1)) {
+                gave_up = it;
+                atomicExch(a.status, 59);
             }
-            float acc[NT][P][4];
+            float y[NT][4];
+            stream_run<T, G, NT, KW>(ring + it % STAGES * Shape::STAGE, at, z_at, lane, xf, sums, y);
+            __syncwarp();
+            if (it + STAGES < its && gave_up < 0) issue(it + STAGES);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t wa = half ? w.z : w.x, wb = half ? w.w : w.y;
-                if ((half * 32) % G == 0)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                for (int e = 0; e < 4; ++e) to[(nt * 8 + (e & 1)) * LD + (e >> 1) * 8] = y[nt][e] * back[nt][e & 1];
+        } else {
 #pragma unroll
-                        for (int p = 0; p < P; ++p) acc[nt][p][0] = acc[nt][p][1] = acc[nt][p][2] = acc[nt][p][3] = 0.f;
-                uint32_t e0, e1, e2, e3, o0, o1, o2, o3;
-                i4_pairs<C8, 0>(wa, e0, e2); i4_pairs<C8, 0>(wb, e1, e3);
-                i4_pairs<C8, 8>(wa, o0, o2); i4_pairs<C8, 8>(wb, o1, o3);
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        i4_mma(acc[nt][p], e0, e1, e2, e3, xf[k][nt][p][half][0], xf[k][nt][p][half][1]);
-                        i4_mma(acc[nt][p], o0, o1, o2, o3, xf[k][nt][p][half][2], xf[k][nt][p][half][3]);
-                    }
-                if ((half * 32 + 32) % G == 0) {
-                    const int g = half * 32 / G;
-                    const float2 fa = i4_step_of<C8>(sa[g]), fb = i4_step_of<C8>(sb[g]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float c[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            c[e] = acc[nt][0][e];
-                            if constexpr (P == 2) c[e] += acc[nt][1][e];
-                        }
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            y[nt][e] = fmaf(fa.x, c[e], fmaf(fa.y, sums[k][g][nt][e], y[nt][e]));
-                            y[nt][2 + e] = fmaf(fb.x, c[2 + e], fmaf(fb.y, sums[k][g][nt][e], y[nt][2 + e]));
-                        }
-                    }
-                }
-            }
+                for (int e = 0; e < 4; ++e) to[(nt * 8 + (e & 1)) * LD + (e >> 1) * 8] = 0.f;
         }
-        __syncwarp();
-        if (ok && it + STAGES < its) issue(it + STAGES);
-        float* mine = part + (it & 1) * (SW * NT * 128) + warp * (NT * 128);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-            *reinterpret_cast<float4*>(mine + nt * 128 + lane * 4) =
-                make_float4(y[nt][0] * back[nt][0], y[nt][1] * back[nt][1], y[nt][2] * back[nt][0], y[nt][3] * back[nt][1]);
+        if ((it + 1) % BATCH && it + 1 < its) continue;
+        // the warps' sums of this batch's tiles, in their order
         __syncthreads();
-        // the warps' sums, in their order; four warps after another take the turn (the buffer is written again two tiles later, behind the
-        // next tile's barrier)
-        const int turn = (warp + SW - it * 4 * NT % SW) % SW;
-        if (turn < 4 * NT) {
-            const float* from = part + (it & 1) * (SW * NT * 128) + turn * 32 + lane;
-            float v = 0.f;
+        const int base = it / BATCH * BATCH;
+        const bool real = sums_here && base + u < its;
+        float v = 0.f;
+        if (real)
 #pragma unroll
-            for (int w = 0; w < SW; ++w) v += from[w * (NT * 128)];
-            total[it * (NT * 128) + turn * 32 + lane] = v;
+            for (int w = 0; w < SW; ++w) v += from[w * SUMS];
+        if (a.slices > 1) {
+            if (real) total[(base + u) * (NT * 128) + t * 16 + row] = v;
+        } else {
+            const float up = __shfl_down_sync(0xffffffffu, v, 8);             // (of a gate row)
+            const int tile_no = first + base + u, n = a.gated ? tile_no * 8 + row : tile_no * 16 + row;
+            if (real && n < a.N && (!a.gated || row < 8)) finish<T>(a.out, (size_t)t * a.ldo + n, a.mode, v, up);
         }
+        if (it + 1 < its) __syncthreads();
     }
     // a wait that gave up leaves copies in flight: they are waited for, with a limit, before the block may end
-    if (!ok)
-        for (int i = gone; i < min(gone + STAGES, its); ++i) wait_full(&full[warp][i % STAGES], (i / STAGES) & 1);
-    if (a.slices > 1) cluster_sync();
-    else __syncthreads();
-    const int outs = units * a.M * 16;
-    for (int o = threadIdx.x + slice * (SW * 32); o < outs; o += a.slices * (SW * 32)) {
-        const int row = o & 15, rest = o >> 4, u = rest / a.M, t = rest - u * a.M, n = (first + u) * 16 + row;
-        const int at = (t >> 3) * 128 + ((row & 7) * 4 + ((t & 7) >> 1)) * 4 + (row >> 3) * 2 + (t & 1);
-        float v[2] = {0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-            const float* p = total + (u * HALVES + h) * (NT * 128) + at;
-            if (a.slices == 1) v[h] = *p;
-            else
-                for (int s = 0; s < a.slices; ++s) v[h] += load_cluster(smem_of(p), s);
-        }
-        if (n < a.N) finish<T>(a.out, (size_t)t * a.ldo + n, a.mode, v[0], v[1]);
+    if (gave_up >= 0)
+        for (int i = gave_up; i < min(gave_up + STAGES, its); ++i) i4_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
+    if (a.slices == 1) return;
+    // the slices' sums, in their order: a block adds up every ``slices``-th run of 512 results of the cluster's
+    cluster_sync();
+    const int results = its * a.M * 16;
+    for (int o = threadIdx.x + slice * (SW * 32); o < (results + 31) / 32 * 32; o += a.slices * (SW * 32)) {
+        const int row = o & 15, rest = o >> 4, u = rest / a.M, t = rest - u * a.M;
+        float v = 0.f;
+        if (o < results)
+            for (int s = 0; s < a.slices; ++s) v += load_cluster(i4_smem(total + u * (NT * 128) + t * 16 + row), s);
+        const float up = __shfl_down_sync(0xffffffffu, v, 8);
+        const int n = a.gated ? (first + u) * 8 + row : (first + u) * 16 + row;
+        if (o < results && n < a.N && (!a.gated || row < 8)) finish<T>(a.out, (size_t)t * a.ldo + n, a.mode, v, up);
     }
-    if (a.slices > 1) cluster_sync();                 // nobody leaves while its totals are read
+    cluster_sync();                                   // nobody leaves while its sums are read
 }
 
 // Returns 1 where the sizes are not this kernel's.
-template <typename T, int G, int NT, int HALVES>
+template <typename T, int G, int NT>
 int launch_stream(StreamArgs a, cudaStream_t stream) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1, KW = 4 / (NT * P);
     using Shape = StreamShape<T, G, NT, KW>;
-    auto kernel = int4_stream_kernel<T, G, NT, KW, HALVES>;
+    auto kernel = int4_stream_kernel<T, G, NT, KW>;
     // slices of K: as few as the registers ask for; more where there are fewer tiles than SMs, down to 1,024 columns a slice
     const int sms = ce_sm_count();
     int slices = (a.kblocks + SW * KW - 1) / (SW * KW);
     while (slices < 8 && a.units * slices * 3 < sms * 2 && a.kblocks / (slices + 1) >= 16) ++slices;
     if (slices > 8) return 1;
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = ce_allow_smem(done, kernel, Shape::smem(Shape::MOST));
+    cudaError_t e = ce_allow_smem(done, kernel, Shape::smem(Shape::MOST, 2));
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_gemm: %s", cudaGetErrorString(e)); }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -474,17 +532,18 @@ int launch_stream(StreamArgs a, cudaStream_t stream) {
         attr[0].val.clusterDim = {(unsigned)slices, 1, 1};
         cfg.numAttrs = 1;
         cfg.gridDim = dim3(slices);
-        cfg.dynamicSmemBytes = Shape::smem(Shape::MOST);
+        cfg.dynamicSmemBytes = Shape::smem(Shape::MOST, 2);
         static CeRoom room[9];
         most = ce_clusters_at_once(room[slices], kernel, cfg);
         if (most < 1) return 1;
     }
     a.slices = slices;
-    a.upb = min((a.units + most - 1) / most, Shape::MOST / HALVES);
-    const int groups = (a.units + a.upb - 1) / a.upb;
+    a.each = (a.units + most - 1) / most;             // tiles a block
+    if (slices > 1) a.each = min(a.each, Shape::MOST);
+    const int groups = (a.units + a.each - 1) / a.each;
     a.overlap = (slices == 1 || groups <= most) && ce_pdl_enabled();
     cfg.gridDim = dim3((unsigned)(groups * slices));
-    cfg.dynamicSmemBytes = Shape::smem(a.upb * HALVES);
+    cfg.dynamicSmemBytes = Shape::smem(a.each, slices);
     cfg.numAttrs = slices > 1 ? 1 : 0;
     if (a.overlap) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -497,25 +556,23 @@ int launch_stream(StreamArgs a, cudaStream_t stream) {
     return ce_check_launch("int4_gemm");
 }
 template <typename T, int G>
-int launch_stream_tiles(const StreamArgs& a, int tiles, bool gated, cudaStream_t stream) {
-    if (tiles == 1) return gated ? launch_stream<T, G, 1, 2>(a, stream) : launch_stream<T, G, 1, 1>(a, stream);
-    return gated ? launch_stream<T, G, 2, 2>(a, stream) : launch_stream<T, G, 2, 1>(a, stream);
+int launch_stream_tiles(const StreamArgs& a, int tiles, cudaStream_t stream) {
+    return tiles == 1 ? launch_stream<T, G, 1>(a, stream) : launch_stream<T, G, 2>(a, stream);
 }
 
 int pieces(int dtype) { return dtype == CE_F32 ? 2 : 1; }
 
 template <typename T, int G, int NT>
-cudaError_t launch(const GemmArgs& a, int row_tiles, bool gated, cudaStream_t stream) {
+cudaError_t launch(const GemmArgs& a, int row_tiles, cudaStream_t stream) {
     ce_note("int4_gemm_kernel");
-    if (gated) return ce_launch(int4_gemm_kernel<T, G, NT, 2>, dim3(row_tiles), dim3(WARPS * 32), 0, stream, a);
-    return ce_launch(int4_gemm_kernel<T, G, NT, 1>, dim3(row_tiles), dim3(WARPS * 32), 0, stream, a);
+    return ce_launch(int4_gemm_kernel<T, G, NT>, dim3(row_tiles), dim3(WARPS * 32), 0, stream, a);
 }
 template <typename T, int G>
-cudaError_t launch_tiles(const GemmArgs& a, int row_tiles, bool gated, cudaStream_t stream) {
-    if (a.tiles == 1) return launch<T, G, 1>(a, row_tiles, gated, stream);
-    if (a.tiles == 2) return launch<T, G, 2>(a, row_tiles, gated, stream);
-    if (a.tiles <= 4) return launch<T, G, 4>(a, row_tiles, gated, stream);
-    return launch<T, G, 8>(a, row_tiles, gated, stream);
+cudaError_t launch_tiles(const GemmArgs& a, int row_tiles, cudaStream_t stream) {
+    if (a.tiles == 1) return launch<T, G, 1>(a, row_tiles, stream);
+    if (a.tiles == 2) return launch<T, G, 2>(a, row_tiles, stream);
+    if (a.tiles <= 4) return launch<T, G, 4>(a, row_tiles, stream);
+    return launch<T, G, 8>(a, row_tiles, stream);
 }
 
 // Whether the stream of weights takes these sizes: up to 16 tokens, K within the registers of 8 blocks
@@ -562,15 +619,15 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
     if (M == 0) return CE_OK;
     const int kept = group < 64 ? group : 64, tiles = (M + 7) / 8, kblocks = (K + 63) / 64;
     const bool gated = mode == SWIGLU || mode == RELUGLU;
-    const int el = dtype == CE_F32 ? 4 : 2;
+    const int el = dtype == CE_F32 ? 4 : 2, row_tiles = gated ? (N + 7) / 8 : (N + 15) / 16;
     const bool vec = ((uintptr_t)x % (4 * el)) == 0 && ldx % 4 == 0;
     if (!scratch) {
         if (!streamed(dtype, M, K)) return ce_fail(CE_ERR_ARG, "int4_gemm: these sizes need scratch memory");
-        StreamArgs a{x, (const unsigned char*)w, out, c->status, ldx, M, N, K, kblocks, ldo, mode, (N + 15) / 16, (N + 15) / 16, 0, 0, 0, vec};
-        const int code = dtype == CE_F32 ? (kept == 32 ? launch_stream_tiles<float, 32>(a, tiles, gated, (cudaStream_t)stream)
-                                                       : launch_stream_tiles<float, 64>(a, tiles, gated, (cudaStream_t)stream))
-                                         : (kept == 32 ? launch_stream_tiles<__nv_bfloat16, 32>(a, tiles, gated, (cudaStream_t)stream)
-                                                       : launch_stream_tiles<__nv_bfloat16, 64>(a, tiles, gated, (cudaStream_t)stream));
+        StreamArgs a{x, (const unsigned char*)w, out, c->status, ldx, M, N, K, kblocks, ldo, mode, gated, row_tiles, 0, 0, 0, vec};
+        const int code = dtype == CE_F32 ? (kept == 32 ? launch_stream_tiles<float, 32>(a, tiles, (cudaStream_t)stream)
+                                                       : launch_stream_tiles<float, 64>(a, tiles, (cudaStream_t)stream))
+                                         : (kept == 32 ? launch_stream_tiles<__nv_bfloat16, 32>(a, tiles, (cudaStream_t)stream)
+                                                       : launch_stream_tiles<__nv_bfloat16, 64>(a, tiles, (cudaStream_t)stream));
         return code == 1 ? ce_fail(CE_ERR_SIZE, "int4_gemm: no room for clusters on this device") : code;
     }
     Operand op;
@@ -582,13 +639,12 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
     cudaError_t e = dtype == CE_F32 ? ce_launch(int4_prepare_kernel<float, 2>, dim3(tiles * 8), dim3(256), 0, (cudaStream_t)stream, p)
                                     : ce_launch(int4_prepare_kernel<__nv_bfloat16, 1>, dim3(tiles * 8), dim3(256), 0, (cudaStream_t)stream, p);
     if (e == cudaSuccess) {
-        const int row_tiles = (N + 15) / 16;
-        GemmArgs a{(const unsigned char*)w, op, out, M, N, kblocks, tiles, ldo, mode, row_tiles};
+        GemmArgs a{(const unsigned char*)w, op, out, M, N, kblocks, tiles, ldo, mode, gated};
         if (dtype == CE_F32)
-            e = kept == 32 ? launch_tiles<float, 32>(a, row_tiles, gated, (cudaStream_t)stream) : launch_tiles<float, 64>(a, row_tiles, gated, (cudaStream_t)stream);
+            e = kept == 32 ? launch_tiles<float, 32>(a, row_tiles, (cudaStream_t)stream) : launch_tiles<float, 64>(a, row_tiles, (cudaStream_t)stream);
         else
-            e = kept == 32 ? launch_tiles<__nv_bfloat16, 32>(a, row_tiles, gated, (cudaStream_t)stream)
-                           : launch_tiles<__nv_bfloat16, 64>(a, row_tiles, gated, (cudaStream_t)stream);
+            e = kept == 32 ? launch_tiles<__nv_bfloat16, 32>(a, row_tiles, (cudaStream_t)stream)
+                           : launch_tiles<__nv_bfloat16, 64>(a, row_tiles, (cudaStream_t)stream);
     }
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_gemm: %s", cudaGetErrorString(e)); }
     return ce_check_launch("int4_gemm");

@@ -36,7 +36,7 @@ _ATTENTION = struct.Struct("=23qdq").pack
 # dtype, x, ldx, w, out, ldo, M, N, K, group, mode, scratch, status, stream
 kernel_lib.declare("ce_int4_gemm", _i, [ctypes.c_char_p])
 _GEMM = struct.Struct("=14q").pack
-# dtype, w, ld, tiles, rows, part, width, group, stream
+# dtype, w, ld, tiles, rows, gated, width, group, stream
 kernel_lib.declare("ce_int4_quantise_weight", _i, [_i, _p, _ll, _p, _i, _i, _i, _i, _p])
 kernel_lib.declare("ce_int4_dequantise_weight", _i, [_i, _p, _ll, _p, _i, _i, _i, _i, _p])
 # each, d, tile
@@ -246,7 +246,7 @@ class Int4Weight:
         #: columns of the result
         self.part = self.rows // 2 if self.gated else self.rows
         kept = min(group, 64)
-        tiles = (self.part + 15) // 16 * (2 if gated else 1)
+        tiles = (self.part + 7) // 8 if gated else (self.part + 15) // 16
         self.kblocks = (self.width + 63) // 64
         self.data = torch.empty((tiles, self.kblocks, 512 + 64 * (64 // kept)), dtype=torch.uint8, device=device)
         #: the word that kernels of products report to (``ops_tensor.gemm_status``)
@@ -261,7 +261,7 @@ class Int4Weight:
         self = cls(weight.shape[0], weight.shape[1], group, gated, weight.device)
         ld = weight.stride(0) if self.rows > 1 else self.width
         ops._ok(kernels().ce_int4_quantise_weight(_code(weight, "weight"), weight.data_ptr(), ld, self.data.data_ptr(),
-                                                  self.rows, self.part, self.width, self.group, _stream(device)), 2)
+                                                  self.rows, int(self.gated), self.width, self.group, _stream(device)), 2)
         return self
 
     def dequantize(self, out: torch.Tensor) -> torch.Tensor:
@@ -271,7 +271,7 @@ class Int4Weight:
             raise KernelError(f"out is {tuple(out.shape)} on {out.device}, not {(self.rows, self.width)} where the weight is ({self.data.device})")
         ld = out.stride(0) if self.rows > 1 else self.width
         ops._ok(kernels().ce_int4_dequantise_weight(_code(out, "out"), out.data_ptr(), ld, self.data.data_ptr(),
-                                                    self.rows, self.part, self.width, self.group, _stream(device)))
+                                                    self.rows, int(self.gated), self.width, self.group, _stream(device)))
         return out
 
 
