@@ -18,6 +18,7 @@
 namespace {
 
 constexpr int WARPS = 8, STAGES = 4;
+constexpr float NOTHING = -1e30f;              // the maximum of no scores
 constexpr float HEADROOM = 5.0f;               // scores may pass the running maximum by this many powers of two before it is moved
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -29,11 +30,15 @@ struct Args {
     int* status;
     float *part_o, *part_ml;       // splits > 1: [row block, split, rows, d], [row block, split, rows, 2]
     long long q_stride;
-    int nh, nkv, page_size, max_pages, num_pages, window, splits, subs;    // subs: row blocks of a sequence (or of a tile of 64 tokens)
-    int vec;
+    int nh, nkv, page_size, max_pages, num_pages, window, splits, share, subs;    // share: tiles of a split; subs: row blocks of a sequence (or of a tile of 64 tokens)
+    int vec, clustered, overlap;   // clustered: the splits of a row block are a cluster and join through shared memory
     float scale;
 };
 
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -81,14 +86,50 @@ __device__ __forceinline__ void load_steps(const unsigned char* p, uint32_t (&v)
     }
 }
 
+// what a run of keys with maximum m and sum l counts for beside the largest maximum (a run that saw nothing: nothing; a sum of NaN stays one)
+__device__ __forceinline__ float weight_of(float m, float l, float M) { return l == 0.f ? 0.f : exp2f(m - M); }
+
+// four channels of a row, rounded once; a row that saw no key becomes zeros
+template <typename T>
+__device__ __forceinline__ void store_row(const Args& a, const Job& j, int row, int d, int ch, float4 v, float L) {
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    const int each = a.nh / a.nkv, rho = j.row0 + row, tok = rho / each;
+    T* dst = (T*)a.out + ((size_t)(j.t0 + tok) * a.nh + j.kvh * each + rho - tok * each) * d + ch;
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(dst) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    } else {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+    }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(uint32_t local, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float load_cluster(uint32_t local, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at_rank(local, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load_cluster4(uint32_t local, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at_rank(local, rank)) : "memory");
+    return v;
+}
+
 template <typename T, int D, int G, int NT>
 __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
     constexpr bool C8 = Pieces<T>::N == 2;            // codes less 8: see i4_pairs
     constexpr int NB = D / 64, NG = D / G, P = Pieces<T>::N, ROWS = 8 * NT, TILE = i4_cache_tile_bytes(D, G), CH = D / 32;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[WARPS][STAGES];
-    __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
-    ce_pdl_begin();
+    __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_join[ROWS][2];
+    if (a.overlap) ce_pdl_launch_dependents();
+    ce_pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3;
     const int split = blockIdx.x % a.splits, job_id = blockIdx.x / a.splits;
     const Job j = job_of(a, job_id, ROWS);
@@ -97,7 +138,8 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
     const int first_pos = j.base + j.row0 / each, last_pos = j.base + (j.row0 + rows - 1) / each;
     const int block_lo = a.window > 0 ? max(0, first_pos - a.window + 1) : 0;
     const int tile_lo = block_lo >> 4, tiles = last_pos < block_lo ? 0 : (last_pos >> 4) + 1 - tile_lo;
-    const int share = (tiles + a.splits - 1) / a.splits, begin = min(split * share, tiles), end = min(begin + share, tiles);
+    // shares of the longest context's length (shorter sequences take fewer blocks), or as many keys as it takes
+    const int share = max(a.share, (tiles + a.splits - 1) / a.splits), begin = min(split * share, tiles), end = min(begin + share, tiles);
     const int mine = end - begin > warp ? (end - begin - warp + WARPS - 1) / WARPS : 0;      // tiles begin + warp, + WARPS, ...
     const int* table = a.block_table + (size_t)j.slot * a.max_pages;
     unsigned char* ring = smem + warp * (STAGES * TILE);
@@ -109,20 +151,20 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    // page ids of 32 of the warp's tiles at a time, one a lane
-    int looked = 0, page_ids = 0;
+    // where 32 of the warp's tiles lie, one a lane
+    int looked = 0;
+    const unsigned char* place = a.pages;
     auto look_up = [&](int from) {
         looked = from;
-        const int i = from + lane, pi = (tile_lo + begin + warp + i * WARPS) / per_page;
-        page_ids = i >= mine ? 0 : pi < a.max_pages ? table[pi] : -1;
-        if (page_ids < 0 || page_ids >= a.num_pages) { atomicExch(a.status, 4); page_ids = 0; }      // (the step's results are not used)
+        const int i = from + lane, t = tile_lo + begin + warp + i * WARPS, pi = t / per_page;
+        int page = i >= mine ? 0 : pi < a.max_pages ? table[pi] : -1;
+        if (page < 0 || page >= a.num_pages) { atomicExch(a.status, 4); page = 0; }      // (the step's results are not used)
+        place = a.pages + (((size_t)page * a.nkv + j.kvh) * per_page + (t - pi * per_page)) * TILE;
     };
     auto issue = [&](int i) {
         if (i >= looked + 32) look_up(i);
-        const int page = __shfl_sync(0xffffffffu, page_ids, i - looked);
-        const int t = tile_lo + begin + warp + i * WARPS, in = t % per_page;
-        if (lane == 0)
-            i4_copy(ring + (i % STAGES) * TILE, a.pages + (((size_t)page * a.nkv + j.kvh) * per_page + in) * TILE, TILE, &full[warp][i % STAGES]);
+        const unsigned char* src = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(place), i - looked));
+        if (lane == 0) i4_copy(ring + (i % STAGES) * TILE, src, TILE, &full[warp][i % STAGES]);
     };
     look_up(0);
     for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
@@ -203,14 +245,18 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
     }
 
     float o[NT][NB * 4][4], oz[NT][NG][2], m[NT][2], sum[NT][2];
-    float top = 0x1p-24f, norm = 1024.0f / top;       // a power of two that no step of V seen so far passes
+    // Weights are kept as 2^(S - m): m follows the scores (within HEADROOM) and, in the same number, the steps: a weight times a step is to lie
+    // near 2^10, so m holds log2(top / 2^10) too, top a power of two that no step of V seen so far passes.  Sums, parts of minima and products
+    // all carry the factor, which falls out at the end.
+    float top = 0x1p-24f, high[NT][2];                // high: what a score (before its row's scale) may reach before m is moved
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < NB * 4; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) oz[nt][g][0] = oz[nt][g][1] = 0.f;
-        m[nt][0] = m[nt][1] = -INFINITY;
+        m[nt][0] = m[nt][1] = NOTHING;
+        high[nt][0] = high[nt][1] = NOTHING;
         sum[nt][0] = sum[nt][1] = 0.f;
     }
     // tiles in [whole_lo, whole_hi] hold only keys that every row sees
@@ -296,17 +342,18 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                s[nt][e] *= row_scale[nt][e];
-                s[nt][2 + e] *= row_scale[nt][e];
                 if (cut) {
                     if (key_a > hi[nt][e] || key_a < lo[nt][e]) s[nt][e] = -INFINITY;
                     if (key_b > hi[nt][e] || key_b < lo[nt][e]) s[nt][2 + e] = -INFINITY;
                 }
-                move = move || fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + HEADROOM;
+                move = move || fmaxf(s[nt][e], s[nt][2 + e]) > high[nt][e];
             }
-        float step_max = 0.f;
+        float fa[NG], fb[NG], step_max = 0.f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) step_max = fmaxf(step_max, fmaxf(i4_unpack(va[g]).x, i4_unpack(vb[g]).x));
+        for (int g = 0; g < NG; ++g) {
+            fa[g] = i4_unpack(va[g]).x; fb[g] = i4_unpack(vb[g]).x;
+            step_max = fmaxf(step_max, fmaxf(fa[g], fb[g]));
+        }
         move = move || step_max > top;
         if (__any_sync(0xffffffffu, move)) {
             // maxima over the 8 lanes that share l, the largest step over all
@@ -315,8 +362,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
             const float before = top;
             // the next power of two: a number's exponent, one up where it has bits below
             if (step_max > top) top = __uint_as_float((__float_as_uint(step_max) + 0x007fffffu) & 0x7f800000u);
-            const float shrink = before / top;
-            norm = 1024.0f / top;
+            const float offset = log2f(top) - 10.0f, grown = log2f(before) - log2f(top);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -325,13 +371,15 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float mn = fmaxf(m[nt][e], mx), alpha = mn == -INFINITY ? 1.0f : exp2f(m[nt][e] - mn);
-                    m[nt][e] = mn;
+                    const float now = fmaxf(m[nt][e] - grown, fmaf(mx, row_scale[nt][e], offset));
+                    const float alpha = m[nt][e] == NOTHING ? 0.0f : exp2f(m[nt][e] - now);
+                    m[nt][e] = mx == -INFINITY && m[nt][e] == NOTHING ? NOTHING : now;
+                    high[nt][e] = m[nt][e] == NOTHING ? NOTHING : (now - offset + HEADROOM) / row_scale[nt][e];
                     sum[nt][e] *= alpha;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) oz[nt][g][e] *= alpha;
 #pragma unroll
-                    for (int i2 = 0; i2 < NB * 4; ++i2) { o[nt][i2][e] *= alpha * shrink; o[nt][i2][2 + e] *= alpha * shrink; }
+                    for (int i2 = 0; i2 < NB * 4; ++i2) { o[nt][i2][e] *= alpha; o[nt][i2][2 + e] *= alpha; }
                 }
         }
         float pr[NT][4];
@@ -339,9 +387,8 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-                pr[nt][e] = ce_exp2_fast(s[nt][e] - base);
-                pr[nt][2 + e] = ce_exp2_fast(s[nt][2 + e] - base);
+                pr[nt][e] = ce_exp2_fast(fmaf(s[nt][e], row_scale[nt][e], -m[nt][e]));
+                pr[nt][2 + e] = ce_exp2_fast(fmaf(s[nt][2 + e], row_scale[nt][e], -m[nt][e]));
                 sum[nt][e] += pr[nt][e] + pr[nt][2 + e];
             }
         // ---- V^T P^T, group by group: the probability carries the step
@@ -353,13 +400,12 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
             for (int half = 0; half < 2; ++half) {
                 const int g = (64 * b + 32 * half) / G;
                 if ((32 * half) % G == 0) {
-                    const float2 fa = i4_step_of<C8>(va[g]), fb = i4_step_of<C8>(vb[g]);
-                    const float sa = fa.x * norm, sb = fb.x * norm;
+                    const float za = i4_step_of<C8>(va[g]).y, zb = i4_step_of<C8>(vb[g]).y;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        oz[nt][g][0] = fmaf(pr[nt][0], fa.y, fmaf(pr[nt][2], fb.y, oz[nt][g][0]));
-                        oz[nt][g][1] = fmaf(pr[nt][1], fa.y, fmaf(pr[nt][3], fb.y, oz[nt][g][1]));
-                        float x0 = pr[nt][0] * sa, x1 = pr[nt][1] * sa, x2 = pr[nt][2] * sb, x3 = pr[nt][3] * sb;
+                        oz[nt][g][0] = fmaf(pr[nt][0], za, fmaf(pr[nt][2], zb, oz[nt][g][0]));
+                        oz[nt][g][1] = fmaf(pr[nt][1], za, fmaf(pr[nt][3], zb, oz[nt][g][1]));
+                        float x0 = pr[nt][0] * fa[g], x1 = pr[nt][1] * fa[g], x2 = pr[nt][2] * fb[g], x3 = pr[nt][3] * fb[g];
 #pragma unroll
                         for (int p = 0; p < P; ++p) {
                             const uint32_t ab = i4_pack(x0, x1), cd = i4_pack(x2, x3);
@@ -407,7 +453,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) t += __shfl_xor_sync(0xffffffffu, t, w);
             if (r == 0) { s_m[warp][row] = m[nt][e]; s_l[warp][row] = t; }
-            const float even = top * (i4_unit<C8> / 1024.0f), odd = even * 0.0625f;
+            constexpr float even = i4_unit<C8>, odd = even * 0.0625f;
             float zs[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -424,32 +470,61 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
         }
     }
     __syncthreads();
+    const bool cluster = a.clustered;
     for (int x = threadIdx.x; x < rows * (D / 4); x += WARPS * 32) {
         const int row = x / (D / 4), ch = (x - row * (D / 4)) * 4;
-        float M = -INFINITY;
+        float M = NOTHING;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][row]);
         float L = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float f = s_m[w][row] == -INFINITY ? (s_l[w][row] == 0.f ? 0.f : 1.f) : exp2f(s_m[w][row] - M);
+            const float f = weight_of(s_m[w][row], s_l[w][row], M);
             const float4 u = *reinterpret_cast<const float4*>(so + (w * ROWS + row) * LD + ch);
             L += s_l[w][row] * f;
             v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
         }
-        if (a.splits > 1) {
+        if (cluster) {
+            // (warp 0's rows: every number of theirs is read by the thread that replaces it)
+            *reinterpret_cast<float4*>(so + row * LD + ch) = v;
+            if (ch == 0) { s_join[row][0] = M; s_join[row][1] = L; }
+        } else if (a.splits > 1) {
             const size_t at = ((size_t)job_id * a.splits + split) * ROWS + row;
             *reinterpret_cast<float4*>(a.part_o + at * D + ch) = v;
             if (ch == 0) { a.part_ml[2 * at] = M; a.part_ml[2 * at + 1] = L; }
         } else {
-            const float inv = L == 0.f ? 0.f : 1.0f / L;
-            const int rho = j.row0 + row, tok = rho / each;
-            T* dst = (T*)a.out + ((size_t)(j.t0 + tok) * a.nh + j.kvh * each + rho - tok * each) * D + ch;
-            CeType<T>::store(dst, v.x * inv); CeType<T>::store(dst + 1, v.y * inv);
-            CeType<T>::store(dst + 2, v.z * inv); CeType<T>::store(dst + 3, v.w * inv);
+            store_row<T>(a, j, row, D, ch, v, L);
         }
     }
+    if (!cluster) return;
+    // the blocks' runs of keys, in their order: each takes a share of the rows' channels
+    cluster_sync();
+    const int all = rows * (D / 4);
+    for (int x = split * (WARPS * 32) + threadIdx.x; x < all; x += a.splits * (WARPS * 32)) {
+        const int row = x / (D / 4), ch = (x - row * (D / 4)) * 4;
+        float M = NOTHING, L = 0.f, ms[8], ls[8];
+        float4 us[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {                 // (one trip to all of them)
+            ms[k] = NOTHING; ls[k] = 0.f; us[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < a.splits) {
+                ms[k] = load_cluster(i4_smem(&s_join[row][0]), k);
+                ls[k] = load_cluster(i4_smem(&s_join[row][1]), k);
+                us[k] = load_cluster4(i4_smem(so + row * LD + ch), k);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) M = fmaxf(M, ms[k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float f = weight_of(ms[k], ls[k], M);
+            L += ls[k] * f;
+            v.x = fmaf(us[k].x, f, v.x); v.y = fmaf(us[k].y, f, v.y); v.z = fmaf(us[k].z, f, v.z); v.w = fmaf(us[k].w, f, v.w);
+        }
+        store_row<T>(a, j, row, D, ch, v, L);
+    }
+    cluster_sync();                                   // nobody leaves while its rows are read
 }
 
 // Joins the runs of keys of a row block, in their order: one block a row, four channels a thread
@@ -462,37 +537,54 @@ __global__ void __launch_bounds__(64) int4_attention_merge_kernel(Args a) {
     if (row >= j.tokens * each - j.row0) return;
     const int ch = threadIdx.x * 4;
     if (ch >= D) return;
-    float M = -INFINITY, L = 0.f;
+    float M = NOTHING, L = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     const size_t at = (size_t)job_id * a.splits * ROWS + row;
     for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (at + (size_t)s * ROWS)]);
     for (int s = 0; s < a.splits; ++s) {
         const size_t p = at + (size_t)s * ROWS;
-        const float ms = a.part_ml[2 * p], ls = a.part_ml[2 * p + 1];
-        const float f = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : exp2f(ms - M);
+        const float ls = a.part_ml[2 * p + 1], f = weight_of(a.part_ml[2 * p], ls, M);
+        if (ls == 0.f) continue;                      // (a run without a key that the row sees wrote nothing else)
         const float4 u = *reinterpret_cast<const float4*>(a.part_o + p * D + ch);
         L += ls * f;
         v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
     }
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
-    const int rho = j.row0 + row, tok = rho / each;
-    T* dst = (T*)a.out + ((size_t)(j.t0 + tok) * a.nh + j.kvh * each + rho - tok * each) * D + ch;
-    CeType<T>::store(dst, v.x * inv); CeType<T>::store(dst + 1, v.y * inv);
-    CeType<T>::store(dst + 2, v.z * inv); CeType<T>::store(dst + 3, v.w * inv);
+    store_row<T>(a, j, row, D, ch, v, L);
 }
 
 template <typename T, int D, int G, int NT>
-int run(const Args& a, int jobs, cudaStream_t stream) {
+int run(Args a, int jobs, cudaStream_t stream) {
     constexpr int TILE = i4_cache_tile_bytes(D, G), RING = WARPS * STAGES * TILE, OUT = WARPS * 8 * NT * (D + 4) * 4;
     constexpr int SMEM = RING > OUT ? RING : OUT;
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = ce_allow_smem(done, int4_attention_kernel<T, D, G, NT>, SMEM);
+    auto kernel = int4_attention_kernel<T, D, G, NT>;
+    cudaError_t e = ce_allow_smem(done, kernel, SMEM);
     if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[2];
+        cfg.gridDim = dim3((unsigned)(jobs * a.splits));
+        cfg.blockDim = dim3(WARPS * 32);
+        cfg.dynamicSmemBytes = SMEM;
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        a.clustered = a.splits > 1 && !a.part_o;
+        a.overlap = ce_pdl_enabled();
+        if (a.clustered) {
+            attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+            attr[cfg.numAttrs++].val.clusterDim = {(unsigned)a.splits, 1, 1};
+            // a grid of more clusters than the chip holds stands alone (ce_clusters_at_once)
+            static CeRoom room[9];
+            a.overlap = a.overlap && jobs <= ce_clusters_at_once(room[a.splits], kernel, cfg);
+        }
+        if (a.overlap) {
+            attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+        }
         ce_note("int4_attention_kernel");
-        e = ce_launch(int4_attention_kernel<T, D, G, NT>, dim3((unsigned)(jobs * a.splits)), dim3(WARPS * 32), SMEM, stream, a);
+        e = cudaLaunchKernelEx(&cfg, kernel, a);
     }
-    if (e == cudaSuccess && a.splits > 1) {
+    if (e == cudaSuccess && a.splits > 1 && !a.clustered) {
         ce_note("int4_attention_merge_kernel");
         e = ce_launch(int4_attention_merge_kernel<T, D, 8 * NT>, dim3((unsigned)(jobs * 8 * NT)), dim3(64), 0, stream, a);
     }
@@ -543,7 +635,7 @@ struct Int4AttentionCall {
     const int *seq_slot, *q_start, *ctx_len, *block_table;
     int* status;
     const int* tiles;              // null: ``n`` one-token sequences
-    long long n, nh, nkv, d, group, page_size, max_pages, num_pages, window, splits;
+    long long n, nh, nkv, d, group, page_size, max_pages, num_pages, window, splits, share;     // without part_o the splits (8 at most) are a cluster
     float *part_o, *part_ml;
     double scale;
     void* stream;
@@ -568,14 +660,16 @@ extern "C" int ce_int4_attention(const Int4AttentionCall* c) {
     if (page_size < 16 || page_size % 16) return ce_fail(CE_ERR_SIZE, "int4_attention: page size %d is not a multiple of 16", page_size);
     if (((uintptr_t)pages & 15) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: the pages do not start on a 16-byte boundary");
     if (max_pages < 1 || num_pages < 1 || splits < 1 || window < 0) return ce_fail(CE_ERR_SIZE, "int4_attention: bad sizes");
-    if (splits > 1 && (!part_o || !part_ml)) return ce_fail(CE_ERR_ARG, "int4_attention: shares of the keys need scratch memory");
+    if (((uintptr_t)out % (dtype == CE_F32 ? 16 : 8)) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: out does not start on a boundary of four elements");
+    if (splits > 8 && (!part_o || !part_ml)) return ce_fail(CE_ERR_ARG, "int4_attention: more than 8 shares of the keys need scratch memory");
+    if (!(c->scale > 0.0)) return ce_fail(CE_ERR_ARG, "int4_attention: a scale that is not positive");
     if (count == 0) return CE_OK;
     const int each = nh / nkv, rows = block_rows(each, d, tiles ? 64 : 1), subs = ((tiles ? 64 : 1) * each + rows - 1) / rows;
     const long long jobs = count * nkv * subs;
     if (count < 0 || jobs * splits * 16 > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_attention: too many rows");
     const int el = dtype == CE_F32 ? 4 : 2;
     Args a{q, out, (const unsigned char*)pages, seq_slot, q_start, ctx_len, block_table, tiles, status, part_o, part_ml, q_stride,
-           nh, nkv, page_size, max_pages, num_pages, window, splits, subs, ((uintptr_t)q % (4 * el)) == 0 && q_stride % 4 == 0, scale};
+           nh, nkv, page_size, max_pages, num_pages, window, splits, (int)c->share, subs, ((uintptr_t)q % (4 * el)) == 0 && q_stride % 4 == 0, 0, 0, scale};
     return dtype == CE_F32 ? run_type<float>(a, d, group, (int)jobs, rows, (cudaStream_t)stream)
                            : run_type<__nv_bfloat16>(a, d, group, (int)jobs, rows, (cudaStream_t)stream);
 }

@@ -11,6 +11,7 @@ tensors' device, which has to be the current one; scratch memory comes from torc
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from typing import Optional
 
@@ -30,9 +31,9 @@ kernel_lib.declare("ce_int4_kv_write", _i, [ctypes.c_char_p])
 kernel_lib.declare("ce_int4_kv_read", _i, [ctypes.c_char_p])
 _KV = struct.Struct("=21q").pack
 # dtype, q, q_stride, pages, out, seq_slot, q_start, ctx_len, block_table, status, tiles, count, nh, nkv, d, group, page_size, max_pages,
-# num_pages, window, splits, part_o, part_ml, scale, stream
+# num_pages, window, splits, share, part_o, part_ml, scale, stream
 kernel_lib.declare("ce_int4_attention", _i, [ctypes.c_char_p])
-_ATTENTION = struct.Struct("=23qdq").pack
+_ATTENTION = struct.Struct("=24qdq").pack
 # dtype, x, ldx, w, out, ldo, M, N, K, group, mode, scratch, status, stream
 kernel_lib.declare("ce_int4_gemm", _i, [ctypes.c_char_p])
 _GEMM = struct.Struct("=14q").pack
@@ -164,11 +165,27 @@ def kv_read(pages: Int4Pages, k_out: torch.Tensor, v_out: torch.Tensor, position
     _kv_call(kernels().ce_int4_kv_read, k_out, v_out, pages, positions, seq_of_token, seq_slot, block_table, status)
 
 
-def _splits(jobs: int, max_ctx: int, window: int, tokens: int) -> int:
-    """Blocks that share a sequence's keys: enough to fill the chip twice, but two tiles of 16 keys a warp at least."""
-    keys = min(max_ctx, window + tokens) if window > 0 else max_ctx
-    most = max(1, (keys + 255) // 256)
-    return max(1, min(most, 64, (2 * 148 + jobs - 1) // jobs))
+@functools.lru_cache(maxsize=4096)
+def _splits(jobs: int, tiles: int):
+    """(blocks that share a row block's keys, tiles of 16 keys a block) for ``jobs`` row blocks of up to ``tiles`` tiles: the least of what the
+    rounds of blocks take, two an SM at a time: 1.1 us for each eighth tile (0.6 with an SM to itself), 4.5 a block to begin and end, a quarter
+    of a round lost at the end, and 2 us where the blocks are joined by a second kernel.  (64 sequences of 8,192 keys, 8 KV heads of 128: 1, 2, 4
+    and 8 blocks a row block 145, 141, 157 and 190 us, of which the rule says 148, 147, 160 and 189.)"""
+    best = (float("inf"), 1, tiles)
+    for splits in (1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64):
+        share = -(-tiles // splits)
+        if splits > 1 and (share < 8 or -(-tiles // share) < splits):
+            continue
+        blocks = jobs * splits
+        rounds = blocks / 296 + 0.25 if blocks > 296 else 1.0
+        cost = rounds * (-(-share // 8) * (1.1 if blocks > 148 else 0.6) + 4.5) + (2.0 if _joined(jobs, splits) else 0.0)
+        best = min(best, (cost, splits, share))
+    return best[1:]
+
+
+def _joined(jobs: int, splits: int) -> bool:
+    """Whether a second kernel joins the splits; up to 8 of few row blocks are a cluster and join through shared memory."""
+    return splits > 8 or (splits > 1 and jobs * splits > 296)
 
 
 def _attend(device, code, q, q_stride, heads, pages, out, seq_slot, q_start, ctx_len, block_table, status, tiles, count, max_ctx, window, scale) -> None:
@@ -176,17 +193,18 @@ def _attend(device, code, q, q_stride, heads, pages, out, seq_slot, q_start, ctx
     each = heads // pages.kv_heads
     tile = 0 if tiles is None else 1
     jobs = count * pages.kv_heads * k.ce_int4_attention_blocks(each, pages.head_dim, tile)
-    splits = _splits(jobs, max_ctx, window, 64 if tile else 1)
+    keys = min(max_ctx, window + (64 if tile else 1) + 15) if window > 0 else max_ctx
+    splits, share = _splits(jobs, max(1, (keys + 15) // 16))
     part_o = part_ml = None
-    if splits > 1:
+    if _joined(jobs, splits):
         rows = jobs * splits * k.ce_int4_attention_rows(each, pages.head_dim, tile)
         part_o = torch.empty(rows * (pages.head_dim + 2), dtype=torch.float32, device=q.device)
         part_ml = part_o.data_ptr() + 4 * rows * pages.head_dim
     ops._ok(k.ce_int4_attention(_ATTENTION(
         code, q.data_ptr(), q_stride, pages.data.data_ptr(), out.data_ptr(), seq_slot.data_ptr(), q_start.data_ptr(), ctx_len.data_ptr(),
         block_table.data_ptr(), status.data_ptr(), 0 if tiles is None else tiles.data_ptr(), count, heads, pages.kv_heads, pages.head_dim,
-        pages.group, pages.page_size, block_table.shape[1], pages.num_pages, window, splits, 0 if part_o is None else part_o.data_ptr(),
-        part_ml or 0, scale, _stream(device))), 2 if splits > 1 else 1)
+        pages.group, pages.page_size, block_table.shape[1], pages.num_pages, window, splits, share,
+        0 if part_o is None else part_o.data_ptr(), part_ml or 0, scale, _stream(device))), 1 if part_o is None else 2)
 
 
 def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor,
@@ -216,6 +234,8 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
     _ints(device, seq_slot=seq_slot, q_start=q_start, ctx_len=ctx_len, block_table=block_table, status=status)
     if block_table.dim() != 2 or window < 0 or n_decode < 0 or max_ctx < 0:
         raise KernelError("attention: a table of [slots, pages], no negative numbers")
+    if not scale > 0.0:
+        raise KernelError(f"attention: a scale of {scale} (it must be positive)")
     seqs = seq_slot.numel()
     if n_decode > seqs or q_start.numel() <= seqs or ctx_len.numel() < seqs:
         raise KernelError("attention: one slot and one length a sequence, one start more")
