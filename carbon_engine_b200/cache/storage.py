@@ -11,7 +11,7 @@ shaped [num_pages, kv_heads, page_size, head_dim].  State caches are tensors
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional
+from typing import Any, Dict, List, Optional
 
 import numpy as np
 import torch
@@ -30,6 +30,8 @@ class LayerCacheView:
     page_size: int = 0
     k_pool: Optional[torch.Tensor] = None
     v_pool: Optional[torch.Tensor] = None
+    #: keys and values in 4 bits (``ops_int4.Int4Pages``), in the place of the two pools
+    int4: Optional[Any] = None
     state: Optional[torch.Tensor] = None        # [max_requests, *shape]
     writes: bool = True
     #: named states of the block around the mixer (a ``BundleCacheSpec``'s ``extra``), each [max_requests, *shape]
@@ -62,6 +64,13 @@ class CacheStorage:
                     # ``num_pages`` counts pages of the engine's size: a group with other pages holds as many tokens
                     groups.append(GroupSpec(ps, max(1, int(n) * int(page_size) // ps), int(spec.window)))
                 g = group_of[(spec.window, ps)]
+                if spec.int4_group is not None:
+                    from ..ops_int4 import Int4Pages
+                    pages = Int4Pages(groups[g].num_pages, spec.kv_heads, ps, spec.head_dim, spec.int4_group, device, poison)
+                    self._entries[cache_id] = LayerCacheView("paged", g, ps, int4=pages)
+                    if cache_id in extras:
+                        raise ValueError("a 4-bit cache beside states of a block is not supported")
+                    continue
                 k = torch.empty((groups[g].num_pages, spec.kv_heads, ps, spec.head_dim), dtype=dtype, device=device)
                 v = torch.empty((groups[g].num_pages, spec.value_heads, ps, spec.value_dim), dtype=dtype, device=device)
                 if poison:          # stale reads then show up as NaN in the logits
@@ -90,15 +99,18 @@ class CacheStorage:
         base = self._entries[call.cache]
         if call.writes:
             return base
-        return LayerCacheView(base.kind, base.group, base.page_size, base.k_pool, base.v_pool, base.state, False, base.extra)
+        return LayerCacheView(base.kind, base.group, base.page_size, base.k_pool, base.v_pool, base.int4, base.state, False, base.extra)
 
     def paged_views(self) -> List[LayerCacheView]:
         return [e for e in self._entries.values() if e.kind == "paged"]
 
     def bytes_per_token(self) -> int:
+        from ..ops_int4 import cache_bytes_per_token
         total = 0
         for e in self._entries.values():
-            if e.kind == "paged":
+            if e.int4 is not None:
+                total += cache_bytes_per_token(e.int4.kv_heads, e.int4.head_dim, e.int4.group)
+            elif e.kind == "paged":
                 total += (e.k_pool.shape[1] * e.k_pool.shape[3] + e.v_pool.shape[1] * e.v_pool.shape[3]) * e.k_pool.element_size()
         return total
 

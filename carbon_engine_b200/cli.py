@@ -34,6 +34,10 @@ def _engine_flags(p: argparse.ArgumentParser) -> None:
                    help="token budget of one step (portions of prompts fill what decoding leaves)")
     p.add_argument("--cuda-graphs", action="store_true", help="replay decode steps as CUDA graphs")
     p.add_argument("--page-size", type=int, default=64, help="tokens per KV page")
+    p.add_argument("--weight-bits", type=int, default=16, choices=[16, 4],
+                   help="4: weights of attention and dense feed-forwards in 4 bits, quantised as they are loaded")
+    p.add_argument("--kv-bits", type=int, default=16, choices=[16, 4], help="4: keys and values in 4 bits, quantised as they enter the cache")
+    p.add_argument("--int4-group", type=int, default=64, help="values that share a step and a minimum: 32 | 64 | 128 (weights; a cache takes 64 at most)")
     p.add_argument("--seed-weights", type=int, default=0, help="seed of --dummy-weight")
 
 
@@ -46,7 +50,8 @@ def _make_engine(a):
     return Engine(a.model, dtype=a.dtype, device=dev, hf_overrides=overrides, dummy_weight=a.dummy_weight,
                   seed=a.seed_weights, kv_tokens=a.kv_tokens, memory_ratio=a.memory_ratio, page_size=a.page_size,
                   max_seq_len=a.max_seq_len, max_running_requests=a.max_running_requests,
-                  max_prefill_tokens=a.max_prefill_tokens, cuda_graphs=a.cuda_graphs)
+                  max_prefill_tokens=a.max_prefill_tokens, cuda_graphs=a.cuda_graphs, weight_bits=a.weight_bits, kv_bits=a.kv_bits,
+                  int4_group=a.int4_group)
 
 
 def _parse_ids(text: str) -> List[int]:

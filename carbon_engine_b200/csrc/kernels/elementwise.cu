@@ -239,7 +239,8 @@ struct QkRopeArgs {
     const int* seq_slot;     // [B]
     const int* block_table;  // [slots, max_pages]
     int* status;
-    int T, nh, nkv, d, rd, page_size, max_pages, num_pages, max_pos, write_kv;
+    int T, nh, nkv, d, rd, page_size, max_pages, num_pages, max_pos;
+    int write_kv;            // 0: query heads only; 1: keys and values into the pages; 2: keys stay in place as queries do, values untouched
     float eps;
     int pairing;             // partners of a rotation: 0 = (i, i + rd/2) ("rotate-half"), 1 = (2i, 2i + 1) (interleaved)
     int weights_ready;       // no kernel in front writes q_weight and k_weight
@@ -254,13 +255,13 @@ __global__ void qk_rope_kvwrite_kernel(QkRopeArgs a) {
     int t = blockIdx.x, hh = blockIdx.y, j = threadIdx.x;
     int d = a.d;
     bool is_q = hh < a.nh, is_k = !is_q && hh < a.nh + a.nkv;
-    if (!is_q && !a.write_kv) return;
+    if (!is_q && (a.write_kv == 0 || (a.write_kv == 2 && !is_k))) return;
     T* src = (T*)a.qkv + (size_t)t * (a.nh + 2 * a.nkv) * d + (size_t)hh * d;
     float v = j < d ? CeType<T>::load(src + j) : 0.f;
     int pos = a.positions[t];
 
     T* dst = nullptr;
-    if (is_q) {
+    if (is_q || a.write_kv == 2) {
         dst = src;
     } else {
         int slot = a.seq_slot[a.seq_of_token[t]];
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(128) qk_rope_kvwrite_warp_kernel(QkRopeArgs a,
     const int t = (int)(wg / groups), g = (int)(wg - (long long)t * groups);
     const int hh0 = g * hpw;
     int hh1 = min(hh0 + hpw, heads_per_token);
-    if (!a.write_kv) hh1 = min(hh1, a.nh);
+    if (a.write_kv != 1) hh1 = min(hh1, a.write_kv == 2 ? a.nh + a.nkv : a.nh);
     if (hh0 >= hh1) return;
     constexpr int half = E * L, d = 2 * half;
     const int e0 = E * (lane % L);
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(128) qk_rope_kvwrite_warp_kernel(QkRopeArgs a,
         rope_load<WF>(a.sin_table + (size_t)pos * half + e0, sn);
     }
     size_t page_row = 0;
-    if (hh1 > a.nh) {                      // a K or V head in this group: where the token's row lies in the pools
+    if (hh1 > a.nh && a.write_kv == 1) {   // a K or V head in this group: where the token's row lies in the pools
         int slot = a.seq_slot[a.seq_of_token[t]];
         int page = a.block_table[(size_t)slot * a.max_pages + pos / a.page_size];
         if (page < 0 || page >= a.num_pages) {
@@ -457,7 +458,7 @@ __global__ void __launch_bounds__(128) qk_rope_kvwrite_warp_kernel(QkRopeArgs a,
             }
             rope_sum<L>(ss, lane);
             if (hh >= hh1) continue;
-            T* dst = kv < 0 ? row + (size_t)hh * d : (T*)(v < 0 ? a.k_pool : a.v_pool) + (page_row + (size_t)(v < 0 ? kv : v) * a.page_size) * d;
+            T* dst = kv < 0 || a.write_kv == 2 ? row + (size_t)hh * d : (T*)(v < 0 ? a.k_pool : a.v_pool) + (page_row + (size_t)(v < 0 ? kv : v) * a.page_size) * d;
             if (w) {
                 const float inv = rsqrtf(fmaf(ss[0], inv_d, a.eps));
 #pragma unroll
@@ -539,7 +540,7 @@ extern "C" int ce_qk_rope_kvwrite(void* qkv, void* k_pool, void* v_pool, int dty
     if (rd < 0 || rd > d || (rd & 1)) return ce_fail(CE_ERR_SIZE, "ce_qk_rope_kvwrite: rotary_dim %d must be even and <= head_dim %d", rd, d);
     if (pairing != 0 && pairing != 1) return ce_fail(CE_ERR_ARG, "ce_qk_rope_kvwrite: pairing %d (0: halves, 1: interleaved)", pairing);
     if (!qkv || !positions || !status) return ce_fail(CE_ERR_ARG, "ce_qk_rope_kvwrite: null pointer");
-    if (write_kv && (!k_pool || !v_pool || !seq_of_token || !seq_slot || !block_table))
+    if (write_kv == 1 && (!k_pool || !v_pool || !seq_of_token || !seq_slot || !block_table))
         return ce_fail(CE_ERR_ARG, "ce_qk_rope_kvwrite: cache pointers missing");
     QkRopeArgs a{qkv, k_pool, v_pool, q_weight, k_weight, cos_table, sin_table, positions, seq_of_token, seq_slot,
                  block_table, status, T, nh, nkv, d, rd, page_size, max_pages, num_pages, max_pos, write_kv, eps, pairing,

@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(256) int4_quantise_weight_kernel(WeightArgs a)
     if ((4 * lane) % kept == 0) *reinterpret_cast<__half2*>(tile + 512 + (in * (64 / kept) + (col & 63) / kept) * 4) = sz;
 }
 
-// Runs behind a weight's quantisation, launched the ordinary way, and so begins when that has ended: from here on, no kernel that starts early
-// beside the one before it can meet a weight that is still being written.
+// Runs behind a kernel that writes a weight, launched the ordinary way, and so begins when that has ended: from here on, no kernel that starts
+// early beside the one before it can meet a weight that is still being written.
 __global__ void int4_weight_done_kernel() {}
 
 template <typename T>
@@ -284,5 +284,6 @@ extern "C" int ce_int4_dequantise_weight(int dtype, void* w, long long ld, const
     const cudaError_t e = dtype == CE_F32 ? ce_launch(int4_dequantise_weight_kernel<float>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a)
                                           : ce_launch(int4_dequantise_weight_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a);
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_dequantise_weight: %s", cudaGetErrorString(e)); }
+    int4_weight_done_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();           // (a product may read its weight ahead of the kernels in front)
     return ce_check_launch("int4_dequantise_weight");
 }

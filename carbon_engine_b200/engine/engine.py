@@ -54,8 +54,9 @@ def require_gpu(device: Union[str, torch.device]) -> torch.device:
 
 def build_model(model_dir: Optional[str], dtype: torch.dtype, device: torch.device, *, config=None,
                 hf_overrides: Optional[Dict[str, Any]] = None, dummy_weight: bool = False, seed: int = 0,
-                max_seq_len: int = 0):
-    """(model, config, max_seq_len): the model of a folder (or of a typed config) with weights loaded."""
+                max_seq_len: int = 0, weight_bits: int = 16, kv_bits: int = 16, int4_group: int = 64, page_size: int = 16):
+    """(model, config, max_seq_len): the model of a folder (or of a typed config) with weights loaded.  ``weight_bits``, ``kv_bits``,
+    ``int4_group``: see :class:`Engine`."""
     if config is None:
         arch, config = load_config(model_dir, hf_overrides)
     else:
@@ -64,11 +65,56 @@ def build_model(model_dir: Optional[str], dtype: torch.dtype, device: torch.devi
     if max_seq_len <= 0:
         max_seq_len = min(config.max_position_embeddings, 32768)
     model = arch.build_model(config, max_seq_len)
+    hold_in_4_bits(model, weight_bits, kv_bits, int4_group, page_size)
     if dummy_weight or model_dir is None:
         load_random(model, seed, device, dtype)
     else:
         load_from_folder(model, model_dir, device, dtype)
     return model, config, max_seq_len
+
+
+def linears(model):
+    """The products of a model's blocks."""
+    from ..parts.linear import Linear
+
+    def walk(part):
+        if isinstance(part, Linear):
+            yield part
+        for child in part.children():
+            yield from walk(child)
+
+    for block in model.blocks:
+        yield from walk(block)
+
+
+def hold_in_4_bits(model, weight_bits: int, kv_bits: int, group: int, page_size: int) -> None:
+    """Mark what a model holds in 4 bits, before its weights are loaded and its cache is laid out: the products that say they can be
+    (``Linear.quantizable``: attention's and the dense feed-forward's; embedding and head stay as they are), and the key/value caches
+    (``PagedAttention``)."""
+    from ..ops_int4 import CACHE_GROUPS, WEIGHT_GROUPS, cache_problem
+    from ..parts.attention import PagedAttention
+    for name, bits in (("weight_bits", weight_bits), ("kv_bits", kv_bits)):
+        if bits not in (4, 16):
+            raise ValueError(f"{name} is 16 (the compute type's own form) or 4, not {bits}")
+
+    if weight_bits == 4:
+        if group not in WEIGHT_GROUPS:
+            raise ValueError(f"int4_group {group} ({', '.join(map(str, WEIGHT_GROUPS))})")
+        found = [p for p in linears(model) if p.quantizable and p.in_features % group == 0 and p.bias_names is None]
+        if not found:
+            raise ValueError(f"no product of this model can be held in 4 bits in groups of {group}")
+        for p in found:
+            p.int4_group = group
+    if kv_bits == 4:
+        mixers = {id(b.mixer): b.mixer for b in model.blocks}.values()
+        for m in mixers:
+            if not isinstance(m, PagedAttention):
+                raise ValueError(f"a 4-bit cache needs paged attention in every layer, not {type(m).__name__}")
+            kept = min(group, max(CACHE_GROUPS))
+            problem = cache_problem(m.head_dim, kept, m.page_size or page_size)
+            if problem:
+                raise ValueError(problem)
+            m.kv_int4_group = kept
 
 
 @dataclass
@@ -112,12 +158,16 @@ class Engine:
                  seed: int = 0, kv_tokens: Optional[int] = None, memory_ratio: float = 0.9, page_size: int = 16,
                  max_seq_len: int = 0, max_running_requests: int = 16, max_prefill_tokens: int = 4096,
                  cuda_graphs: bool = False, poison_cache: bool = False, host_lookahead: bool = True,
-                 run_ahead: bool = True):
+                 run_ahead: bool = True, weight_bits: int = 16, kv_bits: int = 16, int4_group: int = 64):
+        """``weight_bits`` 4: the weights of attention and of dense feed-forwards are held in 4 bits, a step and a minimum (float16) for
+        each ``int4_group`` (32, 64 or 128) neighbouring columns, quantised as they are loaded.  ``kv_bits`` 4: keys and values are
+        quantised as they enter the cache, in groups of ``int4_group`` (at most 64) channels; head sizes 64 to 256 in steps of 64, pages of a
+        multiple of 16 tokens."""
         self.device = require_gpu(device)
         self.dtype = parse_dtype(dtype)
         self.model, self.config, self.max_seq_len = build_model(
             model, self.dtype, self.device, config=config, hf_overrides=hf_overrides, dummy_weight=dummy_weight,
-            seed=seed, max_seq_len=max_seq_len)
+            seed=seed, max_seq_len=max_seq_len, weight_bits=weight_bits, kv_bits=kv_bits, int4_group=int4_group, page_size=int(page_size))
         self.page_size = int(page_size)
         self.max_running = int(max_running_requests)
         self.max_step_tokens = max(int(max_prefill_tokens), self.max_running)
@@ -148,8 +198,9 @@ class Engine:
         from ..parts.base import BundleCacheSpec, PagedCacheSpec
         el = 2 if self.dtype == torch.bfloat16 else 4
         specs = [s.main if isinstance(s, BundleCacheSpec) else s for _, s in self.model.cache_layout()]
-        return sum((s.kv_heads * s.head_dim + s.value_heads * s.value_dim) * el for s in specs
-                   if isinstance(s, PagedCacheSpec))
+        from ..ops_int4 import cache_bytes_per_token
+        return sum(cache_bytes_per_token(s.kv_heads, s.head_dim, s.int4_group) if s.int4_group is not None else
+                   (s.kv_heads * s.head_dim + s.value_heads * s.value_dim) * el for s in specs if isinstance(s, PagedCacheSpec))
 
     def _state_bytes(self) -> int:
         """Bytes of the fixed-size per-request state of every slot (src/model/mod.rs:129-145 counts them too)."""
@@ -176,7 +227,9 @@ class Engine:
         from .. import ops_tensor
         el = 2 if self.dtype == torch.bfloat16 else 4
         step = self.model.step_bytes(self.max_step_tokens, el, rows=self.max_running)
-        return step + step // 4 + 4 * ops_tensor.GEMM_SCRATCH_FLOATS + (256 << 20)
+        # (steps of many tokens read a 4-bit weight back, one at a time)
+        back = max((p.total_out * p.in_features * el for p in linears(self.model) if p.int4 is not None), default=0)
+        return step + step // 4 + 4 * ops_tensor.GEMM_SCRATCH_FLOATS + back + (256 << 20)
 
     def _size_cache(self, kv_tokens: Optional[int], memory_ratio: float) -> int:
         """Pages of the cache: ``kv_tokens`` if given, else what ``memory_ratio`` of the free memory holds

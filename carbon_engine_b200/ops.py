@@ -239,8 +239,10 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, eps: float
 
 def qk_rope_kvwrite(qkv, k_pool, v_pool, q_weight, k_weight, cos, sin, positions, seq_of_token, seq_slot,
                     block_table, status, nh: int, nkv: int, d: int, rotary_dim: int, page_size: int,
-                    eps: float, write_kv: bool = True, pairing: str = "half", weights_ready: bool = False) -> None:
-    """Per-head q/k RMSNorm, rotation, and the write of K and V into the pages.  ``pairing``: which elements
+                    eps: float, write_kv: bool = True, pairing: str = "half", weights_ready: bool = False,
+                    keys_in_place: bool = False) -> None:
+    """Per-head q/k RMSNorm, rotation, and the write of K and V into the pages.  ``keys_in_place``: keys are normed and rotated where they
+    are, like queries, and nothing is written to pages (a cache that is written by another kernel).  ``pairing``: which elements
     of a head turn together, "half" (i with i + rotary_dim/2) or "interleaved" (2i with 2i + 1).  ``cos``, ``sin``, ``positions``
     and the tables of slots and pages may be read while the kernels in front still run, so none of those may write them;
     with ``weights_ready`` the norm weights too.  All other operands are read after them."""
@@ -256,6 +258,8 @@ def qk_rope_kvwrite(qkv, k_pool, v_pool, q_weight, k_weight, cos, sin, positions
     max_pos = cos.shape[0] if cos is not None else 0
     if cos is not None and cos.shape[1] != rotary_dim // 2:
         raise KernelError("qk_rope_kvwrite: rotary table width is not rotary_dim / 2")
+    if keys_in_place:
+        write_kv = False
     if write_kv:
         _need(k_pool, "k_pool", qkv.dtype); _need(v_pool, "v_pool", qkv.dtype)
         if tuple(k_pool.shape[1:]) != (nkv, page_size, d):
@@ -265,7 +269,7 @@ def qk_rope_kvwrite(qkv, k_pool, v_pool, q_weight, k_weight, cos, sin, positions
     _ok(kernels().ce_qk_rope_kvwrite(
         _ptr(qkv), _ptr(k_pool), _ptr(v_pool), dtype_code(qkv.dtype), _ptr(q_weight), _ptr(k_weight), _ptr(cos),
         _ptr(sin), _ptr(positions), _ptr(seq_of_token), _ptr(seq_slot), _ptr(block_table), _ptr(status),
-        T, nh, nkv, d, rotary_dim, page_size, max_pages, num_pages, max_pos, 1 if write_kv else 0, float(eps),
+        T, nh, nkv, d, rotary_dim, page_size, max_pages, num_pages, max_pos, 2 if keys_in_place else 1 if write_kv else 0, float(eps),
         ROPE_PAIRINGS[pairing], int(weights_ready), _stream()))
 
 
@@ -824,6 +828,8 @@ def bias_rope_kvwrite(qkv, k_pool, v_pool, bias, cos, sin, positions, seq_of_tok
         raise KernelError("bias_rope_kvwrite: the bias is shorter than q|k|v")
     if cos is not None and cos.shape[1] != rotary_dim // 2:
         raise KernelError("bias_rope_kvwrite: rotary table width is not rotary_dim / 2")
+    if keys_in_place:
+        write_kv = False
     if write_kv:
         _need(k_pool, "k_pool", qkv.dtype); _need(v_pool, "v_pool", qkv.dtype)
         if tuple(k_pool.shape[1:]) != (nk, page_size, d) or tuple(v_pool.shape[1:]) != (nv, page_size, dv):

@@ -291,7 +291,7 @@ class Int4Weight:
             raise KernelError(f"out is {tuple(out.shape)} on {out.device}, not {(self.rows, self.width)} where the weight is ({self.data.device})")
         ld = out.stride(0) if self.rows > 1 else self.width
         ops._ok(kernels().ce_int4_dequantise_weight(_code(out, "out"), out.data_ptr(), ld, self.data.data_ptr(),
-                                                    self.rows, int(self.gated), self.width, self.group, _stream(device)))
+                                                    self.rows, int(self.gated), self.width, self.group, _stream(device)), 2)
         return out
 
 

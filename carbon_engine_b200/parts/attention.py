@@ -60,8 +60,10 @@ class PagedAttention(Mixer):
         self.scale = float(scale) if scale is not None else 1.0 / math.sqrt(head_dim)
         self.page_size = page_size          # None: the engine's; else this layer's cache has pages of its own size
         self.qkv = Linear(hidden, [heads * head_dim, kv_heads * head_dim, kv_heads * head_dim],
-                          [f"{prefix}.q_proj.weight", f"{prefix}.k_proj.weight", f"{prefix}.v_proj.weight"])
-        self.o = Linear(heads * head_dim, [hidden], [f"{prefix}.o_proj.weight"])
+                          [f"{prefix}.q_proj.weight", f"{prefix}.k_proj.weight", f"{prefix}.v_proj.weight"], quantizable=True)
+        self.o = Linear(heads * head_dim, [hidden], [f"{prefix}.o_proj.weight"], quantizable=True)
+        #: set before the cache is laid out: keys and values are held in 4 bits, a step and a minimum for each group of so many
+        self.kv_int4_group: Optional[int] = None
         self.q_norm_weight: Optional[torch.Tensor] = None
         self.k_norm_weight: Optional[torch.Tensor] = None
 
@@ -86,7 +88,7 @@ class PagedAttention(Mixer):
             self.position.prepare(device)
 
     def cache_spec(self) -> PagedCacheSpec:
-        return PagedCacheSpec(self.kv_heads, self.head_dim, self.window, self.page_size)
+        return PagedCacheSpec(self.kv_heads, self.head_dim, self.window, self.page_size, int4_group=self.kv_int4_group)
 
     def step_bytes(self, tokens: int, element_size: int) -> int:
         return tokens * (2 * self.heads + 2 * self.kv_heads) * self.head_dim * element_size      # q|k|v and the heads' outputs
@@ -135,10 +137,33 @@ class PagedAttention(Mixer):
                             ctx.positions, ctx.seq_of_token, ctx.seq_slot, table, ctx.status, nh, nkv, d,
                             pos.rotary_dim if cos is not None else 0, cache.page_size,
                             self.qk_norm_eps if self.qk_norm_eps is not None else 0.0, write_kv=cache.writes,
-                            pairing=pos.pairing if pos is not None else "half", weights_ready=True)
+                            pairing=pos.pairing if pos is not None else "half", weights_ready=True,
+                            keys_in_place=cache.int4 is not None and cache.writes)
         out = ctx.buffer((T, nh * d))
+        if cache.int4 is not None:
+            self.attend_int4(ctx, qkv, out, cache, table)
+            self.o.forward(out, x, ACCUM if accumulate else STORE_F32)
+            return
         self.attend(ctx, qkv, out, cache, table)
         self.o.forward(out, x, ACCUM if accumulate else STORE_F32)
+
+    def attend_int4(self, ctx, qkv: torch.Tensor, out: torch.Tensor, cache, table: torch.Tensor) -> None:
+        """Quantise the step's keys and values into the pages, then attend over those."""
+        from .. import ops_int4, ops_tensor
+        nh, nkv, d = self.heads, self.kv_heads, self.head_dim
+        plan = ctx.plans[self.plan_key]
+        heads = qkv.view(-1, nh + 2 * nkv, d)
+        if cache.writes:
+            ops_int4.kv_write(cache.int4, heads[:, nh:nh + nkv], heads[:, nh + nkv:], ctx.positions, ctx.seq_of_token, ctx.seq_slot, table,
+                              ctx.status)
+        step = (heads[:, :nh], cache.int4, out.view(-1, nh, d), ctx.seq_slot, ctx.q_start, ctx.ctx_len, table, ctx.status)
+        if ctx.n_decode > 0:
+            # (the plan's bound, and so the launch, is the one a captured step was captured with)
+            ops_int4.attention(*step, n_decode=ctx.n_decode, max_ctx=plan.decode_splits * ops_tensor.decode_split(), window=self.window,
+                               scale=self.scale)
+        if plan.n_tiles > 0:
+            ops_int4.attention(*step, n_decode=0, max_ctx=plan.portion_ctx, tiles=plan.tiles, n_tiles=plan.n_tiles, window=self.window,
+                               scale=self.scale)
 
     def attend(self, ctx, qkv: torch.Tensor, out: torch.Tensor, cache, table: torch.Tensor) -> None:
         nh, nkv, d = self.heads, self.kv_heads, self.head_dim

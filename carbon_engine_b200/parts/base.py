@@ -44,6 +44,8 @@ class PagedCacheSpec:
     #: the value pool's heads and head size where they differ from the keys' (None: the same)
     v_heads: Optional[int] = None
     v_head_dim: Optional[int] = None
+    #: keys and values are held in 4 bits, a step and a minimum for each group of so many (None: in the compute type)
+    int4_group: Optional[int] = None
 
     @property
     def value_heads(self) -> int:

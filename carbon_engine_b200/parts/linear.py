@@ -74,15 +74,27 @@ def matmul_nt(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, mode: int, sc
         raise ValueError(f"unknown epilogue {mode}")
 
 
+def matmul_int4(a: torch.Tensor, w, out: torch.Tensor, mode: int) -> None:
+    """out (op)= a @ w.T with the epilogue ``mode`` and a weight in 4 bits (``ops_int4.Int4Weight``): few tokens read the codes themselves;
+    more take the product of the compute type on the values read back, which are then rounded to it (a step of many tokens is bound
+    by arithmetic: 8 us for the values of 4,096 x 4,096, of a product of some 60 for 2,048 tokens)."""
+    from .. import ops_int4
+    if a.shape[0] <= ops_int4.MAX_TOKENS:
+        ops_int4.matmul(a, w, out, mode)
+    else:
+        matmul_nt(a, w.dequantize(torch.empty((w.rows, w.width), dtype=a.dtype, device=a.device)), out, mode)
+
+
 class Linear(Part):
     def __init__(self, in_features: int, out_features: Sequence[int], names: Sequence[str], init: str = "linear",
                  bias_names: Optional[Sequence[Optional[str]]] = None, pad_rows_to: int = 1,
-                 row_order: Optional[Sequence[Tuple[int, int]]] = None):
+                 row_order: Optional[Sequence[Tuple[int, int]]] = None, quantizable: bool = False, gated: bool = False):
         """``bias_names``: per stored tensor the name of its bias, or None for a tensor without one (a part of
         the concatenation without a bias gets zeros).  ``pad_rows_to``: rows of zeros are appended until the row
         count is a multiple of this, so that the output's row stride keeps an alignment (``padded_out``).
         ``row_order``: (start, stop) ranges of the stored rows in the order in which they are held, where the output's
-        columns are wanted in another order than the checkpoint's."""
+        columns are wanted in another order than the checkpoint's.  ``quantizable``: whoever owns this product reads its weight through
+        :meth:`forward` only, so that it may be held in 4 bits (``int4_group``); ``gated``: its epilogue is a gated activation."""
         if len(out_features) != len(names):
             raise ValueError("one name per stored tensor")
         if bias_names is not None and len(bias_names) != len(names):
@@ -96,6 +108,10 @@ class Linear(Part):
         self.row_order = [(int(a), int(b)) for a, b in row_order] if row_order is not None else None
         if self.row_order is not None and sorted(i for a, b in self.row_order for i in range(a, b)) != list(range(sum(self.out_features))):
             raise ValueError("the row order must name every row once")
+        self.quantizable, self.gated = bool(quantizable), bool(gated)
+        #: set before the weights are loaded: they are held in 4 bits, a step and a minimum for each group of so many columns
+        self.int4_group: Optional[int] = None
+        self.int4 = None                                 # ops_int4.Int4Weight, in the place of ``weight``
         self.weight: Optional[torch.Tensor] = None
         self.bias: Optional[torch.Tensor] = None         # float32 [padded_out], or None
 
@@ -123,6 +139,9 @@ class Linear(Part):
         if pad:
             parts.append(torch.zeros((pad, self.in_features), dtype=dtype, device=device))
         self.weight = parts[0] if len(parts) == 1 else torch.cat(parts, dim=0).contiguous()
+        if self.int4_group is not None:
+            from ..ops_int4 import Int4Weight
+            self.int4, self.weight = Int4Weight.quantize(self.weight, self.int4_group, self.gated), None
         if self.bias_names is not None:
             bias = [get(b).to(device).to(torch.float32) if b else torch.zeros(o, dtype=torch.float32, device=device)
                     for b, o in zip(self.bias_names, self.out_features)]
@@ -136,7 +155,10 @@ class Linear(Part):
     def forward(self, a: torch.Tensor, out: torch.Tensor, mode: int = STORE, add_bias: bool = True, glu=None) -> None:
         """``add_bias=False``: the caller adds ``self.bias`` itself (in a kernel that touches the output anyway).  ``glu``: with
         the clamped gated epilogue, its limit, factor and bias."""
-        matmul_nt(a, self.weight, out, mode, glu=glu, weights_ready=True)
+        if self.int4 is not None:
+            matmul_int4(a, self.int4, out, mode)
+        else:
+            matmul_nt(a, self.weight, out, mode, glu=glu, weights_ready=True)
         if mode == CLAMPGLU:
             return
         if add_bias and self.bias is not None and a.shape[0] > 0:

@@ -36,8 +36,9 @@ class GatedMLP(FeedForward):
         self.limit, self.alpha = float(limit), float(alpha)
         gate, up, down = names
         biases = [f"{prefix}.{b}" for b in bias_names] if bias_names is not None else [None] * 3
-        self.gate_up = Linear(hidden, [intermediate, intermediate], [f"{prefix}.{gate}", f"{prefix}.{up}"], bias_names=biases[:2])
-        self.down = Linear(intermediate, [hidden], [f"{prefix}.{down}"], bias_names=biases[2:])
+        self.gate_up = Linear(hidden, [intermediate, intermediate], [f"{prefix}.{gate}", f"{prefix}.{up}"], bias_names=biases[:2],
+                              quantizable=activation != "clamped", gated=True)
+        self.down = Linear(intermediate, [hidden], [f"{prefix}.{down}"], bias_names=biases[2:], quantizable=True)
 
     def children(self) -> List[Part]:
         return [self.gate_up, self.down]
@@ -65,8 +66,8 @@ class DenseMLP(FeedForward):
         self.epilogue = self._ACTS[activation]
         self.hidden, self.intermediate, self.prefix = hidden, intermediate, prefix
         up, down = names
-        self.up = Linear(hidden, [intermediate], [f"{prefix}.{up}"])
-        self.down = Linear(intermediate, [hidden], [f"{prefix}.{down}"])
+        self.up = Linear(hidden, [intermediate], [f"{prefix}.{up}"], quantizable=True)
+        self.down = Linear(intermediate, [hidden], [f"{prefix}.{down}"], quantizable=True)
 
     def children(self) -> List[Part]:
         return [self.up, self.down]
