@@ -618,6 +618,10 @@ int block_rows(int each, int d, int tokens) { return d <= 128 && each * tokens >
 
 }  // namespace
 
+int ce_int4_attention_tc(const void* q, long long q_stride, const void* pages, void* out, const int* seq_slot, const int* q_start, const int* ctx_len,
+                         const int* block_table, int* status, const int* tiles, int n_tiles, int nh, int nkv, int d, int group, int page_size,
+                         int max_pages, int num_pages, int window, float scale, cudaStream_t stream);
+
 // Rows a block takes, and the row blocks of a one-token sequence (tile 0) or of a tile of 64 tokens (tile 1)
 extern "C" int ce_int4_attention_rows(int each, int d, int tile) { return block_rows(each, d, tile ? 64 : 1); }
 extern "C" int ce_int4_attention_blocks(int each, int d, int tile) {
@@ -635,7 +639,7 @@ struct Int4AttentionCall {
     const int *seq_slot, *q_start, *ctx_len, *block_table;
     int* status;
     const int* tiles;              // null: ``n`` one-token sequences
-    long long n, nh, nkv, d, group, page_size, max_pages, num_pages, window, splits, share;     // without part_o the splits (8 at most) are a cluster
+    long long n, nh, nkv, d, group, page_size, max_pages, num_pages, window, splits, share;     // without part_o the splits (8 at most) are a cluster; 0: the kernel on tcgen05
     float *part_o, *part_ml;
     double scale;
     void* stream;
@@ -659,11 +663,16 @@ extern "C" int ce_int4_attention(const Int4AttentionCall* c) {
     if (group != 32 && group != 64) return ce_fail(CE_ERR_SIZE, "int4_attention: group %d (32 or 64)", group);
     if (page_size < 16 || page_size % 16) return ce_fail(CE_ERR_SIZE, "int4_attention: page size %d is not a multiple of 16", page_size);
     if (((uintptr_t)pages & 15) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: the pages do not start on a 16-byte boundary");
-    if (max_pages < 1 || num_pages < 1 || splits < 1 || window < 0) return ce_fail(CE_ERR_SIZE, "int4_attention: bad sizes");
+    if (max_pages < 1 || num_pages < 1 || splits < 0 || window < 0) return ce_fail(CE_ERR_SIZE, "int4_attention: bad sizes");
     if (((uintptr_t)out % (dtype == CE_F32 ? 16 : 8)) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: out does not start on a boundary of four elements");
     if (splits > 8 && (!part_o || !part_ml)) return ce_fail(CE_ERR_ARG, "int4_attention: more than 8 shares of the keys need scratch memory");
     if (!(c->scale > 0.0)) return ce_fail(CE_ERR_ARG, "int4_attention: a scale that is not positive");
     if (count == 0) return CE_OK;
+    if (splits == 0) {
+        if (dtype != CE_BF16 || !tiles || count < 0 || count > 65535) return ce_fail(CE_ERR_SIZE, "int4_attention: splits of 0 are for tiles of bfloat16");
+        return ce_int4_attention_tc(q, q_stride, pages, out, seq_slot, q_start, ctx_len, block_table, status, tiles, (int)count, nh, nkv, d, group, page_size,
+                                    max_pages, num_pages, window, scale, (cudaStream_t)stream);
+    }
     const int each = nh / nkv, rows = block_rows(each, d, tiles ? 64 : 1), subs = ((tiles ? 64 : 1) * each + rows - 1) / rows;
     const long long jobs = count * nkv * subs;
     if (count < 0 || jobs * splits * 16 > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_attention: too many rows");

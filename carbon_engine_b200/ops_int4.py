@@ -43,6 +43,8 @@ kernel_lib.declare("ce_int4_dequantise_weight", _i, [_i, _p, _ll, _p, _i, _i, _i
 # each, d, tile
 kernel_lib.declare("ce_int4_attention_rows", _i, [_i] * 3)
 kernel_lib.declare("ce_int4_attention_blocks", _i, [_i] * 3)
+# each, d
+kernel_lib.declare("ce_int4_attention_tc_blocks", _i, [_i] * 2)
 # dtype, M, K, group
 kernel_lib.declare("ce_int4_gemm_scratch", _ll, [_i] * 4)
 
@@ -188,16 +190,32 @@ def _joined(jobs: int, splits: int) -> bool:
     return splits > 8 or (splits > 1 and jobs * splits > 296)
 
 
+#: row blocks from which a portion goes to the tcgen05 kernel, which does not share keys among blocks
+TENSOR_BLOCKS = 32
+
+
+@functools.lru_cache(maxsize=256)
+def _row_blocks(each: int, d: int, tile: int):
+    """Blocks a KV head takes of a sequence's token (tile 0) or of a tile of 64 tokens (1), their rows, and blocks of the tcgen05 kernel."""
+    k = kernels()
+    return k.ce_int4_attention_blocks(each, d, tile), k.ce_int4_attention_rows(each, d, tile), k.ce_int4_attention_tc_blocks(each, d) if tile else 0
+
+
 def _attend(device, code, q, q_stride, heads, pages, out, seq_slot, q_start, ctx_len, block_table, status, tiles, count, max_ctx, window, scale) -> None:
     k = kernels()
     each = heads // pages.kv_heads
     tile = 0 if tiles is None else 1
-    jobs = count * pages.kv_heads * k.ce_int4_attention_blocks(each, pages.head_dim, tile)
+    blocks, block_rows, tensor_blocks = _row_blocks(each, pages.head_dim, tile)
+    jobs = count * pages.kv_heads * blocks
     keys = min(max_ctx, window + (64 if tile else 1) + 15) if window > 0 else max_ctx
-    splits, share = _splits(jobs, max(1, (keys + 15) // 16))
+    if (code == ops.BF16 and tensor_blocks * count * pages.kv_heads >= TENSOR_BLOCKS and count <= 65535 and q_stride % 8 == 0
+            and (q.data_ptr() | out.data_ptr()) % 16 == 0):
+        splits = share = 0
+    else:
+        splits, share = _splits(jobs, max(1, (keys + 15) // 16))
     part_o = part_ml = None
     if _joined(jobs, splits):
-        rows = jobs * splits * k.ce_int4_attention_rows(each, pages.head_dim, tile)
+        rows = jobs * splits * block_rows
         part_o = torch.empty(rows * (pages.head_dim + 2), dtype=torch.float32, device=q.device)
         part_ml = part_o.data_ptr() + 4 * rows * pages.head_dim
     ops._ok(k.ce_int4_attention(_ATTENTION(

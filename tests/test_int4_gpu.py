@@ -214,6 +214,57 @@ def test_attention_of_portions(dtype, d, heads, kv_heads, group, page, new, leng
     attend(c, normal((sum(new), heads, d), 9, dtype), k, v, new, lengths, group, window, dtype)
 
 
+@pytest.mark.parametrize("d,heads,kv_heads,group,page,new,lengths,window", [c for c in PORTIONS if c[0] <= 128] + [
+    (128, 4, 1, 32, 16, [64, 1, 200], [64, 700, 260], 0), (64, 4, 4, 64, 32, [129, 70], [129, 1000], 0), (128, 32, 8, 64, 64, [100], [1500], 0),
+    (128, 8, 2, 32, 16, [90], [600], 100), (128, 8, 2, 64, 16, [70], [71], 1), (64, 12, 1, 32, 16, [200], [333], 64), (128, 5, 1, 64, 16, [3], [64], 0)])
+def test_attention_of_portions_on_tcgen05(monkeypatch, d, heads, kv_heads, group, page, new, lengths, window):
+    """The kernel that takes portions of many row blocks, at any number of them."""
+    from carbon_engine_b200 import ops, ops_int4
+    monkeypatch.setattr(ops_int4, "TENSOR_BLOCKS", 1)
+    c, k, v = filled(lengths, kv_heads, d, group, page, BF16)
+    q = normal((sum(new), heads, d), 9, BF16)
+    before = ops.kernel_counts().get("int4_attention_tc_kernel", 0)
+    attend(c, q, k, v, new, lengths, group, window, BF16, n_decode=0)
+    assert ops.kernel_counts()["int4_attention_tc_kernel"] == before + 1
+
+
+def test_portions_on_tcgen05_with_numbers_that_are_none(monkeypatch):
+    from carbon_engine_b200 import ops_int4
+    monkeypatch.setattr(ops_int4, "TENSOR_BLOCKS", 1)
+    for which in ("k", "v", "window"):
+        lengths, new = [150], [140]
+        c = Cache(lengths, 1, 128, 32, 16)
+        k, v = normal((150, 1, 128), 1, BF16), normal((150, 1, 128), 2, BF16)
+        (k if which == "k" else v)[80, 0, 40] = math.nan
+        c.write(k, v)
+        window = 30 if which == "window" else 0
+        out = attend(c, normal((140, 4, 128), 9, BF16), k, v, new, lengths, 32, window, BF16, n_decode=0)
+        seen = out.isnan()
+        last = 80 + 29 - 10 if window else 139
+        assert not bool(seen[:70].any()) and not bool(seen[last + 1:].any())
+        assert bool(seen[70:last + 1].all()) if which == "k" else bool(seen[70:last + 1, :, 32:64].all()) and int(seen.sum()) == (last - 69) * 4 * 32
+    c, k, v = filled([100], 1, 64, 32, 16, BF16)
+    q, out = normal((80, 4, 64), 9, BF16), torch.empty((80, 4, 64), dtype=BF16, device="cuda")
+    q[17, 2, 5], q[40, 0, 0] = math.inf, math.nan
+    c.ops.attention(q, c.pages, out, c.slots, gpu([0, 80]), gpu([100]), c.table, c.status, n_decode=0, max_ctx=100, tiles=gpu([[0, 0], [0, 64]]), scale=0.1)
+    assert bool(out[17, 2].isnan().all()) and bool(out[40, 0].isnan().all()) and int(out.isnan().sum()) == 128
+    # a sequence whose length says that its tokens are not there: rows that see nothing are zeros
+    c.ops.attention(q, c.pages, out, c.slots, gpu([0, 80]), gpu([0]), c.table, c.status, n_decode=0, max_ctx=100, tiles=gpu([[0, 0], [0, 64]]), scale=0.1)
+    assert bool((out == 0).all()) and int(c.status) == 0
+
+
+def test_portions_on_tcgen05_with_scores_far_apart(monkeypatch):
+    from carbon_engine_b200 import ops_int4
+    monkeypatch.setattr(ops_int4, "TENSOR_BLOCKS", 1)
+    for spread in (3.0, 30.0):
+        c = Cache([400], 1, 128, 32, 16)
+        k = normal((400, 1, 128), 1, F32, spread / 11.3)
+        v = normal((400, 1, 128), 2, F32) * torch.logspace(-2, 2, 400, device="cuda")[:, None, None]
+        c.write(k, v)
+        for size in (1.0, 1e-4):
+            attend(c, normal((100, 4, 128), 20, BF16, size), k, v, [100], [400], 32, 0, BF16, n_decode=0)
+
+
 def test_one_token_as_a_portion_is_that_token():
     c, k, v = filled([100, 37], 2, 128, 64, 16, BF16)
     q = normal((2, 8, 128), 9, BF16)
