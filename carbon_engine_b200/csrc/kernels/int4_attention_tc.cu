@@ -3,8 +3,13 @@
 //
 // A block takes up to 256 rows - tokens by the heads that share a KV head, of a tile of 64 tokens - as two products of 128 rows, and all keys
 // they see, 64 at a time.  Four warps bring the keys' and values' codes in from the pages (bulk copies, three tiles of 16 keys a warp on the way)
-// and write them, as float16 values, into the operands' shared tiles; one thread issues the products; eight warps hold a row each for the softmax.  Values of 64 keys serve 256 rows, so that
-// the work of making them (14 instructions for 8 values) stays below the softmax's (some 7 for a score), which is what bounds the kernel.
+// and write them, as float16 values, into the operands' shared tiles; a thread for each 128 rows issues their products; eight warps hold a row a
+// thread for the softmax.  Values of 64 keys serve 256 rows, so that the work of making them (14 instructions for 8 values) stays below the
+// softmax's (some 7 for a score).
+// Tensor memory holds two tiles of scores for each 128 rows and their outputs.  A tile's probabilities take the place of its scores, as the
+// first operand of P V: the products of tile j + 1's scores run while tile j's softmax does, and neither waits for P V of the tile before.  (With
+// one tile of scores, P in shared memory and one issuing thread, a tile of 64 keys took 2.27 us, of which 1.3 were hand-overs that stayed
+// with all work left out.)
 //
 // Roundings: c s + z to float16 once (2^-12 of itself; the codes are exact); a query row brought into [2^14, 2^15) by a power of two is exact in
 // float16 down to 2^-30 of its largest; a probability is kept as 2^(S - m) with m six below the running maximum, so that float16 holds it to
@@ -21,8 +26,8 @@
 
 namespace {
 
-constexpr int BN = 64, STAGES = 2, RAW = 3;      // RAW: tiles of codes a making warp has on the way
-constexpr int MAKERS = 4, SOFTMAX = 8, THREADS = 32 * (1 + MAKERS + SOFTMAX);
+constexpr int BN = 64, STAGES = 3, RAW = 3;      // RAW: tiles of codes a making warp has on the way
+constexpr int MAKERS = 4, SOFTMAX = 8, THREADS = 32 * (2 + MAKERS + SOFTMAX);
 constexpr uint32_t SPIN_LIMIT = 1u << 16;
 constexpr float LIFT = 6.0f, HEADROOM = 8.0f;
 
@@ -68,6 +73,11 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, ui
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
                  ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
+// the same with the first operand in tensor memory
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(i4_smem(bar)) : "memory");
 }
@@ -89,18 +99,13 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
                  "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(taddr), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
-                   "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])),
-                   "r"(__float_as_uint(v[7])), "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])),
-                   "r"(__float_as_uint(v[11])), "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])),
-                   "r"(__float_as_uint(v[15])), "r"(__float_as_uint(v[16])), "r"(__float_as_uint(v[17])), "r"(__float_as_uint(v[18])),
-                   "r"(__float_as_uint(v[19])), "r"(__float_as_uint(v[20])), "r"(__float_as_uint(v[21])), "r"(__float_as_uint(v[22])),
-                   "r"(__float_as_uint(v[23])), "r"(__float_as_uint(v[24])), "r"(__float_as_uint(v[25])), "r"(__float_as_uint(v[26])),
-                   "r"(__float_as_uint(v[27])), "r"(__float_as_uint(v[28])), "r"(__float_as_uint(v[29])), "r"(__float_as_uint(v[30])),
-                   "r"(__float_as_uint(v[31]))
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+                   "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+                   "r"(v[30]), "r"(v[31])
                  : "memory");
 }
 
@@ -125,12 +130,12 @@ __device__ __forceinline__ uint4 values_of(uint32_t w, uint32_t s2, uint32_t z2)
 template <int D, int G>
 struct Shape {
     static constexpr int NB = D / 64;
-    static constexpr uint32_t Q_BYTES = 128 * D * 2, KV_BYTES = BN * D * 2, P_BYTES = 128 * BN * 2;       // of one product's rows, of K or V, of one P
-    static constexpr uint32_t Q = 0, KV = 2 * Q_BYTES, P = KV + STAGES * 2 * KV_BYTES, NAN_KEYS = P + 2 * P_BYTES;
+    static constexpr uint32_t Q_BYTES = 128 * D * 2, KV_BYTES = BN * D * 2;       // of 128 rows, of a tile of K or V
+    static constexpr uint32_t Q = 0, KV = 2 * Q_BYTES, NAN_KEYS = KV + STAGES * 2 * KV_BYTES;
     static constexpr uint32_t CODES = NAN_KEYS + STAGES * 8 * 4 * 2;                                      // (NAN_KEYS: [stage][group][maker] 16 bits)
     static constexpr uint32_t BARS = CODES + MAKERS * RAW * i4_cache_tile_bytes(D, G);
-    static constexpr uint32_t BYTES = BARS + 8 * (20 + MAKERS * RAW);
-    static constexpr uint32_t TMEM = D == 128 ? 512 : 256;
+    static constexpr uint32_t BYTES = BARS + 8 * (24 + 4 * STAGES + MAKERS * RAW);
+    static constexpr uint32_t TMEM = 512;      // scores: 64 columns of tile j of half m at 128 m + 64 (j % 2); outputs from 256 on
 };
 
 template <int D, int G>
@@ -140,10 +145,10 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
     extern __shared__ __align__(1024) unsigned char sm[];
     const uint32_t base = i4_smem(sm);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::BARS);
-    uint64_t &q_full = bars[0], *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7;
-    uint64_t *s_full = bars + 9, *s_free = bars + 11, *p_full = bars + 13, *pv_done = bars + 15;
-    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 17);
-    uint64_t* raw_full = bars + 18;                     // [maker][RAW]
+    uint64_t &q_full = bars[0], *pv_done = bars + 1, *s_full = bars + 3, *p_full = bars + 7;        // s_full, p_full: [half][tile % 2]
+    uint64_t *k_full = bars + 11, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
+    uint64_t* raw_full = v_empty + STAGES;              // [maker][RAW]
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(raw_full + MAKERS * RAW);
     unsigned short* nan_keys = reinterpret_cast<unsigned short*>(sm + S::NAN_KEYS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     ce_pdl_wait();
@@ -169,9 +174,10 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
     }
     if (threadIdx.x == 0) {
         mbar_init(&q_full, SOFTMAX);
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&k_full[s], MAKERS); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], MAKERS); mbar_init(&v_empty[s], 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&k_full[s], MAKERS); mbar_init(&k_empty[s], mts); mbar_init(&v_full[s], MAKERS); mbar_init(&v_empty[s], mts); }
         for (int i = 0; i < MAKERS * RAW; ++i) mbar_init(&raw_full[i], 1);
-        for (int m = 0; m < 2; ++m) { mbar_init(&s_full[m], 1); mbar_init(&s_free[m], 4); mbar_init(&p_full[m], 4); mbar_init(&pv_done[m], 1); }
+        for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+        mbar_init(&pv_done[0], 1); mbar_init(&pv_done[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -184,57 +190,56 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
     ce_pdl_launch_dependents();
     const uint32_t tmem = tmem_slot;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            // ---- the products: S(j) of both halves as soon as their S is free, then O += P(j - 1) V(j - 1)
+    if (warp < 2) {
+        const int m = warp;
+        if (lane == 0 && m < mts) {
+            // ---- the products of 128 rows: S(0) and S(1), then O += P(j) V(j) and S(j + 2), which takes the place of P(j)
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | (8u << 24);
             const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+            const uint32_t tmem_s = tmem + m * 128, tmem_o = tmem + 256 + m * D, q_addr = base + S::Q + m * S::Q_BYTES;
             int where = 62;
             bool ok = mbar_wait(&q_full, 0);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int j = 0; j <= n_kv && ok; ++j) {
-                if (j < n_kv) {
-                    const int s = j % STAGES;
-                    where = 63;
-                    ok = mbar_wait(&k_full[s], (j / STAGES) & 1);
-                    const uint32_t k_addr = base + S::KV + s * 2 * S::KV_BYTES;
-                    for (int m = 0; m < mts && ok; ++m) {
-                        if (j > 0) { where = 64; ok = mbar_wait(&s_free[m], (j - 1) & 1); }
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            auto scores = [&](int j) {
+                const int s = j % STAGES;
+                where = 63;
+                ok = mbar_wait(&k_full[s], (j / STAGES) & 1);
+                if (!ok) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t k_addr = base + S::KV + s * 2 * S::KV_BYTES;
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk)
-                            umma(tmem + m * BN, desc_kmajor(base + S::Q + m * S::Q_BYTES + (kk / 4) * 16384 + (kk % 4) * 32),
-                                 desc_kmajor(k_addr + (kk / 4) * 8192 + (kk % 4) * 32), idesc_s, kk > 0 ? 1u : 0u);
-                        if (m == mts - 1) umma_commit(&k_empty[s]);
-                        umma_commit(&s_full[m]);
-                    }
-                    if (!ok) break;
-                }
-                if (j > 0) {
-                    const int jp = j - 1, s = jp % STAGES;
-                    where = 65;
-                    ok = mbar_wait(&v_full[s], (jp / STAGES) & 1);
-                    const uint32_t v_addr = base + S::KV + s * 2 * S::KV_BYTES + S::KV_BYTES;
-                    for (int m = 0; m < mts && ok; ++m) {
-                        ok = mbar_wait(&p_full[m], jp & 1);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma(tmem_s + (j & 1) * BN, desc_kmajor(q_addr + (kk / 4) * 16384 + (kk % 4) * 32), desc_kmajor(k_addr + (kk / 4) * 8192 + (kk % 4) * 32),
+                         idesc_s, kk > 0 ? 1u : 0u);
+                umma_commit(&s_full[2 * m + (j & 1)]);
+                umma_commit(&k_empty[s]);
+            };
+            if (ok) scores(0);
+            if (ok && n_kv > 1) scores(1);
+            for (int j = 0; j < n_kv && ok; ++j) {
+                const int s = j % STAGES;
+                where = 65;
+                ok = mbar_wait(&v_full[s], (j / STAGES) & 1) && mbar_wait(&p_full[2 * m + (j & 1)], (j >> 1) & 1);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t v_addr = base + S::KV + s * 2 * S::KV_BYTES + S::KV_BYTES;
 #pragma unroll
-                        for (int kk = 0; kk < BN / 16; ++kk)
-                            umma(tmem + 2 * BN + m * D, desc_kmajor(base + S::P + m * S::P_BYTES + kk * 32), desc_mnmajor(v_addr + kk * 16 * 128, 8192),
-                                 idesc_pv, (jp > 0 || kk > 0) ? 1u : 0u);
-                        if (m == mts - 1) umma_commit(&v_empty[s]);
-                        umma_commit(&pv_done[m]);
-                    }
+                for (int kk = 0; kk < BN / 16; ++kk)
+                    umma_ts(tmem_o, tmem_s + (j & 1) * BN + kk * 8, desc_mnmajor(v_addr + kk * 16 * 128, 8192), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+                umma_commit(&pv_done[m]);
+                umma_commit(&v_empty[s]);
+                if (j + 2 < n_kv) {
+                    // (products of different shapes are not promised to run in order: P(j) has been read before its place is written again)
+                    where = 64;
+                    ok = mbar_wait(&pv_done[m], j & 1);
+                    if (ok) scores(j + 2);
                 }
             }
             if (!ok) atomicCAS(a.status, 0, where);
         }
         __syncwarp();
-    } else if (warp <= MAKERS) {
+    } else if (warp < 2 + MAKERS) {
         // ---- keys and values of 16 of every 64 keys
-        const int maker = warp - 1, r = lane >> 2, l = lane & 3, per_page = a.page_size >> 4;
+        const int maker = warp - 2, r = lane >> 2, l = lane & 3, per_page = a.page_size >> 4;
         unsigned char* raw = sm + S::CODES + maker * RAW * TILE;
         uint64_t* raw_bars = raw_full + maker * RAW;
         auto first_key = [&](int j) { return k_begin + j * BN + maker * 16; };
@@ -352,7 +357,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
         }
     } else {
         // ---- softmax: a row a thread
-        const int m = (warp - 1 - MAKERS) >> 2, quad = warp & 3, row = quad * 32 + lane, rr = m * 128 + row;
+        const int m = (warp - 2 - MAKERS) >> 2, quad = warp & 3, row = quad * 32 + lane, rr = m * 128 + row;
         const bool valid = rr < rows;
         const int rho = row0 + rr, tok = rho / each, pos = valid ? pos0 + tok : -1;
         const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
@@ -391,7 +396,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             if (lane == 0) mbar_arrive(&q_full);
         }
         if (m < mts) {
-            const uint32_t lane_base = (uint32_t)(quad * 32) << 16, tmem_s = tmem + m * BN + lane_base, tmem_o = tmem + 2 * BN + m * D + lane_base;
+            const uint32_t lane_base = (uint32_t)(quad * 32) << 16, tmem_s = tmem + m * 128 + lane_base, tmem_o = tmem + 256 + m * D + lane_base;
             float m_run = -INFINITY, l_run = 0.f;
             uint32_t nan_groups = 0;
             bool ok = true;
@@ -399,13 +404,10 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             for (int j = 0; j < n_kv; ++j) {
                 const int k0 = k_begin + j * BN;
                 where = 66;
-                if (!warp_wait(&s_full[m], j & 1)) { ok = false; break; }
+                if (!warp_wait(&s_full[2 * m + (j & 1)], (j >> 1) & 1)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float sv[BN];
-                tmem_ld<BN>(tmem_s, sv);
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_free[m]);
+                tmem_ld<BN>(tmem_s + (j & 1) * BN, sv);
                 const bool full = k0 >= lo && k0 + BN - 1 <= pos;
                 if (!full) {
 #pragma unroll
@@ -435,27 +437,24 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                 }
                 l_run = l_run * alpha + (sum2.x + sum2.y);
                 m_run = m_new;
-                if (j > 0) {
+                // the probabilities, where the scores were: two keys a column
+                tmem_st32(tmem_s + (j & 1) * BN, packed);
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                    // (the product of tile j - 2 is done: this tile's scores were issued behind it)
                     where = 67;
                     if (!warp_wait(&pv_done[m], (j - 1) & 1)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (__any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            float o[32];
-                            tmem_ld<32>(tmem_o + c, o);
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        uint32_t back[32];
+                        tmem_ld<32>(tmem_o + c, o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] *= alpha;
-                            tmem_st32(tmem_o + c, o);
-                        }
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        for (int i = 0; i < 32; ++i) back[i] = __float_as_uint(o[i] * alpha);
+                        tmem_st32(tmem_o + c, back);
                     }
                 }
-                unsigned char* prow = sm + S::P + m * S::P_BYTES + row * 128;
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    *reinterpret_cast<uint4*>(prow + ((c ^ (row & 7)) << 4)) =
-                        make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 // values that are no numbers among this tile's keys
                 where = 68;
                 const int s = j % STAGES;
@@ -473,14 +472,14 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                     for (int g = 0; g < NG; ++g)
                         if (bad[g] & seen) nan_groups |= 1u << g;
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[m]);
+                if (lane == 0) mbar_arrive(&p_full[2 * m + (j & 1)]);
             }
             if (ok) {
                 where = 67;
-                ok = warp_wait(&pv_done[m], (n_kv - 1) & 1);
+                // the last two products may both be under way, and a parity tells one from the next only
+                ok = (n_kv < 2 || warp_wait(&pv_done[m], (n_kv - 2) & 1)) && warp_wait(&pv_done[m], (n_kv - 1) & 1);
             }
             if (!ok && lane == 0) atomicCAS(a.status, 0, where);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
