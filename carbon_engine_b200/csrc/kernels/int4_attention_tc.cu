@@ -2,7 +2,7 @@
 // O += P V are tcgen05.mma instructions (float16 operands, float32 sums in tensor memory).
 //
 // A block takes up to 256 rows - tokens by the heads that share a KV head, of a tile of 64 tokens - as two products of 128 rows, and all keys
-// they see, 64 at a time.  Four warps bring the keys' and values' codes in from the pages (bulk copies, three tiles of 16 keys a warp on the way)
+// they see, 64 at a time.  Six warps bring the keys' and values' codes in from the pages (bulk copies, three tiles of 16 keys a warp on the way)
 // and write them, as float16 values, into the operands' shared tiles; a thread for each 128 rows issues their products; eight warps hold a row a
 // thread for the softmax.  Values of 64 keys serve 256 rows, so that the work of making them (14 instructions for 8 values) stays below the
 // softmax's (some 7 for a score).
@@ -27,7 +27,7 @@
 namespace {
 
 constexpr int BN = 64, STAGES = 3, RAW = 3;      // RAW: tiles of codes a making warp has on the way
-constexpr int MAKERS = 4, SOFTMAX = 8, THREADS = 32 * (2 + MAKERS + SOFTMAX);
+constexpr int MAKERS = 6, SOFTMAX = 8, THREADS = 32 * (2 + MAKERS + SOFTMAX);
 constexpr uint32_t SPIN_LIMIT = 1u << 16;
 constexpr float LIFT = 6.0f, HEADROOM = 8.0f;
 
@@ -69,17 +69,19 @@ __device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
 __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr, uint32_t next) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// One lane of a whole warp issues (always the same one): descriptors stay in registers that a warp shares.
 __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+    asm volatile("{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
                  ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
 // the same with the first operand in tensor memory
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+    asm volatile("{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
                  ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(i4_smem(bar)) : "memory");
+    asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
+                 ::"r"(i4_smem(bar)) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* q) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -127,12 +129,20 @@ __device__ __forceinline__ uint4 values_of(uint32_t w, uint32_t s2, uint32_t z2)
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
+// (s, z) of one token's groups as they lie: N words
+template <int N>
+__device__ __forceinline__ void load_steps(const unsigned char* p, uint32_t (&v)[N]) {
+    if constexpr (N == 1) v[0] = *reinterpret_cast<const uint32_t*>(p);
+    else if constexpr (N == 2) { const uint2 x = *reinterpret_cast<const uint2*>(p); v[0] = x.x; v[1] = x.y; }
+    else { const uint4 x = *reinterpret_cast<const uint4*>(p); v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
+}
+
 template <int D, int G>
 struct Shape {
     static constexpr int NB = D / 64;
     static constexpr uint32_t Q_BYTES = 128 * D * 2, KV_BYTES = BN * D * 2;       // of 128 rows, of a tile of K or V
     static constexpr uint32_t Q = 0, KV = 2 * Q_BYTES, NAN_KEYS = KV + STAGES * 2 * KV_BYTES;
-    static constexpr uint32_t CODES = NAN_KEYS + STAGES * 8 * 4 * 2;                                      // (NAN_KEYS: [stage][group][maker] 16 bits)
+    static constexpr uint32_t CODES = NAN_KEYS + STAGES * 8 * 4 * 2;                                      // (NAN_KEYS: [stage][group][16 keys] 16 bits)
     static constexpr uint32_t BARS = CODES + MAKERS * RAW * i4_cache_tile_bytes(D, G);
     static constexpr uint32_t BYTES = BARS + 8 * (24 + 4 * STAGES + MAKERS * RAW);
     static constexpr uint32_t TMEM = 512;      // scores: 64 columns of tile j of half m at 128 m + 64 (j % 2); outputs from 256 on
@@ -174,7 +184,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
     }
     if (threadIdx.x == 0) {
         mbar_init(&q_full, SOFTMAX);
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&k_full[s], MAKERS); mbar_init(&k_empty[s], mts); mbar_init(&v_full[s], MAKERS); mbar_init(&v_empty[s], mts); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], mts); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], mts); }
         for (int i = 0; i < MAKERS * RAW; ++i) mbar_init(&raw_full[i], 1);
         for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
         mbar_init(&pv_done[0], 1); mbar_init(&pv_done[1], 1);
@@ -192,17 +202,17 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
 
     if (warp < 2) {
         const int m = warp;
-        if (lane == 0 && m < mts) {
+        if (m < mts) {
             // ---- the products of 128 rows: S(0) and S(1), then O += P(j) V(j) and S(j + 2), which takes the place of P(j)
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | (8u << 24);
             const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
             const uint32_t tmem_s = tmem + m * 128, tmem_o = tmem + 256 + m * D, q_addr = base + S::Q + m * S::Q_BYTES;
             int where = 62;
-            bool ok = mbar_wait(&q_full, 0);
+            bool ok = warp_wait(&q_full, 0);
             auto scores = [&](int j) {
                 const int s = j % STAGES;
                 where = 63;
-                ok = mbar_wait(&k_full[s], (j / STAGES) & 1);
+                ok = warp_wait(&k_full[s], (j / STAGES) & 1);
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t k_addr = base + S::KV + s * 2 * S::KV_BYTES;
@@ -218,7 +228,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             for (int j = 0; j < n_kv && ok; ++j) {
                 const int s = j % STAGES;
                 where = 65;
-                ok = mbar_wait(&v_full[s], (j / STAGES) & 1) && mbar_wait(&p_full[2 * m + (j & 1)], (j >> 1) & 1);
+                ok = warp_wait(&v_full[s], (j / STAGES) & 1) && warp_wait(&p_full[2 * m + (j & 1)], (j >> 1) & 1);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t v_addr = base + S::KV + s * 2 * S::KV_BYTES + S::KV_BYTES;
@@ -230,83 +240,78 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                 if (j + 2 < n_kv) {
                     // (products of different shapes are not promised to run in order: P(j) has been read before its place is written again)
                     where = 64;
-                    ok = mbar_wait(&pv_done[m], j & 1);
+                    ok = warp_wait(&pv_done[m], j & 1);
                     if (ok) scores(j + 2);
                 }
             }
-            if (!ok) atomicCAS(a.status, 0, where);
+            if (!ok && lane == 0) atomicCAS(a.status, 0, where);
         }
         __syncwarp();
     } else if (warp < 2 + MAKERS) {
-        // ---- keys and values of 16 of every 64 keys
-        const int maker = warp - 2, r = lane >> 2, l = lane & 3, per_page = a.page_size >> 4;
+        // ---- the tiles of 16 keys, four to every 64, dealt out to the warps in turn: a tile's keys, then its values
+        const int maker = warp - 2, r = lane >> 2, l = lane & 3, per_page = a.page_size >> 4, runs = 4 * n_kv;
         unsigned char* raw = sm + S::CODES + maker * RAW * TILE;
         uint64_t* raw_bars = raw_full + maker * RAW;
-        auto first_key = [&](int j) { return k_begin + j * BN + maker * 16; };
-        auto needed = [&](int j) { return j < n_kv && first_key(j) <= p_last && first_key(j) + 15 >= block_lo; };
+        auto run_of = [&](int i) { return maker + i * MAKERS; };
+        auto first_key = [&](int run) { return k_begin + run * 16; };
+        auto needed = [&](int run) { return run < runs && first_key(run) <= p_last && first_key(run) + 15 >= block_lo; };
         // where 32 of the warp's tiles lie, one a lane
         int looked = 0;
         const unsigned char* place = a.pages;
         auto look_up = [&](int from) {
             looked = from;
-            const int j = from + lane, t = first_key(j) >> 4, pi = t / per_page;
-            int page = !needed(j) ? 0 : pi < a.max_pages ? table[pi] : -1;
+            const int run = run_of(from + lane), t = first_key(run) >> 4, pi = t / per_page;
+            int page = !needed(run) ? 0 : pi < a.max_pages ? table[pi] : -1;
             if (page < 0 || page >= a.num_pages) { atomicExch(a.status, 4); page = 0; }      // (the step's results are not used)
             place = a.pages + (((size_t)page * a.nkv + kvh) * per_page + (t - pi * per_page)) * TILE;
         };
-        auto fetch = [&](int j) {
-            if (j >= looked + 32) look_up(j);
-            const unsigned char* src = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(place), j - looked));
-            if (lane == 0 && needed(j)) i4_copy(raw + j % RAW * TILE, src, TILE, &raw_bars[j % RAW]);
+        auto fetch = [&](int i) {
+            if (i >= looked + 32) look_up(i);
+            const unsigned char* src = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(place), i - looked));
+            if (lane == 0 && needed(run_of(i))) i4_copy(raw + i % RAW * TILE, src, TILE, &raw_bars[i % RAW]);
         };
         look_up(0);
-        for (int j = 0; j < RAW; ++j) fetch(j);
-        // the steps of what lies beyond the block's keys are zeros: anything may lie there
-        struct Steps { uint32_t k[2][NG], v[4][NG]; };
+        for (int i = 0; i < RAW; ++i) fetch(i);
         uint32_t phase = 0;                             // of the RAW barriers
         bool ok = true;
-        for (int j = 0; j < n_kv && ok; ++j) {
-            const int s = j % STAGES;
-            unsigned char* k_tile = sm + S::KV + s * 2 * S::KV_BYTES;
-            unsigned char* v_tile = k_tile + S::KV_BYTES;
-            const bool here = needed(j);
-            const int key0 = first_key(j);
-            const unsigned char* tile = raw + j % RAW * TILE;
+        for (int i = 0; run_of(i) < runs; ++i) {
+            const int run = run_of(i), j = run >> 2, s = j % STAGES, key0 = first_key(run), part = run & 3;
+            const bool here = needed(run), cut = !here || key0 < block_lo || key0 + 15 > p_last;
+            const unsigned char* from = raw + i % RAW * TILE;
+            unsigned char* to = sm + S::KV + s * 2 * S::KV_BYTES;
             uint4 kw[NB], vw[NB];
-            Steps st;
+            uint32_t ks[2][NG], vs[4][NG];              // steps of tokens r and r + 8; of the four tokens of this lane's words of values
+            auto token_of = [&](int e) { return 2 * l + (e & 1) + 8 * (e >> 1); };
             if (here) {
-                ok = __all_sync(0xffffffffu, i4_wait(&raw_bars[j % RAW], phase >> (j % RAW) & 1));
-                phase ^= 1u << (j % RAW);
+                ok = __all_sync(0xffffffffu, i4_wait(&raw_bars[i % RAW], phase >> (i % RAW) & 1));
+                phase ^= 1u << (i % RAW);
                 if (!ok) break;
-                const uint32_t* steps = reinterpret_cast<const uint32_t*>(tile + 16 * D);
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    kw[i] = *reinterpret_cast<const uint4*>(tile + i * 512 + lane * 16);
-                    vw[i] = *reinterpret_cast<const uint4*>(tile + 8 * D + i * 512 + lane * 16);
+                for (int nb = 0; nb < NB; ++nb) {
+                    kw[nb] = *reinterpret_cast<const uint4*>(from + nb * 512 + lane * 16);
+                    vw[nb] = *reinterpret_cast<const uint4*>(from + 8 * D + nb * 512 + lane * 16);
                 }
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    st.k[0][g] = steps[r * NG + g];
-                    st.k[1][g] = steps[(r + 8) * NG + g];
+                for (int e = 0; e < 2; ++e) load_steps<NG>(from + 16 * D + (r + 8 * e) * NG * 4, ks[e]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) st.v[i][g] = steps[16 * NG + (2 * l + (i & 1) + 8 * (i >> 1)) * NG + g];
-                }
+                for (int e = 0; e < 4; ++e) load_steps<NG>(from + 16 * D + 64 * NG + token_of(e) * NG * 4, vs[e]);
+            } else {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) kw[nb] = vw[nb] = make_uint4(0, 0, 0, 0);
             }
             __syncwarp();
-            fetch(j + RAW);
-            if (!here || key0 < block_lo || key0 + 15 > p_last) {
+            fetch(i + RAW);
+            if (cut) {                                  // the steps of what lies beyond the block's keys are zeros: anything may lie there
                 auto in = [&](int token) { return here && key0 + token >= block_lo && key0 + token <= p_last; };
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    if (!in(r)) st.k[0][g] = 0;
-                    if (!in(r + 8)) st.k[1][g] = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!in(2 * l + (i & 1) + 8 * (i >> 1))) st.v[i][g] = 0;
+                    for (int e = 0; e < 2; ++e)
+                        if (!in(r + 8 * e)) ks[e][g] = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!in(token_of(e))) vs[e][g] = 0;
                 }
-                if (!here)
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) kw[i] = vw[i] = make_uint4(0, 0, 0, 0);
             }
             if (j >= STAGES) ok = warp_wait(&k_empty[s], (j / STAGES - 1) & 1);
             if (!ok) break;
@@ -314,10 +319,10 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {           // words of tokens r and r + 8, first and second 32 channels
-                    const int half = e >> 1, row = 16 * maker + r + 8 * (e & 1);
+                    const int half = e >> 1, row = 16 * part + r + 8 * (e & 1);
                     const uint32_t word = e == 0 ? kw[nb].x : e == 1 ? kw[nb].y : e == 2 ? kw[nb].z : kw[nb].w;
-                    const uint32_t p = st.k[e & 1][(64 * nb + 32 * half) / G];
-                    *reinterpret_cast<uint4*>(k_tile + nb * 8192 + row * 128 + (((half * 4 + l) ^ (row & 7)) << 4)) =
+                    const uint32_t p = ks[e & 1][(64 * nb + 32 * half) / G];
+                    *reinterpret_cast<uint4*>(to + nb * 8192 + row * 128 + (((half * 4 + l) ^ (row & 7)) << 4)) =
                         values_of(word, __byte_perm(p, p, 0x1010), __byte_perm(p, p, 0x3232));
                 }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -330,20 +335,22 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             for (int g = 0; g < NG; ++g) {
                 uint32_t bad = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (isnan(i4_unpack(st.v[i][g]).x)) { bad |= 1u << (2 * l + (i & 1) + 8 * (i >> 1)); st.v[i][g] = 0; }
-                bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
-                bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
-                if (lane == 0) nan_keys[(s * 8 + g) * 4 + maker] = (unsigned short)bad;
+                for (int e = 0; e < 4; ++e)
+                    if (isnan(i4_unpack(vs[e][g]).x)) { bad |= 1u << token_of(e); vs[e][g] = 0; }
+                if (__any_sync(0xffffffffu, bad)) {
+                    bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
+                    bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
+                }
+                if (lane == 0) nan_keys[(s * 8 + g) * 4 + part] = (unsigned short)bad;
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = 16 * maker + 2 * l + (i & 1) + 8 * (i >> 1);
-                    const uint32_t word = i == 0 ? vw[nb].x : i == 1 ? vw[nb].y : i == 2 ? vw[nb].z : vw[nb].w;
-                    const uint32_t lo = st.v[i][nb * GB], hi = st.v[i][nb * GB + GB - 1];      // a word's halves lie 32 channels apart
-                    *reinterpret_cast<uint4*>(v_tile + nb * 8192 + row * 128 + ((r ^ (row & 7)) << 4)) =
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 16 * part + token_of(e);
+                    const uint32_t word = e == 0 ? vw[nb].x : e == 1 ? vw[nb].y : e == 2 ? vw[nb].z : vw[nb].w;
+                    const uint32_t lo = vs[e][nb * GB], hi = vs[e][nb * GB + GB - 1];      // a word's halves lie 32 channels apart
+                    *reinterpret_cast<uint4*>(to + S::KV_BYTES + nb * 8192 + row * 128 + ((r ^ (row & 7)) << 4)) =
                         values_of(word, __byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
                 }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
