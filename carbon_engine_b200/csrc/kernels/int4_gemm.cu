@@ -4,9 +4,9 @@
 // The codes are the first operand of mma.sync m16n8k16 (16 rows of the weight), 8 tokens the second; a step scales a group's partial sum in
 // float32, a minimum meets the group's sum of x.  No value of W is ever rounded.
 //
-// int4_prepare_kernel lays the tokens out as that second operand once for all blocks: each token is brought into [2^14, 2^15) by a power of
-// two and rounded to float16 (exact for bfloat16 down to 2^-30 of the token's largest; float32 as two pieces, 22 bits), with the groups' sums of
-// what was rounded.
+// Up to 16 tokens run int4_stream_kernel, more bfloat16 ones int4_gemm_tc.cu, more float32 ones int4_gemm_kernel, for which int4_prepare_kernel
+// lays the tokens out as that second operand: each token is brought into [2^14, 2^15) by a power of two and rounded to two float16 pieces
+// (22 bits), with the groups' sums of what was rounded.
 #include "int4.cuh"
 
 namespace {
@@ -569,11 +569,19 @@ cudaError_t launch(const GemmArgs& a, int row_tiles, cudaStream_t stream) {
 }
 template <typename T, int G>
 cudaError_t launch_tiles(const GemmArgs& a, int row_tiles, cudaStream_t stream) {
-    if (a.tiles == 1) return launch<T, G, 1>(a, row_tiles, stream);
+    if (a.tiles == 1) return launch<T, G, 1>(a, row_tiles, stream);       // (K beyond the stream's registers)
     if (a.tiles == 2) return launch<T, G, 2>(a, row_tiles, stream);
     if (a.tiles <= 4) return launch<T, G, 4>(a, row_tiles, stream);
     return launch<T, G, 8>(a, row_tiles, stream);
 }
+
+}  // namespace
+
+long long ce_int4_gemm_tc_scratch(int M, int K, int kept);
+int ce_int4_gemm_tc(const void* x, long long ldx, const void* w, void* out, int ldo, int M, int N, int K, int kept, int mode, float* scratch, int* status,
+                    cudaStream_t stream);
+
+namespace {
 
 // Whether the stream of weights takes these sizes: up to 16 tokens, K within the registers of 8 blocks
 bool streamed(int dtype, int M, int K) {
@@ -586,6 +594,7 @@ bool streamed(int dtype, int M, int K) {
 // float32 words of scratch memory (0: none) for a product of M tokens and K columns
 extern "C" long long ce_int4_gemm_scratch(int dtype, int M, int K, int group) {
     if (streamed(dtype, M, K)) return 0;
+    if (dtype == CE_BF16) return ce_int4_gemm_tc_scratch(M, K, group < 64 ? group : 64);
     const long long tiles = (M + 7) / 8, kblocks = (K + 63) / 64;
     return kblocks * tiles * pieces(dtype) * 256 + kblocks * (64 / (group < 64 ? group : 64)) * tiles * 8 + tiles * 8;
 }
@@ -630,21 +639,17 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
                                                        : launch_stream_tiles<__nv_bfloat16, 64>(a, tiles, (cudaStream_t)stream));
         return code == 1 ? ce_fail(CE_ERR_SIZE, "int4_gemm: no room for clusters on this device") : code;
     }
+    if (dtype == CE_BF16) return ce_int4_gemm_tc(x, ldx, w, out, ldo, M, N, K, kept, mode, scratch, c->status, (cudaStream_t)stream);
     Operand op;
     op.frag = (uint32_t*)scratch;
     op.sums = scratch + (size_t)kblocks * tiles * pieces(dtype) * 256;
     op.back = op.sums + (size_t)kblocks * (64 / kept) * tiles * 8;
     PrepareArgs p{x, ldx, op, M, K, kblocks, kept, vec};
     ce_note("int4_prepare_kernel");
-    cudaError_t e = dtype == CE_F32 ? ce_launch(int4_prepare_kernel<float, 2>, dim3(tiles * 8), dim3(256), 0, (cudaStream_t)stream, p)
-                                    : ce_launch(int4_prepare_kernel<__nv_bfloat16, 1>, dim3(tiles * 8), dim3(256), 0, (cudaStream_t)stream, p);
+    cudaError_t e = ce_launch(int4_prepare_kernel<float, 2>, dim3(tiles * 8), dim3(256), 0, (cudaStream_t)stream, p);
     if (e == cudaSuccess) {
         GemmArgs a{(const unsigned char*)w, op, out, M, N, kblocks, tiles, ldo, mode, gated};
-        if (dtype == CE_F32)
-            e = kept == 32 ? launch_tiles<float, 32>(a, row_tiles, (cudaStream_t)stream) : launch_tiles<float, 64>(a, row_tiles, (cudaStream_t)stream);
-        else
-            e = kept == 32 ? launch_tiles<__nv_bfloat16, 32>(a, row_tiles, (cudaStream_t)stream)
-                           : launch_tiles<__nv_bfloat16, 64>(a, row_tiles, (cudaStream_t)stream);
+        e = kept == 32 ? launch_tiles<float, 32>(a, row_tiles, (cudaStream_t)stream) : launch_tiles<float, 64>(a, row_tiles, (cudaStream_t)stream);
     }
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_gemm: %s", cudaGetErrorString(e)); }
     return ce_check_launch("int4_gemm");

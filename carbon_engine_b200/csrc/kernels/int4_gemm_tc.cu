@@ -1,0 +1,426 @@
+// Products of up to 64 bfloat16 tokens - the stream of weights (int4_gemm.cu) takes up to 16 - with a weight held in 4 bits (int4.cuh) on the 5th-generation tensor cores.
+//
+//   out[t, n] = sum_g (s_ng (x_tg . (c_ng - 8)) + (z_ng + 8 s_ng) sum x_tg)
+//
+// A block takes 128 rows of the weight (8 tiles of 16) and a slice of K; blocks of a cluster share K.  For each group of columns, tcgen05.mma forms
+// the codes' products with all tokens in a piece of tensor memory of its own; four warps (a row a lane) read it back and add it to their
+// sums in float32, times the row's step: no value of W is ever rounded, and what is read back is as much work as the products are.  Four warps
+// turn codes into float16 integers (c - 8, the even ones, 16 (c - 8), the odd: the tokens are laid out to match), one issues the copies of
+// codes and tokens and one the products.  Slices' sums are added in their order through shared memory.
+//
+// The tokens come prepared (int4_tokens_kernel): each brought into [2^14, 2^15) by a power of two and rounded to float16 - exact for bfloat16 down
+// to 2^-30 of the token's largest - as the second operand's image, swizzle included, and the groups' sums behind it.
+#include "int4.cuh"
+
+namespace {
+
+constexpr int ROWS = 128, MAKERS = 4, THREADS = 32 * (2 + 2 * MAKERS);
+constexpr int RUN = 4, RAW = 4, XS = 6, AS = 3, DS = 8;     // blocks of 64 columns a copy of codes; stages of codes, tokens, operands; pieces of tensor memory
+
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(i4_smem(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(i4_smem(bar)) : "memory");
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, i4_wait(bar, parity)); }
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// one lane of a whole warp issues, always the same one
+__device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+    asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
+                 ::"r"(i4_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* q) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+                   "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]),
+                   "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]),
+                   "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float load_cluster(uint32_t local, int rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+enum { STORE = 0, STORE_F32 = 1, ACCUM_F32 = 2, SWIGLU = 3, RELUGLU = 4, RELU2 = 5 };
+
+// bytes of a block of 64 columns of the prepared tokens: the operand's image, then the groups' sums, token by token
+__host__ __device__ constexpr int tokens_bytes(int tokens, int group) { return tokens * 128 + (64 / group) * tokens * 4; }
+
+struct TokensArgs {
+    const __nv_bfloat16* x;
+    unsigned char* to;             // [kblocks][tokens_bytes], then float32 [tokens]: what a token's sums are multiplied by at the end
+    long long ld;
+    int M, K, kblocks, tokens, group, vec;
+};
+// one block a token (of 32 or 64: those beyond M are zeros)
+__global__ void __launch_bounds__(256) int4_tokens_kernel(TokensArgs a) {
+    ce_pdl_begin();
+    __shared__ float scratch[32];
+    const int t = blockIdx.x, per_block = tokens_bytes(a.tokens, a.group);
+    const bool real = t < a.M;
+    const __nv_bfloat16* src = a.x + (size_t)(real ? t : 0) * a.ld;
+    auto load8 = [&](int c, float (&y)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = 0.f;
+        if (!real || c >= a.K) return;                // (K is a multiple of 32)
+        if (a.vec) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src + c);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { y[2 * i] = __uint_as_float(w[i] << 16); y[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = __bfloat162float(src[c + i]);
+        }
+    };
+    float largest = 0.f;
+    bool finite = true;
+    for (int c = threadIdx.x * 8; c < a.K; c += 2048) {
+        float y[8];
+        load8(c, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { largest = fmaxf(largest, fabsf(y[i])); finite = finite && fabsf(y[i]) <= 3.402823466e38f; }
+    }
+    largest = ce_block_max(finite ? largest : INFINITY, scratch);
+    const float up = i4_row_scale(largest);
+    if (threadIdx.x == 0) reinterpret_cast<float*>(a.to + (size_t)a.kblocks * per_block)[t] = 1.0f / up;
+    for (int c = threadIdx.x * 8; c < a.kblocks * 64; c += 2048) {
+        float y[8], sum = 0.f;
+        load8(c, y);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float f = i & 1 ? 0.0625f : 1.0f, b = i & 1 ? 16.0f : 1.0f;          // odd codes come 16 times too large
+            w[i] = i4_pack(y[i] * up * f, y[i + 4] * up * f);
+            const float2 got = i4_unpack(w[i]);
+            sum += (got.x + got.y) * b;
+        }
+        unsigned char* block = a.to + (size_t)(c >> 6) * per_block;
+        *reinterpret_cast<uint4*>(block + t * 128 + ((((c >> 3) & 7) ^ (t & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        const unsigned here = 0xffu << (threadIdx.x & 24);
+        sum += __shfl_xor_sync(here, sum, 1);
+        sum += __shfl_xor_sync(here, sum, 2);
+        if (a.group == 64) sum += __shfl_xor_sync(here, sum, 4);
+        if (c % a.group == 0) reinterpret_cast<float*>(block + a.tokens * 128)[(c & 63) / a.group * a.tokens + t] = sum;
+    }
+}
+
+struct Args {
+    const unsigned char *w, *x;    // x: as int4_tokens_kernel leaves it
+    const float* back;
+    void* out;
+    int* status;
+    int M, N, kblocks, units, slices, ldo, mode, gated, overlap;      // units: tiles of 16 rows
+};
+
+template <int G, int TOKENS>
+struct Shape {
+    static constexpr int TILE = i4_weight_tile_bytes(G), XB = tokens_bytes(TOKENS, G), XSTEP = (XB + 1023) / 1024 * 1024;
+    static constexpr uint32_t A = 0, X = AS * ROWS * 128, CODES = X + XS * XSTEP, BARS = CODES + RAW * 8 * RUN * TILE;
+    static constexpr uint32_t BYTES = BARS + 8 * (2 * RAW + 2 * XS + 2 * AS + 2 * DS + 2);
+    static constexpr int LD = TOKENS + 1;                               // floats of a row's sums, where the slices are added (in the place of the stages)
+    static_assert(ROWS * LD * 4 <= CODES, "sums");
+};
+
+template <int G, int TOKENS>
+__global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
+    using S = Shape<G, TOKENS>;
+    constexpr int TILE = S::TILE, GB = 64 / G;
+    extern __shared__ __align__(1024) unsigned char sm[];
+    const uint32_t base = i4_smem(sm);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::BARS);
+    uint64_t *raw_full = bars, *raw_empty = bars + RAW, *x_full = raw_empty + RAW, *x_empty = x_full + XS, *a_full = x_empty + XS, *a_empty = a_full + AS;
+    uint64_t *d_full = a_empty + AS, *d_empty = d_full + DS;
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(d_empty + DS);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int slice = blockIdx.x % a.slices, unit0 = blockIdx.x / a.slices * 8, tiles = min(8, a.units - unit0);
+    const int kb_begin = (int)((long long)a.kblocks * slice / a.slices), kb_end = (int)((long long)a.kblocks * (slice + 1) / a.slices);
+    const int n_kb = kb_end - kb_begin, runs = (n_kb + RUN - 1) / RUN;
+    if ((base & 1023u) != 0) {                          // cannot happen with dynamic shared memory alone; refuse rather than mis-swizzle
+        if (threadIdx.x == 0) atomicCAS(a.status, 0, 58);
+        if (a.slices > 1) { cluster_sync(); cluster_sync(); }
+        return;
+    }
+    ce_pdl_wait();                                      // (before tensor memory is taken: a neighbour that this grid waits for may need it)
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 2 * MAKERS); }
+        for (int i = 0; i < XS; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1 + MAKERS); }
+        for (int i = 0; i < AS; ++i) { mbar_init(&a_full[i], MAKERS); mbar_init(&a_empty[i], 1); }
+        for (int i = 0; i < DS; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], MAKERS); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(i4_smem(&tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (a.overlap) ce_pdl_launch_dependents();
+    const uint32_t tmem = tmem_slot;
+    float y[TOKENS];
+    bool ok = true;
+
+    if (warp == 0) {
+        // ---- the products: a group's of all tokens into the next piece of tensor memory
+        const uint32_t idesc = (1u << 4) | ((uint32_t)(TOKENS >> 3) << 17) | (8u << 24);
+        for (int i = 0; i < n_kb && ok; ++i) {
+            ok = warp_wait(&x_full[i % XS], (i / XS) & 1) && warp_wait(&a_full[i % AS], (i / AS) & 1);
+            if (!ok) break;
+            const uint32_t a_addr = base + S::A + i % AS * ROWS * 128, x_addr = base + S::X + i % XS * S::XSTEP;
+#pragma unroll
+            for (int g = 0; g < GB; ++g) {
+                const int d = i * GB + g;
+                if (d >= DS) ok = warp_wait(&d_empty[d % DS], (d / DS - 1) & 1);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int kk = 0; kk < G / 16; ++kk) {
+                    const uint32_t off = (g * (G / 16) + kk) * 32;
+                    umma(tmem + d % DS * 64, desc_kmajor(a_addr + off), desc_kmajor(x_addr + off), idesc, kk > 0 ? 1u : 0u);
+                }
+                umma_commit(&d_full[d % DS]);
+            }
+            umma_commit(&a_empty[i % AS]);
+            umma_commit(&x_empty[i % XS]);
+        }
+        if (!ok && lane == 0) atomicCAS(a.status, 0, 51);
+    } else if (warp == 1) {
+        // ---- the copies, in the order in which they are needed: codes of RUN blocks of columns at a time, tokens block by block
+        if (lane == 0) {
+            int copied = 0, run = 0;
+            for (int i = 0; i < n_kb && ok; ++i) {
+                // codes a few runs ahead of the tokens
+                while (run < runs && run * RUN <= i + (RAW - 1) * RUN && ok) {
+                    if (run >= RAW) ok = i4_wait(&raw_empty[run % RAW], (run / RAW - 1) & 1);
+                    if (!ok) break;
+                    const int count = min(RUN, n_kb - run * RUN);
+                    uint64_t* bar = &raw_full[run % RAW];
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(i4_smem(bar)), "r"(tiles * count * TILE) : "memory");
+                    for (int u = 0; u < tiles; ++u)
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                     ::"r"(base + S::CODES + (run % RAW * 8 + u) * RUN * TILE),
+                                     "l"(a.w + ((size_t)(unit0 + u) * a.kblocks + kb_begin + run * RUN) * TILE), "r"(count * TILE), "r"(i4_smem(bar)) : "memory");
+                    ++run;
+                }
+                if (!ok) break;
+                if (i >= XS) ok = i4_wait(&x_empty[i % XS], (i / XS - 1) & 1);
+                if (!ok) break;
+                i4_copy(sm + S::X + i % XS * S::XSTEP, a.x + (size_t)(kb_begin + i) * S::XB, S::XB, &x_full[i % XS]);
+                copied = i + 1;
+            }
+            if (!ok) {
+                atomicCAS(a.status, 0, 52);
+                // what is on its way lands before the block's memory is another's
+                for (int i = max(0, copied - XS); i < copied; ++i) i4_wait(&x_full[i % XS], (i / XS) & 1);
+                for (int i = max(0, run - RAW); i < run; ++i) i4_wait(&raw_full[i % RAW], (i / RAW) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 2 + MAKERS) {
+        // ---- codes into float16 integers: two tiles of 16 rows a warp
+        const int maker = warp - 2, r = lane >> 2, l = lane & 3;
+        for (int i = 0; i < n_kb && ok; ++i) {
+            const int run = i / RUN;
+            if (i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
+            if (!ok) break;
+            uint4 w[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) w[u] = *reinterpret_cast<const uint4*>(sm + S::CODES + ((run % RAW * 8 + maker * 2 + u) * RUN + i % RUN) * TILE + lane * 16);
+            if (i % RUN == RUN - 1 || i == n_kb - 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
+            }
+            if (i >= AS) ok = warp_wait(&a_empty[i % AS], (i / AS - 1) & 1);
+            if (!ok) break;
+            unsigned char* to = sm + S::A + i % AS * ROWS * 128;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {           // words of rows r and r + 8, first and second 32 columns
+                    const int half = e >> 1, row = 16 * (maker * 2 + u) + r + 8 * (e & 1);
+                    const uint32_t word = e == 0 ? w[u].x : e == 1 ? w[u].y : e == 2 ? w[u].z : w[u].w;
+                    uint32_t v[4];
+                    i4_pairs<true, 0>(word, v[0], v[1]);
+                    i4_pairs<true, 8>(word, v[2], v[3]);
+                    *reinterpret_cast<uint4*>(to + row * 128 + (((half * 4 + l) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[i % AS]);
+        }
+        if (!ok && lane == 0) atomicCAS(a.status, 0, 53);
+    } else {
+        // ---- the sums: a row a lane
+        const int quad = warp & 3, row = quad * 32 + lane, unit = row >> 4;
+        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) y[t] = 0.f;
+        for (int i = 0; i < n_kb && ok; ++i) {
+            const int run = i / RUN;
+            if (i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
+            if (!ok) break;
+            const unsigned char* tile = sm + S::CODES + ((run % RAW * 8 + unit) * RUN + i % RUN) * TILE + 512 + (row & 15) * GB * 4;
+            uint32_t step[GB];
+#pragma unroll
+            for (int g = 0; g < GB; ++g) step[g] = reinterpret_cast<const uint32_t*>(tile)[g];
+            if (i % RUN == RUN - 1 || i == n_kb - 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
+            }
+            ok = warp_wait(&x_full[i % XS], (i / XS) & 1);
+            if (!ok) break;
+            const float* sums = reinterpret_cast<const float*>(sm + S::X + i % XS * S::XSTEP + TOKENS * 128);
+#pragma unroll
+            for (int g = 0; g < GB; ++g) {
+                const int d = i * GB + g;
+                const float2 f = i4_step_of<true>(step[g]);
+                const float2 s2 = make_float2(f.x, f.x), z2 = make_float2(f.y, f.y);
+                // the minimum's part meanwhile
+#pragma unroll
+                for (int t = 0; t < TOKENS; t += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(sums + g * TOKENS + t);
+                    const float2 p = __ffma2_rn(z2, make_float2(v.x, v.y), make_float2(y[t], y[t + 1]));
+                    const float2 q = __ffma2_rn(z2, make_float2(v.z, v.w), make_float2(y[t + 2], y[t + 3]));
+                    y[t] = p.x; y[t + 1] = p.y; y[t + 2] = q.x; y[t + 3] = q.y;
+                }
+                ok = ok && warp_wait(&d_full[d % DS], (d / DS) & 1);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t got[TOKENS];
+#pragma unroll
+                for (int t = 0; t < TOKENS; t += 32) tmem_ld32(tmem + d % DS * 64 + lane_base + t, got + t);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_empty[d % DS]);
+#pragma unroll
+                for (int t = 0; t < TOKENS; t += 2) {
+                    const float2 p = __ffma2_rn(s2, make_float2(__uint_as_float(got[t]), __uint_as_float(got[t + 1])), make_float2(y[t], y[t + 1]));
+                    y[t] = p.x; y[t + 1] = p.y;
+                }
+            }
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&x_empty[i % XS]);
+        }
+        if (!ok && lane == 0) atomicCAS(a.status, 0, 54);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();                                    // the stages are free: the rows' sums take their place
+    if (warp == 0) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+    float* total = reinterpret_cast<float*>(sm);
+    if (warp >= 2 + MAKERS) {
+        const int row = (warp & 3) * 32 + lane;
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) total[row * S::LD + t] = y[t];
+    }
+    if (a.slices > 1) cluster_sync();
+    else __syncthreads();
+    // a row's results of a token: the slices' sums in their order, what was scaled scaled back; a block takes every ``slices``-th run of results
+    const int outs = a.gated ? 64 : ROWS;
+    for (int o = slice * THREADS + threadIdx.x; o < outs * a.M; o += a.slices * THREADS) {
+        const int t = o / outs, i = o - t * outs, row = a.gated ? (i >> 3) * 16 + (i & 7) : i;
+        const int n = a.gated ? unit0 * 8 + i : unit0 * 16 + i;
+        if (n >= a.N) continue;
+        float v = 0.f, u = 0.f;
+        for (int s = 0; s < a.slices; ++s) {
+            v += a.slices > 1 ? load_cluster(i4_smem(total + row * S::LD + t), s) : total[row * S::LD + t];
+            if (a.gated) u += a.slices > 1 ? load_cluster(i4_smem(total + (row + 8) * S::LD + t), s) : total[(row + 8) * S::LD + t];
+        }
+        const float back = a.back[t];
+        v *= back; u *= back;
+        const size_t at = (size_t)t * a.ldo + n;
+        __nv_bfloat16* half = (__nv_bfloat16*)a.out;
+        switch (a.mode) {
+            case STORE_F32: ((float*)a.out)[at] = v; break;
+            case ACCUM_F32: ((float*)a.out)[at] += v; break;
+            case SWIGLU: half[at] = __float2bfloat16_rn(ce_silu_glu(v, u)); break;
+            case RELUGLU: half[at] = __float2bfloat16_rn(fmaxf(v, 0.f) * u); break;
+            case RELU2: v = fmaxf(v, 0.f); half[at] = __float2bfloat16_rn(v * v); break;
+            default: half[at] = __float2bfloat16_rn(v);
+        }
+    }
+    if (a.slices > 1) cluster_sync();                   // nobody leaves while its sums are read
+}
+
+template <int G, int TOKENS>
+int run(TokensArgs p, Args a, cudaStream_t stream) {
+    using S = Shape<G, TOKENS>;
+    auto kernel = int4_gemm_tc_kernel<G, TOKENS>;
+    static std::atomic<unsigned long long> done{0};
+    cudaError_t e = ce_allow_smem(done, kernel, S::BYTES);
+    if (e == cudaSuccess) {
+        ce_note("int4_tokens_kernel");
+        e = ce_launch(int4_tokens_kernel, dim3(TOKENS), dim3(256), 0, stream, p);
+    }
+    if (e == cudaSuccess) {
+        // as many slices of K as fill the chip, of 8 blocks of 64 columns at least
+        const int blocks = (a.units + 7) / 8, sms = ce_sm_count();
+        int slices = 1;
+        while (slices < 8 && blocks * (slices + 1) <= sms && a.kblocks / (slices + 1) >= 8) ++slices;
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[2];
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = S::BYTES;
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        a.overlap = ce_pdl_enabled();
+        static CeRoom room[9];
+        for (;; --slices) {
+            cfg.numAttrs = 0;
+            cfg.gridDim = dim3((unsigned)(blocks * slices));
+            if (slices == 1) break;
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim = {(unsigned)slices, 1, 1};
+            cfg.numAttrs = 1;
+            if (blocks <= ce_clusters_at_once(room[slices], kernel, cfg)) break;       // (clusters that do not all run at once: fewer slices)
+        }
+        a.slices = slices;
+        if (a.overlap) {
+            attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+        }
+        ce_note("int4_gemm_tc_kernel");
+        e = cudaLaunchKernelEx(&cfg, kernel, a);
+    }
+    if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_gemm_tc: %s", cudaGetErrorString(e)); }
+    return ce_check_launch("int4_gemm_tc");
+}
+
+}  // namespace
+
+// float32 words of scratch memory for M tokens (at most 64) of K columns
+long long ce_int4_gemm_tc_scratch(int M, int K, int kept) {
+    const int tokens = M <= 32 ? 32 : 64;
+    return (long long)((K + 63) / 64) * tokens_bytes(tokens, kept) / 4 + tokens;
+}
+
+// The checks of ce_int4_gemm come first: it calls this.  scratch: on a 16-byte boundary; kept: columns of a group in the weight's tiles (32 or 64)
+int ce_int4_gemm_tc(const void* x, long long ldx, const void* w, void* out, int ldo, int M, int N, int K, int kept, int mode, float* scratch, int* status,
+                    cudaStream_t stream) {
+    const int tokens = M <= 32 ? 32 : 64, kblocks = (K + 63) / 64, gated = mode == SWIGLU || mode == RELUGLU;
+    unsigned char* to = (unsigned char*)scratch;
+    TokensArgs p{(const __nv_bfloat16*)x, to, ldx, M, K, kblocks, tokens, kept, ((uintptr_t)x & 15) == 0 && ldx % 8 == 0};
+    Args a{(const unsigned char*)w, to, reinterpret_cast<const float*>(to + (size_t)kblocks * tokens_bytes(tokens, kept)), out, status, M, N, kblocks,
+           gated ? (N + 7) / 8 : (N + 15) / 16, 1, ldo, mode, gated, 0};
+    if (tokens == 32) return kept == 32 ? run<32, 32>(p, a, stream) : run<64, 32>(p, a, stream);
+    return kept == 32 ? run<32, 64>(p, a, stream) : run<64, 64>(p, a, stream);
+}
