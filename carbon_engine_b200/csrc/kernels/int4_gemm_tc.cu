@@ -3,10 +3,11 @@
 //   out[t, n] = sum_g (s_ng (x_tg . (c_ng - 8)) + (z_ng + 8 s_ng) sum x_tg)
 //
 // A block takes 128 rows of the weight (8 tiles of 16) and a slice of K; blocks of a cluster share K.  For each group of columns, tcgen05.mma forms
-// the codes' products with all tokens in a piece of tensor memory of its own; four warps (a row a lane) read it back and add it to their
-// sums in float32, times the row's step: no value of W is ever rounded, and what is read back is as much work as the products are.  Four warps
-// turn codes into float16 integers (c - 8, the even ones, 16 (c - 8), the odd: the tokens are laid out to match), one issues the copies of
-// codes and tokens and one the products.  Slices' sums are added in their order through shared memory.
+// the codes' products with all tokens in a piece of tensor memory of its own; eight warps (a row and half of the tokens a lane) read it back and
+// add it to their sums in float32, times the row's step: no value of W is ever rounded, and what is read back is as much work as the products are.
+// Four warps turn codes into float16 integers (c - 8, the even ones, 16 (c - 8), the odd: the tokens are laid out to match), one issues the
+// copies of codes and tokens and one the products.  Slices' sums are added in their order through shared memory.  The parts hand each other 128
+// columns at a time: a hand-over costs some 0.2 us whatever it hands over.
 //
 // The tokens come prepared (int4_tokens_kernel): each brought into [2^14, 2^15) by a power of two and rounded to float16 - exact for bfloat16 down
 // to 2^-30 of the token's largest - as the second operand's image, swizzle included, and the groups' sums behind it.
@@ -14,8 +15,8 @@
 
 namespace {
 
-constexpr int ROWS = 128, MAKERS = 4, THREADS = 32 * (2 + 2 * MAKERS);
-constexpr int RUN = 4, RAW = 4, XS = 6, AS = 3, DS = 8;     // blocks of 64 columns a copy of codes; stages of codes, tokens, operands; pieces of tensor memory
+constexpr int ROWS = 128, MAKERS = 4, ADDERS = 8, THREADS = 32 * (2 + MAKERS + ADDERS);
+constexpr int RUN = 4, RAW = 4, XS = 4, AS = 2, DS = 8;     // blocks of 64 columns a copy of codes; stages of codes, tokens, operands (two blocks each); pieces of tensor memory
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(i4_smem(bar)), "r"(count));
@@ -36,14 +37,29 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
                  ::"r"(i4_smem(bar)) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* q) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
-                   "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]),
-                   "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]),
-                   "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
-                 : "r"(taddr));
+// N columns of this lane's row (16 or 32): under way until tmem_landed
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&q)[N]) {
+    if constexpr (N == 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+                       "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15])
+                     : "r"(taddr));
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                     "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                     : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+                       "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]),
+                       "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]),
+                       "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+                     : "r"(taddr));
+}
+// (the registers pass through, so that nothing reads them before)
+template <int N>
+__device__ __forceinline__ void tmem_landed(uint32_t (&q)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(q[i]));
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -67,46 +83,53 @@ struct TokensArgs {
     long long ld;
     int M, K, kblocks, tokens, group, vec;
 };
-// one block a token (of 32 or 64: those beyond M are zeros)
-__global__ void __launch_bounds__(256) int4_tokens_kernel(TokensArgs a) {
+// one block a token (of 32 or 64: those beyond M are zeros); up to 16,384 columns are read once and kept in registers
+__global__ void __launch_bounds__(1024) int4_tokens_kernel(TokensArgs a) {
     ce_pdl_begin();
     __shared__ float scratch[32];
     const int t = blockIdx.x, per_block = tokens_bytes(a.tokens, a.group);
     const bool real = t < a.M;
     const __nv_bfloat16* src = a.x + (size_t)(real ? t : 0) * a.ld;
-    auto load8 = [&](int c, float (&y)[8]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = 0.f;
-        if (!real || c >= a.K) return;                // (K is a multiple of 32)
-        if (a.vec) {
-            const uint4 u = *reinterpret_cast<const uint4*>(src + c);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { y[2 * i] = __uint_as_float(w[i] << 16); y[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __bfloat162float(src[c + i]);
-        }
+    auto load8 = [&](int c) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (!real || c >= a.K) return u;              // (K is a multiple of 32)
+        if (a.vec) return *reinterpret_cast<const uint4*>(src + c);
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(src + c);
+        u.x = p[0] | (uint32_t)p[1] << 16; u.y = p[2] | (uint32_t)p[3] << 16; u.z = p[4] | (uint32_t)p[5] << 16; u.w = p[6] | (uint32_t)p[7] << 16;
+        return u;
     };
+    constexpr int KEPT = 2, STEP = 1024 * 8;
+    uint4 kept[KEPT];
     float largest = 0.f;
     bool finite = true;
-    for (int c = threadIdx.x * 8; c < a.K; c += 2048) {
-        float y[8];
-        load8(c, y);
+    auto look = [&](uint4 u) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { largest = fmaxf(largest, fabsf(y[i])); finite = finite && fabsf(y[i]) <= 3.402823466e38f; }
-    }
+        for (int i = 0; i < 4; ++i) {
+            const float p = fabsf(__uint_as_float(w[i] << 16)), q = fabsf(__uint_as_float(w[i] & 0xffff0000u));
+            largest = fmaxf(largest, fmaxf(p, q));
+            finite = finite && p <= 3.402823466e38f && q <= 3.402823466e38f;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) kept[i] = load8(threadIdx.x * 8 + i * STEP);
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) look(kept[i]);
+    for (int c = threadIdx.x * 8 + KEPT * STEP; c < a.K; c += STEP) look(load8(c));
     largest = ce_block_max(finite ? largest : INFINITY, scratch);
     const float up = i4_row_scale(largest);
     if (threadIdx.x == 0) reinterpret_cast<float*>(a.to + (size_t)a.kblocks * per_block)[t] = 1.0f / up;
-    for (int c = threadIdx.x * 8; c < a.kblocks * 64; c += 2048) {
+    auto put = [&](int c, uint4 u) {
+        if (c >= a.kblocks * 64) return;              // (8 threads, a block of 64 columns, together)
+        const uint32_t in[4] = {u.x, u.y, u.z, u.w};
         float y[8], sum = 0.f;
-        load8(c, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { y[2 * i] = __uint_as_float(in[i] << 16) * up; y[2 * i + 1] = __uint_as_float(in[i] & 0xffff0000u) * up; }
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float f = i & 1 ? 0.0625f : 1.0f, b = i & 1 ? 16.0f : 1.0f;          // odd codes come 16 times too large
-            w[i] = i4_pack(y[i] * up * f, y[i + 4] * up * f);
+            w[i] = i4_pack(y[i] * f, y[i + 4] * f);
             const float2 got = i4_unpack(w[i]);
             sum += (got.x + got.y) * b;
         }
@@ -117,7 +140,10 @@ __global__ void __launch_bounds__(256) int4_tokens_kernel(TokensArgs a) {
         sum += __shfl_xor_sync(here, sum, 2);
         if (a.group == 64) sum += __shfl_xor_sync(here, sum, 4);
         if (c % a.group == 0) reinterpret_cast<float*>(block + a.tokens * 128)[(c & 63) / a.group * a.tokens + t] = sum;
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) put(threadIdx.x * 8 + i * STEP, kept[i]);
+    for (int c = threadIdx.x * 8 + KEPT * STEP; c < a.kblocks * 64; c += STEP) put(c, load8(c));
 }
 
 struct Args {
@@ -130,8 +156,8 @@ struct Args {
 
 template <int G, int TOKENS>
 struct Shape {
-    static constexpr int TILE = i4_weight_tile_bytes(G), XB = tokens_bytes(TOKENS, G), XSTEP = (XB + 1023) / 1024 * 1024;
-    static constexpr uint32_t A = 0, X = AS * ROWS * 128, CODES = X + XS * XSTEP, BARS = CODES + RAW * 8 * RUN * TILE;
+    static constexpr int TILE = i4_weight_tile_bytes(G), XB = tokens_bytes(TOKENS, G), XSTEP = (XB + 1023) / 1024 * 1024;     // XSTEP: of a block in shared memory
+    static constexpr uint32_t A = 0, X = AS * 2 * ROWS * 128, CODES = X + XS * 2 * XSTEP, BARS = CODES + RAW * 8 * RUN * TILE;
     static constexpr uint32_t BYTES = BARS + 8 * (2 * RAW + 2 * XS + 2 * AS + 2 * DS + 2);
     static constexpr int LD = TOKENS + 1;                               // floats of a row's sums, where the slices are added (in the place of the stages)
     static_assert(ROWS * LD * 4 <= CODES, "sums");
@@ -150,7 +176,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slice = blockIdx.x % a.slices, unit0 = blockIdx.x / a.slices * 8, tiles = min(8, a.units - unit0);
     const int kb_begin = (int)((long long)a.kblocks * slice / a.slices), kb_end = (int)((long long)a.kblocks * (slice + 1) / a.slices);
-    const int n_kb = kb_end - kb_begin, runs = (n_kb + RUN - 1) / RUN;
+    const int n_kb = kb_end - kb_begin, runs = (n_kb + RUN - 1) / RUN, pairs = (n_kb + 1) / 2;
     if ((base & 1023u) != 0) {                          // cannot happen with dynamic shared memory alone; refuse rather than mis-swizzle
         if (threadIdx.x == 0) atomicCAS(a.status, 0, 58);
         if (a.slices > 1) { cluster_sync(); cluster_sync(); }
@@ -158,10 +184,10 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     }
     ce_pdl_wait();                                      // (before tensor memory is taken: a neighbour that this grid waits for may need it)
     if (threadIdx.x == 0) {
-        for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 2 * MAKERS); }
-        for (int i = 0; i < XS; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1 + MAKERS); }
+        for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], MAKERS + ADDERS); }
+        for (int i = 0; i < XS; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1 + ADDERS); }
         for (int i = 0; i < AS; ++i) { mbar_init(&a_full[i], MAKERS); mbar_init(&a_empty[i], 1); }
-        for (int i = 0; i < DS; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], MAKERS); }
+        for (int i = 0; i < DS; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], ADDERS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -173,26 +199,29 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (a.overlap) ce_pdl_launch_dependents();
     const uint32_t tmem = tmem_slot;
-    float y[TOKENS];
+    constexpr int PART = TOKENS / 2;                    // tokens of a lane that adds
+    float y[PART];
     bool ok = true;
 
     if (warp == 0) {
         // ---- the products: a group's of all tokens into the next piece of tensor memory
         const uint32_t idesc = (1u << 4) | ((uint32_t)(TOKENS >> 3) << 17) | (8u << 24);
-        for (int i = 0; i < n_kb && ok; ++i) {
+        for (int i = 0; i < pairs && ok; ++i) {
             ok = warp_wait(&x_full[i % XS], (i / XS) & 1) && warp_wait(&a_full[i % AS], (i / AS) & 1);
             if (!ok) break;
-            const uint32_t a_addr = base + S::A + i % AS * ROWS * 128, x_addr = base + S::X + i % XS * S::XSTEP;
+            const uint32_t a_addr = base + S::A + i % AS * 2 * ROWS * 128, x_addr = base + S::X + i % XS * 2 * S::XSTEP;
+            const int groups = min(2, n_kb - 2 * i) * GB;
 #pragma unroll
-            for (int g = 0; g < GB; ++g) {
-                const int d = i * GB + g;
-                if (d >= DS) ok = warp_wait(&d_empty[d % DS], (d / DS - 1) & 1);
+            for (int g = 0; g < 2 * GB; ++g) {
+                if (g >= groups) break;
+                const int d = i * 2 * GB + g;
+                if (d >= DS) ok = ok && warp_wait(&d_empty[d % DS], (d / DS - 1) & 1);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                 for (int kk = 0; kk < G / 16; ++kk) {
-                    const uint32_t off = (g * (G / 16) + kk) * 32;
-                    umma(tmem + d % DS * 64, desc_kmajor(a_addr + off), desc_kmajor(x_addr + off), idesc, kk > 0 ? 1u : 0u);
+                    const uint32_t off = (g % GB * (G / 16) + kk) * 32;
+                    umma(tmem + d % DS * 64, desc_kmajor(a_addr + g / GB * ROWS * 128 + off), desc_kmajor(x_addr + g / GB * S::XSTEP + off), idesc, kk > 0 ? 1u : 0u);
                 }
                 umma_commit(&d_full[d % DS]);
             }
@@ -201,12 +230,12 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, 51);
     } else if (warp == 1) {
-        // ---- the copies, in the order in which they are needed: codes of RUN blocks of columns at a time, tokens block by block
+        // ---- the copies, in the order in which they are needed: codes of RUN blocks of columns at a time, tokens of two
         if (lane == 0) {
             int copied = 0, run = 0;
-            for (int i = 0; i < n_kb && ok; ++i) {
+            for (int i = 0; i < pairs && ok; ++i) {
                 // codes a few runs ahead of the tokens
-                while (run < runs && run * RUN <= i + (RAW - 1) * RUN && ok) {
+                while (run < runs && run * RUN <= 2 * i + (RAW - 1) * RUN && ok) {
                     if (run >= RAW) ok = i4_wait(&raw_empty[run % RAW], (run / RAW - 1) & 1);
                     if (!ok) break;
                     const int count = min(RUN, n_kb - run * RUN);
@@ -221,7 +250,13 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 if (!ok) break;
                 if (i >= XS) ok = i4_wait(&x_empty[i % XS], (i / XS - 1) & 1);
                 if (!ok) break;
-                i4_copy(sm + S::X + i % XS * S::XSTEP, a.x + (size_t)(kb_begin + i) * S::XB, S::XB, &x_full[i % XS]);
+                uint64_t* bar = &x_full[i % XS];
+                const int count = min(2, n_kb - 2 * i);
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(i4_smem(bar)), "r"(count * S::XB) : "memory");
+                for (int k = 0; k < count; ++k)
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                 ::"r"(base + S::X + (i % XS * 2 + k) * S::XSTEP), "l"(a.x + (size_t)(kb_begin + 2 * i + k) * S::XB), "r"(S::XB), "r"(i4_smem(bar))
+                                 : "memory");
                 copied = i + 1;
             }
             if (!ok) {
@@ -235,84 +270,89 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     } else if (warp < 2 + MAKERS) {
         // ---- codes into float16 integers: two tiles of 16 rows a warp
         const int maker = warp - 2, r = lane >> 2, l = lane & 3;
-        for (int i = 0; i < n_kb && ok; ++i) {
-            const int run = i / RUN;
-            if (i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
+        for (int i = 0; i < pairs && ok; ++i) {
+            const int run = 2 * i / RUN;
+            if (2 * i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
             if (!ok) break;
-            uint4 w[2];
+            uint4 w[2][2];                              // (an odd last block: the second of the pair holds what lay there, for no product)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) w[u] = *reinterpret_cast<const uint4*>(sm + S::CODES + ((run % RAW * 8 + maker * 2 + u) * RUN + i % RUN) * TILE + lane * 16);
-            if (i % RUN == RUN - 1 || i == n_kb - 1) {
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    w[k][u] = *reinterpret_cast<const uint4*>(sm + S::CODES + ((run % RAW * 8 + maker * 2 + u) * RUN + 2 * i % RUN + k) * TILE + lane * 16);
+            if (2 * i % RUN == RUN - 2 || i == pairs - 1) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
             }
             if (i >= AS) ok = warp_wait(&a_empty[i % AS], (i / AS - 1) & 1);
             if (!ok) break;
-            unsigned char* to = sm + S::A + i % AS * ROWS * 128;
+            unsigned char* to = sm + S::A + i % AS * 2 * ROWS * 128;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {           // words of rows r and r + 8, first and second 32 columns
-                    const int half = e >> 1, row = 16 * (maker * 2 + u) + r + 8 * (e & 1);
-                    const uint32_t word = e == 0 ? w[u].x : e == 1 ? w[u].y : e == 2 ? w[u].z : w[u].w;
-                    uint32_t v[4];
-                    i4_pairs<true, 0>(word, v[0], v[1]);
-                    i4_pairs<true, 8>(word, v[2], v[3]);
-                    *reinterpret_cast<uint4*>(to + row * 128 + (((half * 4 + l) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-                }
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {       // words of rows r and r + 8, first and second 32 columns
+                        const int half = e >> 1, row = 16 * (maker * 2 + u) + r + 8 * (e & 1);
+                        const uint32_t word = e == 0 ? w[k][u].x : e == 1 ? w[k][u].y : e == 2 ? w[k][u].z : w[k][u].w;
+                        uint32_t v[4];
+                        i4_pairs<true, 0>(word, v[0], v[1]);
+                        i4_pairs<true, 8>(word, v[2], v[3]);
+                        *reinterpret_cast<uint4*>(to + k * ROWS * 128 + row * 128 + (((half * 4 + l) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&a_full[i % AS]);
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, 53);
     } else {
-        // ---- the sums: a row a lane
-        const int quad = warp & 3, row = quad * 32 + lane, unit = row >> 4;
-        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+        // ---- the sums: a row and half of the tokens a lane; the next group's products are on their way while this one's are added
+        const int quad = warp & 3, row = quad * 32 + lane, unit = row >> 4, first = (warp - 2 - MAKERS) / 4 * PART;
+        const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + first;
 #pragma unroll
-        for (int t = 0; t < TOKENS; ++t) y[t] = 0.f;
-        for (int i = 0; i < n_kb && ok; ++i) {
-            const int run = i / RUN;
-            if (i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
+        for (int t = 0; t < PART; ++t) y[t] = 0.f;
+        for (int i = 0; i < pairs && ok; ++i) {
+            const int run = 2 * i / RUN, groups = min(2, n_kb - 2 * i) * GB;
+            if (2 * i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
             if (!ok) break;
-            const unsigned char* tile = sm + S::CODES + ((run % RAW * 8 + unit) * RUN + i % RUN) * TILE + 512 + (row & 15) * GB * 4;
-            uint32_t step[GB];
+            uint32_t step[2 * GB];
 #pragma unroll
-            for (int g = 0; g < GB; ++g) step[g] = reinterpret_cast<const uint32_t*>(tile)[g];
-            if (i % RUN == RUN - 1 || i == n_kb - 1) {
+            for (int g = 0; g < 2 * GB; ++g)
+                step[g] = reinterpret_cast<const uint32_t*>(sm + S::CODES + ((run % RAW * 8 + unit) * RUN + 2 * i % RUN + g / GB) * TILE + 512 + (row & 15) * GB * 4)[g % GB];
+            if (2 * i % RUN == RUN - 2 || i == pairs - 1) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
             }
             ok = warp_wait(&x_full[i % XS], (i / XS) & 1);
             if (!ok) break;
-            const float* sums = reinterpret_cast<const float*>(sm + S::X + i % XS * S::XSTEP + TOKENS * 128);
-#pragma unroll
-            for (int g = 0; g < GB; ++g) {
-                const int d = i * GB + g;
-                const float2 f = i4_step_of<true>(step[g]);
-                const float2 s2 = make_float2(f.x, f.x), z2 = make_float2(f.y, f.y);
-                // the minimum's part meanwhile
-#pragma unroll
-                for (int t = 0; t < TOKENS; t += 4) {
-                    const float4 v = *reinterpret_cast<const float4*>(sums + g * TOKENS + t);
-                    const float2 p = __ffma2_rn(z2, make_float2(v.x, v.y), make_float2(y[t], y[t + 1]));
-                    const float2 q = __ffma2_rn(z2, make_float2(v.z, v.w), make_float2(y[t + 2], y[t + 3]));
-                    y[t] = p.x; y[t + 1] = p.y; y[t + 2] = q.x; y[t + 3] = q.y;
-                }
+            uint32_t got[2][PART];
+            auto fetch = [&](int g) {
+                const int d = i * 2 * GB + g;
                 ok = ok && warp_wait(&d_full[d % DS], (d / DS) & 1);
-                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t got[TOKENS];
+                tmem_ld<PART>(from + d % DS * 64, got[g & 1]);
+            };
+            fetch(0);
 #pragma unroll
-                for (int t = 0; t < TOKENS; t += 32) tmem_ld32(tmem + d % DS * 64 + lane_base + t, got + t);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            for (int g = 0; g < 2 * GB; ++g) {
+                if (g >= groups) break;
+                tmem_landed<PART>(got[g & 1]);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&d_empty[d % DS]);
+                if (lane == 0) mbar_arrive(&d_empty[(i * 2 * GB + g) % DS]);
+                if (g + 1 < 2 * GB && g + 1 < groups) fetch(g + 1);
+                const float2 f = i4_step_of<true>(step[g]);
+                const float2 s2 = make_float2(f.x, f.x), z2 = make_float2(f.y, f.y);
+                const float* sums = reinterpret_cast<const float*>(sm + S::X + (i % XS * 2 + g / GB) * S::XSTEP + TOKENS * 128) + g % GB * TOKENS + first;
 #pragma unroll
-                for (int t = 0; t < TOKENS; t += 2) {
-                    const float2 p = __ffma2_rn(s2, make_float2(__uint_as_float(got[t]), __uint_as_float(got[t + 1])), make_float2(y[t], y[t + 1]));
-                    y[t] = p.x; y[t + 1] = p.y;
+                for (int t = 0; t < PART; t += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(sums + t);
+                    const uint32_t* c = &got[g & 1][t];
+                    float2 p = __ffma2_rn(z2, make_float2(v.x, v.y), make_float2(y[t], y[t + 1]));
+                    float2 q = __ffma2_rn(z2, make_float2(v.z, v.w), make_float2(y[t + 2], y[t + 3]));
+                    p = __ffma2_rn(s2, make_float2(__uint_as_float(c[0]), __uint_as_float(c[1])), p);
+                    q = __ffma2_rn(s2, make_float2(__uint_as_float(c[2]), __uint_as_float(c[3])), q);
+                    y[t] = p.x; y[t + 1] = p.y; y[t + 2] = q.x; y[t + 3] = q.y;
                 }
             }
             __syncwarp();
@@ -328,22 +368,33 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     }
     float* total = reinterpret_cast<float*>(sm);
     if (warp >= 2 + MAKERS) {
-        const int row = (warp & 3) * 32 + lane;
+        const int row = (warp & 3) * 32 + lane, first = (warp - 2 - MAKERS) / 4 * PART;
 #pragma unroll
-        for (int t = 0; t < TOKENS; ++t) total[row * S::LD + t] = y[t];
+        for (int t = 0; t < PART; ++t) total[row * S::LD + first + t] = y[t];
     }
     if (a.slices > 1) cluster_sync();
     else __syncthreads();
-    // a row's results of a token: the slices' sums in their order, what was scaled scaled back; a block takes every ``slices``-th run of results
+    // a row's results of a token: the slices' sums in their order (all of them asked for at once), what was scaled scaled back; a block takes
+    // every ``slices``-th run of results
     const int outs = a.gated ? 64 : ROWS;
     for (int o = slice * THREADS + threadIdx.x; o < outs * a.M; o += a.slices * THREADS) {
         const int t = o / outs, i = o - t * outs, row = a.gated ? (i >> 3) * 16 + (i & 7) : i;
         const int n = a.gated ? unit0 * 8 + i : unit0 * 16 + i;
         if (n >= a.N) continue;
-        float v = 0.f, u = 0.f;
-        for (int s = 0; s < a.slices; ++s) {
-            v += a.slices > 1 ? load_cluster(i4_smem(total + row * S::LD + t), s) : total[row * S::LD + t];
-            if (a.gated) u += a.slices > 1 ? load_cluster(i4_smem(total + (row + 8) * S::LD + t), s) : total[(row + 8) * S::LD + t];
+        float v = total[row * S::LD + t], u = a.gated ? total[(row + 8) * S::LD + t] : 0.f;
+        if (a.slices > 1) {
+            float vs[8], us[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                vs[s] = us[s] = 0.f;
+                if (s < a.slices) {
+                    vs[s] = load_cluster(i4_smem(total + row * S::LD + t), s);
+                    if (a.gated) us[s] = load_cluster(i4_smem(total + (row + 8) * S::LD + t), s);
+                }
+            }
+            v = u = 0.f;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) { v += vs[s]; u += us[s]; }
         }
         const float back = a.back[t];
         v *= back; u *= back;
@@ -369,7 +420,7 @@ int run(TokensArgs p, Args a, cudaStream_t stream) {
     cudaError_t e = ce_allow_smem(done, kernel, S::BYTES);
     if (e == cudaSuccess) {
         ce_note("int4_tokens_kernel");
-        e = ce_launch(int4_tokens_kernel, dim3(TOKENS), dim3(256), 0, stream, p);
+        e = ce_launch(int4_tokens_kernel, dim3(TOKENS), dim3(1024), 0, stream, p);
     }
     if (e == cudaSuccess) {
         // as many slices of K as fill the chip, of 8 blocks of 64 columns at least
