@@ -6,7 +6,7 @@
 // the codes' products with all tokens in a piece of tensor memory of its own; eight warps (a row and half of the tokens a lane) read it back and
 // add it to their sums in float32, times the row's step: no value of W is ever rounded, and what is read back is as much work as the products are.
 // Four warps turn codes into float16 integers (c - 8, the even ones, 16 (c - 8), the odd: the tokens are laid out to match), one issues the
-// copies of codes and tokens and one the products.  Slices' sums are added in their order through shared memory.  The parts hand each other 128
+// products, one the copies of codes - before the tokens are there - and one those of tokens.  Slices' sums are added in their order through shared memory.  The parts hand each other 128
 // columns at a time: a hand-over costs some 0.2 us whatever it hands over.
 //
 // The tokens come prepared (int4_tokens_kernel): each brought into [2^14, 2^15) by a power of two and rounded to float16 - exact for bfloat16 down
@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int ROWS = 128, MAKERS = 4, ADDERS = 8, THREADS = 32 * (2 + MAKERS + ADDERS);
+constexpr int ROWS = 128, MAKERS = 4, ADDERS = 8, FIRST = 3, THREADS = 32 * (FIRST + MAKERS + ADDERS);
 constexpr int RUN = 4, RAW = 4, XS = 4, AS = 2, DS = 8;     // blocks of 64 columns a copy of codes; stages of codes, tokens, operands (two blocks each); pieces of tensor memory
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
@@ -159,8 +159,7 @@ struct Shape {
     static constexpr int TILE = i4_weight_tile_bytes(G), XB = tokens_bytes(TOKENS, G), XSTEP = (XB + 1023) / 1024 * 1024;     // XSTEP: of a block in shared memory
     static constexpr uint32_t A = 0, X = AS * 2 * ROWS * 128, CODES = X + XS * 2 * XSTEP, BARS = CODES + RAW * 8 * RUN * TILE;
     static constexpr uint32_t BYTES = BARS + 8 * (2 * RAW + 2 * XS + 2 * AS + 2 * DS + 2);
-    static constexpr int LD = TOKENS + 1;                               // floats of a row's sums, where the slices are added (in the place of the stages)
-    static_assert(ROWS * LD * 4 <= CODES, "sums");
+    static_assert(TOKENS * ROWS * 4 <= CODES, "sums");                   // of the slices, token by token, in the place of the stages
 };
 
 template <int G, int TOKENS>
@@ -182,7 +181,6 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         if (a.slices > 1) { cluster_sync(); cluster_sync(); }
         return;
     }
-    ce_pdl_wait();                                      // (before tensor memory is taken: a neighbour that this grid waits for may need it)
     if (threadIdx.x == 0) {
         for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], MAKERS + ADDERS); }
         for (int i = 0; i < XS; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1 + ADDERS); }
@@ -190,6 +188,21 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         for (int i = 0; i < DS; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], ADDERS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncthreads();
+    // codes of runs of columns, by one lane (not what the kernel in front writes, and what wrote them ended before that one began)
+    auto copy_codes = [&](int run) {
+        const int count = min(RUN, n_kb - run * RUN);
+        uint64_t* bar = &raw_full[run % RAW];
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(i4_smem(bar)), "r"(tiles * count * TILE) : "memory");
+        for (int u = 0; u < tiles; ++u)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(base + S::CODES + (run % RAW * 8 + u) * RUN * TILE),
+                         "l"(a.w + ((size_t)(unit0 + u) * a.kblocks + kb_begin + run * RUN) * TILE), "r"(count * TILE), "r"(i4_smem(bar)) : "memory");
+    };
+    if (warp == 1 && lane == 0)
+        for (int run = 0; run < min(runs, RAW); ++run) copy_codes(run);
+    __syncwarp();
+    ce_pdl_wait();                                      // (before tensor memory is taken: a neighbour that this grid waits for may need it)
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(i4_smem(&tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -230,24 +243,25 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, 51);
     } else if (warp == 1) {
-        // ---- the copies, in the order in which they are needed: codes of RUN blocks of columns at a time, tokens of two
+        // ---- the copies of codes, RUN blocks of columns at a time
         if (lane == 0) {
-            int copied = 0, run = 0;
-            for (int i = 0; i < pairs && ok; ++i) {
-                // codes a few runs ahead of the tokens
-                while (run < runs && run * RUN <= 2 * i + (RAW - 1) * RUN && ok) {
-                    if (run >= RAW) ok = i4_wait(&raw_empty[run % RAW], (run / RAW - 1) & 1);
-                    if (!ok) break;
-                    const int count = min(RUN, n_kb - run * RUN);
-                    uint64_t* bar = &raw_full[run % RAW];
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(i4_smem(bar)), "r"(tiles * count * TILE) : "memory");
-                    for (int u = 0; u < tiles; ++u)
-                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                                     ::"r"(base + S::CODES + (run % RAW * 8 + u) * RUN * TILE),
-                                     "l"(a.w + ((size_t)(unit0 + u) * a.kblocks + kb_begin + run * RUN) * TILE), "r"(count * TILE), "r"(i4_smem(bar)) : "memory");
-                    ++run;
-                }
-                if (!ok) break;
+            int run = min(runs, RAW);
+            for (; run < runs && ok; ++run) {
+                ok = i4_wait(&raw_empty[run % RAW], (run / RAW - 1) & 1);
+                if (ok) copy_codes(run);
+                else break;
+            }
+            if (!ok) {
+                atomicCAS(a.status, 0, 52);
+                for (int i = max(0, run - RAW); i < run; ++i) i4_wait(&raw_full[i % RAW], (i / RAW) & 1);      // what is on its way lands first
+            }
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        // ---- the copies of tokens, two blocks of columns at a time
+        if (lane == 0) {
+            int i = 0;
+            for (; i < pairs && ok; ++i) {
                 if (i >= XS) ok = i4_wait(&x_empty[i % XS], (i / XS - 1) & 1);
                 if (!ok) break;
                 uint64_t* bar = &x_full[i % XS];
@@ -257,19 +271,16 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                                  ::"r"(base + S::X + (i % XS * 2 + k) * S::XSTEP), "l"(a.x + (size_t)(kb_begin + 2 * i + k) * S::XB), "r"(S::XB), "r"(i4_smem(bar))
                                  : "memory");
-                copied = i + 1;
             }
             if (!ok) {
                 atomicCAS(a.status, 0, 52);
-                // what is on its way lands before the block's memory is another's
-                for (int i = max(0, copied - XS); i < copied; ++i) i4_wait(&x_full[i % XS], (i / XS) & 1);
-                for (int i = max(0, run - RAW); i < run; ++i) i4_wait(&raw_full[i % RAW], (i / RAW) & 1);
+                for (int k = max(0, i - XS); k < i; ++k) i4_wait(&x_full[k % XS], (k / XS) & 1);
             }
         }
         __syncwarp();
-    } else if (warp < 2 + MAKERS) {
+    } else if (warp < FIRST + MAKERS) {
         // ---- codes into float16 integers: two tiles of 16 rows a warp
-        const int maker = warp - 2, r = lane >> 2, l = lane & 3;
+        const int maker = warp - FIRST, r = lane >> 2, l = lane & 3;
         for (int i = 0; i < pairs && ok; ++i) {
             const int run = 2 * i / RUN;
             if (2 * i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
@@ -307,7 +318,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         if (!ok && lane == 0) atomicCAS(a.status, 0, 53);
     } else {
         // ---- the sums: a row and half of the tokens a lane; the next group's products are on their way while this one's are added
-        const int quad = warp & 3, row = quad * 32 + lane, unit = row >> 4, first = (warp - 2 - MAKERS) / 4 * PART;
+        const int quad = warp & 3, row = quad * 32 + lane, unit = row >> 4, first = (warp - FIRST - MAKERS) / 4 * PART;
         const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + first;
 #pragma unroll
         for (int t = 0; t < PART; ++t) y[t] = 0.f;
@@ -367,10 +378,10 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
     float* total = reinterpret_cast<float*>(sm);
-    if (warp >= 2 + MAKERS) {
-        const int row = (warp & 3) * 32 + lane, first = (warp - 2 - MAKERS) / 4 * PART;
+    if (warp >= FIRST + MAKERS) {
+        const int row = (warp & 3) * 32 + lane, first = (warp - FIRST - MAKERS) / 4 * PART;
 #pragma unroll
-        for (int t = 0; t < PART; ++t) total[row * S::LD + first + t] = y[t];
+        for (int t = 0; t < PART; ++t) total[(first + t) * ROWS + row] = y[t];
     }
     if (a.slices > 1) cluster_sync();
     else __syncthreads();
@@ -381,15 +392,15 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         const int t = o / outs, i = o - t * outs, row = a.gated ? (i >> 3) * 16 + (i & 7) : i;
         const int n = a.gated ? unit0 * 8 + i : unit0 * 16 + i;
         if (n >= a.N) continue;
-        float v = total[row * S::LD + t], u = a.gated ? total[(row + 8) * S::LD + t] : 0.f;
+        float v = total[t * ROWS + row], u = a.gated ? total[t * ROWS + row + 8] : 0.f;
         if (a.slices > 1) {
             float vs[8], us[8];
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
                 vs[s] = us[s] = 0.f;
                 if (s < a.slices) {
-                    vs[s] = load_cluster(i4_smem(total + row * S::LD + t), s);
-                    if (a.gated) us[s] = load_cluster(i4_smem(total + (row + 8) * S::LD + t), s);
+                    vs[s] = load_cluster(i4_smem(total + t * ROWS + row), s);
+                    if (a.gated) us[s] = load_cluster(i4_smem(total + t * ROWS + row + 8), s);
                 }
             }
             v = u = 0.f;
