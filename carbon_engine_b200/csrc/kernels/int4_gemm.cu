@@ -577,7 +577,7 @@ cudaError_t launch_tiles(const GemmArgs& a, int row_tiles, cudaStream_t stream) 
 
 }  // namespace
 
-long long ce_int4_gemm_tc_scratch(int M, int K, int kept);
+long long ce_int4_gemm_tc_scratch(int M, int K);
 int ce_int4_gemm_tc(const void* x, long long ldx, const void* w, void* out, int ldo, int M, int N, int K, int kept, int mode, float* scratch, int* status,
                     cudaStream_t stream);
 
@@ -594,7 +594,7 @@ bool streamed(int dtype, int M, int K) {
 // float32 words of scratch memory (0: none) for a product of M tokens and K columns
 extern "C" long long ce_int4_gemm_scratch(int dtype, int M, int K, int group) {
     if (streamed(dtype, M, K)) return 0;
-    if (dtype == CE_BF16) return ce_int4_gemm_tc_scratch(M, K, group < 64 ? group : 64);
+    if (dtype == CE_BF16) return ce_int4_gemm_tc_scratch(M, K);
     const long long tiles = (M + 7) / 8, kblocks = (K + 63) / 64;
     return kblocks * tiles * pieces(dtype) * 256 + kblocks * (64 / (group < 64 ? group : 64)) * tiles * 8 + tiles * 8;
 }

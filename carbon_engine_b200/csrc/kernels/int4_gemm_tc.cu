@@ -5,18 +5,21 @@
 // A block takes 128 rows of the weight (8 tiles of 16) and a slice of K; blocks of a cluster share K.  For each group of columns, tcgen05.mma forms
 // the codes' products with all tokens in a piece of tensor memory of its own; eight warps (a row and half of the tokens a lane) read it back and
 // add it to their sums in float32, times the row's step: no value of W is ever rounded, and what is read back is as much work as the products are.
-// Four warps turn codes into float16 integers (c - 8, the even ones, 16 (c - 8), the odd: the tokens are laid out to match), one issues the
-// products, one the copies of codes - before the tokens are there - and one those of tokens.  Slices' sums are added in their order through shared memory.  The parts hand each other 128
-// columns at a time: a hand-over costs some 0.2 us whatever it hands over.
+// The second term is a product too, of 4 columns a group, added up in tensor memory: (s, z, s, z) with the groups' sums in two float16 pieces
+// (8 hi, hi, 8 lo, lo).  (Read from shared memory and added in registers it takes 256 of the 650 cycles of a group: a whole warp's load of the
+// same 16 bytes occupies the pipe as long as one of 512.)  Four warps turn codes into float16 integers (c - 8, the even ones, 16 (c - 8), the odd:
+// the tokens are laid out to match), one issues the products, one the copies of codes - before the tokens are there - and one those of tokens.
+// Slices' sums are added in their order through shared memory.  The parts hand each other 128 columns at a time: a hand-over costs some 0.2 us
+// whatever it hands over.
 //
 // The tokens come prepared (int4_tokens_kernel): each brought into [2^14, 2^15) by a power of two and rounded to float16 - exact for bfloat16 down
-// to 2^-30 of the token's largest - as the second operand's image, swizzle included, and the groups' sums behind it.
+// to 2^-30 of the token's largest - as the second operands' images, swizzle included.
 #include "int4.cuh"
 
 namespace {
 
 constexpr int ROWS = 128, MAKERS = 4, ADDERS = 8, FIRST = 3, THREADS = 32 * (FIRST + MAKERS + ADDERS);
-constexpr int RUN = 4, RAW = 4, XS = 4, AS = 2, DS = 8;     // blocks of 64 columns a copy of codes; stages of codes, tokens, operands (two blocks each); pieces of tensor memory
+constexpr int RUN = 4, RAW = 4, XS = 4, AS = 2, DS = 7;     // blocks of 64 columns a copy of codes; stages of codes, tokens, operands (two blocks each); pieces of tensor memory
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(i4_smem(bar)), "r"(count));
@@ -74,12 +77,18 @@ __device__ __forceinline__ float load_cluster(uint32_t local, int rank) {
 
 enum { STORE = 0, STORE_F32 = 1, ACCUM_F32 = 2, SWIGLU = 3, RELUGLU = 4, RELU2 = 5 };
 
-// bytes of a block of 64 columns of the prepared tokens: the operand's image, then the groups' sums, token by token
-__host__ __device__ constexpr int tokens_bytes(int tokens, int group) { return tokens * 128 + (64 / group) * tokens * 4; }
+// A K-major operand without a swizzle: 8 rows of 16 bytes side by side, groups of 8 rows 128 bytes apart, the second 8 columns ``ahead`` bytes on
+__device__ __forceinline__ uint64_t desc_plain(uint32_t addr, uint32_t ahead) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(ahead >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// bytes of a block of 64 columns of the prepared tokens: the operand's image, then 16 bytes a token of the groups' sums (2^-9 of them, of 64
+// values below 2^15 each, is what float16 holds eight times of)
+__host__ __device__ constexpr int tokens_bytes(int tokens) { return tokens * 144; }
+constexpr float SUMS = 512.0f;
 
 struct TokensArgs {
     const __nv_bfloat16* x;
-    unsigned char* to;             // [kblocks][tokens_bytes], then float32 [tokens]: what a token's sums are multiplied by at the end
+    unsigned char* to;             // [kblocks + 1][tokens_bytes], the last of zeros, then float32 [tokens]: what a token's sums are multiplied by at the end
     long long ld;
     int M, K, kblocks, tokens, group, vec;
 };
@@ -87,7 +96,7 @@ struct TokensArgs {
 __global__ void __launch_bounds__(1024) int4_tokens_kernel(TokensArgs a) {
     ce_pdl_begin();
     __shared__ float scratch[32];
-    const int t = blockIdx.x, per_block = tokens_bytes(a.tokens, a.group);
+    const int t = blockIdx.x, per_block = tokens_bytes(a.tokens);
     const bool real = t < a.M;
     const __nv_bfloat16* src = a.x + (size_t)(real ? t : 0) * a.ld;
     auto load8 = [&](int c) {
@@ -118,9 +127,9 @@ __global__ void __launch_bounds__(1024) int4_tokens_kernel(TokensArgs a) {
     for (int c = threadIdx.x * 8 + KEPT * STEP; c < a.K; c += STEP) look(load8(c));
     largest = ce_block_max(finite ? largest : INFINITY, scratch);
     const float up = i4_row_scale(largest);
-    if (threadIdx.x == 0) reinterpret_cast<float*>(a.to + (size_t)a.kblocks * per_block)[t] = 1.0f / up;
+    if (threadIdx.x == 0) reinterpret_cast<float*>(a.to + (size_t)(a.kblocks + 1) * per_block)[t] = 1.0f / up;
     auto put = [&](int c, uint4 u) {
-        if (c >= a.kblocks * 64) return;              // (8 threads, a block of 64 columns, together)
+        if (c >= (a.kblocks + 1) * 64) return;              // (8 threads, a block of 64 columns, together)
         const uint32_t in[4] = {u.x, u.y, u.z, u.w};
         float y[8], sum = 0.f;
 #pragma unroll
@@ -139,11 +148,18 @@ __global__ void __launch_bounds__(1024) int4_tokens_kernel(TokensArgs a) {
         sum += __shfl_xor_sync(here, sum, 1);
         sum += __shfl_xor_sync(here, sum, 2);
         if (a.group == 64) sum += __shfl_xor_sync(here, sum, 4);
-        if (c % a.group == 0) reinterpret_cast<float*>(block + a.tokens * 128)[(c & 63) / a.group * a.tokens + t] = sum;
+        if (c % a.group == 0) {
+            sum *= 1.0f / SUMS;
+            const float hi = __half2float(__float2half_rn(sum)), lo = sum - hi;
+            const uint32_t first = i4_pack(8.0f * hi, hi), second = i4_pack(8.0f * lo, lo);
+            unsigned char* sums = block + a.tokens * 128 + (t >> 3) * 128 + (t & 7) * 16;
+            if (a.group == 64) *reinterpret_cast<uint4*>(sums) = make_uint4(first, second, 0, 0);
+            else *reinterpret_cast<uint2*>(sums + (c & 32) / 4) = make_uint2(first, second);
+        }
     };
 #pragma unroll
     for (int i = 0; i < KEPT; ++i) put(threadIdx.x * 8 + i * STEP, kept[i]);
-    for (int c = threadIdx.x * 8 + KEPT * STEP; c < a.kblocks * 64; c += STEP) put(c, load8(c));
+    for (int c = threadIdx.x * 8 + KEPT * STEP; c < (a.kblocks + 1) * 64; c += STEP) put(c, load8(c));
 }
 
 struct Args {
@@ -156,8 +172,8 @@ struct Args {
 
 template <int G, int TOKENS>
 struct Shape {
-    static constexpr int TILE = i4_weight_tile_bytes(G), XB = tokens_bytes(TOKENS, G), XSTEP = (XB + 1023) / 1024 * 1024;     // XSTEP: of a block in shared memory
-    static constexpr uint32_t A = 0, X = AS * 2 * ROWS * 128, CODES = X + XS * 2 * XSTEP, BARS = CODES + RAW * 8 * RUN * TILE;
+    static constexpr int TILE = i4_weight_tile_bytes(G), XB = tokens_bytes(TOKENS), XSTEP = (XB + 1023) / 1024 * 1024;     // XSTEP: of a block in shared memory
+    static constexpr uint32_t A = 0, Z = AS * 2 * ROWS * 128, X = Z + AS * ROWS * 32, CODES = X + XS * 2 * XSTEP, BARS = CODES + RAW * 8 * RUN * TILE;
     static constexpr uint32_t BYTES = BARS + 8 * (2 * RAW + 2 * XS + 2 * AS + 2 * DS + 2);
     static_assert(TOKENS * ROWS * 4 <= CODES, "sums");                   // of the slices, token by token, in the place of the stages
 };
@@ -183,7 +199,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], MAKERS + ADDERS); }
-        for (int i = 0; i < XS; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1 + ADDERS); }
+        for (int i = 0; i < XS; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
         for (int i = 0; i < AS; ++i) { mbar_init(&a_full[i], MAKERS); mbar_init(&a_empty[i], 1); }
         for (int i = 0; i < DS; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], ADDERS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -224,6 +240,8 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
             if (!ok) break;
             const uint32_t a_addr = base + S::A + i % AS * 2 * ROWS * 128, x_addr = base + S::X + i % XS * 2 * S::XSTEP;
             const int groups = min(2, n_kb - 2 * i) * GB;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            umma(tmem + DS * 64, desc_plain(base + S::Z + i % AS * ROWS * 32, ROWS * 16), desc_plain(x_addr + TOKENS * 128, S::XSTEP), idesc, i > 0 ? 1u : 0u);
 #pragma unroll
             for (int g = 0; g < 2 * GB; ++g) {
                 if (g >= groups) break;
@@ -265,9 +283,9 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 if (i >= XS) ok = i4_wait(&x_empty[i % XS], (i / XS - 1) & 1);
                 if (!ok) break;
                 uint64_t* bar = &x_full[i % XS];
-                const int count = min(2, n_kb - 2 * i);
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(i4_smem(bar)), "r"(count * S::XB) : "memory");
-                for (int k = 0; k < count; ++k)
+                // (a last block alone: the one behind it comes along, for a product with zeros)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(i4_smem(bar)), "r"(2 * S::XB) : "memory");
+                for (int k = 0; k < 2; ++k)
                     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                                  ::"r"(base + S::X + (i % XS * 2 + k) * S::XSTEP), "l"(a.x + (size_t)(kb_begin + 2 * i + k) * S::XB), "r"(S::XB), "r"(i4_smem(bar))
                                  : "memory");
@@ -291,6 +309,14 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     w[k][u] = *reinterpret_cast<const uint4*>(sm + S::CODES + ((run % RAW * 8 + maker * 2 + u) * RUN + 2 * i % RUN + k) * TILE + lane * 16);
+            uint4 z[2];                                 // of row 32 maker + lane: (s, z, s, z) a group
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t* step = reinterpret_cast<const uint32_t*>(
+                    sm + S::CODES + ((run % RAW * 8 + maker * 2 + (lane >> 4)) * RUN + 2 * i % RUN + k) * TILE + 512 + (lane & 15) * GB * 4);
+                z[k] = make_uint4(0, 0, 0, 0);
+                if (2 * i + k < n_kb) { z[k].x = z[k].y = step[0]; if (GB == 2) z[k].z = z[k].w = step[GB - 1]; }
+            }
             if (2 * i % RUN == RUN - 2 || i == pairs - 1) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
@@ -298,6 +324,8 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
             if (i >= AS) ok = warp_wait(&a_empty[i % AS], (i / AS - 1) & 1);
             if (!ok) break;
             unsigned char* to = sm + S::A + i % AS * 2 * ROWS * 128;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(sm + S::Z + i % AS * ROWS * 32 + k * ROWS * 16 + (maker * 32 + lane) * 16) = z[k];
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -334,8 +362,6 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
             }
-            ok = warp_wait(&x_full[i % XS], (i / XS) & 1);
-            if (!ok) break;
             uint32_t got[2][PART];
             auto fetch = [&](int g) {
                 const int d = i * 2 * GB + g;
@@ -352,23 +378,21 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&d_empty[(i * 2 * GB + g) % DS]);
                 if (g + 1 < 2 * GB && g + 1 < groups) fetch(g + 1);
-                const float2 f = i4_step_of<true>(step[g]);
-                const float2 s2 = make_float2(f.x, f.x), z2 = make_float2(f.y, f.y);
-                const float* sums = reinterpret_cast<const float*>(sm + S::X + (i % XS * 2 + g / GB) * S::XSTEP + TOKENS * 128) + g % GB * TOKENS + first;
+                const float f = i4_step_of<false>(step[g]).x;
 #pragma unroll
-                for (int t = 0; t < PART; t += 4) {
-                    const float4 v = *reinterpret_cast<const float4*>(sums + t);
+                for (int t = 0; t < PART; t += 2) {
                     const uint32_t* c = &got[g & 1][t];
-                    float2 p = __ffma2_rn(z2, make_float2(v.x, v.y), make_float2(y[t], y[t + 1]));
-                    float2 q = __ffma2_rn(z2, make_float2(v.z, v.w), make_float2(y[t + 2], y[t + 3]));
-                    p = __ffma2_rn(s2, make_float2(__uint_as_float(c[0]), __uint_as_float(c[1])), p);
-                    q = __ffma2_rn(s2, make_float2(__uint_as_float(c[2]), __uint_as_float(c[3])), q);
-                    y[t] = p.x; y[t + 1] = p.y; y[t + 2] = q.x; y[t + 3] = q.y;
+                    const float2 p = __ffma2_rn(make_float2(f, f), make_float2(__uint_as_float(c[0]), __uint_as_float(c[1])), make_float2(y[t], y[t + 1]));
+                    y[t] = p.x; y[t + 1] = p.y;
                 }
             }
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(&x_empty[i % XS]);
         }
+        // the second term (its last product was issued before the last group's)
+        uint32_t got[PART];
+        tmem_ld<PART>(from + DS * 64, got);
+        tmem_landed<PART>(got);
+#pragma unroll
+        for (int t = 0; t < PART; ++t) y[t] = fmaf(SUMS, __uint_as_float(got[t]), y[t]);
         if (!ok && lane == 0) atomicCAS(a.status, 0, 54);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -470,9 +494,9 @@ int run(TokensArgs p, Args a, cudaStream_t stream) {
 }  // namespace
 
 // float32 words of scratch memory for M tokens (at most 64) of K columns
-long long ce_int4_gemm_tc_scratch(int M, int K, int kept) {
+long long ce_int4_gemm_tc_scratch(int M, int K) {
     const int tokens = M <= 32 ? 32 : 64;
-    return (long long)((K + 63) / 64) * tokens_bytes(tokens, kept) / 4 + tokens;
+    return (long long)((K + 63) / 64 + 1) * tokens_bytes(tokens) / 4 + tokens;
 }
 
 // The checks of ce_int4_gemm come first: it calls this.  scratch: on a 16-byte boundary; kept: columns of a group in the weight's tiles (32 or 64)
@@ -481,7 +505,7 @@ int ce_int4_gemm_tc(const void* x, long long ldx, const void* w, void* out, int 
     const int tokens = M <= 32 ? 32 : 64, kblocks = (K + 63) / 64, gated = mode == SWIGLU || mode == RELUGLU;
     unsigned char* to = (unsigned char*)scratch;
     TokensArgs p{(const __nv_bfloat16*)x, to, ldx, M, K, kblocks, tokens, kept, ((uintptr_t)x & 15) == 0 && ldx % 8 == 0};
-    Args a{(const unsigned char*)w, to, reinterpret_cast<const float*>(to + (size_t)kblocks * tokens_bytes(tokens, kept)), out, status, M, N, kblocks,
+    Args a{(const unsigned char*)w, to, reinterpret_cast<const float*>(to + (size_t)(kblocks + 1) * tokens_bytes(tokens)), out, status, M, N, kblocks,
            gated ? (N + 7) / 8 : (N + 15) / 16, 1, ldo, mode, gated, 0};
     if (tokens == 32) return kept == 32 ? run<32, 32>(p, a, stream) : run<64, 32>(p, a, stream);
     return kept == 32 ? run<32, 64>(p, a, stream) : run<64, 64>(p, a, stream);
