@@ -77,15 +77,22 @@ __device__ __forceinline__ void i4_mma_first(float (&c)[4], uint32_t a0, uint32_
 }
 
 __device__ __forceinline__ uint32_t i4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// A warp's wait for a copy, with a limit: the thread sleeps in the instruction itself, which leaves the issue slots to the warps that compute
-// (1 token, 75,776 x 4,096: 40.5 us with a loop of tests).
+__device__ __forceinline__ uint32_t i4_arrived(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(i4_smem(bar)), "r"(parity) : "memory");
+    return ok;
+}
+// A lane's wait for a barrier's phase, with a limit: the thread sleeps in the instruction itself.
 __device__ __forceinline__ bool i4_wait(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < (1u << 16); ++i) {
-        uint32_t ok;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(ok) : "r"(i4_smem(bar)), "r"(parity) : "memory");
-        if (ok) return true;
-    }
+    for (uint32_t i = 0; i < (1u << 16); ++i)
+        if (i4_arrived(bar, parity)) return true;
+    return false;
+}
+// A whole warp's: its lanes leave together.
+__device__ __forceinline__ bool i4_warp_wait(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < (1u << 16); ++i)
+        if (__all_sync(0xffffffffu, i4_arrived(bar, parity))) return true;
     return false;
 }
 // A run of bytes into shared memory, counted on the barrier (both addresses and the size in multiples of 16); one lane calls it.

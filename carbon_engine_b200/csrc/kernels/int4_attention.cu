@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
     bool ok = true;
     int gone = 0;                                     // tiles whose copies this warp has waited for
     for (int i = 0; i < mine; ++i, ++gone) {
-        ok = i4_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
+        ok = i4_warp_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
         if (!ok) { if (lane == 0) atomicExch(a.status, 7); break; }
         const unsigned char* tile = ring + (i % STAGES) * TILE;
         const int key0 = (tile_lo + begin + warp + i * WARPS) * 16;

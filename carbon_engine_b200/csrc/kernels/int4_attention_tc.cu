@@ -28,7 +28,6 @@ namespace {
 
 constexpr int BN = 64, STAGES = 3, RAW = 3;      // RAW: tiles of codes a making warp has on the way
 constexpr int MAKERS = 6, SOFTMAX = 8, THREADS = 32 * (2 + MAKERS + SOFTMAX);
-constexpr uint32_t SPIN_LIMIT = 1u << 16;
 constexpr float LIFT = 6.0f, HEADROOM = 8.0f;
 
 struct Args {
@@ -48,19 +47,6 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(i4_smem(bar)) : "memory");
 }
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
-        uint32_t ok;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(ok) : "r"(i4_smem(bar)), "r"(parity) : "memory");
-        if (ok) return true;
-        if (i > 64) __nanosleep(128);
-    }
-    return false;
-}
-// a warp's wait: one verdict for all lanes
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
-
 // Shared-memory operand descriptors, 128-byte swizzle.  K-major: rows of 128 bytes along K, 8-row groups 1024 bytes apart.  MN-major: rows of 128
 // bytes along MN (64 elements), one row per k, 8-row groups 1024 bytes apart, the next 64 MN elements ``next`` bytes further.
 __device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
@@ -208,11 +194,11 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
             const uint32_t tmem_s = tmem + m * 128, tmem_o = tmem + 256 + m * D, q_addr = base + S::Q + m * S::Q_BYTES;
             int where = 62;
-            bool ok = warp_wait(&q_full, 0);
+            bool ok = i4_warp_wait(&q_full, 0);
             auto scores = [&](int j) {
                 const int s = j % STAGES;
                 where = 63;
-                ok = warp_wait(&k_full[s], (j / STAGES) & 1);
+                ok = i4_warp_wait(&k_full[s], (j / STAGES) & 1);
                 if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t k_addr = base + S::KV + s * 2 * S::KV_BYTES;
@@ -228,7 +214,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             for (int j = 0; j < n_kv && ok; ++j) {
                 const int s = j % STAGES;
                 where = 65;
-                ok = warp_wait(&v_full[s], (j / STAGES) & 1) && warp_wait(&p_full[2 * m + (j & 1)], (j >> 1) & 1);
+                ok = i4_warp_wait(&v_full[s], (j / STAGES) & 1) && i4_warp_wait(&p_full[2 * m + (j & 1)], (j >> 1) & 1);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t v_addr = base + S::KV + s * 2 * S::KV_BYTES + S::KV_BYTES;
@@ -240,7 +226,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                 if (j + 2 < n_kv) {
                     // (products of different shapes are not promised to run in order: P(j) has been read before its place is written again)
                     where = 64;
-                    ok = warp_wait(&pv_done[m], j & 1);
+                    ok = i4_warp_wait(&pv_done[m], j & 1);
                     if (ok) scores(j + 2);
                 }
             }
@@ -283,7 +269,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             uint32_t ks[2][NG], vs[4][NG];              // steps of tokens r and r + 8; of the four tokens of this lane's words of values
             auto token_of = [&](int e) { return 2 * l + (e & 1) + 8 * (e >> 1); };
             if (here) {
-                ok = __all_sync(0xffffffffu, i4_wait(&raw_bars[i % RAW], phase >> (i % RAW) & 1));
+                ok = i4_warp_wait(&raw_bars[i % RAW], phase >> (i % RAW) & 1);
                 phase ^= 1u << (i % RAW);
                 if (!ok) break;
 #pragma unroll
@@ -313,7 +299,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                         if (!in(token_of(e))) vs[e][g] = 0;
                 }
             }
-            if (j >= STAGES) ok = warp_wait(&k_empty[s], (j / STAGES - 1) & 1);
+            if (j >= STAGES) ok = i4_warp_wait(&k_empty[s], (j / STAGES - 1) & 1);
             if (!ok) break;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -328,7 +314,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_full[s]);
-            if (j >= STAGES) ok = warp_wait(&v_empty[s], (j / STAGES - 1) & 1);
+            if (j >= STAGES) ok = i4_warp_wait(&v_empty[s], (j / STAGES - 1) & 1);
             if (!ok) break;
             // groups of values that are not numbers: noted, and zeros in the tile
 #pragma unroll
@@ -411,7 +397,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             for (int j = 0; j < n_kv; ++j) {
                 const int k0 = k_begin + j * BN;
                 where = 66;
-                if (!warp_wait(&s_full[2 * m + (j & 1)], (j >> 1) & 1)) { ok = false; break; }
+                if (!i4_warp_wait(&s_full[2 * m + (j & 1)], (j >> 1) & 1)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float sv[BN];
                 tmem_ld<BN>(tmem_s + (j & 1) * BN, sv);
@@ -449,7 +435,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                 if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
                     // (the product of tile j - 2 is done: this tile's scores were issued behind it)
                     where = 67;
-                    if (!warp_wait(&pv_done[m], (j - 1) & 1)) { ok = false; break; }
+                    if (!i4_warp_wait(&pv_done[m], (j - 1) & 1)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
@@ -465,7 +451,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                 // values that are no numbers among this tile's keys
                 where = 68;
                 const int s = j % STAGES;
-                if (!warp_wait(&v_full[s], (j / STAGES) & 1)) { ok = false; break; }
+                if (!i4_warp_wait(&v_full[s], (j / STAGES) & 1)) { ok = false; break; }
                 const unsigned long long* bad = reinterpret_cast<const unsigned long long*>(nan_keys + s * 8 * 4);
                 unsigned long long any = 0;
 #pragma unroll
@@ -486,7 +472,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             if (ok) {
                 where = 67;
                 // the last two products may both be under way, and a parity tells one from the next only
-                ok = (n_kv < 2 || warp_wait(&pv_done[m], (n_kv - 2) & 1)) && warp_wait(&pv_done[m], (n_kv - 1) & 1);
+                ok = (n_kv < 2 || i4_warp_wait(&pv_done[m], (n_kv - 2) & 1)) && i4_warp_wait(&pv_done[m], (n_kv - 1) & 1);
             }
             if (!ok && lane == 0) atomicCAS(a.status, 0, where);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

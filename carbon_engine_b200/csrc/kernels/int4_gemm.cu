@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(SW * 32) int4_stream_kernel(StreamArgs a) {
     for (int it = 0; it < its; ++it) {
         float* to = mine + it % BATCH * (SW * SUMS);
         if (count > 0) {
-            if (gave_up < 0 && !i4_wait(&full[warp][it % STAGES], (it / STAGES) & 1)) {
+            if (gave_up < 0 && !i4_warp_wait(&full[warp][it % STAGES], (it / STAGES) & 1)) {
                 gave_up = it;
                 atomicExch(a.status, 59);
             }

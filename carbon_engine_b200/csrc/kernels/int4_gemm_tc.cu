@@ -19,7 +19,9 @@
 namespace {
 
 constexpr int ROWS = 128, MAKERS = 4, ADDERS = 8, FIRST = 3, THREADS = 32 * (FIRST + MAKERS + ADDERS);
-constexpr int RUN = 4, RAW = 4, XS = 4, AS = 2, DS = 7;     // blocks of 64 columns a copy of codes; stages of codes, tokens, operands (two blocks each); pieces of tensor memory
+constexpr int RUN = 4, RAW = 4, XS = 4, AS = 3, DS = 2;     // blocks of 64 columns a copy of codes; stages of codes, tokens and operands (two blocks each), of sums (two groups each)
+constexpr int SUM_AT = 64 * 2 * DS, A_AT = SUM_AT + 64;      // columns of tensor memory: products, the second term, operands
+static_assert(A_AT + 64 * AS <= 512, "tensor memory");
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(i4_smem(bar)), "r"(count));
@@ -27,7 +29,6 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(i4_smem(bar)) : "memory");
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, i4_wait(bar, parity)); }
 __device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
@@ -35,6 +36,17 @@ __device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
 __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
                  ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// the same with the first operand in tensor memory: a row a lane, two values a column
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// 16 rows of 32 columns: a lane's words of rows lane / 4 (even ones) and 8 on (odd ones), every fourth column
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&q)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::"r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]), "r"(q[4]), "r"(q[5]), "r"(q[6]), "r"(q[7]),
+                   "r"(q[8]), "r"(q[9]), "r"(q[10]), "r"(q[11]), "r"(q[12]), "r"(q[13]), "r"(q[14]), "r"(q[15]), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
@@ -143,7 +155,10 @@ __global__ void __launch_bounds__(1024) int4_tokens_kernel(TokensArgs a) {
             sum += (got.x + got.y) * b;
         }
         unsigned char* block = a.to + (size_t)(c >> 6) * per_block;
-        *reinterpret_cast<uint4*>(block + t * 128 + ((((c >> 3) & 7) ^ (t & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        // columns in the order in which tmem_st lays the codes out: these words are every fourth of 16
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint32_t*>(block + t * 128 + ((((c & 32) / 8 + i) ^ (t & 7)) << 4) + ((c >> 3) & 3) * 4) = w[i];
         const unsigned here = 0xffu << (threadIdx.x & 24);
         sum += __shfl_xor_sync(here, sum, 1);
         sum += __shfl_xor_sync(here, sum, 2);
@@ -173,9 +188,9 @@ struct Args {
 template <int G, int TOKENS>
 struct Shape {
     static constexpr int TILE = i4_weight_tile_bytes(G), XB = tokens_bytes(TOKENS), XSTEP = (XB + 1023) / 1024 * 1024;     // XSTEP: of a block in shared memory
-    static constexpr uint32_t A = 0, Z = AS * 2 * ROWS * 128, X = Z + AS * ROWS * 32, CODES = X + XS * 2 * XSTEP, BARS = CODES + RAW * 8 * RUN * TILE;
+    static constexpr uint32_t X = 0, Z = XS * 2 * XSTEP, CODES = Z + AS * ROWS * 32, BARS = CODES + RAW * 8 * RUN * TILE;
     static constexpr uint32_t BYTES = BARS + 8 * (2 * RAW + 2 * XS + 2 * AS + 2 * DS + 2);
-    static_assert(TOKENS * ROWS * 4 <= CODES, "sums");                   // of the slices, token by token, in the place of the stages
+    static_assert(TOKENS * ROWS * 4 <= BARS, "sums");                   // of the slices, token by token, in the place of the stages
 };
 
 template <int G, int TOKENS>
@@ -236,23 +251,27 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         // ---- the products: a group's of all tokens into the next piece of tensor memory
         const uint32_t idesc = (1u << 4) | ((uint32_t)(TOKENS >> 3) << 17) | (8u << 24);
         for (int i = 0; i < pairs && ok; ++i) {
-            ok = warp_wait(&x_full[i % XS], (i / XS) & 1) && warp_wait(&a_full[i % AS], (i / AS) & 1);
+            ok = i4_warp_wait(&x_full[i % XS], (i / XS) & 1) && i4_warp_wait(&a_full[i % AS], (i / AS) & 1);
             if (!ok) break;
-            const uint32_t a_addr = base + S::A + i % AS * 2 * ROWS * 128, x_addr = base + S::X + i % XS * 2 * S::XSTEP;
+            const uint32_t x_addr = base + S::X + i % XS * 2 * S::XSTEP, a_at = tmem + A_AT + i % AS * 64;
             const int groups = min(2, n_kb - 2 * i) * GB;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            umma(tmem + DS * 64, desc_plain(base + S::Z + i % AS * ROWS * 32, ROWS * 16), desc_plain(x_addr + TOKENS * 128, S::XSTEP), idesc, i > 0 ? 1u : 0u);
+            umma(tmem + SUM_AT, desc_plain(base + S::Z + i % AS * ROWS * 32, ROWS * 16), desc_plain(x_addr + TOKENS * 128, S::XSTEP), idesc, i > 0 ? 1u : 0u);
 #pragma unroll
-            for (int g = 0; g < 2 * GB; ++g) {
-                if (g >= groups) break;
-                const int d = i * 2 * GB + g;
-                if (d >= DS) ok = ok && warp_wait(&d_empty[d % DS], (d / DS - 1) & 1);
+            for (int u = 0; u < GB; ++u) {              // two groups at a time
+                const int d = i * GB + u;
+                if (2 * u >= groups) break;
+                if (d >= DS) ok = ok && i4_warp_wait(&d_empty[d % DS], (d / DS - 1) & 1);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                for (int kk = 0; kk < G / 16; ++kk) {
-                    const uint32_t off = (g % GB * (G / 16) + kk) * 32;
-                    umma(tmem + d % DS * 64, desc_kmajor(a_addr + g / GB * ROWS * 128 + off), desc_kmajor(x_addr + g / GB * S::XSTEP + off), idesc, kk > 0 ? 1u : 0u);
+                for (int g = 2 * u; g < 2 * u + 2; ++g) {
+                    if (g >= groups) break;
+#pragma unroll
+                    for (int kk = 0; kk < G / 16; ++kk) {
+                        const int k16 = g % GB * (G / 16) + kk;
+                        umma_ts(tmem + d % DS * 128 + (g & 1) * 64, a_at + g / GB * 32 + k16 * 8, desc_kmajor(x_addr + g / GB * S::XSTEP + k16 * 32), idesc, kk > 0 ? 1u : 0u);
+                    }
                 }
                 umma_commit(&d_full[d % DS]);
             }
@@ -298,10 +317,10 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         __syncwarp();
     } else if (warp < FIRST + MAKERS) {
         // ---- codes into float16 integers: two tiles of 16 rows a warp
-        const int maker = warp - FIRST, r = lane >> 2, l = lane & 3;
+        const int maker = warp & 3;                         // (whose lanes of tensor memory these are)
         for (int i = 0; i < pairs && ok; ++i) {
             const int run = 2 * i / RUN;
-            if (2 * i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
+            if (2 * i % RUN == 0) ok = i4_warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
             if (!ok) break;
             uint4 w[2][2];                              // (an odd last block: the second of the pair holds what lay there, for no product)
 #pragma unroll
@@ -321,24 +340,27 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
             }
-            if (i >= AS) ok = warp_wait(&a_empty[i % AS], (i / AS - 1) & 1);
+            if (i >= AS) ok = i4_warp_wait(&a_empty[i % AS], (i / AS - 1) & 1);
             if (!ok) break;
-            unsigned char* to = sm + S::A + i % AS * 2 * ROWS * 128;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
             for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(sm + S::Z + i % AS * ROWS * 32 + k * ROWS * 16 + (maker * 32 + lane) * 16) = z[k];
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t v[16];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {       // words of rows r and r + 8, first and second 32 columns
-                        const int half = e >> 1, row = 16 * (maker * 2 + u) + r + 8 * (e & 1);
                         const uint32_t word = e == 0 ? w[k][u].x : e == 1 ? w[k][u].y : e == 2 ? w[k][u].z : w[k][u].w;
-                        uint32_t v[4];
-                        i4_pairs<true, 0>(word, v[0], v[1]);
-                        i4_pairs<true, 8>(word, v[2], v[3]);
-                        *reinterpret_cast<uint4*>(to + k * ROWS * 128 + row * 128 + (((half * 4 + l) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                        uint32_t* at = v + (e >> 1) * 8 + (e & 1);
+                        i4_pairs<true, 0>(word, at[0], at[2]);
+                        i4_pairs<true, 8>(word, at[4], at[6]);
                     }
+                    tmem_st(tmem + A_AT + i % AS * 64 + k * 32 + ((uint32_t)(maker * 32 + u * 16) << 16), v);
+                }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&a_full[i % AS]);
@@ -352,7 +374,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         for (int t = 0; t < PART; ++t) y[t] = 0.f;
         for (int i = 0; i < pairs && ok; ++i) {
             const int run = 2 * i / RUN, groups = min(2, n_kb - 2 * i) * GB;
-            if (2 * i % RUN == 0) ok = warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
+            if (2 * i % RUN == 0) ok = i4_warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
             if (!ok) break;
             uint32_t step[2 * GB];
 #pragma unroll
@@ -362,34 +384,35 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
             }
-            uint32_t got[2][PART];
-            auto fetch = [&](int g) {
-                const int d = i * 2 * GB + g;
-                ok = ok && warp_wait(&d_full[d % DS], (d / DS) & 1);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                tmem_ld<PART>(from + d % DS * 64, got[g & 1]);
-            };
-            fetch(0);
 #pragma unroll
-            for (int g = 0; g < 2 * GB; ++g) {
-                if (g >= groups) break;
-                tmem_landed<PART>(got[g & 1]);
+            for (int u = 0; u < GB; ++u) {
+                const int d = i * GB + u;
+                if (2 * u >= groups) break;
+                ok = ok && i4_warp_wait(&d_full[d % DS], (d / DS) & 1);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t got[2][PART];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) tmem_ld<PART>(from + d % DS * 128 + g * 64, got[g]);     // (of a last group alone, the second is not used)
+#pragma unroll
+                for (int g = 0; g < 2; ++g) tmem_landed<PART>(got[g]);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&d_empty[(i * 2 * GB + g) % DS]);
-                if (g + 1 < 2 * GB && g + 1 < groups) fetch(g + 1);
-                const float f = i4_step_of<false>(step[g]).x;
+                if (lane == 0) mbar_arrive(&d_empty[d % DS]);
 #pragma unroll
-                for (int t = 0; t < PART; t += 2) {
-                    const uint32_t* c = &got[g & 1][t];
-                    const float2 p = __ffma2_rn(make_float2(f, f), make_float2(__uint_as_float(c[0]), __uint_as_float(c[1])), make_float2(y[t], y[t + 1]));
-                    y[t] = p.x; y[t + 1] = p.y;
+                for (int g = 0; g < 2; ++g) {
+                    if (2 * u + g >= groups) break;
+                    const float f = i4_step_of<false>(step[2 * u + g]).x;
+#pragma unroll
+                    for (int t = 0; t < PART; t += 2) {
+                        const float2 p = __ffma2_rn(make_float2(f, f), make_float2(__uint_as_float(got[g][t]), __uint_as_float(got[g][t + 1])), make_float2(y[t], y[t + 1]));
+                        y[t] = p.x; y[t + 1] = p.y;
+                    }
                 }
             }
         }
         // the second term (its last product was issued before the last group's)
         uint32_t got[PART];
-        tmem_ld<PART>(from + DS * 64, got);
+        tmem_ld<PART>(from + SUM_AT, got);
         tmem_landed<PART>(got);
 #pragma unroll
         for (int t = 0; t < PART; ++t) y[t] = fmaf(SUMS, __uint_as_float(got[t]), y[t]);
