@@ -19,7 +19,7 @@
 namespace {
 
 constexpr int ROWS = 128, MAKERS = 4, ADDERS = 8, FIRST = 3, THREADS = 32 * (FIRST + MAKERS + ADDERS);
-constexpr int RUN = 4, RAW = 4, XS = 4, AS = 3, DS = 2;     // blocks of 64 columns a copy of codes; stages of codes, tokens and operands (two blocks each), of sums (two groups each)
+constexpr int RUN = 4, RAW = 4, AS = 3, DS = 2;             // blocks of 64 columns a copy of codes; stages of codes, of operands (two blocks each), of sums (two groups each)
 constexpr int SUM_AT = 64 * 2 * DS, A_AT = SUM_AT + 64;      // columns of tensor memory: products, the second term, operands
 static_assert(A_AT + 64 * AS <= 512, "tensor memory");
 
@@ -79,11 +79,11 @@ __device__ __forceinline__ void tmem_landed(uint32_t (&q)[N]) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float load_cluster(uint32_t local, int rank) {
+__device__ __forceinline__ float4 load_cluster(uint32_t local, int rank) {
     uint32_t at;
-    float v;
+    float4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
 
@@ -93,6 +93,18 @@ enum { STORE = 0, STORE_F32 = 1, ACCUM_F32 = 2, SWIGLU = 3, RELUGLU = 4, RELU2 =
 __device__ __forceinline__ uint64_t desc_plain(uint32_t addr, uint32_t ahead) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(ahead >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
+__device__ __forceinline__ void finish(void* out, size_t at, int mode, float v, float up) {
+    __nv_bfloat16* half = (__nv_bfloat16*)out;
+    switch (mode) {
+        case STORE_F32: ((float*)out)[at] = v; break;
+        case ACCUM_F32: ((float*)out)[at] += v; break;
+        case SWIGLU: half[at] = __float2bfloat16_rn(ce_silu_glu(v, up)); break;
+        case RELUGLU: half[at] = __float2bfloat16_rn(fmaxf(v, 0.f) * up); break;
+        case RELU2: v = fmaxf(v, 0.f); half[at] = __float2bfloat16_rn(v * v); break;
+        default: half[at] = __float2bfloat16_rn(v);
+    }
+}
+
 // bytes of a block of 64 columns of the prepared tokens: the operand's image, then 16 bytes a token of the groups' sums (2^-9 of them, of 64
 // values below 2^15 each, is what float16 holds eight times of)
 __host__ __device__ constexpr int tokens_bytes(int tokens) { return tokens * 144; }
@@ -188,8 +200,8 @@ struct Args {
 template <int G, int TOKENS>
 struct Shape {
     static constexpr int TILE = i4_weight_tile_bytes(G), XB = tokens_bytes(TOKENS), XSTEP = (XB + 1023) / 1024 * 1024;     // XSTEP: of a block in shared memory
-    static constexpr uint32_t X = 0, Z = XS * 2 * XSTEP, CODES = Z + AS * ROWS * 32, BARS = CODES + RAW * 8 * RUN * TILE;
-    static constexpr uint32_t BYTES = BARS + 8 * (2 * RAW + 2 * XS + 2 * AS + 2 * DS + 2);
+    static constexpr uint32_t X = 0, Z = AS * 2 * XSTEP, CODES = Z + AS * ROWS * 32, BARS = CODES + RAW * 8 * RUN * TILE;
+    static constexpr uint32_t BYTES = BARS + 8 * (2 * RAW + 2 * AS + 2 * DS + 2);
     static_assert(TOKENS * ROWS * 4 <= BARS, "sums");                   // of the slices, token by token, in the place of the stages
 };
 
@@ -200,8 +212,8 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     extern __shared__ __align__(1024) unsigned char sm[];
     const uint32_t base = i4_smem(sm);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::BARS);
-    uint64_t *raw_full = bars, *raw_empty = bars + RAW, *x_full = raw_empty + RAW, *x_empty = x_full + XS, *a_full = x_empty + XS, *a_empty = a_full + AS;
-    uint64_t *d_full = a_empty + AS, *d_empty = d_full + DS;
+    uint64_t *raw_full = bars, *raw_empty = bars + RAW, *full = raw_empty + RAW, *empty = full + AS;
+    uint64_t *d_full = empty + AS, *d_empty = d_full + DS;
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(d_empty + DS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slice = blockIdx.x % a.slices, unit0 = blockIdx.x / a.slices * 8, tiles = min(8, a.units - unit0);
@@ -214,8 +226,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], MAKERS + ADDERS); }
-        for (int i = 0; i < XS; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
-        for (int i = 0; i < AS; ++i) { mbar_init(&a_full[i], MAKERS); mbar_init(&a_empty[i], 1); }
+        for (int i = 0; i < AS; ++i) { mbar_init(&full[i], MAKERS + 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < DS; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], ADDERS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -251,9 +262,9 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         // ---- the products: a group's of all tokens into the next piece of tensor memory
         const uint32_t idesc = (1u << 4) | ((uint32_t)(TOKENS >> 3) << 17) | (8u << 24);
         for (int i = 0; i < pairs && ok; ++i) {
-            ok = i4_warp_wait(&x_full[i % XS], (i / XS) & 1) && i4_warp_wait(&a_full[i % AS], (i / AS) & 1);
+            ok = i4_warp_wait(&full[i % AS], (i / AS) & 1);
             if (!ok) break;
-            const uint32_t x_addr = base + S::X + i % XS * 2 * S::XSTEP, a_at = tmem + A_AT + i % AS * 64;
+            const uint32_t x_addr = base + S::X + i % AS * 2 * S::XSTEP, a_at = tmem + A_AT + i % AS * 64;
             const int groups = min(2, n_kb - 2 * i) * GB;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             umma(tmem + SUM_AT, desc_plain(base + S::Z + i % AS * ROWS * 32, ROWS * 16), desc_plain(x_addr + TOKENS * 128, S::XSTEP), idesc, i > 0 ? 1u : 0u);
@@ -275,8 +286,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 }
                 umma_commit(&d_full[d % DS]);
             }
-            umma_commit(&a_empty[i % AS]);
-            umma_commit(&x_empty[i % XS]);
+            umma_commit(&empty[i % AS]);
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, 51);
     } else if (warp == 1) {
@@ -299,19 +309,19 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         if (lane == 0) {
             int i = 0;
             for (; i < pairs && ok; ++i) {
-                if (i >= XS) ok = i4_wait(&x_empty[i % XS], (i / XS - 1) & 1);
+                if (i >= AS) ok = i4_wait(&empty[i % AS], (i / AS - 1) & 1);
                 if (!ok) break;
-                uint64_t* bar = &x_full[i % XS];
+                uint64_t* bar = &full[i % AS];
                 // (a last block alone: the one behind it comes along, for a product with zeros)
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(i4_smem(bar)), "r"(2 * S::XB) : "memory");
                 for (int k = 0; k < 2; ++k)
                     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                                 ::"r"(base + S::X + (i % XS * 2 + k) * S::XSTEP), "l"(a.x + (size_t)(kb_begin + 2 * i + k) * S::XB), "r"(S::XB), "r"(i4_smem(bar))
+                                 ::"r"(base + S::X + (i % AS * 2 + k) * S::XSTEP), "l"(a.x + (size_t)(kb_begin + 2 * i + k) * S::XB), "r"(S::XB), "r"(i4_smem(bar))
                                  : "memory");
             }
             if (!ok) {
                 atomicCAS(a.status, 0, 52);
-                for (int k = max(0, i - XS); k < i; ++k) i4_wait(&x_full[k % XS], (k / XS) & 1);
+                for (int k = max(0, i - AS); k < i; ++k) i4_wait(&full[k % AS], (k / AS) & 1);
             }
         }
         __syncwarp();
@@ -340,7 +350,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
             }
-            if (i >= AS) ok = i4_warp_wait(&a_empty[i % AS], (i / AS - 1) & 1);
+            if (i >= AS) ok = i4_warp_wait(&empty[i % AS], (i / AS - 1) & 1);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -363,7 +373,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[i % AS]);
+            if (lane == 0) mbar_arrive(&full[i % AS]);
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, 53);
     } else {
@@ -432,40 +442,35 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     }
     if (a.slices > 1) cluster_sync();
     else __syncthreads();
-    // a row's results of a token: the slices' sums in their order (all of them asked for at once), what was scaled scaled back; a block takes
+    // four rows' results of a token: the slices' sums in their order (all of them asked for at once), what was scaled scaled back; a block takes
     // every ``slices``-th run of results
-    const int outs = a.gated ? 64 : ROWS;
-    for (int o = slice * THREADS + threadIdx.x; o < outs * a.M; o += a.slices * THREADS) {
-        const int t = o / outs, i = o - t * outs, row = a.gated ? (i >> 3) * 16 + (i & 7) : i;
-        const int n = a.gated ? unit0 * 8 + i : unit0 * 16 + i;
-        if (n >= a.N) continue;
-        float v = total[t * ROWS + row], u = a.gated ? total[t * ROWS + row + 8] : 0.f;
+    const int fours = a.gated ? 16 : ROWS / 4;
+    for (int o = slice * THREADS + threadIdx.x; o < fours * a.M; o += a.slices * THREADS) {
+        const int t = a.gated ? o >> 4 : o >> 5, i = (o & (fours - 1)) * 4, row = a.gated ? (i >> 3) * 16 + (i & 7) : i;
+        const int n = unit0 * (a.gated ? 8 : 16) + i;
+        const float back = a.back[t];
+        float* at = total + t * ROWS + row;
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+        auto add = [](float (&x)[4], float4 y) { x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w; };
         if (a.slices > 1) {
-            float vs[8], us[8];
+            float4 vs[8], us[8];
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
-                vs[s] = us[s] = 0.f;
+                vs[s] = us[s] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (s < a.slices) {
-                    vs[s] = load_cluster(i4_smem(total + t * ROWS + row), s);
-                    if (a.gated) us[s] = load_cluster(i4_smem(total + t * ROWS + row + 8), s);
+                    vs[s] = load_cluster(i4_smem(at), s);
+                    if (a.gated) us[s] = load_cluster(i4_smem(at + 8), s);
                 }
             }
-            v = u = 0.f;
 #pragma unroll
-            for (int s = 0; s < 8; ++s) { v += vs[s]; u += us[s]; }
+            for (int s = 0; s < 8; ++s) { add(v, vs[s]); add(u, us[s]); }
+        } else {
+            add(v, *reinterpret_cast<const float4*>(at));
+            if (a.gated) add(u, *reinterpret_cast<const float4*>(at + 8));
         }
-        const float back = a.back[t];
-        v *= back; u *= back;
-        const size_t at = (size_t)t * a.ldo + n;
-        __nv_bfloat16* half = (__nv_bfloat16*)a.out;
-        switch (a.mode) {
-            case STORE_F32: ((float*)a.out)[at] = v; break;
-            case ACCUM_F32: ((float*)a.out)[at] += v; break;
-            case SWIGLU: half[at] = __float2bfloat16_rn(ce_silu_glu(v, u)); break;
-            case RELUGLU: half[at] = __float2bfloat16_rn(fmaxf(v, 0.f) * u); break;
-            case RELU2: v = fmaxf(v, 0.f); half[at] = __float2bfloat16_rn(v * v); break;
-            default: half[at] = __float2bfloat16_rn(v);
-        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (n + k < a.N) finish(a.out, (size_t)t * a.ldo + n + k, a.mode, v[k] * back, u[k] * back);
     }
     if (a.slices > 1) cluster_sync();                   // nobody leaves while its sums are read
 }
