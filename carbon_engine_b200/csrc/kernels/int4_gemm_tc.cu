@@ -7,7 +7,7 @@
 // add it to their sums in float32, times the row's step: no value of W is ever rounded, and what is read back is as much work as the products are.
 // The second term is a product too, of 4 columns a group, added up in tensor memory: (s, z, s, z) with the groups' sums in two float16 pieces
 // (8 hi, hi, 8 lo, lo).  (Read from shared memory and added in registers it takes 256 of the 650 cycles of a group: a whole warp's load of the
-// same 16 bytes occupies the pipe as long as one of 512.)  Four warps turn codes into float16 integers (c - 8, the even ones, 16 (c - 8), the odd:
+// same 16 bytes occupies the pipe as long as one of 512.)  Eight warps turn codes into float16 integers (c - 8, the even ones, 16 (c - 8), the odd:
 // the tokens are laid out to match), one issues the products, one the copies of codes - before the tokens are there - and one those of tokens.
 // Slices' sums are added in their order through shared memory.  The parts hand each other 128 columns at a time: a hand-over costs some 0.2 us
 // whatever it hands over.
@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr int ROWS = 128, MAKERS = 4, ADDERS = 8, FIRST = 3, THREADS = 32 * (FIRST + MAKERS + ADDERS);
+constexpr int ROWS = 128, MAKERS = 8, ADDERS = 8, FIRST = 3, THREADS = 32 * (FIRST + MAKERS + ADDERS);
 constexpr int RUN = 4, RAW = 4, AS = 3, DS = 2;             // blocks of 64 columns a copy of codes; stages of codes, of operands (two blocks each), of sums (two groups each)
 constexpr int SUM_AT = 64 * 2 * DS, A_AT = SUM_AT + 64;      // columns of tensor memory: products, the second term, operands
 static_assert(A_AT + 64 * AS <= 512, "tensor memory");
@@ -326,26 +326,22 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         }
         __syncwarp();
     } else if (warp < FIRST + MAKERS) {
-        // ---- codes into float16 integers: two tiles of 16 rows a warp
-        const int maker = warp & 3;                         // (whose lanes of tensor memory these are)
+        // ---- codes into float16 integers: two tiles of 16 rows of a block of columns a warp
+        const int maker = warp & 3, k = (warp - FIRST) >> 2;        // (whose lanes of tensor memory these are; which block of a pair)
         for (int i = 0; i < pairs && ok; ++i) {
             const int run = 2 * i / RUN;
             if (2 * i % RUN == 0) ok = i4_warp_wait(&raw_full[run % RAW], (run / RAW) & 1);
             if (!ok) break;
-            uint4 w[2][2];                              // (an odd last block: the second of the pair holds what lay there, for no product)
+            // (an odd last block: the second of the pair is what lay there, for no product)
+            uint4 w[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    w[k][u] = *reinterpret_cast<const uint4*>(sm + S::CODES + ((run % RAW * 8 + maker * 2 + u) * RUN + 2 * i % RUN + k) * TILE + lane * 16);
-            uint4 z[2];                                 // of row 32 maker + lane: (s, z, s, z) a group
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t* step = reinterpret_cast<const uint32_t*>(
-                    sm + S::CODES + ((run % RAW * 8 + maker * 2 + (lane >> 4)) * RUN + 2 * i % RUN + k) * TILE + 512 + (lane & 15) * GB * 4);
-                z[k] = make_uint4(0, 0, 0, 0);
-                if (2 * i + k < n_kb) { z[k].x = z[k].y = step[0]; if (GB == 2) z[k].z = z[k].w = step[GB - 1]; }
-            }
+            for (int u = 0; u < 2; ++u)
+                w[u] = *reinterpret_cast<const uint4*>(sm + S::CODES + ((run % RAW * 8 + maker * 2 + u) * RUN + 2 * i % RUN + k) * TILE + lane * 16);
+            // of row 32 maker + lane: (s, z, s, z) a group
+            const uint32_t* step = reinterpret_cast<const uint32_t*>(
+                sm + S::CODES + ((run % RAW * 8 + maker * 2 + (lane >> 4)) * RUN + 2 * i % RUN + k) * TILE + 512 + (lane & 15) * GB * 4);
+            uint4 z = make_uint4(0, 0, 0, 0);
+            if (2 * i + k < n_kb) { z.x = z.y = step[0]; if (GB == 2) z.z = z.w = step[GB - 1]; }
             if (2 * i % RUN == RUN - 2 || i == pairs - 1) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&raw_empty[run % RAW]);
@@ -353,22 +349,19 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
             if (i >= AS) ok = i4_warp_wait(&empty[i % AS], (i / AS - 1) & 1);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            *reinterpret_cast<uint4*>(sm + S::Z + i % AS * ROWS * 32 + k * ROWS * 16 + (maker * 32 + lane) * 16) = z;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(sm + S::Z + i % AS * ROWS * 32 + k * ROWS * 16 + (maker * 32 + lane) * 16) = z[k];
+            for (int u = 0; u < 2; ++u) {
+                uint32_t v[16];
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    uint32_t v[16];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {       // words of rows r and r + 8, first and second 32 columns
-                        const uint32_t word = e == 0 ? w[k][u].x : e == 1 ? w[k][u].y : e == 2 ? w[k][u].z : w[k][u].w;
-                        uint32_t* at = v + (e >> 1) * 8 + (e & 1);
-                        i4_pairs<true, 0>(word, at[0], at[2]);
-                        i4_pairs<true, 8>(word, at[4], at[6]);
-                    }
-                    tmem_st(tmem + A_AT + i % AS * 64 + k * 32 + ((uint32_t)(maker * 32 + u * 16) << 16), v);
+                for (int e = 0; e < 4; ++e) {           // words of rows r and r + 8, first and second 32 columns
+                    const uint32_t word = e == 0 ? w[u].x : e == 1 ? w[u].y : e == 2 ? w[u].z : w[u].w;
+                    uint32_t* at = v + (e >> 1) * 8 + (e & 1);
+                    i4_pairs<true, 0>(word, at[0], at[2]);
+                    i4_pairs<true, 8>(word, at[4], at[6]);
                 }
+                tmem_st(tmem + A_AT + i % AS * 64 + k * 32 + ((uint32_t)(maker * 32 + u * 16) << 16), v);
+            }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
