@@ -1,8 +1,9 @@
 // Quantisation into 4 bits and back: keys and values as they enter the pages of a cache, weights once when they are loaded (format and layout:
 // int4.cuh).
 //
-// One half of a warp takes 64 neighbouring channels, 4 a lane: a group's extremes are found with shuffles, two lanes put the 8 codes of a word
-// together.  Bound by memory for whole prompts and by the launch for single tokens.
+// Eight lanes take 64 neighbouring channels of a token's head, 8 a lane (a word of a key's codes): a group's extremes are found with shuffles.  A
+// weight's kernels give a lane 4 columns.  Bound by the launch and by four loads that wait for one another (position, request, its slot, its page)
+// for single tokens, by the instructions - some 20 a value - for whole prompts.
 #include "int4.cuh"
 
 namespace {
@@ -38,6 +39,46 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, bool vec, const float (
     else { p[0] = a.x; p[1] = a.y; p[2] = b.x; p[3] = b.y; }
 }
 
+__device__ __forceinline__ void load8(const float* p, bool vec, float (&x)[8]) {
+    float a[4], b[4];
+    load4(p, vec, a);
+    load4(p + 4, vec, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[i + 4] = b[i]; }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool vec, float (&x)[8]) {
+    uint32_t w[4];
+    if (vec) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void store8(float* p, bool vec, const float (&x)[8]) {
+    const float a[4] = {x[0], x[1], x[2], x[3]}, b[4] = {x[4], x[5], x[6], x[7]};
+    store4(p, vec, a);
+    store4(p + 4, vec, b);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, bool vec, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    if (vec) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else {
+        unsigned short* q = reinterpret_cast<unsigned short*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = (unsigned short)(w[i >> 1] >> (i & 1 ? 16 : 0));
+    }
+}
+
 // (s, z) of this lane's group and its four codes as 16 bits; ``lanes``: lanes of a group (8, 16 or 32)
 __device__ __forceinline__ unsigned quantise4(const float (&x)[4], int lanes, __half2& sz) {
     float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
@@ -67,67 +108,91 @@ __device__ __forceinline__ unsigned char* tile_of(const CacheArgs& a, int t, int
     return a.pages + (((size_t)page * a.nkv + h) * (a.page_size >> 4) + (in >> 4)) * (size_t)i4_cache_tile_bytes(a.d, a.group);
 }
 
+// the same for 8 channels a lane; ``lanes`` of a group: 4 or 8
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], int lanes, __half2& sz) {
+    float lo = x[0], hi = x[0];
+    bool ok = fabsf(x[0]) <= I4_LIMIT;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); ok = ok && fabsf(x[i]) <= I4_LIMIT; }
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        ok = __shfl_xor_sync(0xffffffffu, (int)ok, o) && ok;
+    }
+    sz = i4_step(lo, hi, ok);
+    const float s = __low2float(sz), z = __high2float(sz), inv = ok ? i4_inverse(s) : 0.0f;
+    if (!(inv > 0.0f)) return 0u;
+    uint32_t q = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q |= i4_code(x[i], s, z, inv) << (4 * i);
+    return q;
+}
+
+// A thread's place: token t, head h, block b of 64 channels, i: its 8 of them.  It takes the key's and the value's (one search for the page).
+struct Place {
+    int t, h, b, i, channel;
+    bool live;
+};
+__device__ __forceinline__ Place place(const CacheArgs& a) {
+    const unsigned blocks = (unsigned)a.d >> 6, u = blockIdx.x * 32 + (threadIdx.x >> 3), t = u / blocks;
+    Place p;
+    p.live = t < (unsigned)a.T;
+    p.t = p.live ? (int)t : a.T - 1;
+    p.b = (int)(u - t * blocks);
+    p.h = blockIdx.y;
+    p.i = threadIdx.x & 7;
+    p.channel = 64 * p.b + 8 * p.i;
+    return p;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) int4_kv_write_kernel(CacheArgs a) {
     ce_pdl_begin();
-    const int blocks = a.d >> 6, groups = a.d / a.group, lane = threadIdx.x & 15;
-    const long long units = (long long)a.T * a.nkv * 2 * blocks;
-    const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const bool live = u < units;
-    long long rest = live ? u : units - 1;
-    const int b = (int)(rest % blocks); rest /= blocks;
-    const bool is_v = rest & 1; rest >>= 1;
-    const int h = (int)(rest % a.nkv), t = (int)(rest / a.nkv);
-    const T* src = is_v ? (const T*)a.v + t * a.v_token + h * a.v_head : (const T*)a.k + t * a.k_token + h * a.k_head;
-    float x[4];
-    load4(src + 64 * b + 4 * lane, a.vec, x);
-    __half2 sz;
-    const unsigned q = quantise4(x, a.group >> 2, sz);
-    const unsigned near = __shfl_xor_sync(0xffffffffu, q, 1), far = __shfl_xor_sync(0xffffffffu, q, 8);
+    const Place p = place(a);
+    float k[8], v[8];
+    load8((const T*)a.k + p.t * a.k_token + p.h * a.k_head + p.channel, a.vec, k);
+    load8((const T*)a.v + p.t * a.v_token + p.h * a.v_head + p.channel, a.vec, v);
     int at = 0;
-    unsigned char* tile = live ? tile_of(a, t, h, at, 2) : nullptr;
-    if (!tile) return;
-    const int g = (64 * b + 4 * lane) / a.group;
-    const bool first = (4 * lane) % a.group == 0;
-    if (!is_v) {
-        if (!(lane & 1)) *reinterpret_cast<uint32_t*>(tile + i4_k_word(at, 64 * b + 4 * lane)) = q | near << 16;
-        if (first) *reinterpret_cast<__half2*>(tile + i4_k_step(a.d, groups, at, g)) = sz;
-    } else {
-        if (lane < 8) *reinterpret_cast<uint32_t*>(tile + i4_v_word(a.d, at, b, lane)) = q | far << 16;
-        if (first) *reinterpret_cast<__half2*>(tile + i4_v_step(a.d, groups, at, g)) = sz;
+    unsigned char* tile = tile_of(a, p.t, p.h, at, 2);
+    __half2 k_step, v_step;
+    const uint32_t kq = quantise8(k, a.group >> 3, k_step), vq = quantise8(v, a.group >> 3, v_step);
+    // a word of values: channels 4 r .. 4 r + 3 of a block and those 32 further on, which lane i ^ 4 has
+    const bool low = p.i < 4;
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, low ? vq >> 16 : vq & 0xffffu, 4);
+    if (!p.live || !tile) return;
+    const int groups = a.d / a.group, g = p.channel / a.group;
+    *reinterpret_cast<uint32_t*>(tile + i4_k_word(at, p.channel)) = kq;
+    *reinterpret_cast<uint32_t*>(tile + i4_v_word(a.d, at, p.b, 2 * (p.i & 3) + (low ? 0 : 1))) = low ? (vq & 0xffffu) | got << 16 : got | (vq >> 16) << 16;
+    if (p.channel % a.group == 0) {
+        *reinterpret_cast<__half2*>(tile + i4_k_step(a.d, groups, at, g)) = k_step;
+        *reinterpret_cast<__half2*>(tile + i4_v_step(a.d, groups, at, g)) = v_step;
     }
+}
+
+__device__ __forceinline__ void values_of(uint32_t w, __half2 sz, float (&x)[8]) {
+    const float s = __low2float(sz), z = __high2float(sz);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), s, z);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) int4_kv_read_kernel(CacheArgs a) {
     ce_pdl_begin();
-    const int blocks = a.d >> 6, groups = a.d / a.group, lane = threadIdx.x & 15;
-    const long long units = (long long)a.T * a.nkv * 2 * blocks;
-    const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (u >= units) return;
-    long long rest = u;
-    const int b = (int)(rest % blocks); rest /= blocks;
-    const bool is_v = rest & 1; rest >>= 1;
-    const int h = (int)(rest % a.nkv), t = (int)(rest / a.nkv);
+    const Place p = place(a);
     int at = 0;
-    const unsigned char* tile = tile_of(a, t, h, at, 4);
+    const unsigned char* tile = p.live ? tile_of(a, p.t, p.h, at, 4) : nullptr;
     if (!tile) return;
-    const int g = (64 * b + 4 * lane) / a.group;
-    uint32_t w;
-    __half2 sz;
-    if (!is_v) {
-        w = *reinterpret_cast<const uint32_t*>(tile + i4_k_word(at, 64 * b + 4 * lane)) >> (lane & 1 ? 16 : 0);
-        sz = *reinterpret_cast<const __half2*>(tile + i4_k_step(a.d, groups, at, g));
-    } else {
-        w = *reinterpret_cast<const uint32_t*>(tile + i4_v_word(a.d, at, b, lane & 7)) >> (lane & 8 ? 16 : 0);
-        sz = *reinterpret_cast<const __half2*>(tile + i4_v_step(a.d, groups, at, g));
-    }
-    const float s = __low2float(sz), z = __high2float(sz);
-    float x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), s, z);
-    T* dst = is_v ? (T*)a.v + t * a.v_token + h * a.v_head : (T*)a.k + t * a.k_token + h * a.k_head;
-    store4(dst + 64 * b + 4 * lane, a.vec, x);
+    const int groups = a.d / a.group, g = p.channel / a.group;
+    const uint32_t kq = *reinterpret_cast<const uint32_t*>(tile + i4_k_word(at, p.channel));
+    const uint32_t first = *reinterpret_cast<const uint32_t*>(tile + i4_v_word(a.d, at, p.b, 2 * (p.i & 3)));
+    const uint32_t second = *reinterpret_cast<const uint32_t*>(tile + i4_v_word(a.d, at, p.b, 2 * (p.i & 3) + 1));
+    const __half2 k_step = *reinterpret_cast<const __half2*>(tile + i4_k_step(a.d, groups, at, g));
+    const __half2 v_step = *reinterpret_cast<const __half2*>(tile + i4_v_step(a.d, groups, at, g));
+    float x[8];
+    values_of(kq, k_step, x);
+    store8((T*)a.k + p.t * a.k_token + p.h * a.k_head + p.channel, a.vec, x);
+    values_of(__byte_perm(first, second, p.i < 4 ? 0x5410u : 0x7632u), v_step, x);
+    store8((T*)a.v + p.t * a.v_token + p.h * a.v_head + p.channel, a.vec, x);
 }
 
 struct WeightArgs {
@@ -206,12 +271,13 @@ bool aligned4(const void* p, long long s0, long long s1, int dtype) {
 template <typename F32, typename BF16>
 int run_cache(CacheArgs& a, int dtype, F32 f32, BF16 bf16, const char* name, cudaStream_t stream) {
     if (a.T == 0) return CE_OK;
-    a.vec = aligned4(a.k, a.k_token, a.k_head, dtype) && aligned4(a.v, a.v_token, a.v_head, dtype);
-    const long long units = (long long)a.T * a.nkv * 2 * (a.d >> 6), grid = (units + 15) / 16;
-    if (grid > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "%s: too many rows", name);
+    const int wide = dtype == CE_F32 ? 4 : 8;             // values in 16 bytes
+    a.vec = (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0 && a.k_token % wide == 0 && a.k_head % wide == 0 && a.v_token % wide == 0 && a.v_head % wide == 0;
+    const long long units = (long long)a.T * (a.d >> 6);
+    const dim3 grid((unsigned)((units + 31) / 32), (unsigned)a.nkv);
+    if (units > 0x7fffffffll || a.nkv > 65535) return ce_fail(CE_ERR_SIZE, "%s: too many rows", name);
     ce_note(name);
-    const cudaError_t e = dtype == CE_F32 ? ce_launch(f32, dim3((unsigned)grid), dim3(256), 0, stream, a)
-                                          : ce_launch(bf16, dim3((unsigned)grid), dim3(256), 0, stream, a);
+    const cudaError_t e = dtype == CE_F32 ? ce_launch(f32, grid, dim3(256), 0, stream, a) : ce_launch(bf16, grid, dim3(256), 0, stream, a);
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e)); }
     return ce_check_launch(name);
 }
