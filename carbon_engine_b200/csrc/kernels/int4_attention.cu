@@ -18,6 +18,7 @@
 namespace {
 
 constexpr int WARPS = 8, STAGES = 4;
+constexpr int PAIR_UP_TO = 128;
 constexpr float NOTHING = -1e30f;              // the maximum of no scores
 constexpr float HEADROOM = 5.0f;               // scores may pass the running maximum by this many powers of two before it is moved
 constexpr float LOG2E = 1.4426950408889634f;
@@ -122,9 +123,10 @@ __device__ __forceinline__ float4 load_cluster4(uint32_t local, int rank) {
 }
 
 template <typename T, int D, int G, int NT>
-__global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
+__global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_TO ? 2 : 1) int4_attention_kernel(Args a) {
     constexpr bool C8 = Pieces<T>::N == 2;            // codes less 8: see i4_pairs
     constexpr int NB = D / 64, NG = D / G, P = Pieces<T>::N, ROWS = 8 * NT, TILE = i4_cache_tile_bytes(D, G), CH = D / 32;
+    constexpr int PAIR = P * NT * D <= PAIR_UP_TO ? 2 : 1;       // tiles a warp takes at a time
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[WARPS][STAGES];
     __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_join[ROWS][2];
@@ -263,97 +265,124 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
     const int inner_lo = a.window > 0 ? max(0, last_pos - a.window + 1) : 0;
 
     bool ok = true;
-    int gone = 0;                                     // tiles whose copies this warp has waited for
-    for (int i = 0; i < mine; ++i, ++gone) {
-        ok = i4_warp_wait(&full[warp][i % STAGES], (i / STAGES) & 1);
+    int gone = 0;                                     // tiles whose copies this warp has waited for, and whose place others may have taken
+    for (int i = 0; i < mine; i += PAIR) {
+        gone = i;
+        const unsigned char* tile[PAIR];
+        int key0[PAIR];
+        bool cut = false;
+#pragma unroll
+        for (int p = 0; p < PAIR; ++p) {
+            const bool here = p == 0 || i + p < mine;
+            if (here) ok = ok && i4_warp_wait(&full[warp][(i + p) % STAGES], ((i + p) / STAGES) & 1);
+            tile[p] = ring + ((i + p) % STAGES) * TILE;
+            // (a last tile alone: the other's keys are ones that nobody sees)
+            key0[p] = here ? (tile_lo + begin + warp + (i + p) * WARPS) * 16 : last_pos + 1;
+            cut = cut || key0[p] < inner_lo || key0[p] + 15 > first_pos;
+        }
         if (!ok) { if (lane == 0) atomicExch(a.status, 7); break; }
-        const unsigned char* tile = ring + (i % STAGES) * TILE;
-        const int key0 = (tile_lo + begin + warp + i * WARPS) * 16;
-        const bool cut = key0 < inner_lo || key0 + 15 > first_pos;
         // ---- scores of keys r and r + 8 (rows of the tile) for query rows 2 l and 2 l + 1
-        uint32_t ka[NG], kb[NG];
-        load_steps<NG>(tile + 16 * D + r * NG * 4, ka);
-        load_steps<NG>(tile + 16 * D + (r + 8) * NG * 4, kb);
-        float s[NT][4];
+        float s[PAIR][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-        float acc[NT][P][4];
+        for (int p = 0; p < PAIR; ++p) {
+            uint32_t ka[NG], kb[NG];
+            load_steps<NG>(tile[p] + 16 * D + r * NG * 4, ka);
+            load_steps<NG>(tile[p] + 16 * D + (r + 8) * NG * 4, kb);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const uint4 w = *reinterpret_cast<const uint4*>(tile + b * 512 + lane * 16);
+            for (int nt = 0; nt < NT; ++nt) s[p][nt][0] = s[p][nt][1] = s[p][nt][2] = s[p][nt][3] = 0.f;
+            float acc[NT][P][4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int c = 2 * b + half;
-                const uint32_t wa = half ? w.z : w.x, wb = half ? w.w : w.y;
+            for (int b = 0; b < NB; ++b) {
+                const uint4 w = *reinterpret_cast<const uint4*>(tile[p] + b * 512 + lane * 16);
 #pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    uint32_t a0, a1, a2, a3;
-                    if (st) { i4_pairs<C8, 8>(wa, a0, a2); i4_pairs<C8, 8>(wb, a1, a3); }
-                    else { i4_pairs<C8, 0>(wa, a0, a2); i4_pairs<C8, 0>(wb, a1, a3); }
+                for (int half = 0; half < 2; ++half) {
+                    const int c = 2 * b + half;
+                    const uint32_t wa = half ? w.z : w.x, wb = half ? w.w : w.y;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int st = 0; st < 2; ++st) {
+                        uint32_t a0, a1, a2, a3;
+                        if (st) { i4_pairs<C8, 8>(wa, a0, a2); i4_pairs<C8, 8>(wb, a1, a3); }
+                        else { i4_pairs<C8, 0>(wa, a0, a2); i4_pairs<C8, 0>(wb, a1, a3); }
 #pragma unroll
-                        for (int p = 0; p < P; ++p) {
-                            if (st == 0 && (c * 32) % G == 0) i4_mma_first(acc[nt][p], a0, a1, a2, a3, qf[nt][p][c][0], qf[nt][p][c][1]);
-                            else i4_mma(acc[nt][p], a0, a1, a2, a3, qf[nt][p][c][2 * st], qf[nt][p][c][2 * st + 1]);
-                        }
-                }
-                if ((c * 32 + 32) % G == 0) {
-                    const int g = c * 32 / G;
-                    const float2 fa = i4_step_of<C8>(ka[g]), fb = i4_step_of<C8>(kb[g]);
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                            for (int q = 0; q < P; ++q) {
+                                if (st == 0 && (c * 32) % G == 0) i4_mma_first(acc[nt][q], a0, a1, a2, a3, qf[nt][q][c][0], qf[nt][q][c][1]);
+                                else i4_mma(acc[nt][q], a0, a1, a2, a3, qf[nt][q][c][2 * st], qf[nt][q][c][2 * st + 1]);
+                            }
+                    }
+                    if ((c * 32 + 32) % G == 0) {
+                        const int g = c * 32 / G;
+                        const float2 fa = i4_step_of<C8>(ka[g]), fb = i4_step_of<C8>(kb[g]);
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float sa = acc[nt][0][e], sb = acc[nt][0][2 + e];
-                            if constexpr (P == 2) { sa += acc[nt][1][e]; sb += acc[nt][1][2 + e]; }
-                            s[nt][e] = fmaf(fa.x, sa, fmaf(fa.y, qsum[nt][g][e], s[nt][e]));
-                            s[nt][2 + e] = fmaf(fb.x, sb, fmaf(fb.y, qsum[nt][g][e], s[nt][2 + e]));
-                        }
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float sa = acc[nt][0][e], sb = acc[nt][0][2 + e];
+                                if constexpr (P == 2) { sa += acc[nt][1][e]; sb += acc[nt][1][2 + e]; }
+                                s[p][nt][e] = fmaf(fa.x, sa, fmaf(fa.y, qsum[nt][g][e], s[p][nt][e]));
+                                s[p][nt][2 + e] = fmaf(fb.x, sb, fmaf(fb.y, qsum[nt][g][e], s[p][nt][2 + e]));
+                            }
+                    }
                 }
             }
         }
-        const int key_a = key0 + r, key_b = key_a + 8;
         // steps and minima of V; keys outside the block's reach may hold anything
-        uint32_t va[NG], vb[NG];
-        load_steps<NG>(tile + 16 * D + 64 * NG + r * NG * 4, va);
-        load_steps<NG>(tile + 16 * D + 64 * NG + (r + 8) * NG * 4, vb);
+        uint32_t va[PAIR][NG], vb[PAIR][NG];
+#pragma unroll
+        for (int p = 0; p < PAIR; ++p) {
+            load_steps<NG>(tile[p] + 16 * D + 64 * NG + r * NG * 4, va[p]);
+            load_steps<NG>(tile[p] + 16 * D + 64 * NG + (r + 8) * NG * 4, vb[p]);
+        }
         if (cut) {
-            const bool in_a = key_a >= block_lo && key_a <= last_pos, in_b = key_b >= block_lo && key_b <= last_pos;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                // a group that is not a number reaches the rows that see its key, and no others (0 times NaN would)
-                const bool nan_a = isnan(i4_unpack(va[g]).x), nan_b = isnan(i4_unpack(vb[g]).x);
-                if (__any_sync(0xffffffffu, nan_a || nan_b)) {
+            for (int p = 0; p < PAIR; ++p) {
+                const int key_a = key0[p] + r, key_b = key_a + 8;
+                const bool in_a = key_a >= block_lo && key_a <= last_pos, in_b = key_b >= block_lo && key_b <= last_pos;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                for (int g = 0; g < NG; ++g) {
+                    // a group that is not a number reaches the rows that see its key, and no others (0 times NaN would)
+                    const bool nan_a = isnan(i4_unpack(va[p][g]).x), nan_b = isnan(i4_unpack(vb[p][g]).x);
+                    if (__any_sync(0xffffffffu, nan_a || nan_b)) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            if (nan_a && in_a && key_a <= hi[nt][e] && key_a >= lo[nt][e]) oz[nt][g][e] = __int_as_float(0x7fc00000);
-                            if (nan_b && in_b && key_b <= hi[nt][e] && key_b >= lo[nt][e]) oz[nt][g][e] = __int_as_float(0x7fc00000);
-                        }
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                if (nan_a && in_a && key_a <= hi[nt][e] && key_a >= lo[nt][e]) oz[nt][g][e] = __int_as_float(0x7fc00000);
+                                if (nan_b && in_b && key_b <= hi[nt][e] && key_b >= lo[nt][e]) oz[nt][g][e] = __int_as_float(0x7fc00000);
+                            }
+                    }
+                    if (!in_a || nan_a) va[p][g] = 0;
+                    if (!in_b || nan_b) vb[p][g] = 0;
                 }
-                if (!in_a || nan_a) va[g] = 0;
-                if (!in_b || nan_b) vb[g] = 0;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (key_a > hi[nt][e] || key_a < lo[nt][e]) s[p][nt][e] = -INFINITY;
+                        if (key_b > hi[nt][e] || key_b < lo[nt][e]) s[p][nt][2 + e] = -INFINITY;
+                    }
             }
         }
         bool move = false;
+        float mx[NT][2], step_max = 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                if (cut) {
-                    if (key_a > hi[nt][e] || key_a < lo[nt][e]) s[nt][e] = -INFINITY;
-                    if (key_b > hi[nt][e] || key_b < lo[nt][e]) s[nt][2 + e] = -INFINITY;
-                }
-                move = move || fmaxf(s[nt][e], s[nt][2 + e]) > high[nt][e];
-            }
-        float fa[NG], fb[NG], step_max = 0.f;
+                mx[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            fa[g] = i4_unpack(va[g]).x; fb[g] = i4_unpack(vb[g]).x;
-            step_max = fmaxf(step_max, fmaxf(fa[g], fb[g]));
-        }
+                for (int p = 1; p < PAIR; ++p) mx[nt][e] = fmaxf(mx[nt][e], fmaxf(s[p][nt][e], s[p][nt][2 + e]));
+                move = move || mx[nt][e] > high[nt][e];
+            }
+        float fa[PAIR][NG], fb[PAIR][NG];
+#pragma unroll
+        for (int p = 0; p < PAIR; ++p)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                fa[p][g] = i4_unpack(va[p][g]).x; fb[p][g] = i4_unpack(vb[p][g]).x;
+                step_max = fmaxf(step_max, fmaxf(fa[p][g], fb[p][g]));
+            }
         move = move || step_max > top;
         if (__any_sync(0xffffffffu, move)) {
             // maxima over the 8 lanes that share l, the largest step over all
@@ -367,13 +396,13 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float mx = fmaxf(s[nt][e], s[nt][2 + e]);
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float now = fmaxf(m[nt][e] - grown, fmaf(mx, row_scale[nt][e], offset));
+                    float x = mx[nt][e];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float now = fmaxf(m[nt][e] - grown, fmaf(x, row_scale[nt][e], offset));
                     const float alpha = m[nt][e] == NOTHING ? 0.0f : exp2f(m[nt][e] - now);
-                    m[nt][e] = mx == -INFINITY && m[nt][e] == NOTHING ? NOTHING : now;
+                    m[nt][e] = x == -INFINITY && m[nt][e] == NOTHING ? NOTHING : now;
                     high[nt][e] = m[nt][e] == NOTHING ? NOTHING : (now - offset + HEADROOM) / row_scale[nt][e];
                     sum[nt][e] *= alpha;
 #pragma unroll
@@ -382,59 +411,66 @@ __global__ void __launch_bounds__(WARPS * 32) int4_attention_kernel(Args a) {
                     for (int i2 = 0; i2 < NB * 4; ++i2) { o[nt][i2][e] *= alpha; o[nt][i2][2 + e] *= alpha; }
                 }
         }
-        float pr[NT][4];
+        float pr[PAIR][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int p = 0; p < PAIR; ++p)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                pr[nt][e] = ce_exp2_fast(fmaf(s[nt][e], row_scale[nt][e], -m[nt][e]));
-                pr[nt][2 + e] = ce_exp2_fast(fmaf(s[nt][2 + e], row_scale[nt][e], -m[nt][e]));
-                sum[nt][e] += pr[nt][e] + pr[nt][2 + e];
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    pr[p][nt][e] = ce_exp2_fast(fmaf(s[p][nt][e], row_scale[nt][e], -m[nt][e]));
+                    pr[p][nt][2 + e] = ce_exp2_fast(fmaf(s[p][nt][2 + e], row_scale[nt][e], -m[nt][e]));
+                    sum[nt][e] += pr[p][nt][e] + pr[p][nt][2 + e];
+                }
         // ---- V^T P^T, group by group: the probability carries the step
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const uint4 w = *reinterpret_cast<const uint4*>(tile + 8 * D + b * 512 + lane * 16);
-            uint32_t bf[NT][P][2];
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int g = (64 * b + 32 * half) / G;
-                if ((32 * half) % G == 0) {
-                    const float za = i4_step_of<C8>(va[g]).y, zb = i4_step_of<C8>(vb[g]).y;
+            for (int p = 0; p < PAIR; ++p) {
+                const uint4 w = *reinterpret_cast<const uint4*>(tile[p] + 8 * D + b * 512 + lane * 16);
+                uint32_t bf[NT][P][2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        oz[nt][g][0] = fmaf(pr[nt][0], za, fmaf(pr[nt][2], zb, oz[nt][g][0]));
-                        oz[nt][g][1] = fmaf(pr[nt][1], za, fmaf(pr[nt][3], zb, oz[nt][g][1]));
-                        float x0 = pr[nt][0] * fa[g], x1 = pr[nt][1] * fa[g], x2 = pr[nt][2] * fb[g], x3 = pr[nt][3] * fb[g];
+                for (int half = 0; half < 2; ++half) {
+                    const int g = (64 * b + 32 * half) / G;
+                    if ((32 * half) % G == 0) {
+                        const float za = i4_step_of<C8>(va[p][g]).y, zb = i4_step_of<C8>(vb[p][g]).y;
 #pragma unroll
-                        for (int p = 0; p < P; ++p) {
-                            const uint32_t ab = i4_pack(x0, x1), cd = i4_pack(x2, x3);
-                            bf[nt][p][0] = transpose8(ab);
-                            bf[nt][p][1] = transpose8(cd);
-                            if (p + 1 < P) {
-                                const float2 g0 = i4_unpack(ab), g1 = i4_unpack(cd);
-                                x0 -= g0.x; x1 -= g0.y; x2 -= g1.x; x3 -= g1.y;
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const float* w4 = pr[p][nt];
+                            oz[nt][g][0] = fmaf(w4[0], za, fmaf(w4[2], zb, oz[nt][g][0]));
+                            oz[nt][g][1] = fmaf(w4[1], za, fmaf(w4[3], zb, oz[nt][g][1]));
+                            float x0 = w4[0] * fa[p][g], x1 = w4[1] * fa[p][g], x2 = w4[2] * fb[p][g], x3 = w4[3] * fb[p][g];
+#pragma unroll
+                            for (int q = 0; q < P; ++q) {
+                                const uint32_t ab = i4_pack(x0, x1), cd = i4_pack(x2, x3);
+                                bf[nt][q][0] = transpose8(ab);
+                                bf[nt][q][1] = transpose8(cd);
+                                if (q + 1 < P) {
+                                    const float2 g0 = i4_unpack(ab), g1 = i4_unpack(cd);
+                                    x0 -= g0.x; x1 -= g0.y; x2 -= g1.x; x3 -= g1.y;
+                                }
                             }
                         }
                     }
-                }
-                // the halves of a word are the two halves of the block's channels; two tokens' words side by side
-                const uint32_t pick = half ? 0x7632u : 0x5410u;
-                const uint32_t u = __byte_perm(w.x, w.y, pick), v = __byte_perm(w.z, w.w, pick);
+                    // the halves of a word are the two halves of the block's channels; two tokens' words side by side
+                    const uint32_t pick = half ? 0x7632u : 0x5410u;
+                    const uint32_t u = __byte_perm(w.x, w.y, pick), v = __byte_perm(w.z, w.w, pick);
 #pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    uint32_t a0, a1, a2, a3;
-                    if (st) { i4_pairs<C8, 8>(u, a0, a1); i4_pairs<C8, 8>(v, a2, a3); }
-                    else { i4_pairs<C8, 0>(u, a0, a1); i4_pairs<C8, 0>(v, a2, a3); }
+                    for (int st = 0; st < 2; ++st) {
+                        uint32_t a0, a1, a2, a3;
+                        if (st) { i4_pairs<C8, 8>(u, a0, a1); i4_pairs<C8, 8>(v, a2, a3); }
+                        else { i4_pairs<C8, 0>(u, a0, a1); i4_pairs<C8, 0>(v, a2, a3); }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int p = 0; p < P; ++p) i4_mma(o[nt][b * 4 + half * 2 + st], a0, a1, a2, a3, bf[nt][p][0], bf[nt][p][1]);
+                            for (int q = 0; q < P; ++q) i4_mma(o[nt][b * 4 + half * 2 + st], a0, a1, a2, a3, bf[nt][q][0], bf[nt][q][1]);
+                    }
                 }
             }
-        }
         __syncwarp();
-        if (i + STAGES < mine) issue(i + STAGES);
+#pragma unroll
+        for (int p = 0; p < PAIR; ++p)
+            if (i + p + STAGES < mine) issue(i + p + STAGES);
     }
     if (!ok) {
         // the copies still in flight land in this block's memory: wait for them, with a limit, before it is used for anything else
