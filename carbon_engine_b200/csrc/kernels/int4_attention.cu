@@ -17,7 +17,9 @@
 
 namespace {
 
-constexpr int WARPS = 8, STAGES = 4;
+constexpr int WARPS = 8;
+// tiles of a warp's ring: 4, or up to 6 where two blocks of an SM have room for it
+constexpr int ring_tiles(int tile) { return 110592 / (WARPS * tile) < 4 ? 4 : 110592 / (WARPS * tile) > 6 ? 6 : 110592 / (WARPS * tile); }
 constexpr int PAIR_UP_TO = 128;
 constexpr float NOTHING = -1e30f;              // the maximum of no scores
 constexpr float HEADROOM = 5.0f;               // scores may pass the running maximum by this many powers of two before it is moved
@@ -125,7 +127,7 @@ __device__ __forceinline__ float4 load_cluster4(uint32_t local, int rank) {
 template <typename T, int D, int G, int NT>
 __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_TO ? 2 : 1) int4_attention_kernel(Args a) {
     constexpr bool C8 = Pieces<T>::N == 2;            // codes less 8: see i4_pairs
-    constexpr int NB = D / 64, NG = D / G, P = Pieces<T>::N, ROWS = 8 * NT, TILE = i4_cache_tile_bytes(D, G), CH = D / 32;
+    constexpr int NB = D / 64, NG = D / G, P = Pieces<T>::N, ROWS = 8 * NT, TILE = i4_cache_tile_bytes(D, G), CH = D / 32, STAGES = ring_tiles(TILE);
     constexpr int PAIR = P * NT * D <= PAIR_UP_TO ? 2 : 1;       // tiles a warp takes at a time
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[WARPS][STAGES];
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(64) int4_attention_merge_kernel(Args a) {
 
 template <typename T, int D, int G, int NT>
 int run(Args a, int jobs, cudaStream_t stream) {
-    constexpr int TILE = i4_cache_tile_bytes(D, G), RING = WARPS * STAGES * TILE, OUT = WARPS * 8 * NT * (D + 4) * 4;
+    constexpr int TILE = i4_cache_tile_bytes(D, G), RING = WARPS * ring_tiles(TILE) * TILE, OUT = WARPS * 8 * NT * (D + 4) * 4;
     constexpr int SMEM = RING > OUT ? RING : OUT;
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
     static std::atomic<unsigned long long> done{0};
