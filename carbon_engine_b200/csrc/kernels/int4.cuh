@@ -26,6 +26,7 @@
 #pragma once
 #include "common.cuh"
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #define I4_LIMIT 60000.0f
 

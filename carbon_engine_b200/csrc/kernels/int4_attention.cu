@@ -11,13 +11,13 @@
 // row's largest); float32 rows are two float16 pieces, 22 bits.  p_j s_jg is rounded to float16 (2^-12 of itself; two pieces for float32),
 // scaled so that the largest lies near 2^10: sums of thousands of small weights keep their bits.  Everything else is float32.
 //
-// A block takes up to 8 or 16 rows (tokens by heads of the KV head) and a run of the keys; its 8 warps take tiles in turn, each with a ring
-// of its own that one lane fills with bulk copies (a tile is one run of bytes in the page); warps, then blocks, are joined in a fixed order.
+// A block takes up to 8 or 16 rows (tokens by heads of the KV head) and a run of the keys; its 8 or 4 warps take tiles in turn, each with a
+// ring of its own that one lane fills with bulk copies (a tile is one run of bytes in the page); warps, then blocks, are joined in a fixed order.
 #include "int4.cuh"
 
 namespace {
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 8;                       // of a block, at most
 // tiles of a warp's ring: 4, or up to 6 where two blocks of an SM have room for it
 constexpr int ring_tiles(int tile) { return 110592 / (WARPS * tile) < 4 ? 4 : 110592 / (WARPS * tile) > 6 ? 6 : 110592 / (WARPS * tile); }
 constexpr int PAIR_UP_TO = 128;
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_join[ROWS][2];
     if (a.overlap) ce_pdl_launch_dependents();
     ce_pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3, warps = blockDim.x >> 5;
     const int split = blockIdx.x % a.splits, job_id = blockIdx.x / a.splits;
     const Job j = job_of(a, job_id, ROWS);
     const int each = a.nh / a.nkv, rows = min(ROWS, j.tokens * each - j.row0);
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     const int tile_lo = block_lo >> 4, tiles = last_pos < block_lo ? 0 : (last_pos >> 4) + 1 - tile_lo;
     // shares of the longest context's length (shorter sequences take fewer blocks), or as many keys as it takes
     const int share = max(a.share, (tiles + a.splits - 1) / a.splits), begin = min(split * share, tiles), end = min(begin + share, tiles);
-    const int mine = end - begin > warp ? (end - begin - warp + WARPS - 1) / WARPS : 0;      // tiles begin + warp, + WARPS, ...
+    const int mine = end - begin > warp ? (end - begin - warp + warps - 1) / warps : 0;      // tiles begin + warp, + warps, ...
     const int* table = a.block_table + (size_t)j.slot * a.max_pages;
     unsigned char* ring = smem + warp * (STAGES * TILE);
     const int per_page = a.page_size >> 4;
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     const unsigned char* place = a.pages;
     auto look_up = [&](int from) {
         looked = from;
-        const int i = from + lane, t = tile_lo + begin + warp + i * WARPS, pi = t / per_page;
+        const int i = from + lane, t = tile_lo + begin + warp + i * warps, pi = t / per_page;
         int page = i >= mine ? 0 : pi < a.max_pages ? table[pi] : -1;
         if (page < 0 || page >= a.num_pages) { atomicExch(a.status, 4); page = 0; }      // (the step's results are not used)
         place = a.pages + (((size_t)page * a.nkv + j.kvh) * per_page + (t - pi * per_page)) * TILE;
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
             if (here) ok = ok && i4_warp_wait(&full[warp][(i + p) % STAGES], ((i + p) / STAGES) & 1);
             tile[p] = ring + ((i + p) % STAGES) * TILE;
             // (a last tile alone: the other's keys are ones that nobody sees)
-            key0[p] = here ? (tile_lo + begin + warp + (i + p) * WARPS) * 16 : last_pos + 1;
+            key0[p] = here ? (tile_lo + begin + warp + (i + p) * warps) * 16 : last_pos + 1;
             cut = cut || key0[p] < inner_lo || key0[p] + 15 > first_pos;
         }
         if (!ok) { if (lane == 0) atomicExch(a.status, 7); break; }
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     }
     __syncthreads();                                  // the rings are free: the warps' outputs take their place
 
-    float* so = reinterpret_cast<float*>(smem);       // [WARPS][ROWS][D + 4]
+    float* so = reinterpret_cast<float*>(smem);       // [warps][ROWS][D + 4]
     constexpr int LD = D + 4;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -509,20 +509,23 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     }
     __syncthreads();
     const bool cluster = a.clustered;
-    for (int x = threadIdx.x; x < rows * (D / 4); x += WARPS * 32) {
+    for (int x = threadIdx.x; x < rows * (D / 4); x += blockDim.x) {
         const int row = x / (D / 4), ch = (x - row * (D / 4)) * 4;
-        float M = NOTHING;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][row]);
-        float L = 0.f;
+        float M = NOTHING, L = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto join = [&](auto all) {                   // (8 or 4 known to the compiler: the loads go out together)
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float f = weight_of(s_m[w][row], s_l[w][row], M);
-            const float4 u = *reinterpret_cast<const float4*>(so + (w * ROWS + row) * LD + ch);
-            L += s_l[w][row] * f;
-            v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
-        }
+            for (int w = 0; w < all(); ++w) M = fmaxf(M, s_m[w][row]);
+#pragma unroll
+            for (int w = 0; w < all(); ++w) {
+                const float f = weight_of(s_m[w][row], s_l[w][row], M);
+                const float4 u = *reinterpret_cast<const float4*>(so + (w * ROWS + row) * LD + ch);
+                L += s_l[w][row] * f;
+                v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+            }
+        };
+        if (warps == WARPS) join(std::integral_constant<int, WARPS>());
+        else join(std::integral_constant<int, WARPS / 2>());
         if (cluster) {
             // (warp 0's rows: every number of theirs is read by the thread that replaces it)
             *reinterpret_cast<float4*>(so + row * LD + ch) = v;
@@ -539,7 +542,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     // the blocks' runs of keys, in their order: each takes a share of the rows' channels
     cluster_sync();
     const int all = rows * (D / 4);
-    for (int x = split * (WARPS * 32) + threadIdx.x; x < all; x += a.splits * (WARPS * 32)) {
+    for (int x = split * blockDim.x + threadIdx.x; x < all; x += a.splits * blockDim.x) {
         const int row = x / (D / 4), ch = (x - row * (D / 4)) * 4;
         float M = NOTHING, L = 0.f, ms[8], ls[8];
         float4 us[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -565,35 +568,63 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     cluster_sync();                                   // nobody leaves while its rows are read
 }
 
-// Joins the runs of keys of a row block, in their order: one block a row, four channels a thread
+// Joins the runs of keys of a row block: a block a row, its warps - up to 8 - a run in turn (a lane four channels), then the warps' sums, all in a fixed order.
+// (One warp that reads run after run takes 0.5 us for each.)
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(64) int4_attention_merge_kernel(Args a) {
+__global__ void __launch_bounds__(256) int4_attention_merge_kernel(Args a) {
     ce_pdl_begin();
-    const int job_id = blockIdx.x / ROWS, row = blockIdx.x - job_id * ROWS;
+    constexpr int CH = (D + 127) / 128;
+    __shared__ float4 part[8][D / 4];
+    __shared__ float part_l[8];
+    const int job_id = blockIdx.x / ROWS, row = blockIdx.x - job_id * ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const Job j = job_of(a, job_id, ROWS);
     const int each = a.nh / a.nkv;
     if (row >= j.tokens * each - j.row0) return;
-    const int ch = threadIdx.x * 4;
-    if (ch >= D) return;
-    float M = NOTHING, L = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     const size_t at = (size_t)job_id * a.splits * ROWS + row;
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (at + (size_t)s * ROWS)]);
-    for (int s = 0; s < a.splits; ++s) {
+    float M = NOTHING, L = 0.f;
+    for (int s = lane; s < a.splits; s += 32) M = fmaxf(M, a.part_ml[2 * (at + (size_t)s * ROWS)]);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+    float4 v[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = warp; s < a.splits; s += warps) {
         const size_t p = at + (size_t)s * ROWS;
         const float ls = a.part_ml[2 * p + 1], f = weight_of(a.part_ml[2 * p], ls, M);
-        if (ls == 0.f) continue;                      // (a run without a key that the row sees wrote nothing else)
-        const float4 u = *reinterpret_cast<const float4*>(a.part_o + p * D + ch);
         L += ls * f;
-        v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int ch = (c * 32 + lane) * 4;
+            if (ch >= D || ls == 0.f) continue;       // (a run without a key that the row sees wrote nothing else)
+            const float4 u = *reinterpret_cast<const float4*>(a.part_o + p * D + ch);
+            v[c].x = fmaf(u.x, f, v[c].x); v[c].y = fmaf(u.y, f, v[c].y); v[c].z = fmaf(u.z, f, v[c].z); v[c].w = fmaf(u.w, f, v[c].w);
+        }
     }
-    store_row<T>(a, j, row, D, ch, v, L);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        if ((c * 32 + lane) * 4 < D) part[warp][c * 32 + lane] = v[c];
+    if (lane == 0) part_l[warp] = L;
+    __syncthreads();
+    for (int x = threadIdx.x; x < D / 4; x += blockDim.x) {
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+        L = 0.f;
+        for (int w = 0; w < warps; ++w) {
+            const float4 u = part[w][x];
+            L += part_l[w];
+            t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
+        }
+        store_row<T>(a, j, row, D, 4 * x, t, L);
+    }
 }
 
 template <typename T, int D, int G, int NT>
 int run(Args a, int jobs, cudaStream_t stream) {
-    constexpr int TILE = i4_cache_tile_bytes(D, G), RING = WARPS * ring_tiles(TILE) * TILE, OUT = WARPS * 8 * NT * (D + 4) * 4;
-    constexpr int SMEM = RING > OUT ? RING : OUT;
+    constexpr int TILE = i4_cache_tile_bytes(D, G), RING = ring_tiles(TILE) * TILE, OUT = 8 * NT * (D + 4) * 4;
+    constexpr int SMEM = WARPS * (RING > OUT ? RING : OUT);
+    // 8 warps a block as long as the chip takes all blocks at once, two an SM; then 4, four an SM, whose beginnings and ends (some 4.5 us) hide
+    // behind more others: 64 sequences of 8,192 keys in halves 127 us for 135, 128 of 30 to 600 22 us for 30; one of 2,048 8.3 us for 7.5
+    const int warps = (long long)jobs * a.splits <= 2 * ce_sm_count() ? WARPS : WARPS / 2;
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
     static std::atomic<unsigned long long> done{0};
     auto kernel = int4_attention_kernel<T, D, G, NT>;
@@ -602,8 +633,8 @@ int run(Args a, int jobs, cudaStream_t stream) {
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[2];
         cfg.gridDim = dim3((unsigned)(jobs * a.splits));
-        cfg.blockDim = dim3(WARPS * 32);
-        cfg.dynamicSmemBytes = SMEM;
+        cfg.blockDim = dim3(warps * 32);
+        cfg.dynamicSmemBytes = SMEM / WARPS * warps;
         cfg.stream = stream;
         cfg.attrs = attr;
         a.clustered = a.splits > 1 && !a.part_o;
@@ -624,7 +655,7 @@ int run(Args a, int jobs, cudaStream_t stream) {
     }
     if (e == cudaSuccess && a.splits > 1 && !a.clustered) {
         ce_note("int4_attention_merge_kernel");
-        e = ce_launch(int4_attention_merge_kernel<T, D, 8 * NT>, dim3((unsigned)(jobs * 8 * NT)), dim3(64), 0, stream, a);
+        e = ce_launch(int4_attention_merge_kernel<T, D, 8 * NT>, dim3((unsigned)(jobs * 8 * NT)), dim3(32 * (a.splits < 8 ? a.splits : 8)), 0, stream, a);
     }
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_attention: %s", cudaGetErrorString(e)); }
     return ce_check_launch("int4_attention");

@@ -169,18 +169,24 @@ def kv_read(pages: Int4Pages, k_out: torch.Tensor, v_out: torch.Tensor, position
 
 @functools.lru_cache(maxsize=4096)
 def _splits(jobs: int, tiles: int):
-    """(blocks that share a row block's keys, tiles of 16 keys a block) for ``jobs`` row blocks of up to ``tiles`` tiles: the least of what the
-    rounds of blocks take, two an SM at a time: 1.1 us for each eighth tile (0.6 with an SM to itself), 4.5 a block to begin and end, a quarter
-    of a round lost at the end, and 2 us where the blocks are joined by a second kernel.  (64 sequences of 8,192 keys, 8 KV heads of 128: 1, 2, 4
-    and 8 blocks a row block 145, 141, 157 and 190 us, of which the rule says 148, 147, 160 and 189.)"""
+    """(blocks that share a row block's keys, tiles of 16 keys a block) for ``jobs`` row blocks of up to ``tiles`` tiles: what is least by the time
+    that blocks take.  Blocks of 8 warps, two an SM, or of 4, four an SM, where there are more than 296; a block takes 1.03 us for each tile of a
+    warp (0.65 with an SM to itself) and 4.5 to begin and end.  Of more than the chip holds at once, the mean of what it is for requests of one
+    length and for those of half the longest on the average, whose long ones end alone; and what a second kernel takes that joins them.  (64
+    sequences of 8,192 keys, 8 KV heads of 128, in 1, 2, 3, 4 and 8 blocks a row block: 137, 127, 137, 131 and 146 us; 21 of 450 to 9,000
+    keys, groups of 32, in 1 to 6: 78, 58, 70, 57, 51 and 52 us.)"""
     best = (float("inf"), 1, tiles)
     for splits in (1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64):
         share = -(-tiles // splits)
         if splits > 1 and (share < 8 or -(-tiles // share) < splits):
             continue
         blocks = jobs * splits
-        rounds = blocks / 296 + 0.25 if blocks > 296 else 1.0
-        cost = rounds * (-(-share // 8) * (1.1 if blocks > 148 else 0.6) + 4.5) + (2.0 if _joined(jobs, splits) else 0.0)
+        rounds, turns = (blocks / 296, -(-share // 8)) if blocks <= 296 else (blocks / 592, -(-share // 4))
+        cost = turns * (0.65 if blocks <= 96 else 0.85 if blocks <= 148 else 1.03) + 4.5
+        if rounds > 1:
+            cost *= ((rounds + 0.12) + (max(1.0, 0.55 * rounds) + 0.25)) / 2
+        if _joined(jobs, splits):
+            cost += 2.0 + blocks / 500
         best = min(best, (cost, splits, share))
     return best[1:]
 
