@@ -30,12 +30,12 @@ class LayerCacheView:
     page_size: int = 0
     k_pool: Optional[torch.Tensor] = None
     v_pool: Optional[torch.Tensor] = None
-    #: keys and values in 4 bits (``ops_int4.Int4Pages``), in the place of the two pools
-    int4: Optional[Any] = None
     state: Optional[torch.Tensor] = None        # [max_requests, *shape]
     writes: bool = True
     #: named states of the block around the mixer (a ``BundleCacheSpec``'s ``extra``), each [max_requests, *shape]
     extra: Optional[Dict[str, torch.Tensor]] = None
+    #: keys and values in 4 bits (``ops_int4.Int4Pages``), in the place of the two pools
+    int4: Optional[Any] = None
 
 
 class CacheStorage:
@@ -99,7 +99,7 @@ class CacheStorage:
         base = self._entries[call.cache]
         if call.writes:
             return base
-        return LayerCacheView(base.kind, base.group, base.page_size, base.k_pool, base.v_pool, base.int4, base.state, False, base.extra)
+        return LayerCacheView(base.kind, base.group, base.page_size, base.k_pool, base.v_pool, base.state, False, base.extra, base.int4)
 
     def paged_views(self) -> List[LayerCacheView]:
         return [e for e in self._entries.values() if e.kind == "paged"]

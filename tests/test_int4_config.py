@@ -63,3 +63,10 @@ def test_sizes():
 def test_splits_cover_the_keys(jobs, tiles):
     splits, share = ops_int4._splits(jobs, tiles)
     assert splits * share >= tiles and (splits - 1) * share < tiles and 1 <= splits <= 64
+
+
+def test_a_mixer_inside_a_sum_sees_its_own_state():
+    """Views are made field by field in places that know nothing of 4-bit pages."""
+    from carbon_engine_b200.cache.storage import LayerCacheView
+    view = LayerCacheView("paged", 1, 16, "k", "v", "state", False, {"a": "b"})
+    assert (view.state, view.writes, view.extra, view.int4) == ("state", False, {"a": "b"}, None)
