@@ -828,8 +828,6 @@ def bias_rope_kvwrite(qkv, k_pool, v_pool, bias, cos, sin, positions, seq_of_tok
         raise KernelError("bias_rope_kvwrite: the bias is shorter than q|k|v")
     if cos is not None and cos.shape[1] != rotary_dim // 2:
         raise KernelError("bias_rope_kvwrite: rotary table width is not rotary_dim / 2")
-    if keys_in_place:
-        write_kv = False
     if write_kv:
         _need(k_pool, "k_pool", qkv.dtype); _need(v_pool, "v_pool", qkv.dtype)
         if tuple(k_pool.shape[1:]) != (nk, page_size, d) or tuple(v_pool.shape[1:]) != (nv, page_size, dv):
