@@ -643,8 +643,8 @@ int run(Args a, int jobs, cudaStream_t stream) {
             attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
             attr[cfg.numAttrs++].val.clusterDim = {(unsigned)a.splits, 1, 1};
             // a grid of more clusters than the chip holds stands alone (ce_clusters_at_once)
-            static CeRoom room[9];
-            a.overlap = a.overlap && jobs <= ce_clusters_at_once(room[a.splits], kernel, cfg);
+            static CeRoom room[2][9];
+            a.overlap = a.overlap && jobs <= ce_clusters_at_once(room[warps == WARPS][a.splits], kernel, cfg);
         }
         if (a.overlap) {
             attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;

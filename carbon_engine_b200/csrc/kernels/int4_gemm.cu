@@ -630,8 +630,7 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
     const bool gated = mode == SWIGLU || mode == RELUGLU;
     const int el = dtype == CE_F32 ? 4 : 2, row_tiles = gated ? (N + 7) / 8 : (N + 15) / 16;
     const bool vec = ((uintptr_t)x % (4 * el)) == 0 && ldx % 4 == 0;
-    if (!scratch) {
-        if (!streamed(dtype, M, K)) return ce_fail(CE_ERR_ARG, "int4_gemm: these sizes need scratch memory");
+    if (streamed(dtype, M, K)) {
         StreamArgs a{x, (const unsigned char*)w, out, c->status, ldx, M, N, K, kblocks, ldo, mode, gated, row_tiles, 0, 0, 0, vec};
         const int code = dtype == CE_F32 ? (kept == 32 ? launch_stream_tiles<float, 32>(a, tiles, (cudaStream_t)stream)
                                                        : launch_stream_tiles<float, 64>(a, tiles, (cudaStream_t)stream))
@@ -639,6 +638,7 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
                                                        : launch_stream_tiles<__nv_bfloat16, 64>(a, tiles, (cudaStream_t)stream));
         return code == 1 ? ce_fail(CE_ERR_SIZE, "int4_gemm: no room for clusters on this device") : code;
     }
+    if (!scratch) return ce_fail(CE_ERR_ARG, "int4_gemm: these sizes need scratch memory");
     if (dtype == CE_BF16) return ce_int4_gemm_tc(x, ldx, w, out, ldo, M, N, K, kept, mode, scratch, c->status, (cudaStream_t)stream);
     Operand op;
     op.frag = (uint32_t*)scratch;

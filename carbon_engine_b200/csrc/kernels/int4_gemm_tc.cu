@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    // codes of runs of columns, by one lane (not what the kernel in front writes, and what wrote them ended before that one began)
+    // codes of runs of columns, by one lane (a weight is never still being written here: int4_weight_done_kernel)
     auto copy_codes = [&](int run) {
         const int count = min(RUN, n_kb - run * RUN);
         uint64_t* bar = &raw_full[run % RAW];

@@ -282,6 +282,35 @@ def test_slots_strides_and_a_launch_shaped_for_less():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d,heads,kv_heads,group,lengths,window", [
+    (64, 4, 2, 32, [3000, 40, 1, 0], 0), (128, 8, 2, 64, [2500, 17], 0), (128, 12, 1, 32, [2100, 900], 0), (192, 2, 1, 64, [1700, 33], 0),
+    (256, 6, 2, 32, [1600, 5], 0), (128, 5, 1, 32, [3100], 2500)])
+def test_keys_shared_among_blocks(monkeypatch, dtype, d, heads, kv_heads, group, lengths, window):
+    """Blocks that join as a cluster (up to 8 of few row blocks), and by a second kernel."""
+    from carbon_engine_b200 import ops, ops_int4
+    c, k, v = filled(lengths, kv_heads, d, group, 16, dtype)
+    q = normal((len(lengths), heads, d), 9, dtype)
+    tiles = -(-(min(max(lengths), window + 16) if window else max(lengths)) // 16)
+    for splits in (1, 2, 5, 8, 11, 24, 40):
+        monkeypatch.setattr(ops_int4, "_splits", lambda jobs, n: (splits, -(-tiles // splits)))
+        before = ops.kernel_counts().get("int4_attention_merge_kernel", 0)
+        attend(c, q, k, v, [1] * len(lengths), lengths, group, window, dtype)
+        assert ops.kernel_counts().get("int4_attention_merge_kernel", 0) - before == (1 if splits > 8 else 0)
+
+
+@pytest.mark.parametrize("d,heads,kv_heads,group", [(128, 16, 8, 64), (64, 8, 8, 32), (128, 20, 4, 32), (256, 8, 8, 64)])
+def test_more_blocks_than_run_at_once(monkeypatch, d, heads, kv_heads, group):
+    """... which have fewer warps each; alone and with a second kernel that joins them."""
+    from carbon_engine_b200 import ops_int4
+    lengths = [1 + (i * 37) % 230 for i in range(320 // kv_heads)]
+    for splits in (1, 3):
+        monkeypatch.setattr(ops_int4, "_splits", lambda jobs, n: (splits, -(-15 // splits)))
+        for dtype in (BF16, F32):
+            c, k, v = filled(lengths, kv_heads, d, group, 16, dtype)
+            attend(c, normal((len(lengths), heads, d), 9, dtype), k, v, [1] * len(lengths), lengths, group, 0, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_rows_that_see_nothing_are_zeros(dtype):
     c, k, v = filled([20, 0, 33], 2, 64, 32, 16, dtype)
     out = attend(c, normal((3, 4, 64), 9, dtype), k, v, [1, 1, 1], [20, 0, 33], 32, 0, dtype)
@@ -416,6 +445,18 @@ def test_product_with_a_4_bit_weight(dtype, mode, M, N, K, group):
     before = out.clone()
     ops_int4.matmul(x, w4, out, mode)
     check_product(x, w, group, w4, mode, out, before)
+
+
+
+@pytest.mark.parametrize("M,N,K,group", [(20, 24, 16448, 32), (64, 16, 24576, 64), (33, 300, 8192 + 32, 32), (17, 2000, 64, 64), (40, 129, 192, 64), (3, 20, 70016, 64)])
+def test_products_of_wide_narrow_and_odd_weights(M, N, K, group):
+    """Tokens wider than what a thread of their preparation keeps, slices of K of one block of columns and of odd numbers of them."""
+    from carbon_engine_b200 import ops, ops_int4
+    x, w, w4, _ = product_case(BF16, ops.GEMM_STORE_F32, M, N, K, group)
+    out = normal((M, N), 5, F32)
+    ops_int4.matmul(x, w4, out, ops.GEMM_STORE_F32)
+    check_product(x, w, group, w4, ops.GEMM_STORE_F32, out)
+    assert int(w4.status) == 0
 
 
 @pytest.mark.parametrize("M", list(range(1, 65, 3)))
