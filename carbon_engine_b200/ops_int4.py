@@ -69,12 +69,16 @@ def _code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _ints(device: int, **tensors) -> None:
+_I32 = torch.int32
+
+
+def _ints(device: int, names: str, *tensors) -> None:
     """Contiguous int32 tensors on the given device.  (A call's checks are most of its time where the kernel is short: they ask for what is cheap
     to answer, and for the words of an error only when there is one.)"""
-    for name, t in tensors.items():
-        if t.dtype is not torch.int32 or t.get_device() != device or not t.is_contiguous():
-            ops._need(t, name, torch.int32)
+    for t in tensors:
+        if t.dtype is not _I32 or t.get_device() != device or not t.is_contiguous():
+            name = names.split()[[u is t for u in tensors].index(True)]
+            ops._need(t, name, _I32)
             raise KernelError(f"{name} is on {t.device}, the call's other tensors on cuda:{device}")
 
 
@@ -139,7 +143,7 @@ def _kv_call(fn, k, v, pages, positions, seq_of_token, seq_slot, block_table, st
     v_token, v_head, v_channel = v.stride()
     if T and (k_channel != 1 or v_channel != 1):
         raise KernelError("the channels of a head of k and v must lie together")
-    _ints(device, positions=positions, seq_of_token=seq_of_token, seq_slot=seq_slot, block_table=block_table, status=status)
+    _ints(device, "positions seq_of_token seq_slot block_table status", positions, seq_of_token, seq_slot, block_table, status)
     if seq_of_token.numel() != T or block_table.dim() != 2:
         raise KernelError("one position and one sequence a token, and a table of [slots, pages]")
     if T == 0:
@@ -255,7 +259,7 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
         raise KernelError(f"out is {tuple(out.shape)} {out.dtype} on {out.device}, not {tuple(q.shape)} {q.dtype}, contiguous, where q is")
     if pages.data.get_device() != device:
         raise KernelError(f"the pages are on {pages.data.device}, q on {q.device}")
-    _ints(device, seq_slot=seq_slot, q_start=q_start, ctx_len=ctx_len, block_table=block_table, status=status)
+    _ints(device, "seq_slot q_start ctx_len block_table status", seq_slot, q_start, ctx_len, block_table, status)
     if block_table.dim() != 2 or window < 0 or n_decode < 0 or max_ctx < 0:
         raise KernelError("attention: a table of [slots, pages], no negative numbers")
     if not scale > 0.0:
@@ -264,7 +268,7 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
     if n_decode > seqs or q_start.numel() <= seqs or ctx_len.numel() < seqs:
         raise KernelError("attention: one slot and one length a sequence, one start more")
     if tiles is not None:
-        _ints(device, tiles=tiles)
+        _ints(device, "tiles", tiles)
         n_tiles = tiles.numel() // 2 if n_tiles is None else int(n_tiles)
         if n_tiles < 0 or 2 * n_tiles > tiles.numel():
             raise KernelError(f"{n_tiles} tiles in a list of {tiles.numel() // 2}")
