@@ -2,7 +2,7 @@
 // int4.cuh).
 //
 // Eight lanes take 64 neighbouring channels of a token's head, 8 a lane (a word of a key's codes): a group's extremes are found with shuffles.  A
-// weight's kernels give a lane 4 columns.  Bound by the launch and by four loads that wait for one another (position, request, its slot, its page)
+// weight's quantisation gives a lane 4 columns.  Bound by the launch and by four loads that wait for one another (position, request, its slot, its page)
 // for single tokens, by the instructions - some 20 a value - for whole prompts.
 #include "int4.cuh"
 
@@ -201,15 +201,6 @@ struct WeightArgs {
     long long ld;
     int rows, gated, width, kblocks, group, vec;
 };
-// the row tile and the row in it of a weight's row: a gated weight's halves take eight rows of a tile each
-__device__ __forceinline__ int place_of(const WeightArgs& a, int row, int& in) {
-    const int half = a.rows >> 1;
-    if (!a.gated) { in = row & 15; return row >> 4; }
-    const int n = row < half ? row : row - half;
-    in = (n & 7) + (row < half ? 0 : 8);
-    return n >> 3;
-}
-
 // a warp takes 128 neighbouring columns of one row of a tile: rows of padding, and columns beyond the width, hold zeros
 template <typename T>
 __global__ void __launch_bounds__(256) int4_quantise_weight_kernel(WeightArgs a) {
@@ -235,22 +226,26 @@ __global__ void __launch_bounds__(256) int4_quantise_weight_kernel(WeightArgs a)
 // early beside the one before it can meet a weight that is still being written.
 __global__ void int4_weight_done_kernel() {}
 
+// a warp takes a tile: a lane the words of two rows, 8 columns of either half each
 template <typename T>
 __global__ void __launch_bounds__(256) int4_dequantise_weight_kernel(WeightArgs a) {
     ce_pdl_begin();
-    const int lane = threadIdx.x & 15, kept = min(a.group, 64);
-    const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int r = (int)(u / a.kblocks), kb = (int)(u - (long long)r * a.kblocks), col = kb * 64 + 4 * lane;
-    if (r >= a.rows || col >= a.width) return;
-    int in;
-    const int tile_no = place_of(a, r, in);
+    const int lane = threadIdx.x & 31, r = lane >> 2, l = lane & 3, kept = min(a.group, 64), gb = 64 / kept;
+    const int kb = blockIdx.y * 8 + (threadIdx.x >> 5), tile_no = blockIdx.x, half_rows = a.rows >> 1;
+    if (kb >= a.kblocks) return;
     const unsigned char* tile = a.tiles + ((size_t)tile_no * a.kblocks + kb) * i4_weight_tile_bytes(kept);
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + i4_k_word(in, col & 63)) >> (lane & 1 ? 16 : 0);
-    const __half2 sz = *reinterpret_cast<const __half2*>(tile + 512 + (in * (64 / kept) + (col & 63) / kept) * 4);
-    float x[4];
+    const uint4 w = *reinterpret_cast<const uint4*>(tile + lane * 16);
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), __low2float(sz), __high2float(sz));
-    store4((T*)a.w + r * a.ld + col, a.vec, x);
+    for (int e = 0; e < 4; ++e) {                     // rows r and r + 8, first and second 32 columns
+        const int in = r + 8 * (e & 1), col = kb * 64 + 32 * (e >> 1) + 8 * l;
+        const int n = a.gated ? tile_no * 8 + r : tile_no * 16 + in, row = a.gated && (e & 1) ? n + half_rows : n;
+        if (n >= (a.gated ? half_rows : a.rows) || col >= a.width) continue;
+        const __half2 sz = *reinterpret_cast<const __half2*>(tile + 512 + (in * gb + (gb == 2 ? e >> 1 : 0)) * 4);
+        float x[8];
+        values_of(words[e], sz, x);
+        store8((T*)a.w + (long long)row * a.ld + col, a.vec, x);
+    }
 }
 
 int check_cache(const CacheArgs& a, int dtype, const char* who) {
@@ -343,12 +338,12 @@ extern "C" int ce_int4_quantise_weight(int dtype, const void* w, long long ld, v
 extern "C" int ce_int4_dequantise_weight(int dtype, void* w, long long ld, const void* tiles, int rows, int gated, int width, int group, void* stream) {
     WeightArgs a{w, (unsigned char*)tiles, ld, rows, gated, width, (width + 63) / 64, group, 0};
     if (int e = check_weight(a, dtype, "int4_dequantise_weight")) return e;
-    a.vec = aligned4(w, ld, 0, dtype);
-    const long long units = (long long)rows * a.kblocks, grid = (units + 15) / 16;
-    if (grid > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_dequantise_weight: too large");
+    a.vec = ((uintptr_t)w & 15) == 0 && ld % (dtype == CE_F32 ? 4 : 8) == 0;
+    const dim3 grid((unsigned)(gated ? (rows / 2 + 7) / 8 : (rows + 15) / 16), (unsigned)((a.kblocks + 7) / 8));
+    if (grid.y > 65535) return ce_fail(CE_ERR_SIZE, "int4_dequantise_weight: too large");
     ce_note("int4_dequantise_weight_kernel");
-    const cudaError_t e = dtype == CE_F32 ? ce_launch(int4_dequantise_weight_kernel<float>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a)
-                                          : ce_launch(int4_dequantise_weight_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, a);
+    const cudaError_t e = dtype == CE_F32 ? ce_launch(int4_dequantise_weight_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, a)
+                                          : ce_launch(int4_dequantise_weight_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, a);
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_dequantise_weight: %s", cudaGetErrorString(e)); }
     int4_weight_done_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();           // (a product may read its weight ahead of the kernels in front)
     return ce_check_launch("int4_dequantise_weight");

@@ -200,13 +200,17 @@ def _joined(jobs: int, splits: int) -> bool:
     return splits > 8 or (splits > 1 and jobs * splits > 296)
 
 
-#: row blocks from which a portion goes to the tcgen05 kernel, which does not share keys among blocks
-TENSOR_BLOCKS = 32
+#: Query rows (tokens by heads) for each round of its blocks from which portions of bfloat16 go to the tcgen05 kernel, whose blocks take up to 256
+#: rows of a KV head and all of their keys: its time is the rounds' and the keys', that of the kernel on mma.sync the rows' and the keys'.  (8 KV
+#: heads of 128, 2,048 keys: 52 us, against 32 for 2,048 rows, 42 for 4,096, 83 for 8,192; 16,000 keys: 330 us, against 139 for 2,048 rows
+#: and 426 for 8,192.)
+TENSOR_ROWS = 6000
 
 
 @functools.lru_cache(maxsize=256)
 def _row_blocks(each: int, d: int, tile: int):
-    """Blocks a KV head takes of a sequence's token (tile 0) or of a tile of 64 tokens (1), their rows, and blocks of the tcgen05 kernel."""
+    """Blocks a KV head takes of a sequence's token (tile 0) or of a tile of 64 tokens (1), their rows, and blocks
+    of the tcgen05 kernel (0: not such heads)."""
     k = kernels()
     return k.ce_int4_attention_blocks(each, d, tile), k.ce_int4_attention_rows(each, d, tile), k.ce_int4_attention_tc_blocks(each, d) if tile else 0
 
@@ -216,9 +220,9 @@ def _attend(device, code, q, q_stride, heads, pages, out, seq_slot, q_start, ctx
     each = heads // pages.kv_heads
     tile = 0 if tiles is None else 1
     blocks, block_rows, tensor_blocks = _row_blocks(each, pages.head_dim, tile)
-    jobs = count * pages.kv_heads * blocks
+    jobs, tensor_blocks = count * pages.kv_heads * blocks, count * pages.kv_heads * tensor_blocks
     keys = min(max_ctx, window + (64 if tile else 1) + 15) if window > 0 else max_ctx
-    if (code == ops.BF16 and tensor_blocks * count * pages.kv_heads >= TENSOR_BLOCKS and count <= 65535 and q_stride % 8 == 0
+    if (code == ops.BF16 and tensor_blocks and min(64 * count, q.shape[0]) * heads >= TENSOR_ROWS * max(1.0, tensor_blocks / 148) and count <= 65535 and q_stride % 8 == 0
             and (q.data_ptr() | out.data_ptr()) % 16 == 0):
         splits = share = 0
     else:

@@ -220,7 +220,7 @@ def test_attention_of_portions(dtype, d, heads, kv_heads, group, page, new, leng
 def test_attention_of_portions_on_tcgen05(monkeypatch, d, heads, kv_heads, group, page, new, lengths, window):
     """The kernel that takes portions of many row blocks, at any number of them."""
     from carbon_engine_b200 import ops, ops_int4
-    monkeypatch.setattr(ops_int4, "TENSOR_BLOCKS", 1)
+    monkeypatch.setattr(ops_int4, "TENSOR_ROWS", 1)
     c, k, v = filled(lengths, kv_heads, d, group, page, BF16)
     q = normal((sum(new), heads, d), 9, BF16)
     before = ops.kernel_counts().get("int4_attention_tc_kernel", 0)
@@ -230,7 +230,7 @@ def test_attention_of_portions_on_tcgen05(monkeypatch, d, heads, kv_heads, group
 
 def test_portions_on_tcgen05_with_numbers_that_are_none(monkeypatch):
     from carbon_engine_b200 import ops_int4
-    monkeypatch.setattr(ops_int4, "TENSOR_BLOCKS", 1)
+    monkeypatch.setattr(ops_int4, "TENSOR_ROWS", 1)
     for which in ("k", "v", "window"):
         lengths, new = [150], [140]
         c = Cache(lengths, 1, 128, 32, 16)
@@ -255,7 +255,7 @@ def test_portions_on_tcgen05_with_numbers_that_are_none(monkeypatch):
 
 def test_portions_on_tcgen05_with_scores_far_apart(monkeypatch):
     from carbon_engine_b200 import ops_int4
-    monkeypatch.setattr(ops_int4, "TENSOR_BLOCKS", 1)
+    monkeypatch.setattr(ops_int4, "TENSOR_ROWS", 1)
     for spread in (3.0, 30.0):
         c = Cache([400], 1, 128, 32, 16)
         k = normal((400, 1, 128), 1, F32, spread / 11.3)
