@@ -475,8 +475,12 @@ template <int G, int TOKENS>
 int run(TokensArgs p, Args a, cudaStream_t stream) {
     using S = Shape<G, TOKENS>;
     auto kernel = int4_gemm_tc_kernel<G, TOKENS>;
+    // more than it uses: beside a block of another stream's kernel that holds tensor memory, one of this kernel would wait for it inside its
+    // cluster, and that one's cluster, elsewhere, for a block that waits for this kernel's
+    constexpr int SMEM = 220 * 1024;
+    static_assert(S::BYTES <= SMEM, "shared memory");
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = ce_allow_smem(done, kernel, S::BYTES);
+    cudaError_t e = ce_allow_smem(done, kernel, SMEM);
     if (e == cudaSuccess) {
         ce_note("int4_tokens_kernel");
         e = ce_launch(int4_tokens_kernel, dim3(TOKENS), dim3(1024), 0, stream, p);
@@ -489,7 +493,7 @@ int run(TokensArgs p, Args a, cudaStream_t stream) {
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[2];
         cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = S::BYTES;
+        cfg.dynamicSmemBytes = SMEM;
         cfg.stream = stream;
         cfg.attrs = attr;
         a.overlap = ce_pdl_enabled();
