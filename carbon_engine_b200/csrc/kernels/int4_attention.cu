@@ -66,7 +66,7 @@ __device__ __forceinline__ Job job_of(const Args& a, int job, int rows) {
     const int start = a.q_start[j.b], n = a.q_start[j.b + 1] - start;
     j.slot = a.seq_slot[j.b];
     j.t0 = start + q0;
-    j.tokens = a.tiles ? min(64, n - q0) : 1;
+    j.tokens = min(a.tiles ? 64 : 1, n - q0);         // (none: a place of the batch that nobody took)
     j.base = a.ctx_len[j.b] - n + q0;
     j.row0 = sub * rows;
     return j;

@@ -246,7 +246,7 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
 
     ``q`` [T, heads, head_dim] (tokens at any stride, the heads of a token together), ``out`` [T, heads, head_dim] contiguous; sequence b has
     the rows ``q_start[b]`` .. ``q_start[b + 1]`` and ``ctx_len[b]`` keys with them, and its pages in row ``seq_slot[b]`` of ``block_table``.  The first ``n_decode`` sequences bring one
-    token each; the others are listed in ``tiles`` (int32 [n_tiles, 2]: sequence, first of up to 64 of its tokens).  ``max_ctx``: at least the longest
+    token each, or none; the others are listed in ``tiles`` (int32 [n_tiles, 2]: sequence, first of up to 64 of its tokens).  ``max_ctx``: at least the longest
     ``ctx_len`` (it only shapes the launch: a smaller number is slower, not wrong).  ``window`` > 0: a query sees that many keys, itself the last of them.  A row that sees no key becomes zeros; rows of ``out`` that
     belong to no sequence stay as they were.  ``status`` becomes 4 where a page is not held, 7 where a wait gave up."""
     device = _current(q, "q")

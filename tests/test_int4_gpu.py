@@ -271,6 +271,17 @@ def test_one_token_as_a_portion_is_that_token():
     attend(c, q, k, v, [1, 1], [100, 37], 64, 0, BF16, n_decode=0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_places_of_a_batch_that_nobody_took(monkeypatch, dtype):
+    """Among single tokens, at the end too, whether keys are shared among blocks or not."""
+    from carbon_engine_b200 import ops_int4
+    new, lengths = [1, 0, 1, 0, 0], [40, 33, 300, 0, 17]
+    c, k, v = filled(lengths, 2, 64, 32, 16, dtype)
+    for splits in (1, 2, 9):
+        monkeypatch.setattr(ops_int4, "_splits", lambda jobs, n: (splits, -(-19 // splits)))
+        attend(c, normal((2, 4, 64), 9, dtype), k, v, new, lengths, 32, 0, dtype, n_decode=5)
+
+
 def test_slots_strides_and_a_launch_shaped_for_less():
     lengths = [260, 90, 33]
     c, k, v = filled(lengths, 2, 128, 64, 16, BF16, slots=[4, 0, 2])
