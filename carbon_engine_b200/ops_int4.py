@@ -62,6 +62,17 @@ _device = torch._C._cuda_getDevice
 _stream = torch._C._cuda_getCurrentRawStream
 
 
+_entries = {}
+
+
+def _entry(name: str):
+    """An entry point of the kernels' library, looked up (behind that library's lock) once."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(kernels(), name)
+    return fn
+
+
 def _code(t: torch.Tensor, name: str) -> int:
     code = _CODES.get(t.dtype)
     if code is None:
@@ -161,14 +172,14 @@ def kv_write(pages: Int4Pages, k: torch.Tensor, v: torch.Tensor, positions: torc
     """Quantise the keys and values of T tokens into the pages: token t of sequence ``seq_of_token[t]`` (its table row
     ``seq_slot`` of that) goes to position ``positions[t]``.  ``k``, ``v`` [T, kv_heads, head_dim] bfloat16 or float32, tokens and heads at any stride (the columns of a step's
     projection, for instance).  No two tokens of a call may have the same place.  ``status`` becomes 2 where a token's page is not held; its row is dropped then."""
-    _kv_call(kernels().ce_int4_kv_write, k, v, pages, positions, seq_of_token, seq_slot, block_table, status)
+    _kv_call(_entry("ce_int4_kv_write"), k, v, pages, positions, seq_of_token, seq_slot, block_table, status)
 
 
 def kv_read(pages: Int4Pages, k_out: torch.Tensor, v_out: torch.Tensor, positions: torch.Tensor, seq_of_token: torch.Tensor,
             seq_slot: torch.Tensor, block_table: torch.Tensor, status: torch.Tensor) -> None:
     """Read back what T places hold, as :func:`kv_write` names them, rounded once to the outputs' type.  ``status`` becomes 4 where a
     place's page is not held; its rows stay as they were."""
-    _kv_call(kernels().ce_int4_kv_read, k_out, v_out, pages, positions, seq_of_token, seq_slot, block_table, status)
+    _kv_call(_entry("ce_int4_kv_read"), k_out, v_out, pages, positions, seq_of_token, seq_slot, block_table, status)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -216,7 +227,6 @@ def _row_blocks(each: int, d: int, tile: int):
 
 
 def _attend(device, code, q, q_stride, heads, pages, out, seq_slot, q_start, ctx_len, block_table, status, tiles, count, max_ctx, window, scale) -> None:
-    k = kernels()
     each = heads // pages.kv_heads
     tile = 0 if tiles is None else 1
     blocks, block_rows, tensor_blocks = _row_blocks(each, pages.head_dim, tile)
@@ -232,7 +242,7 @@ def _attend(device, code, q, q_stride, heads, pages, out, seq_slot, q_start, ctx
         rows = jobs * splits * block_rows
         part_o = torch.empty(rows * (pages.head_dim + 2), dtype=torch.float32, device=q.device)
         part_ml = part_o.data_ptr() + 4 * rows * pages.head_dim
-    ops._ok(k.ce_int4_attention(_ATTENTION(
+    ops._ok(_entry("ce_int4_attention")(_ATTENTION(
         code, q.data_ptr(), q_stride, pages.data.data_ptr(), out.data_ptr(), seq_slot.data_ptr(), q_start.data_ptr(), ctx_len.data_ptr(),
         block_table.data_ptr(), status.data_ptr(), 0 if tiles is None else tiles.data_ptr(), count, heads, pages.kv_heads, pages.head_dim,
         pages.group, pages.page_size, block_table.shape[1], pages.num_pages, window, splits, share,
@@ -357,12 +367,11 @@ def matmul(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, mode: int = ops.GE
         raise KernelError("the columns of a row of x and out must lie together")
     if M == 1:
         ldx, ldo = w.width, N               # (a single row's stride says nothing)
-    k = kernels()
     # up to 16 tokens that fit the registers of 8 blocks: no scratch memory, one launch (the launcher checks it too)
     scratch = None
     if (M + 7) // 8 * (1 if code else 2) * w.kblocks > 512 or M > 16:
-        scratch = torch.empty(k.ce_int4_gemm_scratch(code, M, w.width, w.group), dtype=torch.float32, device=x.device)
+        scratch = torch.empty(_entry("ce_int4_gemm_scratch")(code, M, w.width, w.group), dtype=torch.float32, device=x.device)
     if ops._profile is not None:
         ops._profile.note_work(w.data.numel() + M * w.width * x.element_size() + out.numel() * out.element_size(), 2 * M * w.rows * w.width)
-    ops._ok(k.ce_int4_gemm(_GEMM(code, x.data_ptr(), ldx, w.data.data_ptr(), out.data_ptr(), ldo, M, N, w.width, w.group, mode,
+    ops._ok(_entry("ce_int4_gemm")(_GEMM(code, x.data_ptr(), ldx, w.data.data_ptr(), out.data_ptr(), ldo, M, N, w.width, w.group, mode,
                                  0 if scratch is None else scratch.data_ptr(), w.status.data_ptr(), _stream(device))), 1 if scratch is None else 2)
