@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, 53);
     } else {
-        // ---- the sums: a row and half of the tokens a lane; the next group's products are on their way while this one's are added
+        // ---- the sums: a row and half of the tokens a lane, two groups at a time
         const int quad = warp & 3, row = quad * 32 + lane, unit = row >> 4, first = (warp - FIRST - MAKERS) / 4 * PART;
         const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + first;
 #pragma unroll
