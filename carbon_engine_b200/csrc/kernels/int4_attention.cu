@@ -76,6 +76,50 @@ template <typename T> struct Pieces;
 template <> struct Pieces<__nv_bfloat16> { static constexpr int N = 1; };
 template <> struct Pieces<float> { static constexpr int N = 2; };
 
+// A lane's channels of a query row, 8 of every 32, as they were read
+template <typename T, int CH> struct Raw;
+template <int CH> struct Raw<__nv_bfloat16, CH> {
+    uint2 w[CH][2];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) w[c][0] = w[c][1] = make_uint2(0, 0);
+    }
+    __device__ __forceinline__ void load(const __nv_bfloat16* src, bool vec) {
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i, p += 4) {
+                w[c][i] = vec ? *reinterpret_cast<const uint2*>(p) : make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
+                if (i) p += 24;
+            }
+    }
+    __device__ __forceinline__ float at(int c, int i) const {
+        const uint32_t v = (i & 2) ? w[c][i >> 2].y : w[c][i >> 2].x;
+        return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
+    }
+};
+template <int CH> struct Raw<float, CH> {
+    float4 w[CH][2];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) w[c][0] = w[c][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __device__ __forceinline__ void load(const float* p, bool vec) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i, p += 4) {
+                w[c][i] = vec ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
+                if (i) p += 24;
+            }
+    }
+    __device__ __forceinline__ float at(int c, int i) const {
+        const float4& v = w[c][i >> 2];
+        return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+    }
+};
+
 // (s, z) of one token's groups out of shared memory, as they lie: NG words
 template <int NG>
 __device__ __forceinline__ void load_steps(const unsigned char* p, uint32_t (&v)[NG]) {
@@ -100,7 +144,7 @@ __device__ __forceinline__ float weight_of(float m, float l, float M) { return l
 template <typename T>
 __device__ __forceinline__ void store_row(const Args& a, const Job& j, int row, int d, int ch, float4 v, float L) {
     const float inv = L == 0.f ? 0.f : 1.0f / L;
-    const int each = a.nh / a.nkv, rho = j.row0 + row, tok = rho / each;
+    const int each = a.nh / a.nkv, rho = j.row0 + row, tok = a.tiles ? rho / each : 0;
     T* dst = (T*)a.out + ((size_t)(j.t0 + tok) * a.nh + j.kvh * each + rho - tok * each) * d + ch;
     if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4*>(dst) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
@@ -145,7 +189,8 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     const Job j = job_of(a, job_id, ROWS);
     const int each = a.nh / a.nkv, rows = min(ROWS, j.tokens * each - j.row0);
     if (rows <= 0) return;                            // a tile with fewer tokens than its row blocks take
-    const int first_pos = j.base + j.row0 / each, last_pos = j.base + (j.row0 + rows - 1) / each;
+    auto token_of = [&](int rho) { return a.tiles ? rho / each : 0; };        // (a single token's rows are its heads)
+    const int first_pos = j.base + token_of(j.row0), last_pos = j.base + token_of(j.row0 + rows - 1);
     const int block_lo = a.window > 0 ? max(0, first_pos - a.window + 1) : 0;
     const int tile_lo = block_lo >> 4, tiles = last_pos < block_lo ? 0 : (last_pos >> 4) + 1 - tile_lo;
     // shares of the longest context's length (shorter sequences take fewer blocks), or as many keys as it takes
@@ -176,6 +221,13 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
         const unsigned char* src = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(place), i - looked));
         if (lane == 0) i4_copy(ring + (i % STAGES) * TILE, src, TILE, &full[warp][i % STAGES]);
     };
+    Raw<T, CH> raw[NT];                               // asked for ahead of the pages: both take a trip
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = nt * 8 + r, rho = j.row0 + row, tok = token_of(rho);
+        raw[nt].clear();
+        if (row < rows) raw[nt].load((const T*)a.q + (size_t)(j.t0 + tok) * a.q_stride + (size_t)(j.kvh * each + rho - tok * each) * D + 8 * l, a.vec);
+    }
     look_up(0);
     for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
 
@@ -186,69 +238,50 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     int hi[NT][2], lo[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int row = nt * 8 + r;
-        float x[CH][8], largest = 0.f;
-        if (row < rows) {
-            const int rho = j.row0 + row, tok = rho / each;
-            const T* src = (const T*)a.q + (size_t)(j.t0 + tok) * a.q_stride + (size_t)(j.kvh * each + rho - tok * each) * D + 8 * l;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                if (a.vec) {
-                    const float4 u = ce_load4(src + 32 * c), v = ce_load4(src + 32 * c + 4);
-                    x[c][0] = u.x; x[c][1] = u.y; x[c][2] = u.z; x[c][3] = u.w; x[c][4] = v.x; x[c][5] = v.y; x[c][6] = v.z; x[c][7] = v.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[c][i] = CeType<T>::load(src + 32 * c + i);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[c][i] = 0.f;
-        }
+        float largest = 0.f;
         bool finite = true;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { largest = fmaxf(largest, fabsf(x[c][i])); finite = finite && fabsf(x[c][i]) <= 3.402823466e38f; }
+            for (int i = 0; i < 8; ++i) { const float x = fabsf(raw[nt].at(c, i)); largest = fmaxf(largest, x); finite = finite && x <= 3.402823466e38f; }
         if (!finite) largest = INFINITY;
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        const float up = i4_row_scale(largest);
-        float sums[NG];
+        const float up = i4_row_scale(largest), up16 = up * 0.0625f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) sums[g] = 0.f;
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            float y[8];
+            for (int i = 0; i < 4; ++i) {
+                float x = raw[nt].at(c, i) * (i & 1 ? up16 : up), y = raw[nt].at(c, i + 4) * (i & 1 ? up16 : up);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[c][i] * up;
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = i & 1 ? 0.0625f : 1.0f;
-                    qf[nt][p][c][i] = i4_pack(y[i] * f, y[i + 4] * f);
-                    const float2 got = i4_unpack(qf[nt][p][c][i]);
-                    const float g0 = got.x * (i & 1 ? 16.0f : 1.0f), g1 = got.y * (i & 1 ? 16.0f : 1.0f);
-                    sums[c * 32 / G] += g0 + g1;
-                    y[i] -= g0; y[i + 4] -= g1;
+                for (int p = 0; p < P; ++p) {
+                    qf[nt][p][c][i] = i4_pack(x, y);
+                    if (p + 1 < P) {
+                        const float2 got = i4_unpack(qf[nt][p][c][i]);
+                        x -= got.x; y -= got.y;
+                    }
                 }
             }
-        }
+        // the groups' sums, where the scores will lie: products with codes of 1, as ordinary numbers
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
-            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+            float acc[P][4];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) qsum[nt][g][e] = __shfl_sync(0xffffffffu, sums[g], 4 * (2 * l + e)) * (1.0f / i4_unit<C8>);
+            for (int c = g * G / 32; c < (g + 1) * G / 32; ++c)
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    if (c == g * G / 32) i4_mma_first(acc[p], 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, qf[nt][p][c][0], qf[nt][p][c][1]);
+                    else i4_mma(acc[p], 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, qf[nt][p][c][0], qf[nt][p][c][1]);
+                    i4_mma(acc[p], 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, qf[nt][p][c][2], qf[nt][p][c][3]);
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qsum[nt][g][e] = (P == 2 ? acc[0][e] + acc[P - 1][e] : acc[0][e]) * (1.0f / i4_unit<C8>);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const float u = __shfl_sync(0xffffffffu, up, 4 * (2 * l + e));
             row_scale[nt][e] = a.scale * LOG2E * i4_unit<C8> / u;
-            const int rr = nt * 8 + 2 * l + e, pos = j.base + (j.row0 + rr) / each;
+            const int rr = nt * 8 + 2 * l + e, pos = j.base + token_of(j.row0 + rr);
             hi[nt][e] = rr < rows ? pos : -1;
             lo[nt][e] = a.window > 0 ? pos - a.window + 1 : 0;
         }
@@ -548,7 +581,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     // the blocks' runs of keys, in their order: each takes a share of the rows' channels
     cluster_sync();
     const int all = rows * (D / 4);
-    for (int x = split * blockDim.x + threadIdx.x; x < all; x += a.splits * blockDim.x) {
+    for (int x = threadIdx.x * a.splits + split; x < all; x += a.splits * blockDim.x) {
         const int row = x / (D / 4), ch = (x - row * (D / 4)) * 4;
         float M = NOTHING, L = 0.f, ms[8], ls[8];
         float4 us[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
