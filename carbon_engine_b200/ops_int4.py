@@ -188,8 +188,8 @@ def _splits(jobs: int, tiles: int):
     that blocks take.  Blocks of 8 warps, two an SM, or of 4, four an SM, where there are more than 296; a block takes 1.03 us for each tile of a
     warp (0.65 with an SM to itself) and 4.5 to begin and end.  Of more than the chip holds at once, the mean of what it is for requests of one
     length and for those of half the longest on the average, whose long ones end alone; and what a second kernel takes that joins them.  (64
-    sequences of 8,192 keys, 8 KV heads of 128, in 1, 2, 3, 4 and 8 blocks a row block: 137, 127, 137, 131 and 146 us; 21 of 450 to 9,000
-    keys, groups of 32, in 1 to 6: 78, 58, 70, 57, 51 and 52 us.)"""
+    sequences of 8,192 keys, 8 KV heads of 128, in 1, 2, 3, 4 and 8 blocks a row block: 136, 137, 135, 130 and 144 us; 21 of 450 to 9,000
+    keys, groups of 32, in 1 to 6: 75, 76, 65, 55, 48 and 49 us.)"""
     best = (float("inf"), 1, tiles)
     for splits in (1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64):
         share = -(-tiles // splits)
