@@ -9,7 +9,7 @@
 // (22 bits), with the groups' sums of what was rounded.
 //
 // The stream is bound by the instructions that take codes apart and by the latencies between them, not by memory: 6,144 x 4,096 for one token
-// 7 us (2.0 TB/s), 12,288 + 12,288 rows of 4,096 for 8 tokens 17.5 us (3.2 TB/s), 75,776 x 4,096 for one token 41 us (4.3 TB/s).  Up to 8 tokens it
+// 6.4 us (2.2 TB/s), 12,288 + 12,288 rows of 4,096 for 8 tokens 17.3 us (3.3 TB/s), 75,776 x 4,096 for one token 40 us (4.4 TB/s).  Up to 8 tokens it
 // is the faster one everywhere; for 9 to 16 it is as long as rows are few (4,096 x 12,288, 16 tokens: 19.6 us, on tcgen05 24; 12,288 + 12,288 x 4,096:
 // 33, 51), and 10 % slower for 75,776 rows of 4,096 (112, 99).
 #include "int4.cuh"
@@ -372,69 +372,129 @@ __global__ void __launch_bounds__(SW * 32) int4_stream_kernel(StreamArgs a) {
     for (int nt = 0; nt < NT; ++nt) {
         const int t = nt * 8 + r;
         const T* src = (const T*)a.x + (size_t)t * a.ldx + kb0 * 64 + 8 * l;
-        float x[KW][2][8], largest = 0.f;
-        bool finite = true;
+        float up;
+        if constexpr (P == 1) {
+            // in pairs, as they lie; the groups' sums as products with codes of 1 (as ordinary numbers): a third of the instructions, which a block runs
+            // once and cold (6,144 x 4,096, one token: 4,500 cycles of 10,800 before)
+            uint32_t x[KW][2][4];
 #pragma unroll
-        for (int k = 0; k < KW; ++k)
+            for (int k = 0; k < KW; ++k)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int c = k * 64 + half * 32;
-                if (t < a.M && k < count && kb0 * 64 + c + 8 * l < a.K) {
-                    if (a.vec) {
-                        const float4 u = ce_load4(src + c), v = ce_load4(src + c + 4);
-                        x[k][half][0] = u.x; x[k][half][1] = u.y; x[k][half][2] = u.z; x[k][half][3] = u.w;
-                        x[k][half][4] = v.x; x[k][half][5] = v.y; x[k][half][6] = v.z; x[k][half][7] = v.w;
-                    } else {
+                for (int half = 0; half < 2; ++half) {
+                    const int c = k * 64 + half * 32;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[k][half][i] = CeType<T>::load(src + c + i);
+                    for (int i = 0; i < 4; ++i) x[k][half][i] = 0;
+                    if (t < a.M && k < count && kb0 * 64 + c + 8 * l < a.K) {
+                        if (a.vec) {
+                            const uint2 u = *reinterpret_cast<const uint2*>(src + c), v = *reinterpret_cast<const uint2*>(src + c + 4);
+                            x[k][half][0] = u.x; x[k][half][1] = u.y; x[k][half][2] = v.x; x[k][half][3] = v.y;
+                        } else {
+                            const unsigned short* p = reinterpret_cast<const unsigned short*>(src + c);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[k][half][i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+                        }
                     }
-                } else {
+                }
+            __nv_bfloat162 most = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[k][half][i] = 0.f;
+            for (int k = 0; k < KW; ++k)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&x[k][half][i])));
+            const float2 two = __bfloat1622float2(most);
+            float largest = two.x <= 3.402823466e38f && two.y <= 3.402823466e38f ? fmaxf(two.x, two.y) : INFINITY;
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+            up = i4_row_scale(largest);
+            const float up16 = up * 0.0625f;                                  // odd codes come 16 times too large
+            sums.b[nt][0] = sums.b[nt][1] = 0;
+#pragma unroll
+            for (int k = 0; k < KW; ++k) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t* v = x[k][half];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        xf[k][nt][0][half][2 * i] = i4_pack(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i + 2] << 16) * up);
+                        xf[k][nt][0][half][2 * i + 1] = i4_pack(__uint_as_float(v[i] & 0xffff0000u) * up16, __uint_as_float(v[i + 2] & 0xffff0000u) * up16);
+                    }
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { largest = fmaxf(largest, fabsf(x[k][half][i])); finite = finite && fabsf(x[k][half][i]) <= 3.402823466e38f; }
-            }
-        if (!finite) largest = INFINITY;
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        const float up = i4_row_scale(largest);
-        if constexpr (P == 1) sums.b[nt][0] = sums.b[nt][1] = 0;
+                for (int g = 0; g < GB; ++g) {
+                    float c[4];
 #pragma unroll
-        for (int k = 0; k < KW; ++k) {
-            float sum[GB];
-#pragma unroll
-            for (int g = 0; g < GB; ++g) sum[g] = 0.f;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float y[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = x[k][half][i] * up;
-#pragma unroll
-                for (int p = 0; p < P; ++p)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float f = i & 1 ? 0.0625f : 1.0f, b = i & 1 ? 16.0f : 1.0f;      // odd codes come 16 times too large
-                        xf[k][nt][p][half][i] = i4_pack(y[i] * f, y[i + 4] * f);
-                        const float2 got = i4_unpack(xf[k][nt][p][half][i]);
-                        sum[half * 32 / G] += (got.x + got.y) * b;
-                        y[i] -= got.x * b; y[i + 4] -= got.y * b;
+                    for (int half = g * G / 32; half < (g + 1) * G / 32; ++half) {
+                        const uint32_t* v = xf[k][nt][0][half];
+                        if (half == g * G / 32) i4_mma_first(c, 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, v[0], v[1]);
+                        else i4_mma(c, 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, v[0], v[1]);
+                        i4_mma(c, 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, v[2], v[3]);
                     }
-            }
-#pragma unroll
-            for (int g = 0; g < GB; ++g) {
-                sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
-                sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
-                if constexpr (P == 2) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) sums.f[k][g][nt][e] = __shfl_sync(0xffffffffu, sum[g], 4 * (2 * l + e)) * (1.0f / i4_unit<C8>);
-                } else {
-                    const float part = sum[g] * (1.0f / 128.0f), high = __half2float(__float2half_rn(part));
+                    // (sums of tokens 2 l and 2 l + 1 are here; of token r wanted)
+                    const float even = __shfl_sync(0xffffffffu, c[0], r >> 1), odd = __shfl_sync(0xffffffffu, c[1], r >> 1);
+                    const float part = (r & 1 ? odd : even) * (1.0f / 128.0f), high = __half2float(__float2half_rn(part));
                     const int at = k * GB + g;                                // of the run's groups
                     if (at >> 1 == l) {
                         sums.b[nt][0] |= i4_pack(at & 1 ? 0.f : part, at & 1 ? part : 0.f);
                         sums.b[nt][1] |= i4_pack(at & 1 ? 0.f : part - high, at & 1 ? part - high : 0.f);
                     }
+                }
+            }
+        } else {
+            float x[KW][2][8], largest = 0.f;
+            bool finite = true;
+#pragma unroll
+            for (int k = 0; k < KW; ++k)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int c = k * 64 + half * 32;
+                    if (t < a.M && k < count && kb0 * 64 + c + 8 * l < a.K) {
+                        if (a.vec) {
+                            const float4 u = ce_load4(src + c), v = ce_load4(src + c + 4);
+                            x[k][half][0] = u.x; x[k][half][1] = u.y; x[k][half][2] = u.z; x[k][half][3] = u.w;
+                            x[k][half][4] = v.x; x[k][half][5] = v.y; x[k][half][6] = v.z; x[k][half][7] = v.w;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) x[k][half][i] = CeType<T>::load(src + c + i);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[k][half][i] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { largest = fmaxf(largest, fabsf(x[k][half][i])); finite = finite && fabsf(x[k][half][i]) <= 3.402823466e38f; }
+                }
+            if (!finite) largest = INFINITY;
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+            up = i4_row_scale(largest);
+#pragma unroll
+            for (int k = 0; k < KW; ++k) {
+                float sum[GB];
+#pragma unroll
+                for (int g = 0; g < GB; ++g) sum[g] = 0.f;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = x[k][half][i] * up;
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float f = i & 1 ? 0.0625f : 1.0f, b = i & 1 ? 16.0f : 1.0f;      // odd codes come 16 times too large
+                            xf[k][nt][p][half][i] = i4_pack(y[i] * f, y[i + 4] * f);
+                            const float2 got = i4_unpack(xf[k][nt][p][half][i]);
+                            sum[half * 32 / G] += (got.x + got.y) * b;
+                            y[i] -= got.x * b; y[i + 4] -= got.y * b;
+                        }
+                }
+#pragma unroll
+                for (int g = 0; g < GB; ++g) {
+                    sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+                    sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) sums.f[k][g][nt][e] = __shfl_sync(0xffffffffu, sum[g], 4 * (2 * l + e)) * (1.0f / i4_unit<C8>);
                 }
             }
         }
