@@ -94,6 +94,19 @@ template <int CH> struct Raw<__nv_bfloat16, CH> {
                 if (i) p += 24;
             }
     }
+    // the largest magnitude, infinity where one is not finite
+    __device__ __forceinline__ float largest() const {
+        __nv_bfloat162 most = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t v = (i & 1) ? w[c][i >> 1].y : w[c][i >> 1].x;
+                most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v)));
+            }
+        const float2 two = __bfloat1622float2(most);
+        return two.x <= 3.402823466e38f && two.y <= 3.402823466e38f ? fmaxf(two.x, two.y) : INFINITY;
+    }
     __device__ __forceinline__ float at(int c, int i) const {
         const uint32_t v = (i & 2) ? w[c][i >> 2].y : w[c][i >> 2].x;
         return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
@@ -113,6 +126,15 @@ template <int CH> struct Raw<float, CH> {
                 w[c][i] = vec ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
                 if (i) p += 24;
             }
+    }
+    __device__ __forceinline__ float largest() const {
+        float most = 0.f;
+        bool finite = true;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { const float x = fabsf(at(c, i)); most = fmaxf(most, x); finite = finite && x <= 3.402823466e38f; }
+        return finite ? most : INFINITY;
     }
     __device__ __forceinline__ float at(int c, int i) const {
         const float4& v = w[c][i >> 2];
@@ -238,13 +260,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
     int hi[NT][2], lo[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        float largest = 0.f;
-        bool finite = true;
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { const float x = fabsf(raw[nt].at(c, i)); largest = fmaxf(largest, x); finite = finite && x <= 3.402823466e38f; }
-        if (!finite) largest = INFINITY;
+        float largest = raw[nt].largest();
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         const float up = i4_row_scale(largest), up16 = up * 0.0625f;
