@@ -14,7 +14,7 @@
 // A block takes up to 8 or 16 rows (tokens by heads of the KV head) and a run of the keys; its 8 or 4 warps take tiles in turn, each with a
 // ring of its own that one lane fills with bulk copies (a tile is one run of bytes in the page); warps, then blocks, are joined in a fixed order.
 //
-// 64 sequences of 8,192 keys of 8 KV heads of 128 take 136 us, 4.4 TB/s: bound by instructions (313 a tile a warp, the ALU pipe, which takes the codes
+// 64 sequences of 8,192 keys of 8 KV heads of 128 take 133 us, 4.5 TB/s: bound by instructions (313 a tile a warp, the ALU pipe, which takes the codes
 // apart, half busy, 2.2 instructions a cycle of an SM).  A block costs some 4 us to begin (place, queries, first tiles) and end (joins), which
 // is what short and uneven requests are bound by (21 of 450 to 9,000 keys: 49 us of which 19.5 are the bytes').
 #include "int4.cuh"
