@@ -1,7 +1,7 @@
 // The 4-bit form of cached keys and values and of weights, shared by the kernels that write, read and multiply it.
 //
 // ``group`` neighbouring values share a minimum z and a step s, both float16; a value is c s + z with a code c of 0 .. 15:
-//   z = float16(min x),  s = float16((max x - z) f) with f the float32 next to 1/15, the difference and the product in float32,
+//   z = float16(min x),  s = float16(max(max x - z, 0) f) with f the float32 next to 1/15, the difference and the product in float32,
 //   c = (x - z) / s rounded to the nearest (ties to even) and cut to 0 .. 15;  s = 0 gives c = 0.
 // A group that holds a value beyond 60,000, or one that is not finite, becomes not a number as a whole (s = z = NaN): c s + z of every
 // other group is a finite float16 after rounding.
@@ -44,10 +44,11 @@ __device__ __forceinline__ int i4_v_word(int d, int token, int b, int r) {
 __device__ __forceinline__ int i4_k_step(int d, int groups, int token, int g) { return 16 * d + (token * groups + g) * 4; }
 __device__ __forceinline__ int i4_v_step(int d, int groups, int token, int g) { return 16 * d + 64 * groups + (token * groups + g) * 4; }
 
-// (s, z) of a group with the extremes lo and hi; ok: all its values are finite and at most I4_LIMIT
+// (s, z) of a group with the extremes lo and hi; ok: all its values are finite and at most I4_LIMIT.  Where rounding takes z above hi (float32
+// groups that are nearly constant), s is 0, as for any group of one value: attention scales its weights by the largest step it meets.
 __device__ __forceinline__ __half2 i4_step(float lo, float hi, bool ok) {
     const __half z = __float2half_rn(lo);
-    const __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, __half2float(z)), 1.0f / 15.0f));
+    const __half s = __float2half_rn(__fmul_rn(fmaxf(__fsub_rn(hi, __half2float(z)), 0.0f), 1.0f / 15.0f));
     return ok ? __halves2half2(s, z) : __halves2half2(__ushort_as_half(0x7e00), __ushort_as_half(0x7e00));
 }
 // The code of x.  (x - z) / s in float32 is off by less than 2^-18 (both factors rounded, the quotient below 16): where it lies that near to the

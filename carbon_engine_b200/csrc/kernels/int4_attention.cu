@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
 
     float o[NT][NB * 4][4], oz[NT][NG][2], m[NT][2], sum[NT][2];
     // Weights are kept as 2^(S - m): m follows the scores (within HEADROOM) and, in the same number, the steps: a weight times a step is to lie
-    // near 2^10, so m holds log2(top / 2^10) too, top a power of two that no step of V seen so far passes.  Sums, parts of minima and products
+    // near 2^10, so m holds log2(top / 2^10) too, top a power of two that no step of V seen so far passes in magnitude.  Sums, parts of minima and products
     // all carry the factor, which falls out at the end.
     float top = 0x1p-24f, high[NT][2];                // high: what a score (before its row's scale) may reach before m is moved
 #pragma unroll
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 fa[p][g] = i4_unpack(va[p][g]).x; fb[p][g] = i4_unpack(vb[p][g]).x;
-                step_max = fmaxf(step_max, fmaxf(fa[p][g], fb[p][g]));
+                step_max = fmaxf(step_max, fmaxf(fabsf(fa[p][g]), fabsf(fb[p][g])));
             }
         move = move || step_max > top;
         if (__any_sync(0xffffffffu, move)) {

@@ -2,7 +2,7 @@
 such a cache, and products of a few tokens with 4-bit weights.
 
 The format (``csrc/kernels/int4.cuh`` has its layout): ``group`` neighbouring values share a minimum z and a step s, both float16; a
-value is c s + z with a code c of 0 .. 15, z = float16(min x), s = float16((max x - z) / 15) (as a product with the float32 next to 1/15), c = (x - z) / s rounded to the nearest.
+value is c s + z with a code c of 0 .. 15, z = float16(min x), s = float16(max(max x - z, 0) / 15) (as a product with the float32 next to 1/15), c = (x - z) / s rounded to the nearest.
 A group that holds a value beyond 60,000 in magnitude, or one that is not finite, reads back as NaN.
 
 Like :mod:`carbon_engine_b200.ops`, every function takes tensors on the GPU, checks them, and launches on the current stream of the
