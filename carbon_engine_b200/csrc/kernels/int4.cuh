@@ -131,6 +131,12 @@ __device__ __forceinline__ float2 i4_step_of(uint32_t v) {
     if (CENTRED) f.y = fmaf(8.0f, f.x, f.y);
     return f;
 }
+// the smaller one; NaN where either is
+__device__ __forceinline__ float i4_min(float a, float b) {
+    float v;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+    return v;
+}
 __device__ __forceinline__ uint32_t i4_pack(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);

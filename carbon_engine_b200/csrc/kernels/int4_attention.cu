@@ -25,8 +25,11 @@ constexpr int WARPS = 8;                       // of a block, at most
 // tiles of a warp's ring: 4, or up to 6 where two blocks of an SM have room for it
 constexpr int ring_tiles(int tile) { return 110592 / (WARPS * tile) < 4 ? 4 : 110592 / (WARPS * tile) > 6 ? 6 : 110592 / (WARPS * tile); }
 constexpr int PAIR_UP_TO = 128;
-constexpr float NOTHING = -1e30f;              // the maximum of no scores
+constexpr float NOTHING = -3.402823466e38f;    // the maximum of no scores
 constexpr float HEADROOM = 5.0f;               // scores may pass the running maximum by this many powers of two before it is moved
+// From this magnitude of m on, float32's steps (0.5 and more) tell in what a weight comes out as: there, weights are cut to the HEADROOM that they
+// may have (m is rounded down: none is lost).  Keys whose scores lie a few such steps below the largest may count for more than they should.
+constexpr float COARSE = 0x1p22f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
                     }
             }
         }
-        bool move = false;
+        bool move = false, coarse = false;            // coarse: a row's m lies beyond COARSE (every turn of such a row moves it)
         float mx[NT][2], step_max = 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -457,16 +460,20 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    const float now = fmaxf(m[nt][e] - grown, fmaf(x, row_scale[nt][e], offset));
+                    const float there = __fmaf_rd(x, row_scale[nt][e], offset);
+                    const float now = m[nt][e] == NOTHING ? there : fmaxf(__fsub_rd(m[nt][e], grown), there);
                     const float alpha = m[nt][e] == NOTHING ? 0.0f : exp2f(m[nt][e] - now);
                     m[nt][e] = x == -INFINITY && m[nt][e] == NOTHING ? NOTHING : now;
-                    high[nt][e] = m[nt][e] == NOTHING ? NOTHING : (now - offset + HEADROOM) / row_scale[nt][e];
+                    const bool far = fabsf(m[nt][e]) >= COARSE;
+                    coarse = coarse || (far && m[nt][e] != NOTHING);
+                    high[nt][e] = far ? NOTHING : (now - offset + HEADROOM) / row_scale[nt][e];
                     sum[nt][e] *= alpha;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) oz[nt][g][e] *= alpha;
 #pragma unroll
                     for (int i2 = 0; i2 < NB * 4; ++i2) { o[nt][i2][e] *= alpha; o[nt][i2][2 + e] *= alpha; }
                 }
+            coarse = __any_sync(0xffffffffu, coarse);
         }
         float pr[PAIR][NT][4];
 #pragma unroll
@@ -475,8 +482,26 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    pr[p][nt][e] = ce_exp2_fast(fmaf(s[p][nt][e], row_scale[nt][e], -m[nt][e]));
-                    pr[p][nt][2 + e] = ce_exp2_fast(fmaf(s[p][nt][2 + e], row_scale[nt][e], -m[nt][e]));
+                    pr[p][nt][e] = fmaf(s[p][nt][e], row_scale[nt][e], -m[nt][e]);
+                    pr[p][nt][2 + e] = fmaf(s[p][nt][2 + e], row_scale[nt][e], -m[nt][e]);
+                }
+        if (coarse) {
+            const float most = 10.0f - log2f(top) + HEADROOM;
+#pragma unroll
+            for (int p = 0; p < PAIR; ++p)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) pr[p][nt][e] = i4_min(pr[p][nt][e], most);
+        }
+#pragma unroll
+        for (int p = 0; p < PAIR; ++p)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    pr[p][nt][e] = ce_exp2_fast(pr[p][nt][e]);
+                    pr[p][nt][2 + e] = ce_exp2_fast(pr[p][nt][2 + e]);
                     sum[nt][e] += pr[p][nt][e] + pr[p][nt][2 + e];
                 }
         // ---- V^T P^T, group by group: the probability carries the step

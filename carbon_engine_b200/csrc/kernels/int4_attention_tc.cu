@@ -33,6 +33,9 @@ namespace {
 constexpr int BN = 64, STAGES = 3, RAW = 3;      // RAW: tiles of codes a making warp has on the way
 constexpr int MAKERS = 6, SOFTMAX = 8, THREADS = 32 * (2 + MAKERS + SOFTMAX);
 constexpr float LIFT = 6.0f, HEADROOM = 8.0f;
+// From this magnitude of the reference on, float32's steps (1 and more) tell in what a probability comes out as: there, they are cut to the LIFT and
+// HEADROOM that they may have (the reference is rounded down: none is lost).
+constexpr float COARSE = 0x1p23f;
 
 struct Args {
     const __nv_bfloat16* q;        // [T, heads, d]: token stride q_stride, heads d apart
@@ -418,20 +421,25 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                     mx4[2] = fmaxf(mx4[2], sv[i + 2]); mx4[3] = fmaxf(mx4[3], sv[i + 3]);
                 }
                 // the reference lies LIFT below the largest score it was set by, and is moved when a score passes that by HEADROOM
-                const float m_tile = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * row_scale - LIFT;
+                const float m_tile = __fmaf_rd(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), row_scale, -LIFT);
                 const bool raise = m_tile > m_run + HEADROOM || (m_run == -INFINITY && m_tile != -INFINITY);
                 const float m_new = raise ? m_tile : m_run, m_use = m_new == -INFINITY ? 0.f : m_new;
                 const float alpha = raise ? ce_exp2_fast(m_run - m_use) : 1.0f;
                 float2 sum2 = make_float2(0.f, 0.f);
                 uint32_t packed[BN / 2];
                 const float2 scale2 = make_float2(row_scale, row_scale), minus_m = make_float2(-m_use, -m_use);
+                auto weights = [&](auto cut) {
 #pragma unroll
-                for (int i = 0; i < BN; i += 2) {
-                    const float2 t = __ffma2_rn(make_float2(sv[i], sv[i + 1]), scale2, minus_m);
-                    const float2 p = make_float2(ce_exp2_fast(t.x), ce_exp2_fast(t.y));
-                    sum2 = __fadd2_rn(sum2, p);
-                    packed[i / 2] = i4_pack(p.x, p.y);
-                }
+                    for (int i = 0; i < BN; i += 2) {
+                        float2 t = __ffma2_rn(make_float2(sv[i], sv[i + 1]), scale2, minus_m);
+                        if (cut()) t = make_float2(i4_min(t.x, LIFT + HEADROOM), i4_min(t.y, LIFT + HEADROOM));
+                        const float2 p = make_float2(ce_exp2_fast(t.x), ce_exp2_fast(t.y));
+                        sum2 = __fadd2_rn(sum2, p);
+                        packed[i / 2] = i4_pack(p.x, p.y);
+                    }
+                };
+                if (__all_sync(0xffffffffu, fabsf(m_use) < COARSE)) weights(std::false_type());
+                else weights(std::true_type());
                 l_run = l_run * alpha + (sum2.x + sum2.y);
                 m_run = m_new;
                 // the probabilities, where the scores were: two keys a column

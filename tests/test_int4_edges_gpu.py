@@ -65,3 +65,92 @@ def test_pages_with_steps_below_zero():
     c.pages.data[..., 16 * 128:] = steps.flatten(-2).view(torch.uint8).reshape(c.pages.data[..., 16 * 128:].shape)
     for dtype in (BF16, F32):
         attend(c, normal((1, 4, 128), 9, dtype), k, v, [1], [40], 64, 0, dtype)
+
+
+# ---- scores of any size
+def decided(q, k, v, new, lengths, off):
+    """The least and the most that attention may return where scores are far apart: the values, channel by channel, of the keys whose scores
+    lie by no more below a row's largest than both may err - ``off`` of the sums of their products' magnitudes each - and 100 (the others' weights,
+    exp(-100) and less, are nothing).  Mostly that is one key."""
+    q, k, v = (t.double().cpu() for t in (q, k, v))
+    each, scale, low, high = q.shape[1] // k.shape[1], 1.0 / math.sqrt(q.shape[2]), torch.zeros_like(q), torch.zeros_like(q)
+    row = first = 0
+    for n, h in zip(new, lengths):
+        for i in range(n):
+            kk, vv = (t[first:first + h - n + i + 1].repeat_interleave(each, dim=1) for t in (k, v))
+            s = (kk * q[row + i]).sum(-1) * scale
+            reach = ((kk * q[row + i]).abs().sum(-1) * scale).max(0).values
+            near = (s >= s.max(0).values - 100.0 - 2.0 * off * reach)[..., None]
+            low[row + i] = torch.where(near, vv, math.inf).amin(0)
+            high[row + i] = torch.where(near, vv, -math.inf).amax(0)
+        row, first = row + n, first + h
+    return low, high
+
+
+def check_decided(c, q, k, v, new, lengths, group, dtype):
+    heads, d = q.shape[1:]
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    decoding = len(new) if max(new) == 1 else 0
+    tiles = [(b, at) for b, n in enumerate(new) if b >= decoding for at in range(0, n, 64)]
+    out = torch.empty_like(q)
+    c.ops.attention(q, c.pages, out, c.slots, gpu(starts), gpu(lengths), c.table, c.status, n_decode=decoding, max_ctx=max(lengths),
+                    tiles=gpu(tiles) if tiles else None, scale=1.0 / math.sqrt(d))
+    # keys are met as they are held (scores err by float32's sums, and by the queries' 22 bits), on tcgen05 rounded to float16 (2^-11 of themselves)
+    on_tcgen05 = c.ops.TENSOR_ROWS == 1 and tiles and dtype == BF16
+    low, high = decided(q, plain.held(k, group), plain.held(v, group), new, lengths, 2.0 ** -10 if on_tcgen05 else 2.0 ** -20)
+    # one weight of 1: its product with the step, or (on tcgen05) the value, is rounded to float16, by 2^-11 of itself at most, of twice the
+    # largest value; float32: two pieces
+    largest = float(plain.held(v, group).abs().max())
+    slack = 2.0 * largest * (2.0 ** -11 if dtype == BF16 else 2.0 ** -22) + largest * 2.0 ** -18
+    got = out.double().cpu()
+    assert int(c.status) == 0
+    assert bool((got >= low - low.abs() * torch.finfo(dtype).eps / 2 - slack).all()) and bool((got <= high + high.abs() * torch.finfo(dtype).eps / 2 + slack).all())
+    return float((low == high).all(-1).double().mean())
+
+
+SIZES = [(1e4, 2e4), (1e8, 2e4), (1e20, 1.0)]          # of queries and keys: scores of 2e8, 2e12 and 1e20
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("q_size,k_size", SIZES)
+def test_single_tokens_with_scores_of_any_size(monkeypatch, dtype, q_size, k_size):
+    """One key decides, and the result is its value: neither infinite nor nothing, though float32's own steps between such scores are large."""
+    from carbon_engine_b200 import ops_int4
+    for d, heads, group in ((128, 8, 64), (64, 4, 32), (256, 4, 32)):
+        lengths = [400, 33, 1, 16]
+        c = Cache(lengths, 1, d, group, 16)
+        k = (normal((450, 1, d), 1, F32) * k_size).clamp(-6e4, 6e4)
+        for v in (normal((450, 1, d), 2, F32), torch.full((450, 1, d), 0.75, device="cuda"), normal((450, 1, d), 2, F32, 1000.0)):
+            c.write(k, v)
+            q = normal((4, heads, d), 3, dtype, q_size)
+            for splits in (1, 3, 11):
+                monkeypatch.setattr(ops_int4, "_splits", lambda jobs, tiles: (splits, -(-25 // splits)))
+                assert check_decided(c, q, k, v, [1] * 4, lengths, group, dtype) > 0.9          # nearly all rows of one key
+
+
+@pytest.mark.parametrize("rows", [1, 10 ** 9])
+@pytest.mark.parametrize("q_size,k_size", SIZES)
+def test_portions_with_scores_of_any_size(monkeypatch, rows, q_size, k_size):
+    from carbon_engine_b200 import ops_int4
+    monkeypatch.setattr(ops_int4, "TENSOR_ROWS", rows)
+    c = Cache([300], 1, 128, 64, 16)
+    k, v = (normal((300, 1, 128), 1, F32) * k_size).clamp(-6e4, 6e4), normal((300, 1, 128), 2, F32)
+    c.write(k, v)
+    check_decided(c, normal((70, 4, 128), 3, BF16, q_size), k, v, [70], [300], 64, BF16)
+
+
+@pytest.mark.parametrize("q_size", [1e4, 1e8])
+def test_equal_keys_share_a_score_of_any_size(q_size):
+    """The same key everywhere: the mean of the values."""
+    c = Cache([16], 1, 128, 64, 16)
+    k, v = normal((1, 1, 128), 1, F32, 2e4).clamp(-6e4, 6e4).expand(16, 1, 128).contiguous(), normal((16, 1, 128), 2, F32)
+    c.write(k, v)
+    for dtype in (BF16, F32):
+        q, out = normal((1, 8, 128), 3, dtype, q_size), torch.empty((1, 8, 128), dtype=dtype, device="cuda")
+        c.ops.attention(q, c.pages, out, c.slots, gpu([0, 1]), gpu([16]), c.table, c.status, n_decode=1, max_ctx=16, scale=0.09)
+        held = plain.held(v, 64)
+        want, largest = held.mean(0).expand(8, 128), float(held.abs().max())
+        slack = 2.0 * largest * (2.0 ** -11 if dtype == BF16 else 2.0 ** -22) + largest * 2.0 ** -18
+        assert bool(((out[0].double() - want).abs() <= want.abs() * torch.finfo(dtype).eps / 2 + slack).all())
