@@ -131,6 +131,7 @@ __device__ __forceinline__ float2 i4_step_of(uint32_t v) {
     if (CENTRED) f.y = fmaf(8.0f, f.x, f.y);
     return f;
 }
+__device__ __forceinline__ float i4_relu(float v) { return v < 0.0f ? 0.0f : v; }        // NaN stays
 // the smaller one; NaN where either is
 __device__ __forceinline__ float i4_min(float a, float b) {
     float v;

@@ -107,8 +107,8 @@ __device__ __forceinline__ void finish(void* out, size_t at, int mode, float v, 
         case STORE_F32: ((float*)out)[at] = v; break;
         case ACCUM_F32: ((float*)out)[at] += v; break;
         case SWIGLU: CeType<T>::store((T*)out + at, ce_silu_glu(v, u)); break;
-        case RELUGLU: CeType<T>::store((T*)out + at, fmaxf(v, 0.f) * u); break;
-        case RELU2: v = fmaxf(v, 0.f); CeType<T>::store((T*)out + at, v * v); break;
+        case RELUGLU: CeType<T>::store((T*)out + at, i4_relu(v) * u); break;
+        case RELU2: v = i4_relu(v); CeType<T>::store((T*)out + at, v * v); break;
         default: CeType<T>::store((T*)out + at, v);
     }
 }

@@ -102,8 +102,8 @@ __device__ __forceinline__ void finish(void* out, size_t at, int mode, float v, 
         case STORE_F32: ((float*)out)[at] = v; break;
         case ACCUM_F32: ((float*)out)[at] += v; break;
         case SWIGLU: half[at] = __float2bfloat16_rn(ce_silu_glu(v, up)); break;
-        case RELUGLU: half[at] = __float2bfloat16_rn(fmaxf(v, 0.f) * up); break;
-        case RELU2: v = fmaxf(v, 0.f); half[at] = __float2bfloat16_rn(v * v); break;
+        case RELUGLU: half[at] = __float2bfloat16_rn(i4_relu(v) * up); break;
+        case RELU2: v = i4_relu(v); half[at] = __float2bfloat16_rn(v * v); break;
         default: half[at] = __float2bfloat16_rn(v);
     }
 }

@@ -345,7 +345,8 @@ _F32_MODES = (ops.GEMM_STORE_F32, ops.GEMM_ACCUM_F32)
 def matmul(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, mode: int = ops.GEMM_STORE) -> None:
     """out (op)= x @ w.T with the epilogue ``mode`` (``ops.GEMM_*``), for up to :data:`MAX_TOKENS` tokens.  ``x`` [M, width]
     bfloat16 or float32; ``out`` [M, rows] (half the rows with a gated epilogue) in the type of x, float32 with ``GEMM_STORE_F32`` and
-    ``GEMM_ACCUM_F32``; rows of both at any stride.  A token of x with a value that is not finite gives a row of NaN."""
+    ``GEMM_ACCUM_F32``; rows of both at any stride.  A token of x with a value that is not finite gives a row of NaN, a group of the weight
+    that reads back as NaN its column."""
     if mode not in _MODES:
         raise KernelError(f"a product with a 4-bit weight has no epilogue {mode}")
     if (mode in _GATED_MODES) != w.gated:

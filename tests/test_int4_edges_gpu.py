@@ -154,3 +154,36 @@ def test_equal_keys_share_a_score_of_any_size(q_size):
         want, largest = held.mean(0).expand(8, 128), float(held.abs().max())
         slack = 2.0 * largest * (2.0 ** -11 if dtype == BF16 else 2.0 ** -22) + largest * 2.0 ** -18
         assert bool(((out[0].double() - want).abs() <= want.abs() * torch.finfo(dtype).eps / 2 + slack).all())
+
+
+# ---- numbers that are none, through every epilogue
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("mode", ["STORE", "STORE_F32", "ACCUM_F32", "SWIGLU", "RELUGLU", "RELU2"])
+@pytest.mark.parametrize("M", [3, 12, 20, 64])
+def test_tokens_and_weights_that_are_no_numbers(dtype, mode, M):
+    """A token with a value that is not finite gives a row of NaN; a group of a weight that is not a number gives its column."""
+    from carbon_engine_b200 import ops, ops_int4
+    mode = getattr(ops, "GEMM_" + mode)
+    gated = mode in (ops.GEMM_SWIGLU, ops.GEMM_RELUGLU)
+    x, w, w4, _ = product_case(dtype, mode, M, 40, 256, 64)
+    kind = F32 if mode in (ops.GEMM_STORE_F32, ops.GEMM_ACCUM_F32) else dtype
+
+    def result(x, w4):
+        out = torch.ones((M, 40), dtype=kind, device="cuda")
+        ops_int4.matmul(x, w4, out, mode)
+        return out
+
+    fine = result(x, w4)
+    assert not bool(fine.isnan().any())
+    bad = x.clone()
+    bad[0, 17], bad[2, 255] = math.nan, -math.inf
+    out = result(bad, w4)
+    assert bool(out[[0, 2]].isnan().all()) and not bool(out[[t for t in range(M) if t not in (0, 2)]].isnan().any())
+    w = w.clone()
+    w[5, 70] = math.inf                                   # (a gate row of gated weights)
+    if gated:
+        w[40 + 9, 3] = math.nan                           # an up row
+    out = result(x, ops_int4.Int4Weight.quantize(w, 64, gated))
+    columns = [5, 9] if gated else [5]
+    others = [n for n in range(40) if n not in columns]
+    assert bool(out[:, columns].isnan().all()) and torch.equal(out[:, others], fine[:, others])
