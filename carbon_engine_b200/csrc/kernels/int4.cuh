@@ -144,6 +144,10 @@ __device__ __forceinline__ uint32_t i4_pack(float lo, float hi) {
 }
 __device__ __forceinline__ float2 i4_unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
+// What a row's scores are multiplied by, kept within float32's normal numbers: beyond them (queries of 2^117 and more, tiny ones beside tiny scales)
+// scores are as far apart, or as near, as makes no difference to a softmax, while infinity and 0 would make NaN of scores that are 0 or hidden.
+// (Comparisons: NaN stays.)
+__device__ __forceinline__ float i4_normal(float v) { return v > 0x1.fffffep127f ? 0x1.fffffep127f : v < 0x1p-126f ? 0x1p-126f : v; }
 // The power of two that brings a row's largest magnitude into [2^14, 2^15): a float16 then holds bfloat16 values exactly down to 2^-30 of the
 // largest.  Its bits are those of 2^14 less the largest's exponent; 1 for a row of zeros, NaN for one that is not finite.
 __device__ __forceinline__ float i4_row_scale(float largest) {

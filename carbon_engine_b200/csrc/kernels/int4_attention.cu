@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(WARPS * 32, Pieces<T>::N * NT * D <= PAIR_UP_T
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const float u = __shfl_sync(0xffffffffu, up, 4 * (2 * l + e));
-            row_scale[nt][e] = a.scale * LOG2E * i4_unit<C8> / u;
+            row_scale[nt][e] = i4_normal(a.scale * LOG2E / u * i4_unit<C8>);        // (in this order nothing passes float32 on the way)
             const int rr = nt * 8 + 2 * l + e, pos = j.base + token_of(j.row0 + rr);
             hi[nt][e] = rr < rows ? pos : -1;
             lo[nt][e] = a.window > 0 ? pos - a.window + 1 : 0;
@@ -815,7 +815,7 @@ extern "C" int ce_int4_attention(const Int4AttentionCall* c) {
     if (max_pages < 1 || num_pages < 1 || splits < 0 || window < 0) return ce_fail(CE_ERR_SIZE, "int4_attention: bad sizes");
     if (((uintptr_t)out % (dtype == CE_F32 ? 16 : 8)) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: out does not start on a boundary of four elements");
     if (splits > 8 && (!part_o || !part_ml)) return ce_fail(CE_ERR_ARG, "int4_attention: more than 8 shares of the keys need scratch memory");
-    if (!(c->scale > 0.0)) return ce_fail(CE_ERR_ARG, "int4_attention: a scale that is not positive");
+    if (!(scale > 0.0f && scale < 0x1p127f)) return ce_fail(CE_ERR_ARG, "int4_attention: a scale that is not a positive number of float32 below 2^127");
     if (count == 0) return CE_OK;
     if (splits == 0) {
         if (dtype != CE_BF16 || !tiles || count < 0 || count > 65535) return ce_fail(CE_ERR_SIZE, "int4_attention: splits of 0 are for tiles of bfloat16");

@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                 }
             }
             const float up = i4_row_scale(finite ? largest : INFINITY);
-            row_scale = a.scale_log2 / up;
+            row_scale = i4_normal(a.scale_log2 / up);
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
                 const uint32_t words[4] = {x[c].x, x[c].y, x[c].z, x[c].w};

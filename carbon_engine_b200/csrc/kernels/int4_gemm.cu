@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(SW * 32) int4_stream_kernel(StreamArgs a) {
             }
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) back[nt][e] = i4_unit<C8> / __shfl_sync(0xffffffffu, up, 4 * (2 * l + e));
+        for (int e = 0; e < 2; ++e) back[nt][e] = 1.0f / __shfl_sync(0xffffffffu, up, 4 * (2 * l + e));      // (not times the unit: of tokens of 2^117 that is no float32)
     }
 
     // a batch's sums, one a thread: of tile u of it, token t, row
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(SW * 32) int4_stream_kernel(StreamArgs a) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) to[(nt * 8 + (e & 1)) * LD + (e >> 1) * 8] = y[nt][e] * back[nt][e & 1];
+                for (int e = 0; e < 4; ++e) to[(nt * 8 + (e & 1)) * LD + (e >> 1) * 8] = y[nt][e] * i4_unit<C8> * back[nt][e & 1];
         } else {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)

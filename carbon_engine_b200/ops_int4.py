@@ -276,8 +276,8 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
     _ints(device, "seq_slot q_start ctx_len block_table status", seq_slot, q_start, ctx_len, block_table, status)
     if block_table.dim() != 2 or window < 0 or n_decode < 0 or max_ctx < 0:
         raise KernelError("attention: a table of [slots, pages], no negative numbers")
-    if not scale > 0.0:
-        raise KernelError(f"attention: a scale of {scale} (it must be positive)")
+    if not 2.0 ** -149 <= scale < 2.0 ** 127:
+        raise KernelError(f"attention: a scale of {scale} (it must be positive, and a number of float32 below 2^127)")
     seqs = seq_slot.numel()
     if n_decode > seqs or q_start.numel() <= seqs or ctx_len.numel() < seqs:
         raise KernelError("attention: one slot and one length a sequence, one start more")

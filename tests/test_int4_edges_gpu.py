@@ -187,3 +187,58 @@ def test_tokens_and_weights_that_are_no_numbers(dtype, mode, M):
     columns = [5, 9] if gated else [5]
     others = [n for n in range(40) if n not in columns]
     assert bool(out[:, columns].isnan().all()) and torch.equal(out[:, others], fine[:, others])
+
+
+# ---- tokens and queries as large and as small as their type holds
+@pytest.mark.parametrize("M", [3, 12, 20])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_tokens_as_large_as_their_type_holds(dtype, M):
+    from carbon_engine_b200 import ops, ops_int4
+    x, w, w4, _ = product_case(dtype, ops.GEMM_STORE_F32, M, 40, 256, 64)
+    for size in (2e35, 4e37, 1e-36):
+        y = x * size                                       # results of up to 1e38: float32 holds them
+        out = torch.empty((M, 40), device="cuda")
+        ops_int4.matmul(y, w4, out, ops.GEMM_STORE_F32)
+        assert bool(out.isfinite().all())
+        if size > 1:
+            check_product(y, w, 64, w4, ops.GEMM_STORE_F32, out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_queries_as_large_as_their_type_holds(monkeypatch, dtype):
+    c = Cache([300, 20], 1, 128, 64, 16)
+    k, v = normal((320, 1, 128), 1, F32, 0.01), normal((320, 1, 128), 2, F32)
+    c.write(k, v)
+    for size in (1e35, 4e37):
+        check_decided(c, normal((2, 8, 128), 3, dtype, size), k, v, [1, 1], [300, 20], 64, dtype)
+    if dtype == BF16:
+        from carbon_engine_b200 import ops_int4
+        monkeypatch.setattr(ops_int4, "TENSOR_ROWS", 1)
+        check_decided(c, normal((20 + 7, 8, 128), 3, dtype, 4e37), k, v, [20, 7], [300, 20], 64, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scales_as_small_as_float32_holds(monkeypatch, dtype):
+    """Every key counts the same, and what is masked counts nothing."""
+    from carbon_engine_b200 import ops_int4
+    c, k, v = filled([30], 1, 64, 32, 16, dtype)
+    for rows in (1, 10 ** 9):
+        monkeypatch.setattr(ops_int4, "TENSOR_ROWS", rows)
+        for n in (1, 5):
+            q = normal((n, 4, 64), 9, dtype, 1e-30)
+            out = torch.empty_like(q)
+            c.ops.attention(q, c.pages, out, c.slots, gpu([0, n]), gpu([30]), c.table, c.status, n_decode=int(n == 1), max_ctx=30,
+                            tiles=gpu([[0, 0]]) if n > 1 else None, scale=1e-37)
+            held = plain.held(v, 32)
+            want = torch.stack([held[:30 - n + i + 1].mean(0).expand(4, 64) for i in range(n)])
+            slack = float(held.abs().max()) * (2.0 ** -10 if dtype == BF16 else 2.0 ** -18)
+            assert bool(((out.double() - want).abs() <= want.abs() * torch.finfo(dtype).eps / 2 + slack).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, 1e-300, math.inf, math.nan, 1e300])
+def test_scales_that_float32_does_not_hold_are_refused(scale):
+    from carbon_engine_b200.csrc.kernel_lib import KernelError
+    c, k, v = filled([30], 1, 64, 32, 16, BF16)
+    q = normal((1, 4, 64), 9, BF16)
+    with pytest.raises(KernelError, match="scale"):
+        c.ops.attention(q, c.pages, torch.empty_like(q), c.slots, gpu([0, 1]), gpu([30]), c.table, c.status, n_decode=1, max_ctx=30, scale=scale)
