@@ -814,6 +814,9 @@ extern "C" int ce_int4_attention(const Int4AttentionCall* c) {
     if (((uintptr_t)pages & 15) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: the pages do not start on a 16-byte boundary");
     if (max_pages < 1 || num_pages < 1 || splits < 0 || window < 0) return ce_fail(CE_ERR_SIZE, "int4_attention: bad sizes");
     if (((uintptr_t)out % (dtype == CE_F32 ? 16 : 8)) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: out does not start on a boundary of four elements");
+    // (a block's first tile of keys is its number times the share)
+    if (c->splits > 1024 || c->share < 0 || c->share > (1ll << 30) / (splits < 1 ? 1 : splits))
+        return ce_fail(CE_ERR_SIZE, "int4_attention: %lld shares of %lld tiles of keys", c->splits, c->share);
     if (splits > 8 && (!part_o || !part_ml)) return ce_fail(CE_ERR_ARG, "int4_attention: more than 8 shares of the keys need scratch memory");
     if (!(scale > 0.0f && scale < 0x1p127f)) return ce_fail(CE_ERR_ARG, "int4_attention: a scale that is not a positive number of float32 below 2^127");
     if (count == 0) return CE_OK;

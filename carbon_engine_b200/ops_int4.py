@@ -206,6 +206,14 @@ def _splits(jobs: int, tiles: int):
     return best[1:]
 
 
+def _shares(jobs: int, max_ctx: int, window: int, tokens: int):
+    """:func:`_splits` for the keys that ``tokens`` tokens side by side may see.  ``max_ctx`` may be any bound: positions are int32."""
+    keys = min(max_ctx, (1 << 31) - 1)
+    if window > 0:
+        keys = min(keys, window + tokens + 15)
+    return _splits(jobs, max(1, (keys + 15) // 16))
+
+
 def _joined(jobs: int, splits: int) -> bool:
     """Whether a second kernel joins the splits; up to 8 of few row blocks are a cluster and join through shared memory."""
     return splits > 8 or (splits > 1 and jobs * splits > 296)
@@ -231,12 +239,11 @@ def _attend(device, code, q, q_stride, heads, pages, out, seq_slot, q_start, ctx
     tile = 0 if tiles is None else 1
     blocks, block_rows, tensor_blocks = _row_blocks(each, pages.head_dim, tile)
     jobs, tensor_blocks = count * pages.kv_heads * blocks, count * pages.kv_heads * tensor_blocks
-    keys = min(max_ctx, window + (64 if tile else 1) + 15) if window > 0 else max_ctx
     if (code == ops.BF16 and tensor_blocks and min(64 * count, q.shape[0]) * heads >= TENSOR_ROWS * max(1.0, tensor_blocks / 148) and count <= 65535 and q_stride % 8 == 0
             and (q.data_ptr() | out.data_ptr()) % 16 == 0):
         splits = share = 0
     else:
-        splits, share = _splits(jobs, max(1, (keys + 15) // 16))
+        splits, share = _shares(jobs, max_ctx, window, 64 if tile else 1)
     part_o = part_ml = None
     if _joined(jobs, splits):
         rows = jobs * splits * block_rows

@@ -242,3 +242,11 @@ def test_scales_that_float32_does_not_hold_are_refused(scale):
     q = normal((1, 4, 64), 9, BF16)
     with pytest.raises(KernelError, match="scale"):
         c.ops.attention(q, c.pages, torch.empty_like(q), c.slots, gpu([0, 1]), gpu([30]), c.table, c.status, n_decode=1, max_ctx=30, scale=scale)
+
+
+# ---- sizes beyond 32 bits
+@pytest.mark.parametrize("max_ctx", [1 << 31, 1 << 36, 1 << 40, (1 << 63) - 1])
+def test_any_bound_on_the_keys(max_ctx):
+    c, k, v = filled([90, 400], 2, 64, 32, 16, BF16)
+    attend(c, normal((2, 4, 64), 9, BF16), k, v, [1, 1], [90, 400], 32, 0, BF16, max_ctx=max_ctx)
+    attend(c, normal((20, 4, 64), 9, BF16), k, v, [12, 8], [90, 400], 32, 0, BF16, n_decode=0, max_ctx=max_ctx)
