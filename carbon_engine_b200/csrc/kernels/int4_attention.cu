@@ -812,7 +812,10 @@ extern "C" int ce_int4_attention(const Int4AttentionCall* c) {
     if (group != 32 && group != 64) return ce_fail(CE_ERR_SIZE, "int4_attention: group %d (32 or 64)", group);
     if (page_size < 16 || page_size % 16) return ce_fail(CE_ERR_SIZE, "int4_attention: page size %d is not a multiple of 16", page_size);
     if (((uintptr_t)pages & 15) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: the pages do not start on a 16-byte boundary");
-    if (max_pages < 1 || num_pages < 1 || splits < 0 || window < 0) return ce_fail(CE_ERR_SIZE, "int4_attention: bad sizes");
+    const long long sizes[] = {c->nh, c->nkv, c->d, c->group, c->page_size, c->max_pages, c->num_pages, c->window, c->splits};
+    for (long long size : sizes)
+        if (size < 0 || size > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "int4_attention: a size of %lld", size);
+    if (max_pages < 1 || num_pages < 1) return ce_fail(CE_ERR_SIZE, "int4_attention: bad sizes");
     if (((uintptr_t)out % (dtype == CE_F32 ? 16 : 8)) != 0) return ce_fail(CE_ERR_ARG, "int4_attention: out does not start on a boundary of four elements");
     // (a block's first tile of keys is its number times the share)
     if (c->splits > 1024 || c->share < 0 || c->share > (1ll << 30) / (splits < 1 ? 1 : splits))

@@ -303,6 +303,12 @@ struct Int4KvCall {
     long long T, nkv, d, group, page_size, max_pages, num_pages;
     void* stream;
 };
+static int check_sizes(const Int4KvCall& c, const char* who) {
+    const long long sizes[] = {c.T, c.nkv, c.d, c.group, c.page_size, c.max_pages, c.num_pages};
+    for (long long size : sizes)
+        if (size < 0 || size > 0x7fffffffll) return ce_fail(CE_ERR_SIZE, "%s: a size of %lld", who, size);
+    return CE_OK;
+}
 static CacheArgs cache_args(const Int4KvCall& c) {
     return CacheArgs{c.k, c.v, (unsigned char*)c.pages, c.positions, c.seq_of_token, c.seq_slot, c.block_table, c.status, c.k_token, c.k_head,
                      c.v_token, c.v_head, (int)c.T, (int)c.nkv, (int)c.d, (int)c.group, (int)c.page_size, (int)c.max_pages, (int)c.num_pages, 0};
@@ -310,6 +316,7 @@ static CacheArgs cache_args(const Int4KvCall& c) {
 
 extern "C" int ce_int4_kv_write(const Int4KvCall* c) {
     CacheArgs a = cache_args(*c);
+    if (int e = check_sizes(*c, "int4_kv_write")) return e;
     if (int e = check_cache(a, (int)c->dtype, "int4_kv_write")) return e;
     return run_cache(a, (int)c->dtype, int4_kv_write_kernel<float>, int4_kv_write_kernel<__nv_bfloat16>, "int4_kv_write_kernel", (cudaStream_t)c->stream);
 }
@@ -317,6 +324,7 @@ extern "C" int ce_int4_kv_write(const Int4KvCall* c) {
 // (writes k and v)
 extern "C" int ce_int4_kv_read(const Int4KvCall* c) {
     CacheArgs a = cache_args(*c);
+    if (int e = check_sizes(*c, "int4_kv_read")) return e;
     if (int e = check_cache(a, (int)c->dtype, "int4_kv_read")) return e;
     return run_cache(a, (int)c->dtype, int4_kv_read_kernel<float>, int4_kv_read_kernel<__nv_bfloat16>, "int4_kv_read_kernel", (cudaStream_t)c->stream);
 }

@@ -96,7 +96,8 @@ struct GemmArgs {
     const unsigned char* w;        // [row tiles][kblocks][tile]
     Operand x;
     void* out;
-    int M, N, kblocks, tiles, ldo, mode, gated;
+    long long ldo;
+    int M, N, kblocks, tiles, mode, gated;
 };
 
 enum { STORE = 0, STORE_F32 = 1, ACCUM_F32 = 2, SWIGLU = 3, RELUGLU = 4, RELU2 = 5 };
@@ -213,8 +214,8 @@ struct StreamArgs {
     const unsigned char* w;
     void* out;
     int* status;
-    long long ldx;
-    int M, N, K, kblocks, ldo, mode, gated, units, each, slices, overlap, vec;
+    long long ldx, ldo;
+    int M, N, K, kblocks, mode, gated, units, each, slices, overlap, vec;
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -643,7 +644,7 @@ cudaError_t launch_tiles(const GemmArgs& a, int row_tiles, cudaStream_t stream) 
 }  // namespace
 
 long long ce_int4_gemm_tc_scratch(int M, int K);
-int ce_int4_gemm_tc(const void* x, long long ldx, const void* w, void* out, int ldo, int M, int N, int K, int kept, int mode, float* scratch, int* status,
+int ce_int4_gemm_tc(const void* x, long long ldx, const void* w, void* out, long long ldo, int M, int N, int K, int kept, int mode, float* scratch, int* status,
                     cudaStream_t stream);
 
 namespace {
@@ -681,14 +682,14 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
     const void *x = c->x, *w = c->w;
     void *out = c->out, *stream = c->stream;
     float* scratch = c->scratch;
-    const long long ldx = c->ldx;
-    const int dtype = (int)c->dtype, ldo = (int)c->ldo, M = (int)c->M, N = (int)c->N, K = (int)c->K, group = (int)c->group, mode = (int)c->mode;
+    const long long ldx = c->ldx, ldo = c->ldo;
+    const int dtype = (int)c->dtype, M = (int)c->M, N = (int)c->N, K = (int)c->K, group = (int)c->group, mode = (int)c->mode;
     if (!x || !w || !out) return ce_fail(CE_ERR_ARG, "int4_gemm: null pointer");
     if (dtype != CE_F32 && dtype != CE_BF16) return ce_fail(CE_ERR_ARG, "int4_gemm: unknown dtype %d", dtype);
     if (group != 32 && group != 64 && group != 128) return ce_fail(CE_ERR_SIZE, "int4_gemm: group %d (32, 64 or 128)", group);
     if (mode < STORE || mode > RELU2) return ce_fail(CE_ERR_SIZE, "int4_gemm: epilogue %d is not one of this product's", mode);
-    if (M < 0 || M > 64 || N < 1 || K < 1 || K % group || ldx < K || ldo < N)
-        return ce_fail(CE_ERR_SIZE, "int4_gemm: %d tokens (at most 64), %d rows of %d (a multiple of the group)", M, N, K);
+    if (c->M < 0 || c->M > 64 || c->N < 1 || c->N > 0x3fffffff || c->K < 1 || c->K > 0x3fffffff || K % group || ldx < K || ldo < N)
+        return ce_fail(CE_ERR_SIZE, "int4_gemm: %lld tokens (at most 64), %lld rows of %lld (a multiple of the group)", c->M, c->N, c->K);
     if (((uintptr_t)w & 15) || ((uintptr_t)scratch & 15)) return ce_fail(CE_ERR_ARG, "int4_gemm: the weight or the scratch memory is not aligned to 16 bytes");
     if (M == 0) return CE_OK;
     const int kept = group < 64 ? group : 64, tiles = (M + 7) / 8, kblocks = (K + 63) / 64;
@@ -696,7 +697,7 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
     const int el = dtype == CE_F32 ? 4 : 2, row_tiles = gated ? (N + 7) / 8 : (N + 15) / 16;
     const bool vec = ((uintptr_t)x % (4 * el)) == 0 && ldx % 4 == 0;
     if (streamed(dtype, M, K)) {
-        StreamArgs a{x, (const unsigned char*)w, out, c->status, ldx, M, N, K, kblocks, ldo, mode, gated, row_tiles, 0, 0, 0, vec};
+        StreamArgs a{x, (const unsigned char*)w, out, c->status, ldx, ldo, M, N, K, kblocks, mode, gated, row_tiles, 0, 0, 0, vec};
         const int code = dtype == CE_F32 ? (kept == 32 ? launch_stream_tiles<float, 32>(a, tiles, (cudaStream_t)stream)
                                                        : launch_stream_tiles<float, 64>(a, tiles, (cudaStream_t)stream))
                                          : (kept == 32 ? launch_stream_tiles<__nv_bfloat16, 32>(a, tiles, (cudaStream_t)stream)
@@ -713,7 +714,7 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
     ce_note("int4_prepare_kernel");
     cudaError_t e = ce_launch(int4_prepare_kernel<float, 2>, dim3(tiles * 8), dim3(256), 0, (cudaStream_t)stream, p);
     if (e == cudaSuccess) {
-        GemmArgs a{(const unsigned char*)w, op, out, M, N, kblocks, tiles, ldo, mode, gated};
+        GemmArgs a{(const unsigned char*)w, op, out, ldo, M, N, kblocks, tiles, mode, gated};
         e = kept == 32 ? launch_tiles<float, 32>(a, row_tiles, (cudaStream_t)stream) : launch_tiles<float, 64>(a, row_tiles, (cudaStream_t)stream);
     }
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_gemm: %s", cudaGetErrorString(e)); }

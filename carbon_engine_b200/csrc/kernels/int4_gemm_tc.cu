@@ -197,7 +197,8 @@ struct Args {
     const float* back;
     void* out;
     int* status;
-    int M, N, kblocks, units, slices, ldo, mode, gated, overlap;      // units: tiles of 16 rows
+    long long ldo;
+    int M, N, kblocks, units, slices, mode, gated, overlap;           // units: tiles of 16 rows
 };
 
 template <int G, int TOKENS>
@@ -528,13 +529,13 @@ long long ce_int4_gemm_tc_scratch(int M, int K) {
 }
 
 // The checks of ce_int4_gemm come first: it calls this.  scratch: on a 16-byte boundary; kept: columns of a group in the weight's tiles (32 or 64)
-int ce_int4_gemm_tc(const void* x, long long ldx, const void* w, void* out, int ldo, int M, int N, int K, int kept, int mode, float* scratch, int* status,
+int ce_int4_gemm_tc(const void* x, long long ldx, const void* w, void* out, long long ldo, int M, int N, int K, int kept, int mode, float* scratch, int* status,
                     cudaStream_t stream) {
     const int tokens = M <= 32 ? 32 : 64, kblocks = (K + 63) / 64, gated = mode == SWIGLU || mode == RELUGLU;
     unsigned char* to = (unsigned char*)scratch;
     TokensArgs p{(const __nv_bfloat16*)x, to, ldx, M, K, kblocks, tokens, kept, ((uintptr_t)x & 15) == 0 && ldx % 8 == 0};
-    Args a{(const unsigned char*)w, to, reinterpret_cast<const float*>(to + (size_t)(kblocks + 1) * tokens_bytes(tokens)), out, status, M, N, kblocks,
-           gated ? (N + 7) / 8 : (N + 15) / 16, 1, ldo, mode, gated, 0};
+    Args a{(const unsigned char*)w, to, reinterpret_cast<const float*>(to + (size_t)(kblocks + 1) * tokens_bytes(tokens)), out, status, ldo, M, N, kblocks,
+           gated ? (N + 7) / 8 : (N + 15) / 16, 1, mode, gated, 0};
     if (tokens == 32) return kept == 32 ? run<32, 32>(p, a, stream) : run<64, 32>(p, a, stream);
     return kept == 32 ? run<32, 64>(p, a, stream) : run<64, 64>(p, a, stream);
 }

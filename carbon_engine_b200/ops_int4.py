@@ -293,11 +293,12 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
         n_tiles = tiles.numel() // 2 if n_tiles is None else int(n_tiles)
         if n_tiles < 0 or 2 * n_tiles > tiles.numel():
             raise KernelError(f"{n_tiles} tiles in a list of {tiles.numel() // 2}")
+    window = min(int(window), (1 << 31) - 1)           # (positions are int32: such a window hides nothing)
     args = (device, code, q, q_token, heads, pages, out, seq_slot, q_start, ctx_len, block_table, status)
     if T and n_decode:
-        _attend(*args, None, n_decode, int(max_ctx), int(window), float(scale))
+        _attend(*args, None, n_decode, int(max_ctx), window, float(scale))
     if T and tiles is not None and n_tiles:
-        _attend(*args, tiles, n_tiles, int(max_ctx), int(window), float(scale))
+        _attend(*args, tiles, n_tiles, int(max_ctx), window, float(scale))
 
 
 class Int4Weight:
@@ -308,9 +309,9 @@ class Int4Weight:
     def __init__(self, rows: int, width: int, group: int = 64, gated: bool = False, device="cuda"):
         if group not in WEIGHT_GROUPS:
             raise KernelError(f"group {group} (a 4-bit weight takes {', '.join(map(str, WEIGHT_GROUPS))})")
-        if rows < 1 or width < 1 or width % group or (gated and rows % 2):
+        if not 0 < rows < 1 << 30 or not 0 < width < 1 << 30 or width % group or (gated and rows % 2):
             raise KernelError(f"a 4-bit weight of {rows} rows of {width}: the width must be a multiple of the group ({group})"
-                              + (", the rows of two" if gated else ""))
+                              + (", the rows of two" if gated else "") + ", both less than 2^30")
         self.rows, self.width, self.group, self.gated = int(rows), int(width), int(group), bool(gated)
         #: columns of the result
         self.part = self.rows // 2 if self.gated else self.rows

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 
 from carbon_engine_b200 import ops_int4
-from carbon_engine_b200.csrc.kernel_lib import kernels
+from carbon_engine_b200.csrc.kernel_lib import KernelError, kernels
 
 ERR_SIZE = -1
 ADDR = 1 << 20                     # an aligned address that nothing reads
@@ -30,3 +30,23 @@ def test_a_bound_on_the_keys_may_be_any_number(max_ctx, window, jobs):
     assert 1 <= splits <= 64 and 1 <= share and splits * share < 1 << 30
     tiles = -(-min(max_ctx, (1 << 31) - 1, window + 16 if window else max_ctx) // 16)
     assert splits * share >= tiles
+
+
+def kv(fn, T=1, page_size=16, max_pages=4, num_pages=8):
+    return fn(ops_int4._KV(1, ADDR, ADDR, 64, 64, 64, 64, ADDR, ADDR, ADDR, ADDR, ADDR, ADDR, T, 1, 64, 32, page_size, max_pages, num_pages, 0))
+
+
+def product(M=2, N=40, K=128, ldo=40):
+    return kernels().ce_int4_gemm(ops_int4._GEMM(1, ADDR, K, ADDR, ADDR, ldo, M, N, K, 64, 0, ADDR, ADDR, 0))
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """(Cut to 32 bits, each would be a size that is taken.)"""
+    beyond = 1 << 32
+    assert attention(window=beyond + 5) == ERR_SIZE and attention(n=beyond * 8 + 1) == ERR_SIZE
+    for fn in (kernels().ce_int4_kv_write, kernels().ce_int4_kv_read):
+        assert kv(fn, T=beyond + 1) == kv(fn, page_size=beyond + 16) == kv(fn, max_pages=beyond + 4) == kv(fn, num_pages=beyond + 8) == ERR_SIZE
+    assert product(M=beyond + 2) == product(N=beyond + 40) == product(K=beyond + 128) == product(ldo=39) == ERR_SIZE
+    for rows, width in ((1 << 30, 64), (64, 1 << 30), ((1 << 32) + 16, 64)):
+        with pytest.raises(KernelError, match="2\\^30"):
+            ops_int4.Int4Weight(rows, width, device="cpu")

@@ -250,3 +250,29 @@ def test_any_bound_on_the_keys(max_ctx):
     c, k, v = filled([90, 400], 2, 64, 32, 16, BF16)
     attend(c, normal((2, 4, 64), 9, BF16), k, v, [1, 1], [90, 400], 32, 0, BF16, max_ctx=max_ctx)
     attend(c, normal((20, 4, 64), 9, BF16), k, v, [12, 8], [90, 400], 32, 0, BF16, n_decode=0, max_ctx=max_ctx)
+
+
+@pytest.mark.parametrize("dtype,K", [(BF16, 128), (BF16, 70016), (F32, 16448)])       # on each of the three kernels
+@pytest.mark.parametrize("stride", [(1 << 31) + 8, (1 << 32) + 40])
+def test_rows_of_a_result_at_strides_beyond_32_bits(dtype, K, stride):
+    from carbon_engine_b200 import ops, ops_int4
+    x, w, w4, _ = product_case(dtype, ops.GEMM_STORE, 2, 40, K, 64)
+    whole = torch.empty(stride + 256, dtype=dtype, device="cuda")
+    out = torch.as_strided(whole, (2, 40), (stride, 1))
+    whole[:256] = 3.0
+    out.fill_(3.0)
+    ops_int4.matmul(x, w4, out, ops.GEMM_STORE)
+    check_product(x, w, 64, w4, ops.GEMM_STORE, out)
+    assert bool((whole[40:256] == 3).all())
+
+
+@pytest.mark.parametrize("window", [(1 << 31) - 1, 1 << 31, (1 << 32) + 5])
+def test_windows_beyond_32_bits_hide_nothing(window):
+    c, k, v = filled([90], 1, 64, 32, 16, BF16)
+    q = normal((1, 4, 64), 9, BF16)
+    outs = []
+    for w in (0, window):
+        out = torch.empty_like(q)
+        c.ops.attention(q, c.pages, out, c.slots, gpu([0, 1]), gpu([90]), c.table, c.status, n_decode=1, max_ctx=90, window=w, scale=0.1)
+        outs.append(out)
+    assert torch.equal(*outs)
