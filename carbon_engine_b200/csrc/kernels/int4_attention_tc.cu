@@ -23,10 +23,12 @@
 // Keys' and values' channels lie in the order in which codes come out of their words; the queries' channels are laid out to match, and
 // the outputs' are put back where they are stored.
 //
-// Every wait on an mbarrier is bounded; on a timeout the block sets a status of 61 to 68, frees its tensor memory and returns.  Tensor memory is
+// Every wait on an mbarrier is bounded; on a timeout the block sets a status of 61 to 68, waits (with the same limit) for its copies and products
+// that are under way, frees its tensor memory and returns.  Tensor memory is
 // taken behind the wait for the kernels in front and before the kernels behind may start: a neighbour that waits for this grid never holds
 // what this grid waits for.
 #include "int4.cuh"
+#include "int4_ring.h"
 
 namespace {
 
@@ -152,6 +154,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
     uint64_t *k_full = bars + 11, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
     uint64_t* raw_full = v_empty + STAGES;              // [maker][RAW]
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(raw_full + MAKERS * RAW);
+    uint64_t* drained = raw_full + MAKERS * RAW + 1;    // [half]: all its products have ended
     unsigned short* nan_keys = reinterpret_cast<unsigned short*>(sm + S::NAN_KEYS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     ce_pdl_wait();
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], mts); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], mts); }
         for (int i = 0; i < MAKERS * RAW; ++i) mbar_init(&raw_full[i], 1);
         for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
-        mbar_init(&pv_done[0], 1); mbar_init(&pv_done[1], 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(&pv_done[i], 1); mbar_init(&drained[i], 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -238,6 +241,9 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                 }
             }
             if (!ok && lane == 0) atomicCAS(a.status, 0, where);
+            // (whoever gave up: no product is under way when tensor and shared memory become another's)
+            umma_commit(&drained[m]);
+            i4_warp_wait(&drained[m], 0);
         }
         __syncwarp();
     } else if (warp < 2 + MAKERS) {
@@ -265,8 +271,10 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
         };
         look_up(0);
         for (int i = 0; i < RAW; ++i) fetch(i);
-        uint32_t phase = 0;                             // of the RAW barriers
+        I4Ring<RAW> ring;
+        auto wait = [&](int at, uint32_t parity) { return i4_warp_wait(&raw_bars[at], parity); };
         bool ok = true;
+        int next = 0;                                   // the tile whose copy is the next to be waited for
         for (int i = 0; run_of(i) < runs; ++i) {
             const int run = run_of(i), j = run >> 2, s = j % STAGES, key0 = first_key(run), part = run & 3;
             const bool here = needed(run), cut = !here || key0 < block_lo || key0 + 15 > p_last;
@@ -276,8 +284,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             uint32_t ks[2][NG], vs[4][NG];              // steps of tokens r and r + 8; of the four tokens of this lane's words of values
             auto token_of = [&](int e) { return 2 * l + (e & 1) + 8 * (e >> 1); };
             if (here) {
-                ok = i4_warp_wait(&raw_bars[i % RAW], phase >> (i % RAW) & 1);
-                phase ^= 1u << (i % RAW);
+                ok = ring.landed(i, wait);
                 if (!ok) break;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
@@ -294,6 +301,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
             }
             __syncwarp();
             fetch(i + RAW);
+            next = i + 1;
             if (cut) {                                  // the steps of what lies beyond the block's keys are zeros: anything may lie there
                 auto in = [&](int token) { return here && key0 + token >= block_lo && key0 + token <= p_last; };
 #pragma unroll
@@ -352,8 +360,7 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
         }
         if (!ok) {
             if (lane == 0) atomicCAS(a.status, 0, 61);
-            // what is on its way lands before the block's memory is another's
-            for (int i = 0; i < RAW; ++i) i4_wait(&raw_bars[i], phase >> i & 1);
+            ring.drain(next, [&](int i) { return needed(run_of(i)); }, wait);
         }
     } else {
         // ---- softmax: a row a thread
@@ -486,7 +493,10 @@ __global__ void __launch_bounds__(THREADS) int4_attention_tc_kernel(Args a) {
                 // the last two products may both be under way, and a parity tells one from the next only
                 ok = (n_kv < 2 || i4_warp_wait(&pv_done[m], (n_kv - 2) & 1)) && i4_warp_wait(&pv_done[m], (n_kv - 1) & 1);
             }
-            if (!ok && lane == 0) atomicCAS(a.status, 0, where);
+            if (!ok) {
+                if (lane == 0) atomicCAS(a.status, 0, where);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (ok) {
                 const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
