@@ -18,6 +18,7 @@
 // The tokens come prepared (int4_tokens_kernel): each brought into [2^14, 2^15) by a power of two and rounded to float16 - exact for bfloat16 down
 // to 2^-30 of the token's largest - as the second operands' images, swizzle included.
 #include "int4.cuh"
+#include "int4_ring.h"
 
 namespace {
 
@@ -219,6 +220,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
     uint64_t *raw_full = bars, *raw_empty = bars + RAW, *full = raw_empty + RAW, *empty = full + AS;
     uint64_t *d_full = empty + AS, *d_empty = d_full + DS;
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(d_empty + DS);
+    uint64_t* drained = d_empty + DS + 1;               // all products have ended
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slice = blockIdx.x % a.slices, unit0 = blockIdx.x / a.slices * 8, tiles = min(8, a.units - unit0);
     const int kb_begin = (int)((long long)a.kblocks * slice / a.slices), kb_end = (int)((long long)a.kblocks * (slice + 1) / a.slices);
@@ -232,6 +234,7 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
         for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], MAKERS + ADDERS); }
         for (int i = 0; i < AS; ++i) { mbar_init(&full[i], MAKERS + 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < DS; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], ADDERS); }
+        mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -293,6 +296,9 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
             umma_commit(&empty[i % AS]);
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, 51);
+        // (whoever gave up: no product is under way when tensor and shared memory become another's)
+        umma_commit(drained);
+        i4_warp_wait(drained, 0);
     } else if (warp == 1) {
         // ---- the copies of codes, RUN blocks of columns at a time
         if (lane == 0) {
@@ -302,10 +308,9 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                 if (ok) copy_codes(run);
                 else break;
             }
-            if (!ok) {
-                atomicCAS(a.status, 0, 52);
-                for (int i = max(0, run - RAW); i < run; ++i) i4_wait(&raw_full[i % RAW], (i / RAW) & 1);      // what is on its way lands first
-            }
+            if (!ok) atomicCAS(a.status, 0, 52);
+            // (whoever gave up: what is on its way lands before the stages are others')
+            i4_drain<RAW>(run, [&](int at, uint32_t parity) { i4_wait(&raw_full[at], parity); });
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -323,10 +328,9 @@ __global__ void __launch_bounds__(THREADS) int4_gemm_tc_kernel(Args a) {
                                  ::"r"(base + S::X + (i % AS * 2 + k) * S::XSTEP), "l"(a.x + (size_t)(kb_begin + 2 * i + k) * S::XB), "r"(S::XB), "r"(i4_smem(bar))
                                  : "memory");
             }
-            if (!ok) {
-                atomicCAS(a.status, 0, 52);
-                for (int k = max(0, i - AS); k < i; ++k) i4_wait(&full[k % AS], (k / AS) & 1);
-            }
+            if (!ok) atomicCAS(a.status, 0, 52);
+            // (a stage that its makers gave up is waited for as long as a wait may take: longer than a copy does)
+            i4_drain<AS>(i, [&](int at, uint32_t parity) { i4_wait(&full[at], parity); });
         }
         __syncwarp();
     } else if (warp < FIRST + MAKERS) {

@@ -23,3 +23,9 @@ template <int N> struct I4Ring {
             if (asked(i)) wait(i % N, (phase >> (i % N)) & 1u);
     }
 };
+
+// A ring that every tile takes in turn, tile i's phase being the (i / N)-th of its place: waits for the last copies of the ``issued`` ones, those that
+// may be under way when nobody is known to have waited for them (which returns at once for all that landed).
+template <int N, typename Wait> I4_BOTH void i4_drain(int issued, Wait wait) {
+    for (int i = issued > N ? issued - N : 0; i < issued; ++i) wait(i % N, (unsigned)(i / N) & 1u);
+}

@@ -82,3 +82,34 @@ def check(tmp_path, text):
 
 def test_a_ring_whose_tiles_may_be_passed_over(tmp_path):
     check(tmp_path, PASSED_OVER)
+
+
+IN_TURN = MODEL + r"""
+// ``issued`` copies, of which each landed or has not, in a ring whose places are taken again once the copy before has landed.
+template <int N> void run(unsigned seed) {
+    std::srand(seed);
+    const int issued = std::rand() % 14, landed_at_least = issued > N ? issued - N : 0;
+    Barrier bars[N];
+    std::set<int> under_way;
+    for (int i = 0; i < issued; ++i) {
+        if (i < landed_at_least || std::rand() % 2) ++bars[i % N].ended;
+        else under_way.insert(i);
+    }
+    i4_drain<N>(issued, [&](int place, unsigned parity) {
+        int tile = -1;
+        for (int t : under_way) if (t % N == place) { CHECK(tile < 0); tile = t; }
+        CHECK(bars[place].wait(parity) == (tile < 0));      // at once for what landed, not before for what did not
+        if (tile >= 0) { under_way.erase(tile); ++bars[place].ended; }
+        CHECK(bars[place].wait(parity));
+    });
+    CHECK(under_way.empty());
+}
+int main() {
+    for (unsigned seed = 0; seed < 20000; ++seed) { run<3>(seed); run<4>(seed); run<1>(seed); }
+    return failures ? 1 : 0;
+}
+"""
+
+
+def test_a_ring_that_tiles_take_in_turn(tmp_path):
+    check(tmp_path, IN_TURN)
