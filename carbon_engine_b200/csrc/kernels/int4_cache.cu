@@ -289,9 +289,6 @@ int check_weight(const WeightArgs& a, int dtype, const char* who) {
 
 }  // namespace
 
-extern "C" int ce_int4_cache_tile_bytes(int d, int group) { return i4_cache_tile_bytes(d, group); }
-extern "C" int ce_int4_weight_tile_bytes(int group) { return i4_weight_tile_bytes(group < 64 ? group : 64); }
-
 // A call's arguments, 8 bytes each in this order: one pointer to pass takes the host a fifth of the time of twenty arguments.
 struct Int4KvCall {
     long long dtype;

@@ -4,8 +4,8 @@
 // The codes are the first operand of mma.sync m16n8k16 (16 rows of the weight), 8 tokens the second; a step scales a group's partial sum in
 // float32, a minimum meets the group's sum of x.  No value of W is ever rounded.
 //
-// Up to 16 tokens run int4_stream_kernel, more bfloat16 ones int4_gemm_tc.cu, more float32 ones int4_gemm_kernel, for which int4_prepare_kernel
-// lays the tokens out as that second operand: each token is brought into [2^14, 2^15) by a power of two and rounded to two float16 pieces
+// Up to 16 tokens run int4_stream_kernel, more bfloat16 ones (or wider) int4_gemm_tc.cu, more float32 ones (or wider) int4_gemm_kernel, for which
+// int4_prepare_kernel lays the tokens out as that second operand: each token is brought into [2^14, 2^15) by a power of two and rounded to two float16 pieces
 // (22 bits), with the groups' sums of what was rounded.
 //
 // The stream is bound by the instructions that take codes apart and by the latencies between them, not by memory: 6,144 x 4,096 for one token
@@ -18,40 +18,41 @@ namespace {
 
 constexpr int WARPS = 8;
 
-struct Operand {                   // what int4_prepare_kernel writes: see operand_floats
-    uint32_t* frag;                // [kblocks][token tiles][pieces][2 halves][32 lanes][4 words]
+constexpr int PIECES = 2;          // float16 numbers of a float32 token's value
+
+struct Operand {                   // what int4_prepare_kernel writes: ce_int4_gemm_scratch counts it
+    uint32_t* frag;                // [kblocks][token tiles][PIECES][2 halves][32 lanes][4 words]
     float* sums;                   // [kblocks * groups of a block][token tiles * 8]
     float* back;                   // [token tiles * 8]: what a token's sums are multiplied by at the end
 };
 
 struct PrepareArgs {
-    const void* x;
+    const float* x;
     long long ld;
     Operand to;
     int M, K, kblocks, group, vec;      // group: 32 or 64
 };
 
 // one block a token of the padded tiles
-template <typename T, int P>
 __global__ void __launch_bounds__(256) int4_prepare_kernel(PrepareArgs a) {
     ce_pdl_begin();
     __shared__ float scratch[32];
     const int t = blockIdx.x, tiles = gridDim.x >> 3, nt = t >> 3, r = t & 7;
     const bool real = t < a.M;
-    const T* src = (const T*)a.x + (size_t)(real ? t : 0) * a.ld;
+    const float* src = a.x + (size_t)(real ? t : 0) * a.ld;
     float largest = 0.f;
     bool finite = true;
     if (real)
         for (int c = threadIdx.x * 8; c < a.K; c += 256 * 8)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = fabsf(CeType<T>::load(src + c + i));
+                const float v = fabsf(src[c + i]);
                 largest = fmaxf(largest, v);
                 finite = finite && v <= 3.402823466e38f;
             }
     largest = ce_block_max(finite ? largest : INFINITY, scratch);
     const float up = i4_row_scale(largest);
-    if (threadIdx.x == 0) a.to.back[t] = i4_unit<P == 2> / up;
+    if (threadIdx.x == 0) a.to.back[t] = 1.0f / up;
     // a thread takes 8 neighbouring columns: the four words of lane (r, l) for a half of a block; four threads hold a run of 32
     const int groups = 64 / a.group;
     for (int c = threadIdx.x * 8; c < a.kblocks * 64; c += 256 * 8) {
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(PrepareArgs a) {
                 y[0] = u.x; y[1] = u.y; y[2] = u.z; y[3] = u.w; y[4] = v.x; y[5] = v.y; y[6] = v.z; y[7] = v.w;
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = CeType<T>::load(src + c + i);
+                for (int i = 0; i < 8; ++i) y[i] = src[c + i];
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] *= up;
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(PrepareArgs a) {
         const int kb = c >> 6, half = (c >> 5) & 1, l = (c >> 3) & 3;
         float sum = 0.f;
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
+        for (int p = 0; p < PIECES; ++p) {
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -82,13 +83,13 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(PrepareArgs a) {
                 sum += (got.x + got.y) * b;
                 y[i] -= got.x * b; y[i + 4] -= got.y * b;
             }
-            *reinterpret_cast<uint4*>(a.to.frag + ((((size_t)kb * tiles + nt) * P + p) * 2 + half) * 128 + (4 * r + l) * 4) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(a.to.frag + ((((size_t)kb * tiles + nt) * PIECES + p) * 2 + half) * 128 + (4 * r + l) * 4) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         const unsigned here = 0xffu << (threadIdx.x & 24);      // the 8 threads of a block of 64 columns: all of them or none are here
         sum += __shfl_xor_sync(here, sum, 1);
         sum += __shfl_xor_sync(here, sum, 2);
         if (a.group == 64) sum += __shfl_xor_sync(here, sum, 4);
-        if (c % a.group == 0) a.to.sums[(size_t)(kb * groups + (c & 63) / a.group) * (tiles * 8) + t] = sum * (1.0f / i4_unit<P == 2>);
+        if (c % a.group == 0) a.to.sums[(size_t)(kb * groups + (c & 63) / a.group) * (tiles * 8) + t] = sum;
     }
 }
 
@@ -115,9 +116,9 @@ __device__ __forceinline__ void finish(void* out, size_t at, int mode, float v, 
 }
 
 // one block a tile of 16 rows: its warps share K
-template <typename T, int G, int NT>
+template <int G, int NT>
 __global__ void __launch_bounds__(WARPS * 32) int4_gemm_kernel(GemmArgs a) {
-    constexpr int P = sizeof(T) == 4 ? 2 : 1, TILE = i4_weight_tile_bytes(G), GB = 64 / G;
+    constexpr int P = PIECES, TILE = i4_weight_tile_bytes(G), GB = 64 / G;
     __shared__ float part[WARPS][16][NT * 8 + 1];
     __shared__ float total[16][NT * 8 + 1];
     ce_pdl_begin();
@@ -141,8 +142,8 @@ __global__ void __launch_bounds__(WARPS * 32) int4_gemm_kernel(GemmArgs a) {
 #pragma unroll
                         for (int p = 0; p < P; ++p) acc[nt][p][0] = acc[nt][p][1] = acc[nt][p][2] = acc[nt][p][3] = 0.f;
                 uint32_t e0, e1, e2, e3, o0, o1, o2, o3;
-                i4_pairs<P == 2, 0>(wa, e0, e2); i4_pairs<P == 2, 0>(wb, e1, e3);
-                i4_pairs<P == 2, 8>(wa, o0, o2); i4_pairs<P == 2, 8>(wb, o1, o3);
+                i4_pairs<true, 0>(wa, e0, e2); i4_pairs<true, 0>(wb, e1, e3);
+                i4_pairs<true, 8>(wa, o0, o2); i4_pairs<true, 8>(wb, o1, o3);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -155,18 +156,15 @@ __global__ void __launch_bounds__(WARPS * 32) int4_gemm_kernel(GemmArgs a) {
                     }
                 if ((half * 32 + 32) % G == 0) {
                     const int g = half * 32 / G;
-                    const float2 fa = i4_step_of<P == 2>(*reinterpret_cast<const uint32_t*>(tile + 512 + (r * GB + g) * 4));
-                    const float2 fb = i4_step_of<P == 2>(*reinterpret_cast<const uint32_t*>(tile + 512 + ((r + 8) * GB + g) * 4));
+                    const float2 fa = i4_step_of<true>(*reinterpret_cast<const uint32_t*>(tile + 512 + (r * GB + g) * 4));
+                    const float2 fb = i4_step_of<true>(*reinterpret_cast<const uint32_t*>(tile + 512 + ((r + 8) * GB + g) * 4));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         if (nt >= a.tiles) continue;
                         const float2 s = *reinterpret_cast<const float2*>(a.x.sums + (size_t)(kb * GB + g) * tokens + nt * 8 + 2 * l);
                         float c[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            c[e] = acc[nt][0][e];
-                            if constexpr (P == 2) c[e] += acc[nt][1][e];
-                        }
+                        for (int e = 0; e < 4; ++e) c[e] = acc[nt][0][e] + acc[nt][1][e];
                         y[nt][0] = fmaf(fa.x, c[0], fmaf(fa.y, s.x, y[nt][0]));
                         y[nt][1] = fmaf(fa.x, c[1], fmaf(fa.y, s.y, y[nt][1]));
                         y[nt][2] = fmaf(fb.x, c[2], fmaf(fb.y, s.x, y[nt][2]));
@@ -194,7 +192,7 @@ __global__ void __launch_bounds__(WARPS * 32) int4_gemm_kernel(GemmArgs a) {
         const int t = i / rows_out, row = i - t * rows_out, n = blockIdx.x * rows_out + row;
         if (t >= a.M || n >= a.N) continue;
         const float back = a.x.back[t];
-        finish<T>(a.out, (size_t)t * a.ldo + n, a.mode, total[row][t] * back, a.gated ? total[row + 8][t] * back : 0.f);
+        finish<float>(a.out, (size_t)t * a.ldo + n, a.mode, total[row][t] * back, a.gated ? total[row + 8][t] * back : 0.f);
     }
 }
 
@@ -626,19 +624,17 @@ int launch_stream_tiles(const StreamArgs& a, int tiles, cudaStream_t stream) {
     return tiles == 1 ? launch_stream<T, G, 1>(a, stream) : launch_stream<T, G, 2>(a, stream);
 }
 
-int pieces(int dtype) { return dtype == CE_F32 ? 2 : 1; }
-
-template <typename T, int G, int NT>
+template <int G, int NT>
 cudaError_t launch(const GemmArgs& a, int row_tiles, cudaStream_t stream) {
     ce_note("int4_gemm_kernel");
-    return ce_launch(int4_gemm_kernel<T, G, NT>, dim3(row_tiles), dim3(WARPS * 32), 0, stream, a);
+    return ce_launch(int4_gemm_kernel<G, NT>, dim3(row_tiles), dim3(WARPS * 32), 0, stream, a);
 }
-template <typename T, int G>
+template <int G>
 cudaError_t launch_tiles(const GemmArgs& a, int row_tiles, cudaStream_t stream) {
-    if (a.tiles == 1) return launch<T, G, 1>(a, row_tiles, stream);       // (K beyond the stream's registers)
-    if (a.tiles == 2) return launch<T, G, 2>(a, row_tiles, stream);
-    if (a.tiles <= 4) return launch<T, G, 4>(a, row_tiles, stream);
-    return launch<T, G, 8>(a, row_tiles, stream);
+    if (a.tiles == 1) return launch<G, 1>(a, row_tiles, stream);          // (K beyond the stream's registers)
+    if (a.tiles == 2) return launch<G, 2>(a, row_tiles, stream);
+    if (a.tiles <= 4) return launch<G, 4>(a, row_tiles, stream);
+    return launch<G, 8>(a, row_tiles, stream);
 }
 
 }  // namespace
@@ -651,7 +647,7 @@ namespace {
 
 // Whether the stream of weights takes these sizes: up to 16 tokens, K within the registers of 8 blocks
 bool streamed(int dtype, int M, int K) {
-    const int tiles = (M + 7) / 8, nt_p = tiles * pieces(dtype);
+    const int tiles = (M + 7) / 8, nt_p = tiles * (dtype == CE_F32 ? PIECES : 1);
     return tiles <= 2 && (K + 63) / 64 <= 8 * SW * (4 / nt_p);
 }
 
@@ -662,7 +658,7 @@ extern "C" long long ce_int4_gemm_scratch(int dtype, int M, int K, int group) {
     if (streamed(dtype, M, K)) return 0;
     if (dtype == CE_BF16) return ce_int4_gemm_tc_scratch(M, K);
     const long long tiles = (M + 7) / 8, kblocks = (K + 63) / 64;
-    return kblocks * tiles * pieces(dtype) * 256 + kblocks * (64 / (group < 64 ? group : 64)) * tiles * 8 + tiles * 8;
+    return kblocks * tiles * PIECES * 256 + kblocks * (64 / (group < 64 ? group : 64)) * tiles * 8 + tiles * 8;
 }
 
 // A call's arguments, 8 bytes each in this order.  N: columns of the result (a gated weight has N gate rows and N up rows).
@@ -708,14 +704,14 @@ extern "C" int ce_int4_gemm(const Int4GemmCall* c) {
     if (dtype == CE_BF16) return ce_int4_gemm_tc(x, ldx, w, out, ldo, M, N, K, kept, mode, scratch, c->status, (cudaStream_t)stream);
     Operand op;
     op.frag = (uint32_t*)scratch;
-    op.sums = scratch + (size_t)kblocks * tiles * pieces(dtype) * 256;
+    op.sums = scratch + (size_t)kblocks * tiles * PIECES * 256;
     op.back = op.sums + (size_t)kblocks * (64 / kept) * tiles * 8;
-    PrepareArgs p{x, ldx, op, M, K, kblocks, kept, vec};
+    PrepareArgs p{(const float*)x, ldx, op, M, K, kblocks, kept, vec};
     ce_note("int4_prepare_kernel");
-    cudaError_t e = ce_launch(int4_prepare_kernel<float, 2>, dim3(tiles * 8), dim3(256), 0, (cudaStream_t)stream, p);
+    cudaError_t e = ce_launch(int4_prepare_kernel, dim3(tiles * 8), dim3(256), 0, (cudaStream_t)stream, p);
     if (e == cudaSuccess) {
         GemmArgs a{(const unsigned char*)w, op, out, ldo, M, N, kblocks, tiles, mode, gated};
-        e = kept == 32 ? launch_tiles<float, 32>(a, row_tiles, (cudaStream_t)stream) : launch_tiles<float, 64>(a, row_tiles, (cudaStream_t)stream);
+        e = kept == 32 ? launch_tiles<32>(a, row_tiles, (cudaStream_t)stream) : launch_tiles<64>(a, row_tiles, (cudaStream_t)stream);
     }
     if (e != cudaSuccess) { (void)cudaGetLastError(); return ce_fail(CE_ERR_CUDA, "int4_gemm: %s", cudaGetErrorString(e)); }
     return ce_check_launch("int4_gemm");

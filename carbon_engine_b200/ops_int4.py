@@ -22,8 +22,6 @@ from .csrc import kernel_lib
 from .csrc.kernel_lib import KernelError, kernels
 
 _i, _ll, _p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
-kernel_lib.declare("ce_int4_cache_tile_bytes", _i, [_i, _i])
-kernel_lib.declare("ce_int4_weight_tile_bytes", _i, [_i])
 # These take one pointer to their arguments, 8 bytes each (ctypes takes 0.2 us for every argument of its own):
 # dtype, k, v, strides of k and v (token, head), pages, positions, seq_of_token, seq_slot, block_table, status,
 # T, nkv, d, group, page_size, max_pages, num_pages, stream

@@ -276,3 +276,16 @@ def test_windows_beyond_32_bits_hide_nothing(window):
         c.ops.attention(q, c.pages, out, c.slots, gpu([0, 1]), gpu([90]), c.table, c.status, n_decode=1, max_ctx=90, window=w, scale=0.1)
         outs.append(out)
     assert torch.equal(*outs)
+
+
+# ---- float32 tokens on either side of what the stream's registers hold
+@pytest.mark.parametrize("M,K,streamed", [(8, 16384, True), (5, 16448, False), (16, 8192, True), (12, 8256, False), (1, 16448, False)])
+def test_float32_products_beyond_the_streams_registers(M, K, streamed):
+    from carbon_engine_b200 import ops, ops_int4
+    for group, mode in ((64, ops.GEMM_STORE_F32), (32, ops.GEMM_SWIGLU)):
+        x, w, w4, _ = product_case(F32, mode, M, 33, K, group)
+        out = torch.empty((M, 33), device="cuda")
+        before = ops.kernel_counts().get("int4_gemm_kernel", 0)
+        ops_int4.matmul(x, w4, out, mode)
+        check_product(x, w, group, w4, mode, out)
+        assert ops.kernel_counts().get("int4_gemm_kernel", 0) - before == (0 if streamed else 1)
