@@ -17,9 +17,10 @@ from .sampling.params import SamplingParams
 
 class BenchHarness:
     def __init__(self, cfg, max_batch: int, context: int, new_tokens: int, graphs: bool = True,
-                 page_size: int = 64, seed: int = 0, step_tokens: int = 4096):
+                 page_size: int = 64, seed: int = 0, step_tokens: int = 4096, weight_bits: int = 16, kv_bits: int = 16,
+                 int4_group: int = 64):
         """``cfg``: the sizes of a Qwen3 dense model as a dict, or a typed configuration of any registered
-        architecture."""
+        architecture.  ``weight_bits``, ``kv_bits``, ``int4_group``: see :class:`Engine`."""
         if isinstance(cfg, dict):
             raw = dict(cfg, architectures=["Qwen3ForCausalLM"], model_type="qwen3")
             self.config = Qwen3Config.from_dict(raw)
@@ -31,14 +32,30 @@ class BenchHarness:
         self.max_seq_len = max(4096, per_seq)
         self.engine = Engine(config=self.config, dtype="bfloat16", dummy_weight=True, seed=seed,
                              kv_tokens=max_batch * per_seq + 4096, page_size=page_size, max_seq_len=max(4096, per_seq),
-                             max_running_requests=max_batch, max_prefill_tokens=step_tokens, cuda_graphs=graphs)
+                             max_running_requests=max_batch, max_prefill_tokens=step_tokens, cuda_graphs=graphs,
+                             weight_bits=weight_bits, kv_bits=kv_bits, int4_group=int4_group)
         self.graphs = bool(graphs and self.engine.runner.graphs_enabled)
         self.rng = np.random.default_rng(seed)
         self._next = 1 << 40
         g = torch.Generator(device=self.engine.device).manual_seed(seed)
         for view in self.engine.storage.paged_views():          # a cache that holds plausible keys and values
+            if view.int4 is not None:
+                self._fill(view.int4, g)
+                continue
             for pool in (view.k_pool, view.v_pool):
                 pool.normal_(0.0, 1.0, generator=g)
+
+    def _fill(self, pages, generator) -> None:
+        """Normal keys and values in all 4-bit pages."""
+        from . import ops_int4
+        device = self.engine.device
+        table = torch.arange(pages.num_pages, dtype=torch.int32, device=device)[None]
+        slot, status = torch.zeros(1, dtype=torch.int32, device=device), torch.zeros(1, dtype=torch.int32, device=device)
+        for at in range(0, pages.num_pages * pages.page_size, 16384):
+            pos = torch.arange(at, min(at + 16384, pages.num_pages * pages.page_size), dtype=torch.int32, device=device)
+            k, v = (torch.empty((len(pos), pages.kv_heads, pages.head_dim), dtype=torch.bfloat16, device=device).normal_(0.0, 1.0, generator=generator)
+                    for _ in "kv")
+            ops_int4.kv_write(pages, k, v, pos, torch.zeros_like(pos), slot, table, status)
 
     def _tokens(self, n: int) -> List[int]:
         return self.rng.integers(0, self.config.vocab_size, size=n).tolist()

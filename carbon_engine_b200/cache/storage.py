@@ -105,11 +105,10 @@ class CacheStorage:
         return [e for e in self._entries.values() if e.kind == "paged"]
 
     def bytes_per_token(self) -> int:
-        from ..ops_int4 import cache_bytes_per_token
         total = 0
         for e in self._entries.values():
             if e.int4 is not None:
-                total += cache_bytes_per_token(e.int4.kv_heads, e.int4.head_dim, e.int4.group)
+                total += e.int4.bytes_per_token()
             elif e.kind == "paged":
                 total += (e.k_pool.shape[1] * e.k_pool.shape[3] + e.v_pool.shape[1] * e.v_pool.shape[3]) * e.k_pool.element_size()
         return total

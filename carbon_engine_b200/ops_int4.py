@@ -139,6 +139,10 @@ class Int4Pages:
         """Bytes a key or value takes, steps and minima included."""
         return 0.5 + 4.0 / self.group
 
+    def bytes_per_token(self) -> int:
+        """Bytes a token's keys and values take."""
+        return cache_bytes_per_token(self.kv_heads, self.head_dim, self.group)
+
 
 def _kv_call(fn, k, v, pages, positions, seq_of_token, seq_slot, block_table, status) -> None:
     device = _current(k, "k")
@@ -328,6 +332,8 @@ class Int4Weight:
             raise KernelError("a weight is [rows, width], the columns of a row together")
         self = cls(weight.shape[0], weight.shape[1], group, gated, weight.device)
         ld = weight.stride(0) if self.rows > 1 else self.width
+        if ops._profile is not None:
+            ops._profile.note_work(weight.numel() * weight.element_size() + self.data.numel(), 0)
         ops._ok(kernels().ce_int4_quantise_weight(_code(weight, "weight"), weight.data_ptr(), ld, self.data.data_ptr(),
                                                   self.rows, int(self.gated), self.width, self.group, _stream(device)), 2)
         return self
@@ -338,6 +344,8 @@ class Int4Weight:
         if out.shape != (self.rows, self.width) or out.stride(1) != 1 or self.data.get_device() != device:
             raise KernelError(f"out is {tuple(out.shape)} on {out.device}, not {(self.rows, self.width)} where the weight is ({self.data.device})")
         ld = out.stride(0) if self.rows > 1 else self.width
+        if ops._profile is not None:
+            ops._profile.note_work(self.data.numel() + out.numel() * out.element_size(), 0)
         ops._ok(kernels().ce_int4_dequantise_weight(_code(out, "out"), out.data_ptr(), ld, self.data.data_ptr(),
                                                     self.rows, int(self.gated), self.width, self.group, _stream(device)), 2)
         return out

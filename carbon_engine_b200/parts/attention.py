@@ -157,13 +157,28 @@ class PagedAttention(Mixer):
             ops_int4.kv_write(cache.int4, heads[:, nh:nh + nkv], heads[:, nh + nkv:], ctx.positions, ctx.seq_of_token, ctx.seq_slot, table,
                               ctx.status)
         step = (heads[:, :nh], cache.int4, out.view(-1, nh, d), ctx.seq_slot, ctx.q_start, ctx.ctx_len, table, ctx.status)
+        prof = ops.profiling()
         if ctx.n_decode > 0:
+            if prof is not None:
+                prof.note_work(*self.int4_work(ctx, cache.int4, qkv.element_size(), 0, ctx.n_decode))
             # (the plan's bound, and so the launch, is the one a captured step was captured with)
             ops_int4.attention(*step, n_decode=ctx.n_decode, max_ctx=plan.decode_splits * ops_tensor.decode_split(), window=self.window,
                                scale=self.scale)
         if plan.n_tiles > 0:
+            if prof is not None:
+                prof.note_work(*self.int4_work(ctx, cache.int4, qkv.element_size(), ctx.n_decode, ctx.B))
             ops_int4.attention(*step, n_decode=0, max_ctx=plan.portion_ctx, tiles=plan.tiles, n_tiles=plan.n_tiles, window=self.window,
                                scale=self.scale)
+
+    def int4_work(self, ctx, pages, el: int, first: int, last: int):
+        """Bytes that attention of sequences first .. last - 1 over 4-bit pages reads and writes once, and its operations."""
+        keys = pairs = tokens = 0
+        for b in range(first, last):
+            n, before = ctx.h_q_start[b + 1] - ctx.h_q_start[b], ctx.h_ctx_before[b]
+            keys += before + n - (max(0, before + 1 - self.window) if self.window else 0)
+            pairs += sum(min(p + 1, self.window or p + 1) for p in range(before, before + n))
+            tokens += n
+        return keys * pages.bytes_per_token() + 2 * tokens * self.heads * self.head_dim * el, 4 * pairs * self.heads * self.head_dim
 
     def attend(self, ctx, qkv: torch.Tensor, out: torch.Tensor, cache, table: torch.Tensor) -> None:
         nh, nkv, d = self.heads, self.kv_heads, self.head_dim
