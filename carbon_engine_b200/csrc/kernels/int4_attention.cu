@@ -7,9 +7,12 @@
 // (keys) or the probability (values), a minimum takes part in float32.  Keys (values' channels) are the 16 rows of mma.sync m16n8k16, query
 // rows its 8 columns, which is how the heads of a group that share a KV head fill a tile.
 //
-// Roundings: a query row is brought into [2^14, 2^15) by a power of two and rounded to float16, which is exact for bfloat16 (to 2^-30 of the
-// row's largest); float32 rows are two float16 pieces, 22 bits.  p_j s_jg is rounded to float16 (2^-12 of itself; two pieces for float32),
-// scaled so that the largest lies near 2^10: sums of thousands of small weights keep their bits.  Everything else is float32.
+// Roundings: a query row is brought into [2^14, 2^15) by a power of two and rounded to float16, which is exact for bfloat16 values down to 2^-27 of
+// the row's largest (half of them divided by 16, for codes that come 16 times too large); float32 rows are two float16 pieces, 22 bits.  p_j s_jg is
+// rounded to float16 (by 2^-11 of itself at most; two pieces for float32), scaled so that the largest probability times the largest step that the warp
+// has met in any group lies near 2^10: sums of thousands of small weights keep their bits.  Below 2^-14 float16's steps are fixed, so that each key may
+// err by 15 2^-34 of that largest step, in units of the largest probability: what a group with far smaller steps than its neighbours' loses.
+// Everything else is float32.
 //
 // A block takes up to 8 or 16 rows (tokens by heads of the KV head) and a run of the keys; its 8 or 4 warps take tiles in turn, each with a
 // ring of its own that one lane fills with bulk copies (a tile is one run of bytes in the page); warps, then blocks, are joined in a fixed order.

@@ -289,3 +289,30 @@ def test_float32_products_beyond_the_streams_registers(M, K, streamed):
         ops_int4.matmul(x, w4, out, mode)
         check_product(x, w, group, w4, mode, out)
         assert ops.kernel_counts().get("int4_gemm_kernel", 0) - before == (0 if streamed else 1)
+
+
+# ---- groups of very different steps side by side
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("spread", [1.0, 8.0])
+def test_small_groups_beside_large_ones(dtype, spread):
+    """Each group with a tolerance of its own.  A weight's product with its step is rounded by 2^-11 of itself (2^-22 for float32's two pieces), and
+    below 2^-14 by float16's fixed half step of 2^-25.  The row's largest weight is 2^10 over a power of two that is less than twice the largest
+    step s met, so in units of that weight 2^-25 is at most 2^-34 s; a key's codes are at most 15, and n keys err by n 15 2^-34 s together."""
+    n, d, group = 800, 128, 32
+    c = Cache([n], 1, d, group, 16)
+    sizes = torch.tensor([1000.0, 1e-2, 1.0, 0.1], device="cuda").repeat_interleave(group)
+    k, v = normal((n, 1, d), 1, F32, spread / 11.3), normal((n, 1, d), 2, F32) * sizes
+    c.write(k, v)
+    q, scale = normal((1, 8, d), 3, dtype), 1.0 / math.sqrt(d)
+    out = torch.empty_like(q)
+    c.ops.attention(q, c.pages, out, c.slots, gpu([0, 1]), gpu([n]), c.table, c.status, n_decode=1, max_ctx=n, scale=scale)
+    held = plain.held(v, group).cpu()
+    want, reach, _ = plain.attend(q.cpu(), plain.held(k, group).cpu(), held, [1], [n], scale, 0)
+    largest_step = float((held.unflatten(-1, (-1, group)).amax(-1) - held.unflatten(-1, (-1, group)).amin(-1)).max()) / 15
+    for g in range(d // group):
+        part = slice(g * group, (g + 1) * group)
+        largest = float(held[..., part].abs().max())
+        tolerance = want[..., part].abs() * torch.finfo(dtype).eps / 2 + 2.0 * largest * (reach + 4.0) * 2.0 ** -21 \
+            + 2.0 * largest * (2.0 ** -11 if dtype == BF16 else 2.0 ** -22) + n * 15 * 2.0 ** -34 * largest_step + largest * (n / 128 + 32) * 2.0 ** -23
+        off = (out[..., part].double().cpu() - want[..., part]).abs()
+        assert bool((off <= tolerance).all()), (g, float(off.max()), float(tolerance.max()))
