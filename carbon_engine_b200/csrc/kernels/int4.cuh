@@ -149,7 +149,7 @@ __device__ __forceinline__ float2 i4_unpack(uint32_t v) { return __half22float2(
 // (Comparisons: NaN stays.)
 __device__ __forceinline__ float i4_normal(float v) { return v > 0x1.fffffep127f ? 0x1.fffffep127f : v < 0x1p-126f ? 0x1p-126f : v; }
 // The power of two that brings a row's largest magnitude into [2^14, 2^15): a float16 then holds bfloat16 values exactly down to 2^-30 of the
-// largest.  Its bits are those of 2^14 less the largest's exponent; 1 for a row of zeros, NaN for one that is not finite.
+// largest, and a 16th of them (for codes that come 16 times too large) down to 2^-27.  Its bits are those of 2^14 less the largest's exponent; 1 for a row of zeros, NaN for one that is not finite.
 __device__ __forceinline__ float i4_row_scale(float largest) {
     if (!(largest <= 3.402823466e38f)) return __int_as_float(0x7fc00000);
     const int e = (int)(__float_as_uint(largest) >> 23) - 127;          // subnormal numbers count as 2^-127

@@ -17,7 +17,7 @@
 // A block takes up to 8 or 16 rows (tokens by heads of the KV head) and a run of the keys; its 8 or 4 warps take tiles in turn, each with a
 // ring of its own that one lane fills with bulk copies (a tile is one run of bytes in the page); warps, then blocks, are joined in a fixed order.
 //
-// 64 sequences of 8,192 keys of 8 KV heads of 128 take 133 us, 4.5 TB/s: bound by instructions (313 a tile a warp, the ALU pipe, which takes the codes
+// 64 sequences of 8,192 keys of 8 KV heads of 128 take 135 us, 4.5 TB/s: bound by instructions (313 a tile a warp, the ALU pipe, which takes the codes
 // apart, half busy, 2.2 instructions a cycle of an SM).  A block costs some 4 us to begin (place, queries, first tiles) and end (joins), which
 // is what short and uneven requests are bound by (21 of 450 to 9,000 keys: 49 us of which 19.5 are the bytes').
 #include "int4.cuh"
@@ -706,7 +706,8 @@ int run(Args a, int jobs, cudaStream_t stream) {
     constexpr int TILE = i4_cache_tile_bytes(D, G), RING = ring_tiles(TILE) * TILE, OUT = 8 * NT * (D + 4) * 4;
     constexpr int SMEM = WARPS * (RING > OUT ? RING : OUT);
     // 8 warps a block as long as the chip takes all blocks at once, two an SM; then 4, four an SM, whose beginnings and ends (some 4.5 us) hide
-    // behind more others: 64 sequences of 8,192 keys in quarters 134 us for 151, 128 of 30 to 600 22 us for 30; one of 2,048 in eighths 8.3 us for 7.5
+    // behind more others: 64 sequences of 8,192 keys in quarters (ops_int4._splits takes thirds there) 134 us for 151, 128 of 30 to 600 22 us for 30;
+    // one of 2,048 in eighths 8.3 us for 7.5
     const int warps = (long long)jobs * a.splits <= 2 * ce_sm_count() ? WARPS : WARPS / 2;
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
     static std::atomic<unsigned long long> done{0};

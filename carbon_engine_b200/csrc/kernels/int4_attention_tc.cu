@@ -11,13 +11,13 @@
 // one tile of scores, P in shared memory and one issuing thread, a tile of 64 keys took 2.27 us, of which 1.3 were hand-overs that stayed
 // with all work left out.)
 //
-// 1,733 tokens after 6,000, 32 heads over 8 of 128: 288 us, 0.41 of the arithmetic peak: a tile of 64 keys takes some 2,500 cycles, of which the
+// 1,733 tokens after 6,000, 32 heads over 8 of 128: 294 us, 0.40 of the arithmetic peak: a tile of 64 keys takes some 2,500 cycles, of which the
 // exponentials of 256 rows take 1,024, the products 1,300, and the softmax's chain (scores there, 1,550 cycles of arithmetic, probabilities
 // stored, products issued) is the longest; 224 blocks for 148 SMs take one and a half rounds.
 //
-// Roundings: c s + z to float16 once (2^-12 of itself; the codes are exact); a query row brought into [2^14, 2^15) by a power of two is exact in
+// Roundings: c s + z to float16 once (by 2^-11 of itself at most; the codes are exact); a query row brought into [2^14, 2^15) by a power of two is exact in
 // float16 down to 2^-30 of its largest; a probability is kept as 2^(S - m) with m six below the running maximum, so that float16 holds it to
-// 2^-12 of itself down to 2^-20 of the largest.  A group of values that is not a number is put into the tile as zeros and reaches the rows that
+// 2^-11 of itself down to 2^-20 of the largest.  A group of values that is not a number is put into the tile as zeros and reaches the rows that
 // see its key at the end.
 //
 // Keys' and values' channels lie in the order in which codes come out of their words; the queries' channels are laid out to match, and

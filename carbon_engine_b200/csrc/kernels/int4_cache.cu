@@ -3,8 +3,8 @@
 //
 // Eight lanes take 64 neighbouring channels of a token's head, 8 a lane (a word of a key's codes): a group's extremes are found with shuffles.  A
 // weight's quantisation gives a lane 4 columns.  Bound by the launch and by four loads that wait for one another (position, request, its slot, its
-// page) for single tokens (2.7 us of the GPU's time), by the instructions - some 20 a value - for whole prompts (2,048 tokens of 8 heads of 128
-// written and read back: 12.7 us, 1.7 TB/s).
+// page) for single tokens (2.7 us of the GPU's time), by the instructions - some 60 a value by the
+// counters - for whole prompts (2,048 tokens of 8 heads of 128: written in 8.2 us, read back in 4.6).
 #include "int4.cuh"
 
 namespace {

@@ -5,13 +5,13 @@
 // float32, a minimum meets the group's sum of x.  No value of W is ever rounded.
 //
 // Up to 16 tokens run int4_stream_kernel, more bfloat16 ones (or wider) int4_gemm_tc.cu, more float32 ones (or wider) int4_gemm_kernel, for which
-// int4_prepare_kernel lays the tokens out as that second operand: each token is brought into [2^14, 2^15) by a power of two and rounded to two float16 pieces
-// (22 bits), with the groups' sums of what was rounded.
+// int4_prepare_kernel lays the tokens out as that second operand: each token is brought into [2^14, 2^15) by a power of two and rounded to two
+// float16 pieces (22 bits), with the groups' sums of what was rounded (4,096 x 4,096: 27 us for 17 tokens, 53 for 64).
 //
 // The stream is bound by the instructions that take codes apart and by the latencies between them, not by memory: 6,144 x 4,096 for one token
 // 6.4 us (2.2 TB/s), 12,288 + 12,288 rows of 4,096 for 8 tokens 17.3 us (3.3 TB/s), 75,776 x 4,096 for one token 40 us (4.4 TB/s).  Up to 8 tokens it
 // is the faster one everywhere; for 9 to 16 it is as long as rows are few (4,096 x 12,288, 16 tokens: 19.6 us, on tcgen05 24; 12,288 + 12,288 x 4,096:
-// 33, 51), and 10 % slower for 75,776 rows of 4,096 (112, 99).
+// 33, 51), and 10 % slower for 75,776 rows of 4,096 (112, 99).  Warm weights; past cold ones 12,288 + 12,288 x 4,096 take 21 us for 8 tokens, 40 for 16.
 #include "int4.cuh"
 
 namespace {

@@ -13,10 +13,11 @@
 //
 // 64 tokens x 12,288 columns x 4,096 rows take 29 us in groups of 32, 25.5 in groups of 64 (9 tokens: 26 and 24): what bounds it is the chain of
 // hand-overs - 1,300 cycles for 128 columns, of which the products take some 300 - and the 10 us before the first and behind the last of them
-// (tokens prepared, slices joined), neither memory (5 us) nor the tensor cores.
+// (tokens prepared, slices joined), neither memory (5 us) nor the tensor cores.  The 16-bit product of these sizes takes no longer (gemm_tc.cu:
+// past cold weights 24 to 30 us for 17 to 64 tokens, this one 27 to 34): a 4-bit weight of so many tokens saves memory, not time.
 //
 // The tokens come prepared (int4_tokens_kernel): each brought into [2^14, 2^15) by a power of two and rounded to float16 - exact for bfloat16 down
-// to 2^-30 of the token's largest - as the second operands' images, swizzle included.
+// to 2^-27 of the token's largest - as the second operands' images, swizzle included.
 #include "int4.cuh"
 #include "int4_ring.h"
 

@@ -189,9 +189,10 @@ def _splits(jobs: int, tiles: int):
     """(blocks that share a row block's keys, tiles of 16 keys a block) for ``jobs`` row blocks of up to ``tiles`` tiles: what is least by the time
     that blocks take.  Blocks of 8 warps, two an SM, or of 4, four an SM, where there are more than 296; a block takes 1.03 us for each tile of a
     warp (0.65 with an SM to itself) and 4.5 to begin and end.  Of more than the chip holds at once, the mean of what it is for requests of one
-    length and for those of half the longest on the average, whose long ones end alone; and what a second kernel takes that joins them.  (64
-    sequences of 8,192 keys, 8 KV heads of 128, in 1, 2, 3, 4 and 8 blocks a row block: 136, 137, 135, 130 and 144 us; 21 of 450 to 9,000
-    keys, groups of 32, in 1 to 6: 75, 76, 65, 55, 48 and 49 us.)"""
+    length and for those of half the longest on the average, whose long ones end alone; and what a second kernel takes that joins them.  The model
+    lies within a tenth of the best: 64 sequences of 8,192 keys, 8 KV heads of 128, in 1, 2, 3, 4 and 8 blocks a row block take 138, 138, 135, 130 and
+    144 us, and it takes 3; 21 of 450 to 9,000 keys, groups of 32, in 1 to 6 take 74, 76, 65, 56, 49 and 50 us, and it takes 6.  (Its numbers are the
+    B200's: 148 SMs, 296 blocks of 8 warps or 592 of 4 at once.)"""
     best = (float("inf"), 1, tiles)
     for splits in (1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64):
         share = -(-tiles // splits)
@@ -267,7 +268,8 @@ def attention(q: torch.Tensor, pages: Int4Pages, out: torch.Tensor, seq_slot: to
     the rows ``q_start[b]`` .. ``q_start[b + 1]`` and ``ctx_len[b]`` keys with them, and its pages in row ``seq_slot[b]`` of ``block_table``.  The first ``n_decode`` sequences bring one
     token each, or none; the others are listed in ``tiles`` (int32 [n_tiles, 2]: sequence, first of up to 64 of its tokens).  ``max_ctx``: at least the longest
     ``ctx_len`` (it only shapes the launch: a smaller number is slower, not wrong).  ``window`` > 0: a query sees that many keys, itself the last of them.  A row that sees no key becomes zeros; rows of ``out`` that
-    belong to no sequence stay as they were.  ``status`` becomes 4 where a page is not held, 7 where a wait gave up."""
+    belong to no sequence stay as they were.  ``status`` becomes 4 where a page is not held, 7 or 61 to 69 where a wait gave up (61 on: portions on
+    tcgen05).  Scores may have any size that float32 holds; those within a few of its steps of a row's largest may count alike."""
     device = _current(q, "q")
     code = _code(q, "q")
     if q.dim() != 3:
@@ -357,7 +359,8 @@ _F32_MODES = (ops.GEMM_STORE_F32, ops.GEMM_ACCUM_F32)
 
 
 def matmul(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, mode: int = ops.GEMM_STORE) -> None:
-    """out (op)= x @ w.T with the epilogue ``mode`` (``ops.GEMM_*``), for up to :data:`MAX_TOKENS` tokens.  ``x`` [M, width]
+    """out (op)= x @ w.T with the epilogue ``mode`` (``ops.GEMM_*``), for up to :data:`MAX_TOKENS` tokens (faster than the 16-bit product for up to
+    some 16 of them).  Waits that gave up are reported as 51 to 59 in the weight's ``status``.  ``x`` [M, width]
     bfloat16 or float32; ``out`` [M, rows] (half the rows with a gated epilogue) in the type of x, float32 with ``GEMM_STORE_F32`` and
     ``GEMM_ACCUM_F32``; rows of both at any stride.  A token of x with a value that is not finite gives a row of NaN, a group of the weight
     that reads back as NaN its column."""
