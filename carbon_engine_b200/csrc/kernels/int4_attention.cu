@@ -706,7 +706,7 @@ int run(Args a, int jobs, cudaStream_t stream) {
     constexpr int TILE = i4_cache_tile_bytes(D, G), RING = ring_tiles(TILE) * TILE, OUT = 8 * NT * (D + 4) * 4;
     constexpr int SMEM = WARPS * (RING > OUT ? RING : OUT);
     // 8 warps a block as long as the chip takes all blocks at once, two an SM; then 4, four an SM, whose beginnings and ends (some 4.5 us) hide
-    // behind more others: 64 sequences of 8,192 keys in quarters (ops_int4._splits takes thirds there) 134 us for 151, 128 of 30 to 600 22 us for 30;
+    // behind more others: 64 sequences of 8,192 keys in quarters (ops_int4._splits takes thirds there) 134 us for 151, 128 of 30 to 600 22 us for 30 (19 since);
     // one of 2,048 in eighths 8.3 us for 7.5
     const int warps = (long long)jobs * a.splits <= 2 * ce_sm_count() ? WARPS : WARPS / 2;
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
