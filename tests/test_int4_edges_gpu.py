@@ -316,3 +316,41 @@ def test_small_groups_beside_large_ones(dtype, spread):
             + 2.0 * largest * (2.0 ** -11 if dtype == BF16 else 2.0 ** -22) + n * 15 * 2.0 ** -34 * largest_step + largest * (n / 128 + 32) * 2.0 ** -23
         off = (out[..., part].double().cpu() - want[..., part]).abs()
         assert bool((off <= tolerance).all()), (g, float(off.max()), float(tolerance.max()))
+
+
+# ---- as they are used: the tcgen05 forms
+def test_graphs_and_streams_of_portions_and_of_many_tokens():
+    """Two captured steps (write, attend, a product of many tokens) replayed on two streams at once, and eager calls beside them."""
+    from carbon_engine_b200 import ops, ops_int4
+    jobs = []
+    for seed, d, heads, kv_heads in ((0, 128, 32, 8), (100, 64, 48, 4)):
+        c, k, v = filled([900], kv_heads, d, 64, 16, BF16, seed=seed)
+        q = normal((500, heads, d), seed + 9, BF16)
+        out, y = torch.empty_like(q), torch.empty((40, 700), dtype=BF16, device="cuda")
+        w4 = ops_int4.Int4Weight.quantize(normal((700, heads * d), seed + 3, BF16, 0.05), 64)
+        starts, held, tiles = gpu([0, 500]), gpu([900]), gpu([(0, at) for at in range(0, 500, 64)])
+
+        def step(c=c, k=k, v=v, q=q, out=out, y=y, w4=w4, starts=starts, held=held, tiles=tiles):
+            c.write(k, v)
+            c.ops.attention(q, c.pages, out, c.slots, starts, held, c.table, c.status, n_decode=0, max_ctx=900, tiles=tiles, scale=0.09)
+            ops_int4.matmul(out.flatten(1)[:40], w4, y, ops.GEMM_STORE)
+
+        before = [ops.kernel_counts().get(n, 0) for n in ("int4_attention_tc_kernel", "int4_gemm_tc_kernel")]
+        step()
+        torch.cuda.synchronize()
+        assert [ops.kernel_counts().get(n, 0) for n in ("int4_attention_tc_kernel", "int4_gemm_tc_kernel")] == [n + 1 for n in before]
+        want = out.clone(), y.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        jobs.append((graph, step, out, y, want, c, w4))
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for run in (lambda job: job[0].replay(), lambda job: job[1]()):
+        for _ in range(5):
+            for s, job in zip(streams, jobs):
+                with torch.cuda.stream(s):
+                    job[2].zero_(); job[3].zero_()
+                    run(job)
+        torch.cuda.synchronize()
+        for _, _, out, y, want, c, w4 in jobs:
+            assert torch.equal(out, want[0]) and torch.equal(y, want[1]) and int(c.status) == 0 and int(w4.status) == 0
